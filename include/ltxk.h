@@ -377,6 +377,26 @@ int ltxk_attention(void *out, const void *q, int64_t q_bstride, int64_t q_tstrid
                    int64_t batch, int64_t tokens_q, int64_t tokens_k, int64_t heads, int64_t head_dim, float scale,
                    void *workspace, int64_t workspace_bytes, void *stream);
 
+/* Bytes of workspace ltxk_cross_attention needs for this shape. */
+int64_t ltxk_cross_attention_workspace_bytes(int64_t batch, int64_t tokens_q, int64_t tokens_k, int64_t heads,
+                                             int64_t head_dim);
+
+/* ltxk_attention over the keys that `keep` names, for prompts of different lengths
+ * in one batch: keep is one byte per key (non-zero: attended) at keep +
+ * b*keep_bstride + j, of any pattern (NULL: every key).  Keys and values left out
+ * are not read, so they may hold anything; a batch item without a kept key gives
+ * zeros.  The work is that of the kept keys.  The gated output rounds once:
+ *   out[b*Tq + t, h, :] = round(sum * 2*sigmoid(logits[b*Tq + t, h]))
+ * Everything else as ltxk_attention, but `workspace` holds
+ * ltxk_cross_attention_workspace_bytes.
+ * Stands in for SDPA with a mask that closes the context's padding
+ * (standalone/ltx_nn.py:22-26, ltx_dit.py:237-248). */
+int ltxk_cross_attention(void *out, const void *q, int64_t q_bstride, int64_t q_tstride, const void *k,
+                         int64_t k_bstride, int64_t k_tstride, const void *v, int64_t v_bstride, int64_t v_tstride,
+                         const void *keep, int64_t keep_bstride, const void *logits, int64_t batch, int64_t tokens_q,
+                         int64_t tokens_k, int64_t heads, int64_t head_dim, float scale, void *workspace,
+                         int64_t workspace_bytes, void *stream);
+
 /* Bytes of workspace ltxk_linear needs for this shape (at most 64 MB). */
 int64_t ltxk_linear_workspace_bytes(int64_t m, int64_t n, int64_t k);
 
@@ -401,6 +421,52 @@ int ltxk_linear(void *y, const void *x, const void *w, const void *bias, int64_t
  * stream's rows. */
 int ltxk_linear_layers(void *const *y, const void *x, const void *const *w, const void *const *bias,
                        const int64_t *n, int64_t layers, int64_t m, int64_t k, void *stream);
+
+/* ----------------------------------------------------------------------- */
+/* 8-bit linear layers                                                     */
+/* ----------------------------------------------------------------------- */
+
+/* Rows of k values in blocks of 128 e4m3 values (OCP, largest 448) with a
+ * power-of-two scale each; the last block of a row may be short.  With a the
+ * largest magnitude of a block and e the least integer with a <= 448 * 2^e, at
+ * least -127, a value x is held as q = e4m3(x * 2^-e) (to nearest even), which
+ * stands for q * 2^e.  An infinity or NaN makes its whole block NaN.  In memory:
+ *   values  [rows, 128*blocks] bytes, blocks = ceil(k/128), zeros past k
+ *   scales  [ceil(blocks/4), rows, 4] bytes: e + 127 of block 4*i + j of a row
+ *           (255: a NaN block; zeros past the last block)
+ * Both 16-byte aligned. */
+
+/* Values and scales of x [rows, k] (bf16, k a multiple of 8). */
+int ltxk_quantize_fp8(void *q, void *q_scale, const void *x, int64_t rows, int64_t k, void *stream);
+
+/* ltxk_add_norm_modulate with the modulated rows as blocks, not rounded to bf16
+ * before:
+ *   x_out = round(x + f*gate*mask);  q, q_scale = blocks(rms(x_out)*(1 + scale) + shift)
+ * Without f (then x_out, gate and mask are NULL, too): of x itself, as
+ * ltxk_norm_modulate.  x_out may be x. */
+int ltxk_add_norm_modulate_fp8(void *x_out, void *q, void *q_scale, const void *x, const void *f,
+                               const ltxk_ada *gate, const void *mask, int64_t rows, int64_t tokens, int64_t dim,
+                               float eps, const ltxk_ada *shift, const ltxk_ada *scale, void *stream);
+
+/* Bytes of workspace ltxk_linear_fp8 (gelu 0) or ltxk_linear_gelu_fp8 (gelu 1)
+ * needs for this shape. */
+int64_t ltxk_linear_fp8_workspace_bytes(int64_t m, int64_t n, int64_t k, int gelu);
+
+/* y = round(x w^T + bias) for x [m, k] and w [n, k] in blocks, y [m, n] and bias
+ * [n] (or NULL) bf16: exact products of the held values, fp32 sums, one rounding.
+ * n and k are multiples of 8; x, w and y hold fewer than 2^31 values each.
+ * `workspace`: device memory of ltxk_linear_fp8_workspace_bytes, 16-byte aligned
+ * (NULL if that is 0), in use until the call's work has run.  For the linear
+ * layers of the DiT blocks (standalone/ltx_nn.py:188-192,205-207,247-248). */
+int ltxk_linear_fp8(void *y, const void *x, const void *x_scale, const void *w, const void *w_scale, const void *bias,
+                    int64_t m, int64_t n, int64_t k, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* q, q_scale = blocks(gelu_tanh(x w^T + bias)) of [m, n], fp32 up to the blocks:
+ * the first layer of a feed-forward whose second one reads blocks
+ * (standalone/ltx_nn.py:247-248). */
+int ltxk_linear_gelu_fp8(void *q, void *q_scale, const void *x, const void *x_scale, const void *w,
+                         const void *w_scale, const void *bias, int64_t m, int64_t n, int64_t k, void *workspace,
+                         int64_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -57,6 +57,8 @@ struct FlashParams {
     int whole;              // query tiles of an XCD that one workgroup takes alone
     int rest, parts;        // the others, each cut into `parts` units over the keys
     float scale2;           // scale * log2(e)
+    bool round;             // the output rounds to bf16 before the gate, too
+    const int *count, *list;  // kept keys only: how many of each batch item's, and which (batch, tk)
 };
 
 // Query tile t of XCD x: all query tiles of a head go to one XCD, whose L2 then
@@ -94,15 +96,21 @@ typedef __attribute__((address_space(3))) char lds_char;
 template <int D>
 constexpr int kLoads = kKeys * D * 2 / 1024 / kWaves;  // load instructions of a wave for a tile
 
+// The row of a tile that this lane loads in part j.
+template <int D>
+__device__ __forceinline__ int part_row(int j, int wave, int lane)
+{
+    return (wave * kLoads<D> + j) * (1024 / (2 * D)) + lane / (D / 8);
+}
+
 template <int D, bool V>
-__device__ __forceinline__ void load_part(rsrc_t r, char *lds, int j, int first_row, int last_row, uint32_t stride,
-                                          int wave, int lane)
+__device__ __forceinline__ void load_part(rsrc_t r, char *lds, int j, int key, uint32_t stride, int wave, int lane)
 {
     const int at = wave * kLoads<D> + j;
-    const int row = at * (1024 / (2 * D)) + lane / (D / 8);
+    const int row = part_row<D>(j, wave, lane);
     const int pos = lane % (D / 8);
     const int c = V ? v_pos<D>(row, pos) : k_pos<D>(row, pos);  // the permutations are involutions
-    const uint32_t off = static_cast<uint32_t>(min(first_row + row, last_row)) * stride + c * 16;
+    const uint32_t off = static_cast<uint32_t>(key) * stride + c * 16;
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_char *)(lds + at * 1024), 16, off, 0, 0, 0);
 }
 
@@ -123,10 +131,14 @@ __device__ __forceinline__ float pair_sum(float v)
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// The gate 2*sigmoid(logit), and a gated output: the output rounds to bf16 first,
-// as the tensor that the gate multiplies does.
+// The gate 2*sigmoid(logit), and a gated output: in ltxk_attention the output rounds to
+// bf16 first, as the tensor that the gate multiplies does (relative error 2.5e-3 against
+// 1.9e-3 without).
 __device__ __forceinline__ float head_gate(uint16_t logit) { return 2.0f / (1.0f + expf(-bf16_to_f32(logit))); }
-__device__ __forceinline__ float gated(float o, float gate) { return bf16_to_f32(f32_to_bf16(o)) * gate; }
+__device__ __forceinline__ float gated(float o, float gate, bool round)
+{
+    return (round ? bf16_to_f32(f32_to_bf16(o)) : o) * gate;
+}
 
 // This wave's loads have landed and its LDS reads returned, then all waves'.
 __device__ __forceinline__ void tile_barrier()
@@ -137,7 +149,9 @@ __device__ __forceinline__ void tile_barrier()
     asm volatile("" ::: "memory");
 }
 
-template <int D>
+// KEPT: over the keys that p.list names, which it gathers: a batch item's work is
+// that of its kept keys, and nothing of the others is read.
+template <int D, bool KEPT>
 __global__ void __launch_bounds__(kWaves * 64, 2) flash_kernel(FlashParams p)
 {
     constexpr int KS = D / 16;               // contraction steps of the scores
@@ -155,20 +169,54 @@ __global__ void __launch_bounds__(kWaves * 64, 2) flash_kernel(FlashParams p)
     const int unit = j - p.whole, part = split ? unit % p.parts : 0;
     int b, head, first;
     if (!query_tile(p, xcd, split ? p.whole + unit / p.parts : j, b, head, first)) return;
-    const int t0 = split ? part * p.tiles / p.parts : 0;
-    const int t1 = split ? (part + 1) * p.tiles / p.parts : p.tiles;
-    const int n = t1 - t0;  // at least one tile: the host takes no more parts than tiles
+    const int keys = KEPT ? p.count[b] : p.tk;
+    const int tiles = KEPT ? (keys + kKeys - 1) / kKeys : p.tiles;
+    const int t0 = split ? part * tiles / p.parts : 0;
+    const int t1 = split ? (part + 1) * tiles / p.parts : tiles;
+    const int n = t1 - t0;  // at least one tile (the host takes no more parts than tiles), but where keys are left out
     const int last = p.tk - 1;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int l32 = lane & 31, half = lane >> 5;
+    if constexpr (KEPT) {
+        if (n == 0) {  // nothing to attend to: a weight of zero, or an output of zero
+            if (split) {
+                if (half == 0)
+                    p.stats[(static_cast<int64_t>(xcd) * p.rest * p.parts + unit) * kRows + wave * 32 + l32] =
+                        make_float2(-FLT_MAX, 0.f);
+            } else {
+                for (int i = threadIdx.x; i < kRows * (D / 8); i += kWaves * 64) {
+                    const int r = first + i / (D / 8);
+                    if (r < p.tq)
+                        *reinterpret_cast<u32x4 *>(
+                            p.out + ((static_cast<int64_t>(b) * p.tq + r) * p.heads + head) * D + i % (D / 8) * 8) = u32x4{};
+                }
+            }
+            return;
+        }
+    }
     const rsrc_t kr = make_rsrc(p.k + b * p.kbs + head * D, static_cast<uint32_t>(last) * p.kts + 2 * D);
     const rsrc_t vr = make_rsrc(p.v + b * p.vbs + head * D, static_cast<uint32_t>(last) * p.vts + 2 * D);
 
-    auto load_k = [&](int i, int part, char *dst) {
-        load_part<D, false>(kr, dst, part, (t0 + i) * kKeys, last, p.kts, wave, lane);
+    // Kept keys: the rows that this lane loads of tile i (values), i + 1 (keys) and,
+    // on their way, i + 2.
+    int at_v[kLoads<D>], at_k[kLoads<D>], at_next[kLoads<D>];
+    auto listed = [&](int i, int *at) {
+        const int *list = p.list + static_cast<int64_t>(b) * p.tk;
+#pragma unroll
+        for (int c = 0; c < kLoads<D>; ++c)
+            at[c] = list[min((t0 + min(i, n - 1)) * kKeys + part_row<D>(c, wave, lane), keys - 1)];
     };
-    auto load_v = [&](int i, int part, char *dst) {
-        load_part<D, true>(vr, dst, part, (t0 + i) * kKeys, last, p.vts, wave, lane);
+    if constexpr (KEPT) {
+        listed(0, at_k);
+        listed(1, at_next);
+    }
+    auto load_k = [&](int i, int c, char *dst) {
+        const int key = KEPT ? at_k[c] : min((t0 + i) * kKeys + part_row<D>(c, wave, lane), last);
+        load_part<D, false>(kr, dst, c, key, p.kts, wave, lane);
+    };
+    auto load_v = [&](int i, int c, char *dst) {
+        const int key = KEPT ? at_v[c] : min((t0 + i) * kKeys + part_row<D>(c, wave, lane), last);
+        load_part<D, true>(vr, dst, c, key, p.vts, wave, lane);
     };
 #pragma unroll
     for (int c = 0; c < kLoads<D>; ++c) load_k(0, c, k0);
@@ -244,7 +292,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) flash_kernel(FlashParams p)
     // if a row's maximum grew, its weights.
     auto softmax = [&](int i) __attribute__((always_inline)) {
         if (i == n - 1) {  // keys past the last get weight zero
-            const int valid = p.tk - (t0 + i) * kKeys;
+            const int valid = keys - (t0 + i) * kKeys;
             if (valid < kKeys)
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
@@ -304,6 +352,14 @@ __global__ void __launch_bounds__(kWaves * 64, 2) flash_kernel(FlashParams p)
                     __attribute__((always_inline)) {
         constexpr int kEvery = from == 0 ? 3 : 2;
         const int next = min(i + 1, n - 1);
+        if constexpr (KEPT) {
+#pragma unroll
+            for (int c = 0; c < kLoads<D>; ++c) {
+                at_v[c] = at_k[c];
+                at_k[c] = at_next[c];
+            }
+            listed(i + 2, at_next);
+        }
         products(from, integral_constant<int, NV + NK>{}, vp, kc, [&](int j) __attribute__((always_inline)) {
             if (j % kEvery) return;
             const int c = j / kEvery;
@@ -349,14 +405,14 @@ __global__ void __launch_bounds__(kWaves * 64, 2) flash_kernel(FlashParams p)
         for (int c = 0; c < 4; ++c) {
             float f[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) f[r] = gated(o[t][4 * c + r] * inv, gate);
+            for (int r = 0; r < 4; ++r) f[r] = gated(o[t][4 * c + r] * inv, gate, p.round);
             *reinterpret_cast<uint2 *>(op + 32 * t + 8 * c) =
                 make_uint2(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]));
         }
 }
 
 // Merges the units of the split query tiles: 8 columns of one query a thread.
-template <int D>
+template <int D, bool KEPT>
 __global__ void __launch_bounds__(256) flash_merge_kernel(FlashParams p)
 {
     constexpr int kChunks = D / 8;
@@ -370,6 +426,7 @@ __global__ void __launch_bounds__(256) flash_merge_kernel(FlashParams p)
     float acc[8] = {}, sum = 0.f;
     for (int k = 0; k < p.parts; ++k) {
         const float2 st = p.stats[u + k * kRows];
+        if (KEPT && st.y == 0.f) continue;  // no kept key: this unit wrote no sums
         const float w = __builtin_amdgcn_exp2f(st.x - m);
         const f32x4 *x = reinterpret_cast<const f32x4 *>(p.part + (u + k * kRows) * D + c * 8);
         const f32x4 lo = x[0], hi = x[1];
@@ -381,9 +438,9 @@ __global__ void __launch_bounds__(256) flash_merge_kernel(FlashParams p)
         }
     }
     const int64_t tok = (static_cast<int64_t>(b) * p.tq + first + r) * p.heads + head;
-    const float gate = p.logits ? head_gate(p.logits[tok]) : 1.f, inv = 1.f / sum;
+    const float gate = p.logits ? head_gate(p.logits[tok]) : 1.f, inv = KEPT && sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] = gated(acc[e] * inv, gate);
+    for (int e = 0; e < 8; ++e) acc[e] = gated(acc[e] * inv, gate, p.round);
     *reinterpret_cast<u32x4 *>(p.out + tok * D + c * 8) = pack8v(acc);
 }
 
@@ -412,11 +469,41 @@ FlashCut cut(int64_t bh, int64_t tokens_q, int64_t tokens_k)
     return c;
 }
 
-template <int D>
+template <int D, bool KEPT>
 void launch(const FlashParams &p, hipStream_t s)
 {
-    flash_kernel<D><<<8u * (p.whole + p.rest * p.parts), kWaves * 64, 0, s>>>(p);
-    if (p.rest) flash_merge_kernel<D><<<8u * (p.rest * (kRows * D / 8) / 256), 256, 0, s>>>(p);
+    flash_kernel<D, KEPT><<<8u * (p.whole + p.rest * p.parts), kWaves * 64, 0, s>>>(p);
+    if (p.rest) flash_merge_kernel<D, KEPT><<<8u * (p.rest * (kRows * D / 8) / 256), 256, 0, s>>>(p);
+}
+
+// The kept keys of each batch item in their order, a workgroup an item: 1024 keys a
+// round, each wave's by a ballot, the waves' counts added up in LDS.
+__global__ void __launch_bounds__(1024) keep_kernel(const uint8_t *keep, int64_t stride, int tk, int *count, int *list)
+{
+    __shared__ int waves[2][16];
+    const int64_t b = blockIdx.x;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    int before = 0;
+    for (int first = 0, round = 0; first < tk; first += 1024, round ^= 1) {
+        const int i = first + threadIdx.x;
+        const bool kept = i < tk && keep[b * stride + i];
+        const uint64_t ballot = __ballot(kept);
+        if (lane == 0) waves[round][wave] = __popcll(ballot);
+        __syncthreads();
+        int at = before;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) {
+            if (w < wave) at += waves[round][w];
+            before += waves[round][w];
+        }
+        if (kept) list[b * tk + at + __popcll(ballot & ((uint64_t{1} << lane) - 1))] = i;
+    }
+    if (threadIdx.x == 0) count[b] = before;
+}
+
+int64_t list_bytes(int64_t batch, int64_t tokens_k)
+{
+    return (batch * (tokens_k + 1) * 4 + 15) / 16 * 16;
 }
 
 }  // namespace
@@ -432,13 +519,14 @@ extern "C" int64_t ltxk_attention_workspace_bytes(int64_t batch, int64_t tokens_
     return 8 * c.rest * c.parts * kRows * (head_dim + 2) * 4;
 }
 
-extern "C" int ltxk_attention(void *out, const void *q, int64_t q_bstride, int64_t q_tstride, const void *k,
-                              int64_t k_bstride, int64_t k_tstride, const void *v, int64_t v_bstride,
-                              int64_t v_tstride, const void *logits, int64_t batch, int64_t tokens_q,
-                              int64_t tokens_k, int64_t heads, int64_t head_dim, float scale, void *workspace,
-                              int64_t workspace_bytes, void *stream)
+// The checks and the launch of both entry points; `lists` bytes of the workspace are
+// for the kept keys' list.
+static int attend(const char *what, bool round, int64_t lists, void *out, const void *q, int64_t q_bstride, int64_t q_tstride, const void *k,
+                  int64_t k_bstride, int64_t k_tstride, const void *v, int64_t v_bstride, int64_t v_tstride,
+                  const void *keep, int64_t keep_bstride, const void *logits, int64_t batch, int64_t tokens_q,
+                  int64_t tokens_k, int64_t heads, int64_t head_dim, float scale, void *workspace,
+                  int64_t workspace_bytes, void *stream)
 {
-    static const char *what = "attention";
     clear_error();
     if (batch < 0 || tokens_q < 0 || tokens_k < 0 || heads <= 0)
         return fail(LTXK_E_ARG, "%s: bad shape batch=%lld tokens_q=%lld tokens_k=%lld heads=%lld", what,
@@ -469,16 +557,17 @@ extern "C" int ltxk_attention(void *out, const void *q, int64_t q_bstride, int64
     // a launch holds fewer than 2^32 threads
     if (c.whole + c.rest * c.parts >= (int64_t{1} << 32) / (8 * kWaves * 64))
         return fail(LTXK_E_ARG, "%s: too many query tiles", what);
-    if (c.rest && (!workspace || !aligned16(workspace) ||
-                   workspace_bytes < ltxk_attention_workspace_bytes(batch, tokens_q, tokens_k, heads, head_dim)))
-        return fail(LTXK_E_ARG, "%s: the workspace must hold ltxk_attention_workspace_bytes, 16-byte aligned", what);
+    if ((c.rest || lists) &&
+        (!workspace || !aligned16(workspace) ||
+         workspace_bytes < lists + ltxk_attention_workspace_bytes(batch, tokens_q, tokens_k, heads, head_dim)))
+        return fail(LTXK_E_ARG, "%s: the workspace must hold ltxk_%s_workspace_bytes, 16-byte aligned", what, what);
     FlashParams p{};
     p.q = static_cast<const uint16_t *>(q);
     p.k = static_cast<const uint16_t *>(k);
     p.v = static_cast<const uint16_t *>(v);
     p.logits = static_cast<const uint16_t *>(logits);
     p.out = static_cast<uint16_t *>(out);
-    p.part = static_cast<float *>(workspace);
+    p.part = reinterpret_cast<float *>(static_cast<char *>(workspace) + lists);
     p.stats = reinterpret_cast<float2 *>(p.part + 8 * c.rest * c.parts * kRows * head_dim);
     p.qbs = q_bstride;
     p.kbs = k_bstride;
@@ -496,9 +585,56 @@ extern "C" int ltxk_attention(void *out, const void *q, int64_t q_bstride, int64
     p.rest = static_cast<int>(c.rest);
     p.parts = static_cast<int>(c.parts);
     p.scale2 = scale2;
-    if (head_dim == 128)
-        launch<128>(p, static_cast<hipStream_t>(stream));
-    else
-        launch<64>(p, static_cast<hipStream_t>(stream));
+    p.round = round;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (keep) {
+        int *count = static_cast<int *>(workspace), *list = count + batch;
+        p.count = count;
+        p.list = list;
+        keep_kernel<<<static_cast<unsigned>(batch), 1024, 0, s>>>(static_cast<const uint8_t *>(keep), keep_bstride, p.tk,
+                                                                  count, list);
+        if (head_dim == 128)
+            launch<128, true>(p, s);
+        else
+            launch<64, true>(p, s);
+    } else if (head_dim == 128) {
+        launch<128, false>(p, s);
+    } else {
+        launch<64, false>(p, s);
+    }
     return check_launch(what);
+}
+
+extern "C" int ltxk_attention(void *out, const void *q, int64_t q_bstride, int64_t q_tstride, const void *k,
+                              int64_t k_bstride, int64_t k_tstride, const void *v, int64_t v_bstride,
+                              int64_t v_tstride, const void *logits, int64_t batch, int64_t tokens_q,
+                              int64_t tokens_k, int64_t heads, int64_t head_dim, float scale, void *workspace,
+                              int64_t workspace_bytes, void *stream)
+{
+    return attend("attention", true, 0, out, q, q_bstride, q_tstride, k, k_bstride, k_tstride, v, v_bstride, v_tstride, nullptr,
+                  0, logits, batch, tokens_q, tokens_k, heads, head_dim, scale, workspace, workspace_bytes, stream);
+}
+
+extern "C" int64_t ltxk_cross_attention_workspace_bytes(int64_t batch, int64_t tokens_q, int64_t tokens_k,
+                                                        int64_t heads, int64_t head_dim)
+{
+    if (batch <= 0 || tokens_q <= 0 || tokens_k <= 0 || heads <= 0 || head_dim <= 0) return 0;
+    return list_bytes(batch, tokens_k) + ltxk_attention_workspace_bytes(batch, tokens_q, tokens_k, heads, head_dim);
+}
+
+extern "C" int ltxk_cross_attention(void *out, const void *q, int64_t q_bstride, int64_t q_tstride, const void *k,
+                                    int64_t k_bstride, int64_t k_tstride, const void *v, int64_t v_bstride,
+                                    int64_t v_tstride, const void *keep, int64_t keep_bstride, const void *logits,
+                                    int64_t batch, int64_t tokens_q, int64_t tokens_k, int64_t heads, int64_t head_dim,
+                                    float scale, void *workspace, int64_t workspace_bytes, void *stream)
+{
+    static const char *what = "cross_attention";
+    clear_error();
+    if (keep_bstride < 0) return fail(LTXK_E_ARG, "%s: keep's stride must not be negative", what);
+    // the list's size once batch and tokens_k are known to be in range
+    const int64_t lists = batch > 0 && batch <= (1 << 20) && tokens_k > 0 && tokens_k < 0x7fffffff
+                              ? list_bytes(batch, tokens_k) : 0;
+    return attend(what, false, lists, out, q, q_bstride, q_tstride, k, k_bstride, k_tstride, v, v_bstride, v_tstride, keep,
+                  keep_bstride, logits, batch, tokens_q, tokens_k, heads, head_dim, scale, workspace, workspace_bytes,
+                  stream);
 }

@@ -133,6 +133,20 @@ SIGNATURES = {
         [_c_vp, _c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_i64,
          _c_i64, _c_i64, _c_float, _c_vp, _c_i64, _c_vp],
     ),
+    "ltxk_cross_attention_workspace_bytes": (_c_i64, [_c_i64] * 5),
+    "ltxk_cross_attention": (
+        _c_int,
+        [_c_vp, _c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64,
+         _c_i64, _c_i64, _c_i64, _c_i64, _c_float, _c_vp, _c_i64, _c_vp],
+    ),
+    "ltxk_quantize_fp8": (_c_int, [_c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_vp]),
+    "ltxk_add_norm_modulate_fp8": (
+        _c_int,
+        [_c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _ADA_P, _c_vp, _c_i64, _c_i64, _c_i64, _c_float, _ADA_P, _ADA_P, _c_vp],
+    ),
+    "ltxk_linear_fp8_workspace_bytes": (_c_i64, [_c_i64, _c_i64, _c_i64, _c_int]),
+    "ltxk_linear_fp8": (_c_int, [_c_vp] * 6 + [_c_i64] * 3 + [_c_vp, _c_i64, _c_vp]),
+    "ltxk_linear_gelu_fp8": (_c_int, [_c_vp] * 7 + [_c_i64] * 3 + [_c_vp, _c_i64, _c_vp]),
 }
 
 _lib = None
@@ -272,6 +286,19 @@ def _stream(t: torch.Tensor) -> int:
     if _raw_stream is not None:
         return _raw_stream(t.get_device())
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _one_device(t: torch.Tensor, *others: torch.Tensor | None) -> None:
+    """All operands on one device, and that the current one, on whose stream the call runs."""
+    device = t.get_device()
+    for o in others:
+        if o is not None and o.get_device() != device:
+            raise ValueError(f"operands are on {t.device} and {o.device}")
+    if device != _current_device():
+        raise RuntimeError(f"operands are on {t.device}, which is not the current device (torch.cuda.set_device)")
 
 
 def _ptr(t: torch.Tensor | None) -> int | None:
@@ -889,6 +916,252 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: int, log
     rc = lib.ltxk_attention(_ptr(out), q.data_ptr(), tq * d, d, k.data_ptr(), tk * d, d, v.data_ptr(), tk * d, d,
                             _ptr(logits), b, tq, tk, heads, dh, dh ** -0.5, _ptr(ws), nbytes, _stream(q))
     _check_rc(rc, "attention")
+    return out
+
+
+def _rows_of(x: torch.Tensor, name: str, b: int, t: int, d: int) -> torch.Tensor:
+    """x if it is bf16 (b, t, d) with contiguous rows that the kernels can read through its
+    batch and token strides (not negative, multiples of 8), else an error."""
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if x.device.type != "cuda":
+        raise RuntimeError(f"{name} is on {x.device}; ltxk kernels run on the ROCm device only")
+    if x.dtype != torch.bfloat16:
+        raise ValueError(f"{name} has dtype {x.dtype}, expected torch.bfloat16")
+    if tuple(x.shape) != (b, t, d):
+        raise ValueError(f"{name} is {tuple(x.shape)}, expected {(b, t, d)}")
+    if x.numel() and ((d > 1 and x.stride(2) != 1) or x.stride(0) % 8 or x.stride(1) % 8
+                      or (t > 1 and x.stride(1) < d)):
+        raise ValueError(f"{name}'s rows must be contiguous, with batch and token strides (multiples of 8) that cover "
+                         f"them; got {x.stride()}")
+    return x
+
+
+def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: int, keep: torch.Tensor | None = None,
+                    logits: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """attention of q (B, Tq, H*Dh) over the kept ones of an encoder's states: k and v (B, Tk, H*Dh), heads of 64 or
+    128, keep (B or 1, Tk) bool or uint8 (True: attended; None: all are), logits (B, Tq, H) as in `attention`, the
+    gated result rounded once.
+
+    q, k and v may be views of wider rows (one projection's key and value halves).  Keys and values that are not kept
+    are not read and cost no time, whatever their pattern; where nothing is kept (or Tk is 0) the result is zero."""
+    if not all(isinstance(x, torch.Tensor) and x.ndim == 3 for x in (q, k, v)):
+        raise ValueError("q, k and v must be (B, T, H*Dh) tensors")
+    (b, tq, d), tk = q.shape, k.shape[1]
+    for x, name, t in ((q, "q", tq), (k, "k", tk), (v, "v", tk)):
+        _rows_of(x, name, b, t, d)
+    dh = d // heads if heads > 0 else 0
+    if d != heads * dh or dh not in ATTENTION_HEAD_DIMS:
+        raise ValueError(f"width {d} is not {heads} heads of 64 or 128")
+    if keep is not None:
+        _dev(keep, "keep", (torch.bool, torch.uint8))
+        if keep.ndim != 2 or keep.shape[0] not in (1, b) or keep.shape[1] != tk:
+            raise ValueError(f"keep {tuple(keep.shape)} must be ({b} or 1, {tk})")
+    if logits is not None:
+        _dev(logits, "logits")
+        if tuple(logits.shape) != (b, tq, heads):
+            raise ValueError(f"logits {tuple(logits.shape)} != {(b, tq, heads)}")
+    if out is None:
+        out = torch.empty((b, tq, d), device=q.device, dtype=q.dtype)
+    else:
+        _dev(out, "out")
+        if tuple(out.shape) != (b, tq, d):
+            raise ValueError(f"out {tuple(out.shape)} != {(b, tq, d)}")
+    _one_device(q, k, v, keep, logits, out)
+    if out.numel() == 0:
+        return out
+    if tk == 0:
+        return out.zero_()
+    lib = load()
+    # a stride that is never taken (one token, one batch item) may be anything in torch
+    strides = [s for x, t in ((q, tq), (k, tk), (v, tk)) for s in (x.stride(0) if b > 1 else 0,
+                                                                    x.stride(1) if t > 1 else d)]
+    (qb, qt, kb, kt, vb, vt), st = strides, _stream(q)
+    nbytes = lib.ltxk_cross_attention_workspace_bytes(b, tq, tk, heads, dh)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    rc = lib.ltxk_cross_attention(_ptr(out), q.data_ptr(), qb, qt, k.data_ptr(), kb, kt, v.data_ptr(), vb, vt,
+                                  _ptr(keep), tk if keep is not None and keep.shape[0] > 1 else 0, _ptr(logits), b, tq,
+                                  tk, heads, dh, dh ** -0.5, ws.data_ptr(), nbytes, st)
+    _check_rc(rc, "cross_attention")
+    return out
+
+
+# --------------------------------------------------------------------------
+# 8-bit linear layers
+# --------------------------------------------------------------------------
+
+FP8_BLOCK, FP8_GROUP = 128, 4
+
+
+class Fp8Blocks:
+    """Rows in blocks of 128 e4m3 values with a power-of-two scale each, as the 8-bit
+    linear layers read them.
+
+    shape (..., K): what is held.  data: float8_e4m3fn (rows, 128 * ceil(K / 128)), zeros past K.
+    scale: uint8 (ceil(blocks / 4), rows, 4), the exponent + 127 of block 4 i + j of row r at [i, r, j];
+    255 marks a block that held an infinity or NaN.  K is a multiple of 8.  Made by quantize_fp8 and the
+    kernels that write blocks; a program that keeps quantised weights may build it from its own tensors."""
+
+    __slots__ = ("data", "scale", "shape")
+
+    def __init__(self, data: torch.Tensor, scale: torch.Tensor, shape):
+        shape = tuple(shape)
+        _dev(data, "data", torch.float8_e4m3fn)
+        _dev(scale, "scale", torch.uint8)
+        if not shape or shape[-1] <= 0 or shape[-1] % 8:
+            raise ValueError(f"shape {shape} must end in a positive multiple of 8")
+        rows, blocks = _fp8_extent(shape)
+        if tuple(data.shape) != (rows, blocks * FP8_BLOCK):
+            raise ValueError(f"data {tuple(data.shape)} does not hold {shape}: expected {(rows, blocks * FP8_BLOCK)}")
+        want = (-(-blocks // FP8_GROUP), rows, FP8_GROUP)
+        if tuple(scale.shape) != want:
+            raise ValueError(f"scale {tuple(scale.shape)} does not hold {shape}: expected {want}")
+        if data.get_device() != scale.get_device():
+            raise ValueError(f"data is on {data.device}, scale on {scale.device}")
+        self.data, self.scale, self.shape = data, scale, shape
+
+    @classmethod
+    def _made(cls, shape, device) -> "Fp8Blocks":
+        """Uninitialised blocks for a kernel to fill."""
+        rows, blocks = _fp8_extent(shape)
+        self = object.__new__(cls)
+        self.shape = tuple(shape)
+        self.data = torch.empty(rows, blocks * FP8_BLOCK, device=device, dtype=torch.float8_e4m3fn)
+        self.scale = torch.empty(-(-blocks // FP8_GROUP), rows, FP8_GROUP, device=device, dtype=torch.uint8)
+        return self
+
+    @property
+    def device(self) -> torch.device:
+        return self.data.device
+
+    def float(self) -> torch.Tensor:
+        """The values held, in fp32 (exact but where they leave fp32's range), by torch operations."""
+        rows, blocks = _fp8_extent(self.shape)
+        e = self.scale.transpose(0, 1).reshape(rows, -1)[:, :blocks, None].to(torch.int32)
+        power = torch.where(e == 0, 1 << 22, e << 23).view(torch.float32)  # 2^(e - 127), 2^-127 a subnormal; 255: infinite
+        v = self.data.float().view(rows, blocks, FP8_BLOCK) * power
+        v = v.masked_fill(e == 255, float("nan"))
+        return v.reshape(rows, -1)[:, :self.shape[-1]].reshape(self.shape)
+
+    def view(self, *shape) -> "Fp8Blocks":
+        """The same rows under another leading shape."""
+        lead = 1
+        for s in shape[:-1]:
+            lead *= s
+        if not shape or shape[-1] != self.shape[-1] or lead != self.data.shape[0]:
+            raise ValueError(f"{self.shape} has no view {shape}: the last dimension stays")
+        return Fp8Blocks(self.data, self.scale, shape)
+
+
+def _fp8_extent(shape) -> tuple[int, int]:
+    """(rows, blocks of a row)."""
+    rows = 1
+    for s in shape[:-1]:
+        rows *= s
+    return rows, -(-shape[-1] // FP8_BLOCK)
+
+
+def quantize_fp8(x: torch.Tensor) -> Fp8Blocks:
+    """x (..., K) bf16 in blocks; K a positive multiple of 8."""
+    _dev(x, "x")
+    if x.ndim == 0 or x.shape[-1] == 0 or x.shape[-1] % 8:
+        raise ValueError(f"x {tuple(x.shape)} must end in a positive multiple of 8")
+    _one_device(x)
+    out = Fp8Blocks._made(x.shape, x.device)
+    rc = load().ltxk_quantize_fp8(out.data.data_ptr(), out.scale.data_ptr(), x.data_ptr(), out.data.shape[0],
+                                  x.shape[-1], _stream(x))
+    _check_rc(rc, "quantize_fp8")
+    return out
+
+
+def norm_modulate_fp8(x: torch.Tensor, shift: AdaRef | None = None, scale: AdaRef | None = None,
+                      eps: float = 1e-6) -> Fp8Blocks:
+    """rms(x)*(1+scale)+shift in blocks, not rounded to bf16 before."""
+    return _norm_fp8(x, None, None, None, shift, scale, eps, None)[1]
+
+
+def add_norm_modulate_fp8(x: torch.Tensor, f: torch.Tensor, gate: AdaRef | None = None,
+                          mask: torch.Tensor | None = None, shift: AdaRef | None = None, scale: AdaRef | None = None,
+                          eps: float = 1e-6, x_out: torch.Tensor | None = None) -> tuple[torch.Tensor, Fp8Blocks]:
+    """x' = x + f*gate*mask; returns (x', rms(x')*(1+scale)+shift in blocks): `add_norm_modulate` for an 8-bit layer."""
+    if f is None:
+        raise ValueError("add_norm_modulate_fp8 needs f (norm_modulate_fp8 takes x alone)")
+    return _norm_fp8(x, f, gate, mask, shift, scale, eps, x_out)
+
+
+def _norm_fp8(x, f, gate, mask, shift, scale, eps, x_out):
+    b, t, d = _btd(x, "x")
+    if f is not None:
+        _dev(f, "f")
+        if f.shape != x.shape:
+            raise ValueError(f"x {tuple(x.shape)} and f {tuple(f.shape)} differ")
+        x_out = _out_like(x_out, x, "x_out")
+    if mask is not None:
+        _dev(mask, "mask")
+        if mask.numel() != b:
+            raise ValueError(f"mask must hold one value per batch item ({b}), got {mask.numel()}")
+    if d == 0 or d % 8:
+        raise ValueError(f"x {tuple(x.shape)} must end in a positive multiple of 8")
+    _one_device(x, f, mask, *[o for a in (gate, shift, scale) if a is not None for o in (a.table, a.emb)])
+    out = Fp8Blocks._made(x.shape, x.device)
+    if x.numel() == 0:
+        return x_out, out
+    rc = load().ltxk_add_norm_modulate_fp8(
+        _ptr(x_out), out.data.data_ptr(), out.scale.data_ptr(), _ptr(x), _ptr(f), _ada_arg(gate, b, t, d), _ptr(mask),
+        b * t, t, d, eps, _ada_arg(shift, b, t, d), _ada_arg(scale, b, t, d), _stream(x))
+    _check_rc(rc, "add_norm_modulate_fp8")
+    return x_out, out
+
+
+def _fp8_operands(x, weight: Fp8Blocks, bias: torch.Tensor | None) -> Fp8Blocks:
+    """x in blocks, after the checks that both 8-bit layers share."""
+    if not isinstance(weight, Fp8Blocks):
+        raise TypeError("weight must be Fp8Blocks (quantize_fp8)")
+    if len(weight.shape) != 2 or weight.shape[0] == 0 or weight.shape[0] % 8:
+        raise ValueError(f"weight {weight.shape} must be (N, K), N a positive multiple of 8")
+    if not isinstance(x, Fp8Blocks):
+        _dev(x, "x")
+    if len(x.shape) == 0 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"x {tuple(x.shape)} does not end in the weight's {weight.shape[1]} columns")
+    if bias is not None:
+        _dev(bias, "bias")
+        if tuple(bias.shape) != (weight.shape[0],):
+            raise ValueError(f"bias {tuple(bias.shape)} must be ({weight.shape[0]},)")
+    x = x if isinstance(x, Fp8Blocks) else quantize_fp8(x)
+    _one_device(x.data, weight.data, bias)
+    return x
+
+
+def _fp8_workspace(lib, m: int, n: int, k: int, gelu: int, device) -> tuple:
+    nbytes = lib.ltxk_linear_fp8_workspace_bytes(m, n, k, gelu)
+    return (torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None), nbytes
+
+
+def linear_fp8(x: torch.Tensor | Fp8Blocks, weight: Fp8Blocks, bias: torch.Tensor | None = None) -> torch.Tensor:
+    """x (..., K) weight (N, K)^T + bias (N) as bf16, over blocks: x as it is held, or quantised first if it is bf16.
+    Exact products of the held values, fp32 sums, one rounding; N a multiple of 8."""
+    x = _fp8_operands(x, weight, bias)
+    (n, k), m = weight.shape, x.data.shape[0]
+    out = torch.empty(*x.shape[:-1], n, device=x.device, dtype=torch.bfloat16)
+    lib = load()
+    ws, nbytes = _fp8_workspace(lib, m, n, k, 0, x.device)
+    rc = lib.ltxk_linear_fp8(out.data_ptr(), x.data.data_ptr(), x.scale.data_ptr(), weight.data.data_ptr(),
+                             weight.scale.data_ptr(), _ptr(bias), m, n, k, _ptr(ws), nbytes, _stream(x.data))
+    _check_rc(rc, "linear_fp8")
+    return out
+
+
+def linear_gelu_fp8(x: torch.Tensor | Fp8Blocks, weight: Fp8Blocks, bias: torch.Tensor | None = None) -> Fp8Blocks:
+    """gelu_tanh(x weight^T + bias) in blocks, fp32 up to them: a feed-forward's first layer for an 8-bit second."""
+    x = _fp8_operands(x, weight, bias)
+    (n, k), m = weight.shape, x.data.shape[0]
+    out = Fp8Blocks._made((*x.shape[:-1], n), x.device)
+    lib = load()
+    ws, nbytes = _fp8_workspace(lib, m, n, k, 1, x.device)
+    rc = lib.ltxk_linear_gelu_fp8(out.data.data_ptr(), out.scale.data_ptr(), x.data.data_ptr(), x.scale.data_ptr(),
+                                  weight.data.data_ptr(), weight.scale.data_ptr(), _ptr(bias), m, n, k, _ptr(ws),
+                                  nbytes, _stream(x.data))
+    _check_rc(rc, "linear_gelu_fp8")
     return out
 
 
