@@ -11,6 +11,9 @@
 // the result's rounding to bf16.  Everything past a group of 8 is fp32.
 #include "fp8_blocks.h"
 
+#include <algorithm>
+#include <type_traits>
+
 namespace ltxk {
 namespace {
 
@@ -24,6 +27,9 @@ struct Fp8Params {
     uint8_t *q, *qs;   // its blocks after GELU
     float *part;       // fp32 sums (m, np)
     int m, n, kp, blocks, np;
+    int tiles_m, tiles_n;
+    int whole, rest, parts;  // tiles that one workgroup takes alone; the others, cut into parts over K
+    int per;                 // units of the cut tiles an XCD
 };
 
 __device__ __forceinline__ i32x8 cat(i32x4 a, i32x4 b)
@@ -38,6 +44,716 @@ __device__ __forceinline__ float gelu(float x)
     constexpr float kC1 = -2.0f * 1.4426950408889634f * 0.7978845608028654f, kC2 = kC1 * 0.044715f;
     return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * __builtin_fmaf(kC2, x * x, kC1)));
 }
+
+// --------------------------------------------------------------------- tiles --
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) char lds_char;
+
+// LDS position of 16-byte chunk c of a tile's row of 128 values: 16 rows of one
+// chunk column, which a fragment read takes at a time, cover all banks.
+__device__ __forceinline__ int chunk_pos(int row, int c) { return c ^ ((row >> 1) & 7); }
+
+// 64 lanes x 16 (4) bytes from memory straight to LDS at `lds`, through m0.  In assembly
+// because the compiler, which cannot tell the buffers of a ring apart, would wait
+// for every load in flight before each LDS read; it has no output register, and its
+// wait is step_barrier's.  The wait states cover scalar operands that a vector
+// instruction has just written.  Nothing else in the kernel may use m0.
+__device__ __forceinline__ void load_lds16(const u32x4 &rsrc, uint32_t lds, uint32_t off, uint32_t soff)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                 ::"s"(lds), "v"(off), "s"(rsrc), "s"(soff)
+                 : "memory");
+}
+__device__ __forceinline__ void load_lds4(const u32x4 &rsrc, uint32_t lds, uint32_t off, uint32_t soff)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, %3 offen lds"
+                 ::"s"(lds), "v"(off), "s"(rsrc), "s"(soff)
+                 : "memory");
+}
+
+// At most `N` of this wave's loads in flight (none without `more`) and its LDS
+// reads returned, then all waves'.
+template <int N>
+__device__ __forceinline__ void step_barrier(bool more)
+{
+    asm volatile("" ::: "memory");
+    if (more)
+        __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | (N >> 4 << 14));  // vmcnt(N) lgkmcnt(0)
+    else
+        __builtin_amdgcn_s_waitcnt(0x0070);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+__device__ __forceinline__ u32x4 whole_memory(const void *base)
+{
+    const uint64_t a = reinterpret_cast<uint64_t>(base);
+    return u32x4{static_cast<uint32_t>(a), static_cast<uint32_t>(a >> 32) & 0xffff, 0xffffffffu, 0x00020000u};
+}
+
+constexpr int kBand = 4;  // tiles of x that a band of the tile order holds
+
+// A workgroup's tile: SIZE rows of x and as many of w, WM x WN waves.  Steps of 128 values
+// are held in LDS, the first DEEP of a wave's loads for a step (rows of x first, then of
+// w) RD steps deep, the others RS.
+template <int SIZE, int WM_, int WN_, int DEEP, int RD_, int RS_>
+struct Tile {
+    static constexpr int size = SIZE;
+    static constexpr int WM = WM_, WN = WN_, waves = WM * WN;
+    static constexpr int MT = SIZE / WM / 32, NT = SIZE / WN / 32;  // 32-row tiles of a wave
+    static constexpr int L = 2 * SIZE / 8 / waves, LD = DEEP, LS = L - LD;  // loads of a wave for a step
+    static constexpr int RD = RD_, RS = RS_;
+    static constexpr int deep_rows = LD * waves * 8, deep_bytes = LD * waves * 1024, shallow_bytes = LS * waves * 1024;
+    static constexpr int shallow_at = RD * deep_bytes, scale_at = shallow_at + RS * shallow_bytes;
+    static constexpr int lds = scale_at + 4 * SIZE * 4;  // two groups' scales of x and w
+    static_assert(LS == 0 ? RS == RD : RS == 2 && RD == 3, "the waits below");
+    static_assert(deep_rows % (MT * 32) == 0 && (deep_rows <= SIZE || LS == 0), "a wave's rows of x have one depth");
+};
+
+// The rows of x and w that tile t takes: bands kBand tiles of x deep.
+template <int TILE>
+__device__ __forceinline__ void tile_rows(const Fp8Params &p, int t, int &m0, int &n0)
+{
+    const int band = t / (kBand * p.tiles_n), at = t % (kBand * p.tiles_n);
+    const int deep = min(kBand, p.tiles_m - band * kBand);
+    m0 = (band * kBand + at % deep) * TILE;
+    n0 = at / deep * TILE;
+}
+
+template <typename T, bool GELU>
+__global__ void __launch_bounds__(T::waves * 64, T::waves / 4) tile_kernel(Fp8Params p)
+{
+    constexpr int MT = T::MT, NT = T::NT, L = T::L, LD = T::LD, LS = T::LS, RD = T::RD, RS = T::RS, TILE = T::size;
+    __shared__ __attribute__((aligned(1024))) char smem[T::lds];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int l32 = lane & 31, half = lane >> 5;
+
+    // A run of neighbouring tiles per XCD (workgroups are dealt to the XCDs in
+    // turn), so that its L2 serves a tile of either side to several workgroups.
+    const int xcd = blockIdx.x & 7, j = blockIdx.x >> 3, whole_per = p.whole >> 3;
+    int tile, part = -1;
+    if (j < whole_per) {
+        tile = xcd * whole_per + j;
+    } else {
+        const int per = (p.rest * p.parts + 7) >> 3, unit = xcd * per + j - whole_per;
+        if (j - whole_per >= per || unit >= p.rest * p.parts) return;
+        part = p.parts == 1 ? -1 : unit / p.rest;
+        tile = p.whole + unit % p.rest;
+    }
+    int m0, n0;
+    tile_rows<TILE>(p, tile, m0, n0);
+    // parts * blocks stays below 2^32: 256 parts at most of fewer than 2^24 blocks
+    auto from = [&](int i) { return static_cast<int>(static_cast<uint32_t>(i) * p.blocks / static_cast<uint32_t>(p.parts)); };
+    const int first = part < 0 ? 0 : from(part), n = (part < 0 ? p.blocks : from(part + 1)) - first;
+
+    const u32x4 xr = whole_memory(p.x), wr = whole_memory(p.w);
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char *)smem));
+    // Load c of a step: rows (c * waves + wave) * 8 .. + 7 of the tile's x and w together.
+    // Rows past the last repeat it; their results are not stored.
+    uint32_t at[L];
+#pragma unroll
+    for (int c = 0; c < L; ++c) {
+        const int row = (c * T::waves + wave) * 8 + (lane >> 3);
+        const bool is_x = c * T::waves * 8 < TILE;
+        at[c] = static_cast<uint32_t>(is_x ? min(m0 + row, p.m - 1) : min(n0 + row - TILE, p.n - 1)) *
+                    static_cast<uint32_t>(p.kp) + chunk_pos(row, lane & 7) * 16;
+    }
+    // Scales, 64 rows a load: x's first, then w's.
+    constexpr int kScaleLoads = 2 * TILE / 64 / T::waves;
+    static_assert(kScaleLoads * T::waves * 64 == 2 * TILE && TILE / 64 % kScaleLoads == 0, "a wave loads x's or w's");
+    const bool sx = wave * kScaleLoads < TILE / 64;
+    const u32x4 sr = whole_memory(sx ? p.xs : p.ws);
+    const int s_rows = sx ? p.m : p.n;
+    uint32_t so[kScaleLoads];
+#pragma unroll
+    for (int c = 0; c < kScaleLoads; ++c)
+        so[c] = static_cast<uint32_t>(min((sx ? m0 : n0 - TILE) + (wave * kScaleLoads + c) * 64 + lane, s_rows - 1)) * 4;
+    const int groups = (p.blocks + 3) >> 2;
+    // A group's scales, into its half of their place; past the last group the last one's, which nothing reads.
+    auto load_scales = [&](int group) {
+#pragma unroll
+        for (int c = 0; c < kScaleLoads; ++c)
+            load_lds4(sr, __builtin_amdgcn_readfirstlane(lds0 + T::scale_at + (group & 1) * (2 * TILE * 4) +
+                                                         (wave * kScaleLoads + c) * 256), so[c],
+                      __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(min(group, groups - 1)) * s_rows * 4));
+    };
+    // Load c of step i, into place `slot` of its ring.
+    auto load = [&](int i, int c, int slot) {
+        const int to = c < LD ? slot * T::deep_bytes + c * T::waves * 1024
+                              : T::shallow_at + slot * T::shallow_bytes + (c - LD) * T::waves * 1024;
+        load_lds16(c * T::waves * 8 < TILE ? xr : wr, __builtin_amdgcn_readfirstlane(lds0 + to + wave * 1024), at[c],
+                   __builtin_amdgcn_readfirstlane((first + i) * kFp8Block));
+    };
+    load_scales(first >> 2);
+    load_scales((first >> 2) + 1);
+    for (int i = 0; i < RD && i < n; ++i) {
+        if (i < RS)
+#pragma unroll
+            for (int c = LD; c < L; ++c) load(i, c, i);
+#pragma unroll
+        for (int c = 0; c < LD; ++c) load(i, c, i);
+    }
+
+    int off[4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) off[s] = l32 * 128 + chunk_pos(l32, 2 * s + half) * 16;
+    const int wm = wave / T::WN * (MT * 32), wn = wave % T::WN * (NT * 32);  // this wave's rows
+
+    // acc[i][j]: lane l holds row 32 i + l % 32 of x; register r row 32 j + 8 (r/4) + 4 half + r % 4 of w
+    f32x16 acc[MT][NT] = {};
+    // Fragments of a half step (64 values): x's in two sets, w's in one whose second half is
+    // read while the first is multiplied, which is what the registers hold.
+    constexpr int kEarly = NT / 2;
+    i32x8 xf[2][MT], wf[NT];
+    int xs[MT], ws[NT], xs_next[MT], ws_next[NT];  // scales of this step and the next
+    auto fragment = [&](int base, int s) {
+        const i32x4 *lo = reinterpret_cast<const i32x4 *>(smem + base + off[2 * s]);
+        const i32x4 *hi = reinterpret_cast<const i32x4 *>(smem + base + off[2 * s + 1]);
+        return cat(*lo, *hi);
+    };
+    // This wave's rows of x and w in LDS, by the places of a step in the two rings
+    auto rows_at = [&](int row, int deep, int shallow) {
+        return row < T::deep_rows ? deep * T::deep_bytes + row * 128
+                                  : T::shallow_at + shallow * T::shallow_bytes + (row - T::deep_rows) * 128;
+    };
+    auto read_x = [&](int base, int s, int t) { xf[s][t] = fragment(base + t * 4096, s); };
+    auto read_w = [&](int base, int s, int t) { wf[t] = fragment(base + t * 4096, s); };
+    const int scale_row = T::scale_at + (wm + l32) * 4, scale_row_w = T::scale_at + (TILE + wn + l32) * 4;
+    auto read_scales = [&](int abs) {
+        const char *at = smem + (abs >> 2 & 1) * (2 * TILE * 4) + (abs & 3);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) xs_next[t] = *reinterpret_cast<const uint8_t *>(at + scale_row + t * 128);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) ws_next[t] = *reinterpret_cast<const uint8_t *>(at + scale_row_w + t * 128);
+    };
+
+    // Loads that may be in flight when a step has to be there: those issued after its last
+    constexpr int kNewer = (RS - 2) * L + (RD - RS) * LD;
+    step_barrier<kNewer + L>(n >= RD);
+    read_scales(first);
+    int deep = 0, shallow = 0, x_at = rows_at(wm, 0, 0), w_at = rows_at(TILE + wn, 0, 0);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) read_x(x_at, 0, t);
+#pragma unroll
+    for (int t = 0; t < kEarly; ++t) read_w(w_at, 0, t);
+
+    // Step i, without a branch inside (the compiler would move the products past it).  Between
+    // its products are the loads of steps i + RS (with `near`) and i + RD (with `far`).
+    auto step = [&](int i, auto near, auto far) __attribute__((always_inline)) {
+        // Products before the turn: beside one each the second half of this half step's w is
+        // read, the last one covers those reads.  Past it the next half step's x and first half of w.
+        constexpr int kProducts = MT * NT, kTurn = NT - kEarly + 1, kSlots = kProducts - kTurn;
+        constexpr int kReads = (MT + kEarly + kSlots - 1) / kSlots, kLoads = (L + kSlots - 1) / kSlots;
+        const int deep_next = deep + 1 == RD ? 0 : deep + 1, shallow_next = shallow + 1 == RS ? 0 : shallow + 1;
+        const int x_next = rows_at(wm, deep_next, shallow_next), w_next = rows_at(TILE + wn, deep_next, shallow_next);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) xs[t] = xs_next[t];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) ws[t] = ws_next[t];
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int e = 0; e < kProducts; ++e) {
+                if (e < kTurn) {
+                    if (kEarly + e < NT) read_w(w_at, s, kEarly + e);
+                } else {
+                    // step i + 1 is there, and all waves have read step i whole, so its places
+                    // go to steps i + RS and i + RD
+                    if (s == 1 && e == kTurn) {
+                        step_barrier<far ? kNewer : 0>(true);
+                        __builtin_amdgcn_sched_barrier(0);
+                        if constexpr (near) load_scales(((first + i) >> 2) + 1);
+                        read_scales(first + i + 1);
+                    }
+#pragma unroll
+                    for (int t = (e - kTurn) * kReads; t < (e - kTurn + 1) * kReads && t < MT + kEarly; ++t) {
+                        if (t < MT)
+                            read_x(s == 0 ? x_at : x_next, s ^ 1, t);
+                        else
+                            read_w(s == 0 ? w_at : w_next, s ^ 1, t - MT);
+                    }
+                    if (s == 1)
+#pragma unroll
+                        for (int c = (e - kTurn) * kLoads; c < (e - kTurn + 1) * kLoads && c < L; ++c) {
+                            if constexpr (near)
+                                if (c < LS) load(i + RS, LD + c, shallow);
+                            if constexpr (far)
+                                if (c >= LS) load(i + RD, c - LS, deep);
+                        }
+                }
+                const int ni = e / MT, mi = e % MT;
+                acc[mi][ni] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[ni], xf[s][mi], acc[mi][ni], 0, 0, 0,
+                                                                             ws[ni], 0, xs[mi]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        deep = deep_next, shallow = shallow_next, x_at = x_next, w_at = w_next;
+    };
+    constexpr std::true_type yes{};
+    constexpr std::false_type no{};
+    int i = 0;
+    for (; i + RD < n; ++i) step(i, yes, yes);
+    if (RS < RD && i + RS < n) step(i++, yes, no);
+    for (; i < n; ++i) step(i, no, no);
+
+    if (part >= 0) {
+        float *sums = p.part + (static_cast<int64_t>(part) * p.rest + tile - p.whole) * (TILE * TILE);
+#pragma unroll
+        for (int mi = 0; mi < MT; ++mi)
+#pragma unroll
+            for (int ni = 0; ni < NT; ++ni)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    *reinterpret_cast<f32x4 *>(sums + (wm + mi * 32 + l32) * TILE + wn + ni * 32 + 8 * q + 4 * half) =
+                        f32x4{acc[mi][ni][4 * q], acc[mi][ni][4 * q + 1], acc[mi][ni][4 * q + 2], acc[mi][ni][4 * q + 3]};
+        return;
+    }
+    // a bias past the last column reads the last ones; not stored
+    if (p.bias)
+#pragma unroll
+        for (int ni = 0; ni < NT; ++ni)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const uint16_t *b = p.bias + min(n0 + wn + ni * 32 + 8 * q + 4 * half, p.n - 4);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int mi = 0; mi < MT; ++mi) acc[mi][ni][4 * q + e] += bf16_to_f32(b[e]);
+            }
+    if constexpr (!GELU) {
+#pragma unroll
+        for (int mi = 0; mi < MT; ++mi) {
+            const int row = m0 + wm + mi * 32 + l32;
+            if (row >= p.m) continue;
+#pragma unroll
+            for (int ni = 0; ni < NT; ++ni)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int col = n0 + wn + ni * 32 + 8 * q + 4 * half;
+                    if (col >= p.n) continue;
+                    *reinterpret_cast<uint2 *>(p.y + static_cast<int64_t>(row) * p.n + col) =
+                        make_uint2(pack_bf16x2(acc[mi][ni][4 * q], acc[mi][ni][4 * q + 1]),
+                                   pack_bf16x2(acc[mi][ni][4 * q + 2], acc[mi][ni][4 * q + 3]));
+                }
+        }
+        return;
+    }
+    // GELU, the largest magnitude of each row's block of 128 columns (a wave's, or
+    // that of two waves side by side), the block
+    static_assert(NT * 32 == 128 || NT * 32 == 64, "a block is one wave's or two's");
+    uint32_t top[MT];
+#pragma unroll
+    for (int mi = 0; mi < MT; ++mi) {
+        top[mi] = 0;
+#pragma unroll
+        for (int ni = 0; ni < NT; ++ni)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const bool in = n0 + wn + ni * 32 + 8 * (r >> 2) + 4 * half < p.n;
+                const float g = in ? gelu(acc[mi][ni][r]) : 0.f;
+                acc[mi][ni][r] = g;
+                top[mi] = max(top[mi], magnitude(g));
+            }
+        const auto both = __builtin_amdgcn_permlane32_swap(top[mi], top[mi], false, false);
+        top[mi] = max(static_cast<uint32_t>(both[0]), static_cast<uint32_t>(both[1]));
+    }
+    if constexpr (NT * 32 == 64) {
+        uint32_t *tops = reinterpret_cast<uint32_t *>(smem);
+        __syncthreads();  // all waves are done with the tiles
+        if (half == 0)
+#pragma unroll
+            for (int mi = 0; mi < MT; ++mi) tops[wave * (MT * 32) + mi * 32 + l32] = top[mi];
+        __syncthreads();
+#pragma unroll
+        for (int mi = 0; mi < MT; ++mi) top[mi] = max(top[mi], tops[(wave ^ 1) * (MT * 32) + mi * 32 + l32]);
+    }
+    const int block = (n0 + wn) / kFp8Block, last = p.np / kFp8Block - 1;
+    if (block > last) return;
+#pragma unroll
+    for (int mi = 0; mi < MT; ++mi) {
+        const int row = m0 + wm + mi * 32 + l32;
+        if (row >= p.m) continue;
+        const uint32_t scale = fp8_scale(top[mi]);
+        const float inv = fp8_inverse(scale == 255 ? 127 : scale);
+#pragma unroll
+        for (int ni = 0; ni < NT; ++ni)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const uint32_t v = fp8_pack4(acc[mi][ni][4 * q], acc[mi][ni][4 * q + 1], acc[mi][ni][4 * q + 2],
+                                             acc[mi][ni][4 * q + 3], inv);
+                *reinterpret_cast<uint32_t *>(p.q + static_cast<int64_t>(row) * p.np + n0 + wn + ni * 32 + 8 * q + 4 * half) =
+                    scale == 255 ? 0x7f7f7f7fu : v;
+            }
+        if (half || wn % kFp8Block) continue;
+        // the last block's lane also fills its group
+        for (int b = block; b == block || (block == last && b <= (last | 3)); ++b)
+            p.qs[(static_cast<int64_t>(b >> 2) * p.m + row) * 4 + (b & 3)] = b == block ? static_cast<uint8_t>(scale) : 0;
+    }
+}
+
+// ------------------------------------------------------------------ large tiles --
+// 256 x 256 tiles, four waves of 128 x 128 (a third less read from LDS than by eight of
+// 64 x 128), one workgroup a compute unit that takes its tiles (and parts of tiles) one
+// after another: the loads run two steps ahead of the products, into the next tile
+// where this one ends, so that they go on during the epilogue.
+constexpr int kBig = 256, kBigWaves = 4, kBigLoads = 2 * kBig / 8 / kBigWaves;
+constexpr int kDeepLoads = 6;                                  // of a wave: 192 rows of x, three steps in LDS
+constexpr int kNearLoads = kBigLoads - kDeepLoads;             // the other rows of x and w: two steps
+constexpr int kDeepRows = kDeepLoads * kBigWaves * 8;
+constexpr int kDeepBytes = kDeepRows * 128, kNearBytes = (2 * kBig - kDeepRows) * 128;
+constexpr int kNearAt = 3 * kDeepBytes, kScalesAt = kNearAt + 2 * kNearBytes, kScaleBytes = 2 * kBig * 4;
+constexpr int kBigLds = kScalesAt + 3 * kScaleBytes;
+constexpr int kCus = 32;  // workgroups of an XCD at a time
+
+struct Unit {
+    int tile, part;   // part < 0: the whole of K
+    int m0, n0, first, n;
+};
+
+__device__ __forceinline__ Unit unit_at(const Fp8Params &p, int xcd, int j)
+{
+    Unit u;
+    const int whole_per = p.whole >> 3;
+    u.part = -1;
+    if (j < whole_per) {
+        u.tile = xcd * whole_per + j;
+    } else {
+        const int i = xcd * p.per + j - whole_per;
+        u.part = p.parts == 1 ? -1 : i / p.rest;
+        u.tile = p.whole + i % p.rest;
+    }
+    tile_rows<kBig>(p, u.tile, u.m0, u.n0);
+    // parts * blocks stays below 2^32: 256 parts at most of fewer than 2^24 blocks
+    auto from = [&](int i) { return static_cast<int>(static_cast<uint32_t>(i) * p.blocks / static_cast<uint32_t>(p.parts)); };
+    u.first = u.part < 0 ? 0 : from(u.part);
+    u.n = (u.part < 0 ? p.blocks : from(u.part + 1)) - u.first;
+    return u;
+}
+
+// Units of an XCD: its whole tiles, then its share of the cut ones.
+__device__ __forceinline__ int units_of(const Fp8Params &p, int xcd)
+{
+    return (p.whole >> 3) + max(0, min(p.per, p.rest * p.parts - xcd * p.per));
+}
+
+// An accumulator's value where the epilogue uses it: in assembly because the compiler
+// otherwise copies all 256 of them to vector registers at once, and spills.  It does not
+// see that a product wrote them, so settle() comes first: 32 wait states, of which a product needs 19.
+__device__ __forceinline__ float taken(float acc)
+{
+    float v;
+    asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v) : "a"(acc));
+    return v;
+}
+__device__ __forceinline__ void settle() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
+
+// The bias of four columns from `col`; past the last column the last ones' (not stored).
+__device__ __forceinline__ void bias4(const Fp8Params &p, int col, float b[4])
+{
+    b[0] = b[1] = b[2] = b[3] = 0.f;
+    if (!p.bias) return;
+    const uint2 v = *reinterpret_cast<const uint2 *>(p.bias + min(col, p.n - 4));
+    b[0] = __uint_as_float(v.x << 16);
+    b[1] = __uint_as_float(v.x & 0xffff0000u);
+    b[2] = __uint_as_float(v.y << 16);
+    b[3] = __uint_as_float(v.y & 0xffff0000u);
+}
+
+template <bool GELU>
+__global__ void __launch_bounds__(kBigWaves * 64, 1) big_kernel(Fp8Params p)
+{
+    constexpr int MT = 4, NT = 4;
+    __shared__ __attribute__((aligned(1024))) char smem[kBigLds];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int l32 = lane & 31, half = lane >> 5;
+    const int wm = (wave >> 1) * 128, wn = (wave & 1) * 128;  // this wave's rows
+    const int xcd = blockIdx.x & 7, units = units_of(p, xcd);
+    int j = blockIdx.x >> 3;
+    if (j >= units) return;
+
+    const u32x4 xr = whole_memory(p.x), wr = whole_memory(p.w), xsr = whole_memory(p.xs), wsr = whole_memory(p.ws);
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char *)smem));
+    // Load c of a step: rows (4 c + wave) * 8 .. + 7 of the tile's x and w together, and rows
+    // 64 wave .. of x's scales and of w's.  Rows past the last repeat it; their results
+    // are not stored.
+    uint32_t at[kBigLoads], at_s[2];
+    auto address = [&](const Unit &u) {
+#pragma unroll
+        for (int c = 0; c < kBigLoads; ++c) {
+            const int row = (c * kBigWaves + wave) * 8 + (lane >> 3);
+            const int r = c * kBigWaves * 8 < kBig ? min(u.m0 + row, p.m - 1) : min(u.n0 + row - kBig, p.n - 1);
+            at[c] = static_cast<uint32_t>(r) * static_cast<uint32_t>(p.kp) + chunk_pos(row, lane & 7) * 16;
+        }
+        at_s[0] = static_cast<uint32_t>(min(u.m0 + wave * 64 + lane, p.m - 1)) * 4;
+        at_s[1] = static_cast<uint32_t>(min(u.n0 + wave * 64 + lane, p.n - 1)) * 4;
+    };
+    // of step `abs` of K, into places `deep` and `near` of the rings
+    auto load = [&](int abs, int c, int deep, int near) {
+        const int to = c < kDeepLoads ? deep * kDeepBytes + c * kBigWaves * 1024
+                                      : kNearAt + near * kNearBytes + (c - kDeepLoads) * kBigWaves * 1024;
+        load_lds16(c * kBigWaves * 8 < kBig ? xr : wr, __builtin_amdgcn_readfirstlane(lds0 + to + wave * 1024), at[c],
+                   __builtin_amdgcn_readfirstlane(abs * kFp8Block));
+    };
+    auto load_scales = [&](int abs, int c, int deep) {
+        load_lds4(c ? wsr : xsr,
+                  __builtin_amdgcn_readfirstlane(lds0 + kScalesAt + deep * kScaleBytes + c * kBig * 4 + wave * 256), at_s[c],
+                  __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(abs >> 2) * (c ? p.n : p.m) * 4));
+    };
+
+    int off[4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) off[s] = l32 * 128 + chunk_pos(l32, 2 * s + half) * 16;
+    // A row's place in LDS as deep * DEEP + near * NEAR + c: rows of this wave's first 64 of x are
+    // deep (0 and 128), those of w near, the other 64 of x (64 and 192) one or the other.
+    const bool x1_deep = wm + 64 < kDeepRows;
+    const int x1_d = x1_deep ? kDeepBytes : 0, x1_n = x1_deep ? 0 : kNearBytes;
+    const int x1_c = x1_deep ? (wm + 64) * 128 : kNearAt + (wm + 64 - kDeepRows) * 128;
+    auto x0_at = [&](int deep) { return deep * kDeepBytes + wm * 128; };
+    auto x1_at = [&](int deep, int near) { return deep * x1_d + near * x1_n + x1_c; };
+    auto w_at = [&](int near) { return kNearAt + near * kNearBytes + (kBig + wn - kDeepRows) * 128; };
+    // Fragments of a half step (64 values): x's in two sets, w's in one whose second half is
+    // read while the first is multiplied.
+    i32x8 xf[2][MT], wf[NT];
+    int xs[MT], ws[NT], xs_next[MT], ws_next[NT];  // scales of this step and the next
+    auto fragment = [&](int base, int s) {
+        const i32x4 *lo = reinterpret_cast<const i32x4 *>(smem + base + off[2 * s]);
+        const i32x4 *hi = reinterpret_cast<const i32x4 *>(smem + base + off[2 * s + 1]);
+        return cat(*lo, *hi);
+    };
+    const int scale_row = kScalesAt + (wm + l32) * 4, scale_row_w = kScalesAt + (kBig + wn + l32) * 4;
+    auto read_scale = [&](int t, int abs, int deep) {
+        const char *s = smem + deep * kScaleBytes + (abs & 3);
+        if (t < MT)
+            xs_next[t] = *reinterpret_cast<const uint8_t *>(s + scale_row + t * 128);
+        else
+            ws_next[t - MT] = *reinterpret_cast<const uint8_t *>(s + scale_row_w + (t - MT) * 128);
+    };
+
+    Unit u = unit_at(p, xcd, j);
+    address(u);
+    for (int i = 0; i < 2; ++i) {  // a unit has two steps at least
+#pragma unroll
+        for (int c = 0; c < 2; ++c) load_scales(u.first + i, c, i);
+#pragma unroll
+        for (int c = 0; c < kBigLoads; ++c) load(u.first + i, c, i, i);
+    }
+    step_barrier<kBigLoads + 2>(true);
+    int deep = 0, near = 0;
+#pragma unroll
+    for (int t = 0; t < MT + NT; ++t) read_scale(t, u.first, 0);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) xf[0][t] = fragment((t < 2 ? x0_at(0) : x1_at(0, 0)) + (t & 1) * 4096, 0);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) wf[t] = fragment(w_at(0) + t * 4096, 0);
+
+    f32x16 acc[MT][NT];
+    // One step: 32 products a wave.  Between them, of the step after it the scales (`next`
+    // says which of their four bytes) and the first fragments are read, and step `ahead` of
+    // the address is loaded, two further on.  No branch inside: the compiler would move the
+    // products past it.
+    auto step = [&](int next, int ahead) __attribute__((always_inline)) {
+        const int deep1 = deep == 2 ? 0 : deep + 1, deep2 = deep1 == 2 ? 0 : deep1 + 1;
+        const int x0 = x0_at(deep), x1 = x1_at(deep, near), w0 = w_at(near);
+        const int x0n = x0_at(deep1), x1n = x1_at(deep1, near ^ 1), w0n = w_at(near ^ 1);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) xs[t] = xs_next[t];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) ws[t] = ws_next[t];
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int e = 0; e < MT * NT; ++e) {
+                if (e < 2) wf[2 + e] = fragment(w0 + (2 + e) * 4096, s);
+                if (s == 1 && e == 3) {
+                    // the next step is there but for what this one's first half has issued, and all
+                    // waves have read this one whole
+                    step_barrier<kDeepLoads + 2>(true);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                if (e >= 4 && e < 16 && e % 2 == 0) {
+                    const int t = (e - 4) / 2;
+                    if (t < MT)
+                        xf[s ^ 1][t] = fragment((s == 0 ? (t < 2 ? x0 : x1) : (t < 2 ? x0n : x1n)) + (t & 1) * 4096, s ^ 1);
+                    else
+                        wf[t - MT] = fragment((s == 0 ? w0 : w0n) + (t - MT) * 4096, s ^ 1);
+                }
+                if (s == 0 && e % 2 == 1) {
+                    const int c = e / 2;
+                    if (c < 2)
+                        load_scales(ahead, c, deep2);
+                    else
+                        load(ahead, c - 2, deep2, near);
+                }
+                if (s == 1 && e >= 4 && e - 4 < kNearLoads) load(ahead, kDeepLoads + e - 4, deep2, near);
+                if (s == 1 && e >= 5 && e - 5 < MT + NT) read_scale(e - 5, next, deep1);
+                const int ni = e / MT, mi = e % MT;
+                acc[mi][ni] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[ni], xf[s][mi], acc[mi][ni], 0, 0, 0,
+                                                                             ws[ni], 0, xs[mi]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        deep = deep1, near ^= 1;
+    };
+
+    for (;;) {
+#pragma unroll
+        for (int mi = 0; mi < MT; ++mi)
+#pragma unroll
+            for (int ni = 0; ni < NT; ++ni) acc[mi][ni] = f32x16{};
+        const Unit done = u;
+        bool more = true;
+        int ahead = u.first + 2, next = u.first + 1;
+        for (int left = done.n; left > 0; --left) {
+            if (left == 2) {  // the loads go on in the next unit; past the last one they repeat it unread
+                j += kCus;
+                more = j < units;
+                if (more) u = unit_at(p, xcd, j);
+                address(u);
+                ahead = u.first;
+            }
+            if (left == 1) next = u.first;
+            step(next, ahead);
+            ++ahead, ++next;
+        }
+
+        // acc[i][j]: lane l holds row 32 i + l % 32 of x; register r row 32 j + 8 (r/4) + 4 half + r % 4 of w
+        const int m0 = done.m0 + wm, n0 = done.n0 + wn;
+        settle();
+        if (done.part >= 0) {
+            float *sums = p.part + (static_cast<int64_t>(done.part) * p.rest + done.tile - p.whole) * (kBig * kBig);
+#pragma unroll
+            for (int mi = 0; mi < MT; ++mi)
+#pragma unroll
+                for (int ni = 0; ni < NT; ++ni)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        f32x4 v;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] = taken(acc[mi][ni][4 * q + e]);
+                        *reinterpret_cast<f32x4 *>(sums + (wm + mi * 32 + l32) * kBig + wn + ni * 32 + 8 * q + 4 * half) = v;
+                    }
+        } else if constexpr (!GELU) {
+#pragma unroll
+            for (int ni = 0; ni < NT; ++ni) {
+                float b[4][4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) bias4(p, n0 + ni * 32 + 8 * q + 4 * half, b[q]);
+#pragma unroll
+                for (int mi = 0; mi < MT; ++mi) {
+                    const int row = m0 + mi * 32 + l32;
+                    uint32_t v[4][2];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        float f[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) f[e] = taken(acc[mi][ni][4 * q + e]) + b[q][e];
+                        v[q][0] = pack_bf16x2(f[0], f[1]);
+                        v[q][1] = pack_bf16x2(f[2], f[3]);
+                    }
+#pragma unroll
+                    for (int q = 0; q < 4; q += 2) {
+                        // lanes l and l + 32 swap halves of two runs of eight columns: one each
+                        const auto lo = __builtin_amdgcn_permlane32_swap(v[q][0], v[q + 1][0], false, false);
+                        const auto hi = __builtin_amdgcn_permlane32_swap(v[q][1], v[q + 1][1], false, false);
+                        const int col = n0 + ni * 32 + 8 * (q + half);
+                        if (row < p.m && col < p.n)
+                            *reinterpret_cast<u32x4 *>(p.y + static_cast<int64_t>(row) * p.n + col) =
+                                u32x4{lo[0], hi[0], lo[1], hi[1]};
+                    }
+                }
+            }
+        } else {
+            // GELU, and each row's 128 columns, a block
+            const int block = n0 / kFp8Block, last = p.np / kFp8Block - 1;
+#pragma unroll
+            for (int mi = 0; mi < MT; ++mi) {
+                float g[NT][16], top = 0.f;
+                bool bad = false;
+#pragma unroll
+                for (int ni = 0; ni < NT; ++ni)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int col = n0 + ni * 32 + 8 * q + 4 * half;
+                        float b[4];
+                        bias4(p, col, b);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float v = gelu(taken(acc[mi][ni][4 * q + e]) + b[e]);
+                            g[ni][4 * q + e] = col < p.n ? v : 0.f;
+                            bad |= v != v;
+                            top = fmaxf(top, fabsf(g[ni][4 * q + e]));
+                        }
+                    }
+                const uint32_t t = bad ? 0x7fffffffu : __float_as_uint(top);
+                const auto both = __builtin_amdgcn_permlane32_swap(t, t, false, false);
+                const uint32_t scale = fp8_scale(max(static_cast<uint32_t>(both[0]), static_cast<uint32_t>(both[1])));
+                const float inv = fp8_inverse(scale == 255 ? 127 : scale);
+                const int row = m0 + mi * 32 + l32;
+                const bool in = row < p.m && block <= last;
+#pragma unroll
+                for (int ni = 0; ni < NT; ++ni)
+#pragma unroll
+                    for (int q = 0; q < 4; q += 2) {
+                        const float *f = &g[ni][4 * q];
+                        uint32_t lo = fp8_pack4(f[0], f[1], f[2], f[3], inv), hi = fp8_pack4(f[4], f[5], f[6], f[7], inv);
+                        if (scale == 255) lo = hi = 0x7f7f7f7fu;
+                        const auto v = __builtin_amdgcn_permlane32_swap(lo, hi, false, false);
+                        if (in)
+                            *reinterpret_cast<uint2 *>(p.q + static_cast<int64_t>(row) * p.np + n0 + ni * 32 + 8 * (q + half)) =
+                                make_uint2(v[0], v[1]);
+                    }
+                // the last block's lane also fills its group
+                if (in && half == 0)
+                    for (int b = block; b == block || (block == last && b <= (last | 3)); ++b)
+                        p.qs[(static_cast<int64_t>(b >> 2) * p.m + row) * 4 + (b & 3)] = b == block ? static_cast<uint8_t>(scale) : 0;
+            }
+        }
+        if (!more) break;
+    }
+    step_barrier<0>(true);  // no load may write LDS that is no longer this workgroup's
+}
+
+// Adds the parts of the cut tiles in their order, then the bias, and rounds, or makes
+// blocks: 8 columns a thread, 16 neighbouring lanes a block.
+template <int TILE, bool GELU>
+__global__ void __launch_bounds__(256) tile_sum_kernel(Fp8Params p)
+{
+    constexpr int kPer = TILE * TILE / 8 / 256;  // workgroups a tile
+    const int t = blockIdx.x / kPer, i = (blockIdx.x % kPer * 256 + threadIdx.x) * 8;
+    int m0, n0;
+    tile_rows<TILE>(p, p.whole + t, m0, n0);
+    const int row = m0 + i / TILE, col = n0 + i % TILE;
+    if (row >= p.m || col >= (GELU ? p.np : p.n)) return;  // whole blocks of lanes
+    float f[8] = {};
+    if (col < p.n) {
+        const float *s = p.part + static_cast<int64_t>(t) * (TILE * TILE) + i;
+        f32x4 lo = {}, hi = {};
+        for (int k = 0; k < p.parts; ++k, s += static_cast<int64_t>(p.rest) * (TILE * TILE)) {
+            lo += *reinterpret_cast<const f32x4 *>(s);
+            hi += *reinterpret_cast<const f32x4 *>(s + 4);
+        }
+        float b[8] = {};
+        if (p.bias) unpack8v(*reinterpret_cast<const u32x4 *>(p.bias + col), b);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            f[e] = lo[e] + b[e];
+            f[4 + e] = hi[e] + b[4 + e];
+        }
+        if constexpr (GELU)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = gelu(f[e]);
+    }
+    if constexpr (!GELU) {
+        *reinterpret_cast<u32x4 *>(p.y + static_cast<int64_t>(row) * p.n + col) = pack8v(f);
+    } else {
+        uint32_t scale;
+        *reinterpret_cast<uint2 *>(p.q + static_cast<int64_t>(row) * p.np + col) = fp8_quantize8(f, scale);
+        const int block = col / kFp8Block, last = p.np / kFp8Block - 1;
+        if (threadIdx.x & 15) return;
+        for (int b = block; b == block || (block == last && b <= (last | 3)); ++b)
+            p.qs[(static_cast<int64_t>(b >> 2) * p.m + row) * 4 + (b & 3)] = b == block ? static_cast<uint8_t>(scale) : 0;
+    }
+}
+
+typedef Tile<128, 2, 2, 8, 4, 4> Medium;
 
 // ------------------------------------------------------------------ few rows --
 // 16 rows of w and 16 * MT of x a workgroup; its waves take every kWaves-th block of
@@ -132,9 +848,46 @@ void launch_few(const Fp8Params &p, hipStream_t s)
         few_kernel<4, SUMS><<<across * static_cast<unsigned>((p.m + 63) / 64), kWaves * 64, 0, s>>>(p);
 }
 
+// How a product is cut: the kernel, and for tiles the ones past the last full wave of
+// the chip, dealt to its units in parts of K of at least 8 steps each.
+struct Cut {
+    int tile;  // 0: few rows
+    int64_t tiles_m, tiles_n, whole, rest, parts;
+};
+
+Cut cut(int64_t m, int64_t n, int64_t k)
+{
+    Cut c{};
+    if (m <= 64) return c;
+    c.tile = (m + 255) / 256 * ((n + 255) / 256) >= 192 && k > 128 ? 256 : 128;
+    c.tiles_m = (m + c.tile - 1) / c.tile;
+    c.tiles_n = (n + c.tile - 1) / c.tile;
+    c.rest = c.tiles_m * c.tiles_n % 256;
+    c.whole = c.tiles_m * c.tiles_n - c.rest;
+    c.parts = 1;
+    const int64_t blocks = fp8_blocks(k);
+    if (c.rest) {
+        c.parts = 256 / c.rest;
+        if (c.parts > blocks / 8) c.parts = blocks / 8;
+        if (c.parts < 1) c.parts = 1;
+    }
+    return c;
+}
+
 int64_t workspace_bytes(int64_t m, int64_t n, int64_t k, bool gelu)
 {
+    const Cut c = cut(m, n, k);
+    if (c.tile) return c.parts > 1 ? c.rest * c.parts * c.tile * c.tile * 4 : 0;
     return gelu ? m * fp8_blocks(n) * kFp8Block * 4 : 0;
+}
+
+template <typename T, bool GELU>
+void launch_tiles(const Fp8Params &p, hipStream_t s)
+{
+    const unsigned grid = 8u * static_cast<unsigned>(p.whole / 8 + (p.rest * p.parts + 7) / 8);
+    tile_kernel<T, GELU><<<grid, T::waves * 64, 0, s>>>(p);
+    if (p.rest && p.parts > 1)
+        tile_sum_kernel<T::size, GELU><<<static_cast<unsigned>(p.rest) * (T::size * T::size / 8 / 256), 256, 0, s>>>(p);
 }
 
 // The checks and the launch of both entry points.
@@ -175,8 +928,30 @@ int linear(const char *what, void *y, void *y_scale, bool gelu, const void *x, c
     p.kp = static_cast<int>(kp);
     p.blocks = static_cast<int>(kp / kFp8Block);
     p.np = static_cast<int>(np);
+    const Cut c = cut(m, n, k);
+    p.tiles_m = static_cast<int>(c.tiles_m);
+    p.tiles_n = static_cast<int>(c.tiles_n);
+    p.whole = static_cast<int>(c.whole);
+    p.rest = static_cast<int>(c.rest);
+    p.parts = static_cast<int>(c.parts);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (gelu) {
+    if (c.tile == 256) {
+        p.per = static_cast<int>((c.rest * c.parts + 7) / 8);
+        const unsigned grid = 8u * static_cast<unsigned>(std::min<int64_t>(kCus, c.whole / 8 + p.per));
+        if (gelu)
+            big_kernel<true><<<grid, kBigWaves * 64, 0, s>>>(p);
+        else
+            big_kernel<false><<<grid, kBigWaves * 64, 0, s>>>(p);
+        if (c.parts > 1) {
+            const unsigned sums = static_cast<unsigned>(c.rest) * (kBig * kBig / 8 / 256);
+            if (gelu)
+                tile_sum_kernel<kBig, true><<<sums, 256, 0, s>>>(p);
+            else
+                tile_sum_kernel<kBig, false><<<sums, 256, 0, s>>>(p);
+        }
+    } else if (c.tile == 128) {
+        gelu ? launch_tiles<Medium, true>(p, s) : launch_tiles<Medium, false>(p, s);
+    } else if (gelu) {
         launch_few<true>(p, s);
         gelu_quantize_kernel<<<static_cast<unsigned>((m * fp8_groups(n) + 3) / 4), 256, 0, s>>>(p);
     } else {
