@@ -447,15 +447,16 @@ __device__ __forceinline__ float taken(float acc)
 __device__ __forceinline__ void settle() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
 
 // The bias of four columns from `col`; past the last column the last ones' (not stored).
-__device__ __forceinline__ void bias4(const Fp8Params &p, int col, float b[4])
+__device__ __forceinline__ uint2 bias4(const Fp8Params &p, int col)
 {
-    b[0] = b[1] = b[2] = b[3] = 0.f;
-    if (!p.bias) return;
-    const uint2 v = *reinterpret_cast<const uint2 *>(p.bias + min(col, p.n - 4));
-    b[0] = __uint_as_float(v.x << 16);
-    b[1] = __uint_as_float(v.x & 0xffff0000u);
-    b[2] = __uint_as_float(v.y << 16);
-    b[3] = __uint_as_float(v.y & 0xffff0000u);
+    return p.bias ? *reinterpret_cast<const uint2 *>(p.bias + min(col, p.n - 4)) : make_uint2(0, 0);
+}
+__device__ __forceinline__ void widen(const uint2 &v, float f[4])
+{
+    f[0] = __uint_as_float(v.x << 16);
+    f[1] = __uint_as_float(v.x & 0xffff0000u);
+    f[2] = __uint_as_float(v.y << 16);
+    f[3] = __uint_as_float(v.y & 0xffff0000u);
 }
 
 template <bool GELU>
@@ -631,33 +632,43 @@ __global__ void __launch_bounds__(kBigWaves * 64, 1) big_kernel(Fp8Params p)
                         *reinterpret_cast<f32x4 *>(sums + (wm + mi * 32 + l32) * kBig + wn + ni * 32 + 8 * q + 4 * half) = v;
                     }
         } else if constexpr (!GELU) {
+            uint2 b[NT][4];
 #pragma unroll
-            for (int ni = 0; ni < NT; ++ni) {
-                float b[4][4];
+            for (int ni = 0; ni < NT; ++ni)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) bias4(p, n0 + ni * 32 + 8 * q + 4 * half, b[q]);
+                for (int q = 0; q < 4; ++q) b[ni][q] = bias4(p, n0 + ni * 32 + 8 * q + 4 * half);
 #pragma unroll
-                for (int mi = 0; mi < MT; ++mi) {
-                    const int row = m0 + mi * 32 + l32;
+            for (int mi = 0; mi < MT; ++mi) {
+#pragma unroll
+                for (int ni = 0; ni < NT; ++ni) {
                     uint32_t v[4][2];
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        float f[4];
+                        float f[4], c[4];
+                        widen(b[ni][q], c);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) f[e] = taken(acc[mi][ni][4 * q + e]) + b[q][e];
+                        for (int e = 0; e < 4; ++e) f[e] = taken(acc[mi][ni][4 * q + e]) + c[e];
                         v[q][0] = pack_bf16x2(f[0], f[1]);
                         v[q][1] = pack_bf16x2(f[2], f[3]);
                     }
+                    // lanes l and l + 32, then l and l + 16, swap: 16 rows of 32 columns a store,
+                    // 64 bytes a row (32 rows of 16: 309 against 302 us on [24576, 4096] x 4096)
+                    u32x4 lo, hi;
 #pragma unroll
-                    for (int q = 0; q < 4; q += 2) {
-                        // lanes l and l + 32 swap halves of two runs of eight columns: one each
-                        const auto lo = __builtin_amdgcn_permlane32_swap(v[q][0], v[q + 1][0], false, false);
-                        const auto hi = __builtin_amdgcn_permlane32_swap(v[q][1], v[q + 1][1], false, false);
-                        const int col = n0 + ni * 32 + 8 * (q + half);
-                        if (row < p.m && col < p.n)
-                            *reinterpret_cast<u32x4 *>(p.y + static_cast<int64_t>(row) * p.n + col) =
-                                u32x4{lo[0], hi[0], lo[1], hi[1]};
+                    for (int e = 0; e < 2; ++e) {
+                        const auto first = __builtin_amdgcn_permlane32_swap(v[0][e], v[1][e], false, false);
+                        const auto second = __builtin_amdgcn_permlane32_swap(v[2][e], v[3][e], false, false);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const auto rows = __builtin_amdgcn_permlane16_swap(first[i], second[i], false, false);
+                            lo[2 * i + e] = rows[0], hi[2 * i + e] = rows[1];
+                        }
                     }
+                    const int row = m0 + mi * 32 + (lane & 15), col = n0 + ni * 32 + 8 * half + (lane & 16);
+                    if (row < p.m && col < p.n)
+                        *reinterpret_cast<u32x4 *>(p.y + static_cast<int64_t>(row) * p.n + col) = lo;
+                    if (row + 16 < p.m && col < p.n)
+                        *reinterpret_cast<u32x4 *>(p.y + static_cast<int64_t>(row + 16) * p.n + col) = hi;
                 }
             }
         } else {
@@ -673,7 +684,7 @@ __global__ void __launch_bounds__(kBigWaves * 64, 1) big_kernel(Fp8Params p)
                     for (int q = 0; q < 4; ++q) {
                         const int col = n0 + ni * 32 + 8 * q + 4 * half;
                         float b[4];
-                        bias4(p, col, b);
+                        widen(bias4(p, col), b);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const float v = gelu(taken(acc[mi][ni][4 * q + e]) + b[e]);
@@ -686,20 +697,27 @@ __global__ void __launch_bounds__(kBigWaves * 64, 1) big_kernel(Fp8Params p)
                 const auto both = __builtin_amdgcn_permlane32_swap(t, t, false, false);
                 const uint32_t scale = fp8_scale(max(static_cast<uint32_t>(both[0]), static_cast<uint32_t>(both[1])));
                 const float inv = fp8_inverse(scale == 255 ? 127 : scale);
+#pragma unroll
+                for (int ni = 0; ni < NT; ++ni) {
+                    uint32_t v[4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const float *f = &g[ni][4 * q];
+                        v[q] = scale == 255 ? 0x7f7f7f7fu : fp8_pack4(f[0], f[1], f[2], f[3], inv);
+                    }
+                    // as above: 16 rows of 32 columns a store
+                    const auto first = __builtin_amdgcn_permlane32_swap(v[0], v[1], false, false);
+                    const auto second = __builtin_amdgcn_permlane32_swap(v[2], v[3], false, false);
+                    const auto lo = __builtin_amdgcn_permlane16_swap(first[0], second[0], false, false);
+                    const auto hi = __builtin_amdgcn_permlane16_swap(first[1], second[1], false, false);
+                    const int row = m0 + mi * 32 + (lane & 15), col = n0 + ni * 32 + 8 * half + (lane & 16);
+                    if (row < p.m && block <= last)
+                        *reinterpret_cast<uint2 *>(p.q + static_cast<int64_t>(row) * p.np + col) = make_uint2(lo[0], hi[0]);
+                    if (row + 16 < p.m && block <= last)
+                        *reinterpret_cast<uint2 *>(p.q + static_cast<int64_t>(row + 16) * p.np + col) = make_uint2(lo[1], hi[1]);
+                }
                 const int row = m0 + mi * 32 + l32;
                 const bool in = row < p.m && block <= last;
-#pragma unroll
-                for (int ni = 0; ni < NT; ++ni)
-#pragma unroll
-                    for (int q = 0; q < 4; q += 2) {
-                        const float *f = &g[ni][4 * q];
-                        uint32_t lo = fp8_pack4(f[0], f[1], f[2], f[3], inv), hi = fp8_pack4(f[4], f[5], f[6], f[7], inv);
-                        if (scale == 255) lo = hi = 0x7f7f7f7fu;
-                        const auto v = __builtin_amdgcn_permlane32_swap(lo, hi, false, false);
-                        if (in)
-                            *reinterpret_cast<uint2 *>(p.q + static_cast<int64_t>(row) * p.np + n0 + ni * 32 + 8 * (q + half)) =
-                                make_uint2(v[0], v[1]);
-                    }
                 // the last block's lane also fills its group
                 if (in && half == 0)
                     for (int b = block; b == block || (block == last && b <= (last | 3)); ++b)
