@@ -449,11 +449,14 @@ int ltxk_add_norm_modulate_fp8(void *x_out, void *q, void *q_scale, const void *
                                float eps, const ltxk_ada *shift, const ltxk_ada *scale, void *stream);
 
 /* Bytes of workspace ltxk_linear_fp8 (gelu 0) or ltxk_linear_gelu_fp8 (gelu 1)
- * needs for this shape. */
-int64_t ltxk_linear_fp8_workspace_bytes(int64_t m, int64_t n, int64_t k, int gelu);
+ * needs for this shape, with x in blocks (quantize 0) or in bf16 (quantize 1). */
+int64_t ltxk_linear_fp8_workspace_bytes(int64_t m, int64_t n, int64_t k, int gelu, int quantize);
 
 /* y = round(x w^T + bias) for x [m, k] and w [n, k] in blocks, y [m, n] and bias
- * [n] (or NULL) bf16: exact products of the held values, fp32 sums, one rounding.
+ * [n] (or NULL) bf16: products of the held values, fp32 sums, one rounding.  With
+ * x_scale NULL x is bf16 [m, k] instead and quantised in `workspace` as by
+ * ltxk_quantize_fp8.  (The matrix cores cut the products of 8 neighbouring values
+ * of k off at 2^-13 of the largest of them before they are added up in fp32.)
  * n and k are multiples of 8; x, w and y hold fewer than 2^31 values each.
  * `workspace`: device memory of ltxk_linear_fp8_workspace_bytes, 16-byte aligned
  * (NULL if that is 0), in use until the call's work has run.  For the linear

@@ -774,64 +774,151 @@ __global__ void __launch_bounds__(256) tile_sum_kernel(Fp8Params p)
 typedef Tile<128, 2, 2, 8, 4, 4> Medium;
 
 // ------------------------------------------------------------------ few rows --
-// 16 rows of w and 16 * MT of x a workgroup; its waves take every kWaves-th block of
-// K, straight from memory to registers, and their sums are added in LDS.
-constexpr int kWaves = 8;
+// 32 * MT rows of x and 32 * NT of w a workgroup.  Each of its four waves takes every fourth
+// block of K, through LDS of its own (so that the loads read whole rows of 128 bytes; straight
+// to registers a load of 16 lanes touches 16 rows), RING blocks ahead and without a barrier;
+// their sums are added in LDS at the end.
+constexpr int kFewWaves = 4;
 
-template <int MT, bool SUMS>
-__global__ void __launch_bounds__(kWaves * 64) few_kernel(Fp8Params p)
+template <int MT_, int NT_, int RING_>
+struct Few {
+    static constexpr int MT = MT_, NT = NT_, RING = RING_;
+    static constexpr int loads = 4 * (MT + NT) + 2;               // of a block: 8 rows each, and both sides' scales
+    static constexpr int scales_at = (MT + NT) * 4096, bytes = scales_at + 512;
+    static constexpr int sums = kFewWaves * MT * NT * 4096;
+    static constexpr int lds = RING * bytes * kFewWaves > sums ? RING * bytes * kFewWaves : sums;
+    static_assert(MT <= 2 && NT <= 2 && loads * (RING - 1) < 64, "a load takes 64 rows of scales, a wait counts to 63");
+};
+
+// This wave's loads but the newest `n` have landed.
+__device__ __forceinline__ void wait_loads(int n)
 {
-    __shared__ f32x4 sums[kWaves][MT][64];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int across = (p.n + 15) / 16;
-    const int n0 = blockIdx.x % across * 16, m0 = blockIdx.x / across * 16 * MT;
-    const int l16 = lane & 15, quad = lane >> 4;
-    // rows past the last repeat it; their results are not stored
-    const int nr = min(n0 + l16, p.n - 1);
-    const uint8_t *wp = p.w + static_cast<int64_t>(nr) * p.kp + quad * 32;
-    const uint8_t *xp[MT];
-    int mr[MT];
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        mr[t] = min(m0 + t * 16 + l16, p.m - 1);
-        xp[t] = p.x + static_cast<int64_t>(mr[t]) * p.kp + quad * 32;
+    asm volatile("" ::: "memory");
+    switch (n) {
+#define LTXK_WAIT(N) case N: __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | (N >> 4 << 14)); break;
+    LTXK_WAIT(10)
+    LTXK_WAIT(14)
+    LTXK_WAIT(18)
+    LTXK_WAIT(20)
+    LTXK_WAIT(28)
+    LTXK_WAIT(30)
+#undef LTXK_WAIT
+    default: __builtin_amdgcn_s_waitcnt(0x0f70);
     }
-    f32x4 acc[MT] = {};
-    for (int b = wave; b < p.blocks; b += kWaves) {
-        const int64_t off = static_cast<int64_t>(b) * kFp8Block;
-        const i32x4 *wv = reinterpret_cast<const i32x4 *>(wp + off);
-        const i32x8 wf = cat(wv[0], wv[1]);
-        const int ws = p.ws[(static_cast<int64_t>(b >> 2) * p.n + nr) * 4 + (b & 3)];
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            const i32x4 *xv = reinterpret_cast<const i32x4 *>(xp[t] + off);
-            const i32x8 xf = cat(xv[0], xv[1]);
-            const int xs = p.xs[(static_cast<int64_t>(b >> 2) * p.m + mr[t]) * 4 + (b & 3)];
-            acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf, xf, acc[t], 0, 0, 0, ws, 0, xs);
-        }
-    }
-#pragma unroll
-    for (int t = 0; t < MT; ++t) sums[wave][t][lane] = acc[t];
-    __syncthreads();
-    if (wave >= MT) return;
-    // lane l: row l % 16 of x, rows 4 (l / 16) .. + 3 of w
-    f32x4 v = sums[0][wave][lane];
-#pragma unroll
-    for (int i = 1; i < kWaves; ++i) v += sums[i][wave][lane];
-    const int row = m0 + wave * 16 + l16, col = n0 + quad * 4;
-    if (row >= p.m || col >= p.n) return;
-    if (p.bias)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] += bf16_to_f32(p.bias[col + e]);
-    if constexpr (SUMS)
-        *reinterpret_cast<f32x4 *>(p.part + static_cast<int64_t>(row) * p.np + col) = v;
-    else
-        *reinterpret_cast<uint2 *>(p.y + static_cast<int64_t>(row) * p.n + col) =
-            make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+    asm volatile("" ::: "memory");
 }
 
-// blocks(gelu(sums)): 16 lanes a block, as quantize_fp8.
-__global__ void __launch_bounds__(256) gelu_quantize_kernel(Fp8Params p)
+template <typename F, bool SUMS>
+__global__ void __launch_bounds__(kFewWaves * 64) few_kernel(Fp8Params p)
+{
+    constexpr int MT = F::MT, NT = F::NT, R = F::RING;
+    __shared__ __attribute__((aligned(1024))) char smem[F::lds];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int l32 = lane & 31, half = lane >> 5;
+    // a tile of w goes to one XCD for all tiles of x, and all parts of a tile, too
+    const int at_x = blockIdx.x >> 3;
+    const int tn = at_x / p.tiles_m / p.parts * 8 + (blockIdx.x & 7), tm = at_x % p.tiles_m, part = at_x / p.tiles_m % p.parts;
+    if (tn >= p.tiles_n) return;
+    const int m0 = tm * 32 * MT, n0 = tn * 32 * NT;
+    // blocks of this part, then every fourth of them for this wave
+    const int from = static_cast<int>(static_cast<uint32_t>(part) * p.blocks / p.parts);
+    const int to = static_cast<int>(static_cast<uint32_t>(part + 1) * p.blocks / p.parts);
+    const int first = from + wave, n = max(0, (to - first + kFewWaves - 1) / kFewWaves);
+
+    const u32x4 xr = whole_memory(p.x), wr = whole_memory(p.w), xsr = whole_memory(p.xs), wsr = whole_memory(p.ws);
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char *)smem)) + wave * R * F::bytes;
+    // rows past the last repeat it; their results are not stored
+    uint32_t xo[4 * MT], wo[4 * NT];
+    const uint32_t chunk = chunk_pos(lane >> 3, lane & 7) * 16, chunk_odd = chunk_pos(8 + (lane >> 3), lane & 7) * 16;
+#pragma unroll
+    for (int c = 0; c < 4 * MT; ++c)
+        xo[c] = static_cast<uint32_t>(min(m0 + c * 8 + (lane >> 3), p.m - 1)) * static_cast<uint32_t>(p.kp) + (c & 1 ? chunk_odd : chunk);
+#pragma unroll
+    for (int c = 0; c < 4 * NT; ++c)
+        wo[c] = static_cast<uint32_t>(min(n0 + c * 8 + (lane >> 3), p.n - 1)) * static_cast<uint32_t>(p.kp) + (c & 1 ? chunk_odd : chunk);
+    const uint32_t xso = static_cast<uint32_t>(min(m0 + lane, p.m - 1)) * 4, wso = static_cast<uint32_t>(min(n0 + lane, p.n - 1)) * 4;
+    auto load = [&](int i, int slot) {
+        const int b = first + i * kFewWaves;
+        const uint32_t at = lds0 + slot * F::bytes;
+        const uint32_t k = __builtin_amdgcn_readfirstlane(b * kFp8Block), g = __builtin_amdgcn_readfirstlane(b >> 2);
+#pragma unroll
+        for (int c = 0; c < 4 * NT; ++c) load_lds16(wr, __builtin_amdgcn_readfirstlane(at + (MT * 4 + c) * 1024), wo[c], k);
+#pragma unroll
+        for (int c = 0; c < 4 * MT; ++c) load_lds16(xr, __builtin_amdgcn_readfirstlane(at + c * 1024), xo[c], k);
+        load_lds4(xsr, __builtin_amdgcn_readfirstlane(at + F::scales_at), xso, __builtin_amdgcn_readfirstlane(g * p.m * 4));
+        load_lds4(wsr, __builtin_amdgcn_readfirstlane(at + F::scales_at + 256), wso, __builtin_amdgcn_readfirstlane(g * p.n * 4));
+    };
+    for (int i = 0; i < R && i < n; ++i) load(i, i);
+
+    int off[4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) off[s] = l32 * 128 + chunk_pos(l32, 2 * s + half) * 16;
+    f32x16 acc[MT][NT] = {};
+    int slot = 0;
+    for (int i = 0; i < n; ++i) {
+        wait_loads(min(R - 1, n - 1 - i) * F::loads);
+        const char *at = smem + (wave * R + slot) * F::bytes;
+        i32x8 f[2][MT + NT];
+        int scale[MT + NT];
+#pragma unroll
+        for (int t = 0; t < MT + NT; ++t) {
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+                f[s][t] = cat(*reinterpret_cast<const i32x4 *>(at + t * 4096 + off[2 * s]),
+                              *reinterpret_cast<const i32x4 *>(at + t * 4096 + off[2 * s + 1]));
+            scale[t] = *reinterpret_cast<const uint8_t *>(at + F::scales_at + (t < MT ? t * 128 : 256 + (t - MT) * 128) + l32 * 4 +
+                                                          ((first + i * kFewWaves) & 3));
+        }
+        // read whole: its place goes to block i + R
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+        asm volatile("" ::: "memory");
+        if (i + R < n) load(i + R, slot);
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int ni = 0; ni < NT; ++ni)
+#pragma unroll
+                for (int mi = 0; mi < MT; ++mi)
+                    acc[mi][ni] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(f[s][MT + ni], f[s][mi], acc[mi][ni], 0, 0, 0,
+                                                                                 scale[MT + ni], 0, scale[mi]);
+        slot = slot + 1 == R ? 0 : slot + 1;
+    }
+
+    // lane l: row l % 32 of x, rows 8 q + 4 (l / 32) .. + 3 of w in registers 4 q ..
+    __syncthreads();  // all waves are done with their places
+    f32x4 *sums = reinterpret_cast<f32x4 *>(smem);
+#pragma unroll
+    for (int t = 0; t < MT * NT; ++t)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const f32x16 &a = acc[t / NT][t % NT];
+            sums[((wave * MT * NT + t) * 4 + q) * 64 + lane] = f32x4{a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]};
+        }
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < MT * NT; ++t) {  // this wave's q of each tile
+        f32x4 v = {};
+#pragma unroll
+        for (int w = 0; w < kFewWaves; ++w) v += sums[((w * MT * NT + t) * 4 + wave) * 64 + lane];
+        const int row = m0 + t / NT * 32 + l32, col = n0 + t % NT * 32 + 8 * wave + 4 * half;
+        if (row >= p.m || col >= p.n) continue;
+        if constexpr (SUMS) {
+            *reinterpret_cast<f32x4 *>(p.part + (static_cast<int64_t>(part) * p.m + row) * p.np + col) = v;
+        } else {
+            if (p.bias)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] += bf16_to_f32(p.bias[col + e]);
+            *reinterpret_cast<uint2 *>(p.y + static_cast<int64_t>(row) * p.n + col) =
+                make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+        }
+    }
+}
+
+// Adds the parts of a cut K in their order, then the bias, and rounds, or makes blocks
+// of the GELU: 8 columns a thread, 16 neighbouring lanes a block, as quantize_fp8.
+template <bool GELU>
+__global__ void __launch_bounds__(256) few_sum_kernel(Fp8Params p)
 {
     const int64_t unit = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63, row = static_cast<int>(unit % p.m);
@@ -839,51 +926,85 @@ __global__ void __launch_bounds__(256) gelu_quantize_kernel(Fp8Params p)
     if (group * 512 >= p.np) return;
     float f[8] = {};
     if (col < p.n) {
-        const f32x4 *s = reinterpret_cast<const f32x4 *>(p.part + static_cast<int64_t>(row) * p.np + col);
-        const f32x4 lo = s[0], hi = s[1];
+        const float *s = p.part + static_cast<int64_t>(row) * p.np + col;
+        f32x4 lo = {}, hi = {};
+        for (int k = 0; k < p.parts; ++k, s += static_cast<int64_t>(p.m) * p.np) {
+            lo += *reinterpret_cast<const f32x4 *>(s);
+            hi += *reinterpret_cast<const f32x4 *>(s + 4);
+        }
+        float b[8] = {};
+        if (p.bias) unpack8v(*reinterpret_cast<const u32x4 *>(p.bias + col), b);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            f[e] = gelu(lo[e]);
-            f[4 + e] = gelu(hi[e]);
+            f[e] = lo[e] + b[e];
+            f[4 + e] = hi[e] + b[4 + e];
         }
+        if constexpr (GELU)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = gelu(f[e]);
+        else
+            *reinterpret_cast<u32x4 *>(p.y + static_cast<int64_t>(row) * p.n + col) = pack8v(f);
     }
-    uint32_t scale;
-    const uint2 q = fp8_quantize8(f, scale);
-    if (col < p.np) *reinterpret_cast<uint2 *>(p.q + static_cast<int64_t>(row) * p.np + col) = q;
-    if ((lane & 15) == 0)
-        p.qs[(static_cast<int64_t>(group) * p.m + row) * 4 + (lane >> 4)] = static_cast<uint8_t>(scale);
+    if constexpr (GELU) {
+        uint32_t scale;
+        const uint2 q = fp8_quantize8(f, scale);
+        if (col < p.np) *reinterpret_cast<uint2 *>(p.q + static_cast<int64_t>(row) * p.np + col) = q;
+        if ((lane & 15) == 0)
+            p.qs[(static_cast<int64_t>(group) * p.m + row) * 4 + (lane >> 4)] = static_cast<uint8_t>(scale);
+    }
 }
 
-template <bool SUMS>
-void launch_few(const Fp8Params &p, hipStream_t s)
+template <typename F>
+void few_rows(const Fp8Params &p, bool gelu, hipStream_t s)
 {
-    const unsigned across = static_cast<unsigned>((p.n + 15) / 16);
-    if (p.m <= 16)
-        few_kernel<1, SUMS><<<across, kWaves * 64, 0, s>>>(p);
-    else if (p.m <= 32)
-        few_kernel<2, SUMS><<<across, kWaves * 64, 0, s>>>(p);
-    else
-        few_kernel<4, SUMS><<<across * static_cast<unsigned>((p.m + 63) / 64), kWaves * 64, 0, s>>>(p);
+    const unsigned grid = 8u * static_cast<unsigned>((p.tiles_n + 7) / 8) * static_cast<unsigned>(p.tiles_m) * static_cast<unsigned>(p.parts);
+    if (gelu || p.parts > 1) {
+        few_kernel<F, true><<<grid, kFewWaves * 64, 0, s>>>(p);
+        const unsigned sums = static_cast<unsigned>((static_cast<int64_t>(p.m) * ((p.np + 511) / 512) + 3) / 4);
+        if (gelu)
+            few_sum_kernel<true><<<sums, 256, 0, s>>>(p);
+        else
+            few_sum_kernel<false><<<sums, 256, 0, s>>>(p);
+    } else {
+        few_kernel<F, false><<<grid, kFewWaves * 64, 0, s>>>(p);
+    }
 }
 
-// How a product is cut: the kernel, and for tiles the ones past the last full wave of
-// the chip, dealt to its units in parts of K of at least 8 steps each.
+// The kernel that a product takes, and how it is cut over K.
+//
+// Few rows: up to 32, and outputs of at most 256 tiles of 64 x 64, one a compute unit (tiles of
+// 64 x 32 where there are at most 128).  Cold operands, this kernel / 128 x 128 tiles, us, M x N x
+// K: 126 x 2048 x 2048 7 / 15, 126 x 8192 x 2048 11 / 19, 504 x 2048 x 8192 21 / 25, 256 x 4096 x
+// 4096 15 / 22;  512 tiles, 512 x 4096 x 4096 25 / 25;  1024, 504 x 8192 x 2048 32 / 17.
+// K is cut from 128 blocks on where the tiles leave units idle, into parts of at least 16; the
+// second launch costs 5 us: 1 x 1024 x 16384 19 us whole, 12 in 8 parts; 126 x 1024 x 16384 28 and
+// 17; 126 x 2048 x 8192 17 and 17.
 struct Cut {
-    int tile;  // 0: few rows
+    int tile;  // rows of x and of w; few rows: 32, 48 (64 and 32) and 64
     int64_t tiles_m, tiles_n, whole, rest, parts;
 };
 
 Cut cut(int64_t m, int64_t n, int64_t k)
 {
     Cut c{};
-    if (m <= 64) return c;
+    const int64_t blocks = fp8_blocks(k), tiles64 = (m + 63) / 64 * ((n + 63) / 64);
+    c.parts = 1;
+    if (m <= 32 || tiles64 <= 256) {
+        const int mt = m <= 32 ? 1 : 2, nt = m <= 32 || tiles64 <= 128 ? 1 : 2;
+        c.tile = 16 * (mt + nt);
+        c.tiles_m = (m + 32 * mt - 1) / (32 * mt);
+        c.tiles_n = (n + 32 * nt - 1) / (32 * nt);
+        if (blocks >= 128)
+            while (c.tiles_m * c.tiles_n * c.parts * 2 <= 256 && blocks >= c.parts * 2 * 16) c.parts *= 2;
+        return c;
+    }
+    // Tiles: those past the last full wave of the chip are dealt to its units in parts of
+    // K of at least 8 steps each.
     c.tile = (m + 255) / 256 * ((n + 255) / 256) >= 192 && k > 128 ? 256 : 128;
     c.tiles_m = (m + c.tile - 1) / c.tile;
     c.tiles_n = (n + c.tile - 1) / c.tile;
     c.rest = c.tiles_m * c.tiles_n % 256;
     c.whole = c.tiles_m * c.tiles_n - c.rest;
-    c.parts = 1;
-    const int64_t blocks = fp8_blocks(k);
     if (c.rest) {
         c.parts = 256 / c.rest;
         if (c.parts > blocks / 8) c.parts = blocks / 8;
@@ -895,8 +1016,8 @@ Cut cut(int64_t m, int64_t n, int64_t k)
 int64_t workspace_bytes(int64_t m, int64_t n, int64_t k, bool gelu)
 {
     const Cut c = cut(m, n, k);
-    if (c.tile) return c.parts > 1 ? c.rest * c.parts * c.tile * c.tile * 4 : 0;
-    return gelu ? m * fp8_blocks(n) * kFp8Block * 4 : 0;
+    if (c.tile >= 128) return c.parts > 1 ? c.rest * c.parts * c.tile * c.tile * 4 : 0;
+    return gelu || c.parts > 1 ? c.parts * m * fp8_blocks(n) * kFp8Block * 4 : 0;
 }
 
 template <typename T, bool GELU>
@@ -908,6 +1029,8 @@ void launch_tiles(const Fp8Params &p, hipStream_t s)
         tile_sum_kernel<T::size, GELU><<<static_cast<unsigned>(p.rest) * (T::size * T::size / 8 / 256), 256, 0, s>>>(p);
 }
 
+int64_t round16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
+
 // The checks and the launch of both entry points.
 int linear(const char *what, void *y, void *y_scale, bool gelu, const void *x, const void *x_scale, const void *w,
            const void *w_scale, const void *bias, int64_t m, int64_t n, int64_t k, void *workspace,
@@ -918,8 +1041,7 @@ int linear(const char *what, void *y, void *y_scale, bool gelu, const void *x, c
         return fail(LTXK_E_ARG, "%s: bad shape m=%lld n=%lld k=%lld (n and k positive multiples of 8)", what,
                     (long long)m, (long long)n, (long long)k);
     if (m == 0) return LTXK_OK;
-    if (!y || (gelu && !y_scale) || !x || !x_scale || !w || !w_scale)
-        return fail(LTXK_E_ARG, "%s: null operand", what);
+    if (!y || (gelu && !y_scale) || !x || !w || !w_scale) return fail(LTXK_E_ARG, "%s: null operand", what);
     for (const void *v : {static_cast<const void *>(y), static_cast<const void *>(y_scale), x, x_scale, w, w_scale, bias})
         if (!aligned16(v)) return fail(LTXK_E_ALIGN, "%s: operands must be 16-byte aligned", what);
     // operands are read through 32-bit offsets, outputs counted by 32-bit tiles
@@ -928,7 +1050,8 @@ int linear(const char *what, void *y, void *y_scale, bool gelu, const void *x, c
     const int64_t kp = fp8_blocks(k) * kFp8Block, np = fp8_blocks(n) * kFp8Block;
     if (m > (kMax - 1) / kp || n > (kMax - 1) / kp || m > (kMax - 1) / np)
         return fail(LTXK_E_ARG, "%s: x, w or y holds 2^31 values or more", what);
-    const int64_t need = workspace_bytes(m, n, k, gelu);
+    const int64_t values = x_scale ? 0 : m * kp, scales = x_scale ? 0 : m * fp8_groups(k) * kFp8Group;
+    const int64_t blocks_at = round16(values) + round16(scales), need = blocks_at + workspace_bytes(m, n, k, gelu);
     if (need && (!workspace || !aligned16(workspace) || workspace_size < need))
         return fail(LTXK_E_ARG, "%s: the workspace must hold ltxk_linear_fp8_workspace_bytes, 16-byte aligned", what);
     Fp8Params p{};
@@ -940,7 +1063,14 @@ int linear(const char *what, void *y, void *y_scale, bool gelu, const void *x, c
     p.y = gelu ? nullptr : static_cast<uint16_t *>(y);
     p.q = gelu ? static_cast<uint8_t *>(y) : nullptr;
     p.qs = static_cast<uint8_t *>(y_scale);
-    p.part = static_cast<float *>(workspace);
+    p.part = reinterpret_cast<float *>(static_cast<char *>(workspace) + blocks_at);
+    if (!x_scale) {
+        char *q = static_cast<char *>(workspace), *q_scale = q + round16(values);
+        const int rc = ltxk_quantize_fp8(q, q_scale, x, m, k, stream);
+        if (rc) return rc;
+        p.x = reinterpret_cast<const uint8_t *>(q);
+        p.xs = reinterpret_cast<const uint8_t *>(q_scale);
+    }
     p.m = static_cast<int>(m);
     p.n = static_cast<int>(n);
     p.kp = static_cast<int>(kp);
@@ -969,11 +1099,12 @@ int linear(const char *what, void *y, void *y_scale, bool gelu, const void *x, c
         }
     } else if (c.tile == 128) {
         gelu ? launch_tiles<Medium, true>(p, s) : launch_tiles<Medium, false>(p, s);
-    } else if (gelu) {
-        launch_few<true>(p, s);
-        gelu_quantize_kernel<<<static_cast<unsigned>((m * fp8_groups(n) + 3) / 4), 256, 0, s>>>(p);
+    } else if (c.tile == 64) {
+        few_rows<Few<2, 2, 2>>(p, gelu, s);
+    } else if (c.tile == 48) {
+        few_rows<Few<2, 1, 3>>(p, gelu, s);
     } else {
-        launch_few<false>(p, s);
+        few_rows<Few<1, 1, 2>>(p, gelu, s);
     }
     return check_launch(what);
 }
@@ -983,10 +1114,13 @@ int linear(const char *what, void *y, void *y_scale, bool gelu, const void *x, c
 
 using namespace ltxk;
 
-extern "C" int64_t ltxk_linear_fp8_workspace_bytes(int64_t m, int64_t n, int64_t k, int gelu)
+extern "C" int64_t ltxk_linear_fp8_workspace_bytes(int64_t m, int64_t n, int64_t k, int gelu, int quantize)
 {
     if (m <= 0 || n <= 0 || k <= 0) return 0;
-    return workspace_bytes(m, n, k, gelu != 0);
+    const int64_t kMax = int64_t{1} << 31;  // sizes that the calls refuse
+    if (m >= kMax || n >= kMax || k >= kMax) return 0;
+    const int64_t blocks = quantize ? round16(m * fp8_blocks(k) * kFp8Block) + round16(m * fp8_groups(k) * kFp8Group) : 0;
+    return blocks + workspace_bytes(m, n, k, gelu != 0);
 }
 
 extern "C" int ltxk_linear_fp8(void *y, const void *x, const void *x_scale, const void *w, const void *w_scale,

@@ -144,7 +144,7 @@ SIGNATURES = {
         _c_int,
         [_c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _ADA_P, _c_vp, _c_i64, _c_i64, _c_i64, _c_float, _ADA_P, _ADA_P, _c_vp],
     ),
-    "ltxk_linear_fp8_workspace_bytes": (_c_i64, [_c_i64, _c_i64, _c_i64, _c_int]),
+    "ltxk_linear_fp8_workspace_bytes": (_c_i64, [_c_i64, _c_i64, _c_i64, _c_int, _c_int]),
     "ltxk_linear_fp8": (_c_int, [_c_vp] * 6 + [_c_i64] * 3 + [_c_vp, _c_i64, _c_vp]),
     "ltxk_linear_gelu_fp8": (_c_int, [_c_vp] * 7 + [_c_i64] * 3 + [_c_vp, _c_i64, _c_vp]),
 }
@@ -292,7 +292,7 @@ _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device
 
 
 def _one_device(t: torch.Tensor, *others: torch.Tensor | None) -> None:
-    """All operands on one device, and that the current one, on whose stream the call runs."""
+    """All operands on one device, and that the current one: a launch goes to the current device."""
     device = t.get_device()
     for o in others:
         if o is not None and o.get_device() != device:
@@ -919,22 +919,30 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: int, log
     return out
 
 
-def _rows_of(x: torch.Tensor, name: str, b: int, t: int, d: int) -> torch.Tensor:
-    """x if it is bf16 (b, t, d) with contiguous rows that the kernels can read through its
-    batch and token strides (not negative, multiples of 8), else an error."""
+def _attention_rows(x: torch.Tensor, name: str, b: int, t: int, d: int) -> tuple[int, int]:
+    """(batch stride, token stride) of a bf16 (b, t, d) whose rows are contiguous, or an error.  A stride that is never
+    taken (one token, one batch item) may be anything in torch: the contiguous one stands for it."""
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
     if x.device.type != "cuda":
         raise RuntimeError(f"{name} is on {x.device}; ltxk kernels run on the ROCm device only")
     if x.dtype != torch.bfloat16:
         raise ValueError(f"{name} has dtype {x.dtype}, expected torch.bfloat16")
-    if tuple(x.shape) != (b, t, d):
+    if x.shape != (b, t, d):
         raise ValueError(f"{name} is {tuple(x.shape)}, expected {(b, t, d)}")
-    if x.numel() and ((d > 1 and x.stride(2) != 1) or x.stride(0) % 8 or x.stride(1) % 8
-                      or (t > 1 and x.stride(1) < d)):
+    if x.is_contiguous():
+        return t * d, d
+    sb, st, sd = x.stride()
+    sb, st = sb if b > 1 else 0, st if t > 1 else d
+    if sd != 1 or sb % 8 or st % 8 or st < d:
         raise ValueError(f"{name}'s rows must be contiguous, with batch and token strides (multiples of 8) that cover "
                          f"them; got {x.stride()}")
-    return x
+    return sb, st
+
+
+@functools.lru_cache(maxsize=4096)
+def _cross_attention_workspace_bytes(b: int, tq: int, tk: int, heads: int, dh: int) -> int:
+    return load().ltxk_cross_attention_workspace_bytes(b, tq, tk, heads, dh)
 
 
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: int, keep: torch.Tensor | None = None,
@@ -945,43 +953,42 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: in
 
     q, k and v may be views of wider rows (one projection's key and value halves).  Keys and values that are not kept
     are not read and cost no time, whatever their pattern; where nothing is kept (or Tk is 0) the result is zero."""
-    if not all(isinstance(x, torch.Tensor) and x.ndim == 3 for x in (q, k, v)):
+    if getattr(q, "ndim", 0) != 3 or getattr(k, "ndim", 0) != 3:
         raise ValueError("q, k and v must be (B, T, H*Dh) tensors")
     (b, tq, d), tk = q.shape, k.shape[1]
-    for x, name, t in ((q, "q", tq), (k, "k", tk), (v, "v", tk)):
-        _rows_of(x, name, b, t, d)
+    qb, qt = _attention_rows(q, "q", b, tq, d)
+    kb, kt = _attention_rows(k, "k", b, tk, d)
+    vb, vt = _attention_rows(v, "v", b, tk, d)
     dh = d // heads if heads > 0 else 0
     if d != heads * dh or dh not in ATTENTION_HEAD_DIMS:
         raise ValueError(f"width {d} is not {heads} heads of 64 or 128")
+    keep_stride = 0
     if keep is not None:
-        _dev(keep, "keep", (torch.bool, torch.uint8))
+        _dev(keep, "keep", torch.bool if keep.dtype == torch.bool else torch.uint8)
         if keep.ndim != 2 or keep.shape[0] not in (1, b) or keep.shape[1] != tk:
             raise ValueError(f"keep {tuple(keep.shape)} must be ({b} or 1, {tk})")
+        if keep.shape[0] > 1:
+            keep_stride = tk
     if logits is not None:
         _dev(logits, "logits")
-        if tuple(logits.shape) != (b, tq, heads):
+        if logits.shape != (b, tq, heads):
             raise ValueError(f"logits {tuple(logits.shape)} != {(b, tq, heads)}")
     if out is None:
         out = torch.empty((b, tq, d), device=q.device, dtype=q.dtype)
     else:
         _dev(out, "out")
-        if tuple(out.shape) != (b, tq, d):
+        if out.shape != (b, tq, d):
             raise ValueError(f"out {tuple(out.shape)} != {(b, tq, d)}")
     _one_device(q, k, v, keep, logits, out)
     if out.numel() == 0:
         return out
     if tk == 0:
         return out.zero_()
-    lib = load()
-    # a stride that is never taken (one token, one batch item) may be anything in torch
-    strides = [s for x, t in ((q, tq), (k, tk), (v, tk)) for s in (x.stride(0) if b > 1 else 0,
-                                                                    x.stride(1) if t > 1 else d)]
-    (qb, qt, kb, kt, vb, vt), st = strides, _stream(q)
-    nbytes = lib.ltxk_cross_attention_workspace_bytes(b, tq, tk, heads, dh)
+    nbytes = _cross_attention_workspace_bytes(b, tq, tk, heads, dh)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-    rc = lib.ltxk_cross_attention(_ptr(out), q.data_ptr(), qb, qt, k.data_ptr(), kb, kt, v.data_ptr(), vb, vt,
-                                  _ptr(keep), tk if keep is not None and keep.shape[0] > 1 else 0, _ptr(logits), b, tq,
-                                  tk, heads, dh, dh ** -0.5, ws.data_ptr(), nbytes, st)
+    rc = load().ltxk_cross_attention(out.data_ptr(), q.data_ptr(), qb, qt, k.data_ptr(), kb, kt, v.data_ptr(), vb, vt,
+                                     _ptr(keep), keep_stride, _ptr(logits), b, tq, tk, heads, dh, dh ** -0.5,
+                                     ws.data_ptr(), nbytes, _stream(q))
     _check_rc(rc, "cross_attention")
     return out
 
@@ -1011,11 +1018,11 @@ class Fp8Blocks:
         if not shape or shape[-1] <= 0 or shape[-1] % 8:
             raise ValueError(f"shape {shape} must end in a positive multiple of 8")
         rows, blocks = _fp8_extent(shape)
-        if tuple(data.shape) != (rows, blocks * FP8_BLOCK):
+        if data.shape != (rows, blocks * FP8_BLOCK):
             raise ValueError(f"data {tuple(data.shape)} does not hold {shape}: expected {(rows, blocks * FP8_BLOCK)}")
-        want = (-(-blocks // FP8_GROUP), rows, FP8_GROUP)
-        if tuple(scale.shape) != want:
-            raise ValueError(f"scale {tuple(scale.shape)} does not hold {shape}: expected {want}")
+        if scale.shape != (-(-blocks // FP8_GROUP), rows, FP8_GROUP):
+            raise ValueError(f"scale {tuple(scale.shape)} does not hold {shape}: expected "
+                             f"{(-(-blocks // FP8_GROUP), rows, FP8_GROUP)}")
         if data.get_device() != scale.get_device():
             raise ValueError(f"data is on {data.device}, scale on {scale.device}")
         self.data, self.scale, self.shape = data, scale, shape
@@ -1113,56 +1120,58 @@ def _norm_fp8(x, f, gate, mask, shift, scale, eps, x_out):
     return x_out, out
 
 
-def _fp8_operands(x, weight: Fp8Blocks, bias: torch.Tensor | None) -> Fp8Blocks:
-    """x in blocks, after the checks that both 8-bit layers share."""
+@functools.lru_cache(maxsize=4096)
+def _fp8_workspace_bytes(m: int, n: int, k: int, gelu: bool, quantize: bool) -> int:
+    """A function of the sizes alone; asked for each call it takes the host 1 us of about 10."""
+    return load().ltxk_linear_fp8_workspace_bytes(m, n, k, gelu, quantize)
+
+
+def _fp8_linear(x, weight: Fp8Blocks, bias: torch.Tensor | None, gelu: bool):
+    """Both 8-bit layers: x in blocks, or bf16 and quantised by the same call."""
     if not isinstance(weight, Fp8Blocks):
         raise TypeError("weight must be Fp8Blocks (quantize_fp8)")
     if len(weight.shape) != 2 or weight.shape[0] == 0 or weight.shape[0] % 8:
         raise ValueError(f"weight {weight.shape} must be (N, K), N a positive multiple of 8")
-    if not isinstance(x, Fp8Blocks):
+    n, k = weight.shape
+    held = isinstance(x, Fp8Blocks)
+    if not held:
         _dev(x, "x")
-    if len(x.shape) == 0 or x.shape[-1] != weight.shape[1]:
-        raise ValueError(f"x {tuple(x.shape)} does not end in the weight's {weight.shape[1]} columns")
+    lead = x.shape[:-1]
+    if len(x.shape) == 0 or x.shape[-1] != k:
+        raise ValueError(f"x {tuple(x.shape)} does not end in the weight's {k} columns")
     if bias is not None:
         _dev(bias, "bias")
-        if tuple(bias.shape) != (weight.shape[0],):
-            raise ValueError(f"bias {tuple(bias.shape)} must be ({weight.shape[0]},)")
-    x = x if isinstance(x, Fp8Blocks) else quantize_fp8(x)
-    _one_device(x.data, weight.data, bias)
-    return x
-
-
-def _fp8_workspace(lib, m: int, n: int, k: int, gelu: int, device) -> tuple:
-    nbytes = lib.ltxk_linear_fp8_workspace_bytes(m, n, k, gelu)
-    return (torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None), nbytes
+        if bias.shape != (n,):
+            raise ValueError(f"bias {tuple(bias.shape)} must be ({n},)")
+    data, scale = (x.data, x.scale) if held else (x, None)
+    w = weight.data
+    _one_device(data, w, bias)
+    m = data.shape[0] if held else x.numel() // k
+    if gelu:
+        out = Fp8Blocks._made((*lead, n), w.device)
+    else:
+        out = torch.empty((*lead, n), device=w.device, dtype=torch.bfloat16)
+    nbytes = _fp8_workspace_bytes(m, n, k, gelu, not held)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=w.device) if nbytes else None
+    lib = load()
+    rest = (data.data_ptr(), _ptr(scale), w.data_ptr(), weight.scale.data_ptr(), _ptr(bias), m, n, k, _ptr(ws), nbytes,
+            _stream(w))
+    if gelu:
+        _check_rc(lib.ltxk_linear_gelu_fp8(out.data.data_ptr(), out.scale.data_ptr(), *rest), "linear_gelu_fp8")
+    else:
+        _check_rc(lib.ltxk_linear_fp8(out.data_ptr(), *rest), "linear_fp8")
+    return out
 
 
 def linear_fp8(x: torch.Tensor | Fp8Blocks, weight: Fp8Blocks, bias: torch.Tensor | None = None) -> torch.Tensor:
     """x (..., K) weight (N, K)^T + bias (N) as bf16, over blocks: x as it is held, or quantised first if it is bf16.
-    Exact products of the held values, fp32 sums, one rounding; N a multiple of 8."""
-    x = _fp8_operands(x, weight, bias)
-    (n, k), m = weight.shape, x.data.shape[0]
-    out = torch.empty(*x.shape[:-1], n, device=x.device, dtype=torch.bfloat16)
-    lib = load()
-    ws, nbytes = _fp8_workspace(lib, m, n, k, 0, x.device)
-    rc = lib.ltxk_linear_fp8(out.data_ptr(), x.data.data_ptr(), x.scale.data_ptr(), weight.data.data_ptr(),
-                             weight.scale.data_ptr(), _ptr(bias), m, n, k, _ptr(ws), nbytes, _stream(x.data))
-    _check_rc(rc, "linear_fp8")
-    return out
+    Products of the held values, fp32 sums, one rounding; N a multiple of 8."""
+    return _fp8_linear(x, weight, bias, False)
 
 
 def linear_gelu_fp8(x: torch.Tensor | Fp8Blocks, weight: Fp8Blocks, bias: torch.Tensor | None = None) -> Fp8Blocks:
     """gelu_tanh(x weight^T + bias) in blocks, fp32 up to them: a feed-forward's first layer for an 8-bit second."""
-    x = _fp8_operands(x, weight, bias)
-    (n, k), m = weight.shape, x.data.shape[0]
-    out = Fp8Blocks._made((*x.shape[:-1], n), x.device)
-    lib = load()
-    ws, nbytes = _fp8_workspace(lib, m, n, k, 1, x.device)
-    rc = lib.ltxk_linear_gelu_fp8(out.data.data_ptr(), out.scale.data_ptr(), x.data.data_ptr(), x.scale.data_ptr(),
-                                  weight.data.data_ptr(), weight.scale.data_ptr(), _ptr(bias), m, n, k, _ptr(ws),
-                                  nbytes, _stream(x.data))
-    _check_rc(rc, "linear_gelu_fp8")
-    return out
+    return _fp8_linear(x, weight, bias, True)
 
 
 def gelu_tanh(x: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:

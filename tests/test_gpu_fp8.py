@@ -279,8 +279,8 @@ def test_outputs_behind_the_rows_stay():
         assert lib.ltxk_quantize_fp8(q.data_ptr(), s.data_ptr(), x.data_ptr(), m, k, st) == 0
         assert (q[rows * kp:] == 77).all() and (s[xb.scale.numel():] == 77).all()
         y = torch.full((m * n + 256,), 7.0, device=DEV, dtype=torch.bfloat16)
-        ws = torch.empty(max(16, lib.ltxk_linear_fp8_workspace_bytes(m, n, k, 0), lib.ltxk_linear_fp8_workspace_bytes(m, n, k, 1)),
-                         dtype=torch.uint8, device=DEV)
+        ws = torch.empty(max(16, *(lib.ltxk_linear_fp8_workspace_bytes(m, n, k, g, 0) for g in (0, 1))), dtype=torch.uint8,
+                         device=DEV)
         ops = [t.data_ptr() for t in (xb.data, xb.scale, w.data, w.scale)]
         assert lib.ltxk_linear_fp8(y.data_ptr(), *ops, None, m, n, k, ws.data_ptr(), ws.numel(), st) == 0
         assert (y[m * n:] == 7).all() and torch.equal(y[:m * n].view(m, n), ltxk.linear_fp8(xb, w))
