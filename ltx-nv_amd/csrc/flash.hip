@@ -58,7 +58,9 @@ struct FlashParams {
     int rest, parts;        // the others, each cut into `parts` units over the keys
     float scale2;           // scale * log2(e)
     bool round;             // the output rounds to bf16 before the gate, too
-    const int *count, *list;  // kept keys only: how many of each batch item's, and which (batch, tk)
+    const uint8_t *keep;    // kept keys only: a byte per key, batch items keep_bs apart,
+    int64_t keep_bs;
+    const int *count, *list;  // or how many of each batch item's are kept, and which (batch, tk)
 };
 
 // Query tile t of XCD x: all query tiles of a head go to one XCD, whose L2 then
@@ -149,11 +151,53 @@ __device__ __forceinline__ void tile_barrier()
     asm volatile("" ::: "memory");
 }
 
-// KEPT: over the keys that p.list names, which it gathers: a batch item's work is
-// that of its kept keys, and nothing of the others is read.
-template <int D, bool KEPT>
+// Over which keys: all of them, or the kept ones, which it gathers (a batch item's work is
+// that of its kept keys, and nothing of the others is read): the workgroup lists them in LDS
+// for itself up to kMaxListed of them, as far as two workgroups' lists fit beside their
+// tiles, else keep_kernel has.
+enum Keys { kAll, kKept, kListed };
+constexpr int kMaxListed = 8192;
+
+// The kept of tk keys in their order into `list`, their count returned: 1024 keys a round,
+// four a thread, each wave's by ballots, the waves' counts added up in LDS (`counts`, 8).
+__device__ __forceinline__ int list_kept(const uint8_t *keep, int tk, uint16_t *list, int *counts)
+{
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const uint64_t below = (uint64_t{1} << lane) - 1;
+    int before = 0;
+    for (int first = 0, round = 0; first < tk; first += 1024, round ^= 1) {
+        const int i = first + threadIdx.x * 4;
+        uint8_t kept[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) kept[j] = i + j < tk ? keep[i + j] : 0;
+        int at = 0, total = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint64_t b = __ballot(kept[j] != 0);
+            at += __popcll(b & below);
+            total += __popcll(b);
+        }
+        if (lane == 0) counts[round * kWaves + wave] = total;
+        __syncthreads();
+        at += before;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const int c = counts[round * kWaves + w];
+            if (w < wave) at += c;
+            before += c;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (kept[j]) list[at++] = static_cast<uint16_t>(i + j);
+    }
+    __syncthreads();
+    return before;
+}
+
+template <int D, Keys KEYS>
 __global__ void __launch_bounds__(kWaves * 64, 2) flash_kernel(FlashParams p)
 {
+    constexpr bool KEPT = KEYS != kAll;
     constexpr int KS = D / 16;               // contraction steps of the scores
     constexpr int MT = D / 32;               // output tiles
     constexpr int NK = 2 * KS, NV = 4 * MT;  // K and V fragments of a tile
@@ -169,7 +213,10 @@ __global__ void __launch_bounds__(kWaves * 64, 2) flash_kernel(FlashParams p)
     const int unit = j - p.whole, part = split ? unit % p.parts : 0;
     int b, head, first;
     if (!query_tile(p, xcd, split ? p.whole + unit / p.parts : j, b, head, first)) return;
-    const int keys = KEPT ? p.count[b] : p.tk;
+    __shared__ uint16_t kept[KEYS == kKept ? kMaxListed : 1];
+    int keys = p.tk;
+    if constexpr (KEYS == kKept) keys = list_kept(p.keep + b * p.keep_bs, p.tk, kept, reinterpret_cast<int *>(k0));
+    if constexpr (KEYS == kListed) keys = p.count[b];
     const int tiles = KEPT ? (keys + kKeys - 1) / kKeys : p.tiles;
     const int t0 = split ? part * tiles / p.parts : 0;
     const int t1 = split ? (part + 1) * tiles / p.parts : tiles;
@@ -201,10 +248,11 @@ __global__ void __launch_bounds__(kWaves * 64, 2) flash_kernel(FlashParams p)
     // on their way, i + 2.
     int at_v[kLoads<D>], at_k[kLoads<D>], at_next[kLoads<D>];
     auto listed = [&](int i, int *at) {
-        const int *list = p.list + static_cast<int64_t>(b) * p.tk;
 #pragma unroll
-        for (int c = 0; c < kLoads<D>; ++c)
-            at[c] = list[min((t0 + min(i, n - 1)) * kKeys + part_row<D>(c, wave, lane), keys - 1)];
+        for (int c = 0; c < kLoads<D>; ++c) {
+            const int j = min((t0 + min(i, n - 1)) * kKeys + part_row<D>(c, wave, lane), keys - 1);
+            at[c] = KEYS == kKept ? kept[j] : p.list[static_cast<int64_t>(b) * p.tk + j];
+        }
     };
     if constexpr (KEPT) {
         listed(0, at_k);
@@ -469,11 +517,11 @@ FlashCut cut(int64_t bh, int64_t tokens_q, int64_t tokens_k)
     return c;
 }
 
-template <int D, bool KEPT>
+template <int D, Keys KEYS>
 void launch(const FlashParams &p, hipStream_t s)
 {
-    flash_kernel<D, KEPT><<<8u * (p.whole + p.rest * p.parts), kWaves * 64, 0, s>>>(p);
-    if (p.rest) flash_merge_kernel<D, KEPT><<<8u * (p.rest * (kRows * D / 8) / 256), 256, 0, s>>>(p);
+    flash_kernel<D, KEYS><<<8u * (p.whole + p.rest * p.parts), kWaves * 64, 0, s>>>(p);
+    if (p.rest) flash_merge_kernel<D, KEYS != kAll><<<8u * (p.rest * (kRows * D / 8) / 256), 256, 0, s>>>(p);
 }
 
 // The kept keys of each batch item in their order, a workgroup an item: 1024 keys a
@@ -503,7 +551,7 @@ __global__ void __launch_bounds__(1024) keep_kernel(const uint8_t *keep, int64_t
 
 int64_t list_bytes(int64_t batch, int64_t tokens_k)
 {
-    return (batch * (tokens_k + 1) * 4 + 15) / 16 * 16;
+    return tokens_k <= kMaxListed ? 0 : (batch * (tokens_k + 1) * 4 + 15) / 16 * 16;
 }
 
 }  // namespace
@@ -587,20 +635,20 @@ static int attend(const char *what, bool round, int64_t lists, void *out, const 
     p.scale2 = scale2;
     p.round = round;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (keep) {
+    const bool wide = head_dim == 128;
+    if (!keep) {
+        wide ? launch<128, kAll>(p, s) : launch<64, kAll>(p, s);
+    } else if (tokens_k <= kMaxListed) {
+        p.keep = static_cast<const uint8_t *>(keep);
+        p.keep_bs = keep_bstride;
+        wide ? launch<128, kKept>(p, s) : launch<64, kKept>(p, s);
+    } else {
         int *count = static_cast<int *>(workspace), *list = count + batch;
         p.count = count;
         p.list = list;
         keep_kernel<<<static_cast<unsigned>(batch), 1024, 0, s>>>(static_cast<const uint8_t *>(keep), keep_bstride, p.tk,
                                                                   count, list);
-        if (head_dim == 128)
-            launch<128, true>(p, s);
-        else
-            launch<64, true>(p, s);
-    } else if (head_dim == 128) {
-        launch<128, false>(p, s);
-    } else {
-        launch<64, false>(p, s);
+        wide ? launch<128, kListed>(p, s) : launch<64, kListed>(p, s);
     }
     return check_launch(what);
 }

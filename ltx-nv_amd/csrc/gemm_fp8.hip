@@ -22,11 +22,12 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 struct Fp8Params {
     const uint8_t *x, *xs, *w, *ws;  // values and scales
+    const uint16_t *x16;             // x in bf16 instead, rows of k
     const uint16_t *bias;
     uint16_t *y;       // bf16 result, or
     uint8_t *q, *qs;   // its blocks after GELU
     float *part;       // fp32 sums (m, np)
-    int m, n, kp, blocks, np;
+    int m, n, k, kp, blocks, np;
     int tiles_m, tiles_n;
     int whole, rest, parts;  // tiles that one workgroup takes alone; the others, cut into parts over K
     int per;                 // units of the cut tiles an XCD
@@ -780,15 +781,24 @@ typedef Tile<128, 2, 2, 8, 4, 4> Medium;
 // their sums are added in LDS at the end.
 constexpr int kFewWaves = 4;
 
-template <int MT_, int NT_, int RING_>
+// X16: x is bf16, and each workgroup quantises all of it into LDS while its first loads of w are
+// on their way: for x of at most kInline bytes there (a launch less).
+constexpr int kInline = 17408;  // with the ring a third of LDS
+
+template <int MT_, int NT_, int RING_, bool X16_ = false>
 struct Few {
     static constexpr int MT = MT_, NT = NT_, RING = RING_;
-    static constexpr int loads = 4 * (MT + NT) + 2;               // of a block: 8 rows each, and both sides' scales
-    static constexpr int scales_at = (MT + NT) * 4096, bytes = scales_at + 512;
-    static constexpr int sums = kFewWaves * MT * NT * 4096;
-    static constexpr int lds = RING * bytes * kFewWaves > sums ? RING * bytes * kFewWaves : sums;
+    static constexpr bool X16 = X16_;
+    static constexpr int loads = X16 ? 4 * NT + 1 : 4 * (MT + NT) + 2;  // of a block: 8 rows each, and the scales
+    static constexpr int w_at = X16 ? 0 : MT * 4096, scales_at = w_at + NT * 4096, bytes = scales_at + (X16 ? 256 : 512);
+    static constexpr int ring = RING * bytes * kFewWaves, sums = kFewWaves * MT * NT * 4096;
+    static constexpr int x_at = ring > sums ? ring : sums, lds = x_at + (X16 ? kInline : 0);
     static_assert(MT <= 2 && NT <= 2 && loads * (RING - 1) < 64, "a load takes 64 rows of scales, a wait counts to 63");
 };
+
+// x in LDS: rows of the values, 16 bytes apart from a multiple of 128 (so that 32 rows cover
+// the banks), then rows of the scales.
+__host__ __device__ inline int64_t inline_bytes(int64_t m, int64_t kp) { return m * (kp + 16 + kp / kFp8Block); }
 
 // This wave's loads but the newest `n` have landed.
 __device__ __forceinline__ void wait_loads(int n)
@@ -796,6 +806,7 @@ __device__ __forceinline__ void wait_loads(int n)
     asm volatile("" ::: "memory");
     switch (n) {
 #define LTXK_WAIT(N) case N: __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | (N >> 4 << 14)); break;
+    LTXK_WAIT(5)
     LTXK_WAIT(10)
     LTXK_WAIT(14)
     LTXK_WAIT(18)
@@ -842,13 +853,44 @@ __global__ void __launch_bounds__(kFewWaves * 64) few_kernel(Fp8Params p)
         const uint32_t at = lds0 + slot * F::bytes;
         const uint32_t k = __builtin_amdgcn_readfirstlane(b * kFp8Block), g = __builtin_amdgcn_readfirstlane(b >> 2);
 #pragma unroll
-        for (int c = 0; c < 4 * NT; ++c) load_lds16(wr, __builtin_amdgcn_readfirstlane(at + (MT * 4 + c) * 1024), wo[c], k);
+        for (int c = 0; c < 4 * NT; ++c) load_lds16(wr, __builtin_amdgcn_readfirstlane(at + F::w_at + c * 1024), wo[c], k);
+        load_lds4(wsr, __builtin_amdgcn_readfirstlane(at + F::scales_at), wso, __builtin_amdgcn_readfirstlane(g * p.n * 4));
+        if constexpr (!F::X16) {
 #pragma unroll
-        for (int c = 0; c < 4 * MT; ++c) load_lds16(xr, __builtin_amdgcn_readfirstlane(at + c * 1024), xo[c], k);
-        load_lds4(xsr, __builtin_amdgcn_readfirstlane(at + F::scales_at), xso, __builtin_amdgcn_readfirstlane(g * p.m * 4));
-        load_lds4(wsr, __builtin_amdgcn_readfirstlane(at + F::scales_at + 256), wso, __builtin_amdgcn_readfirstlane(g * p.n * 4));
+            for (int c = 0; c < 4 * MT; ++c) load_lds16(xr, __builtin_amdgcn_readfirstlane(at + c * 1024), xo[c], k);
+            load_lds4(xsr, __builtin_amdgcn_readfirstlane(at + F::scales_at + 256), xso, __builtin_amdgcn_readfirstlane(g * p.m * 4));
+        }
     };
     for (int i = 0; i < R && i < n; ++i) load(i, i);
+    char *xl = smem + F::x_at, *xsl = xl + p.m * (p.kp + 16);
+    if constexpr (F::X16) {
+        // a block 16 lanes, as quantize_fp8; the loads of kBatch blocks together
+        constexpr int kBatch = 4, kStride = kFewWaves * 4;
+        const int units = p.m * p.blocks;
+        for (int u0 = threadIdx.x >> 4; u0 < units; u0 += kBatch * kStride) {
+            u32x4 raw[kBatch];
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {  // past the last: read again, not stored
+                const int u = min(u0 + i * kStride, units - 1), row = u / p.blocks, col = u % p.blocks * kFp8Block + (lane & 15) * 8;
+                raw[i] = *reinterpret_cast<const u32x4 *>(p.x16 + static_cast<int64_t>(row) * p.k + min(col, p.k - 8));
+                if (col >= p.k) raw[i] = u32x4{};
+            }
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                const int u = u0 + i * kStride, row = u / p.blocks, b = u % p.blocks;
+                float f[8];
+                unpack8v(raw[i], f);
+                uint32_t scale;
+                const uint2 q = fp8_quantize8(f, scale);
+                if (u >= units) continue;
+                *reinterpret_cast<uint2 *>(xl + row * (p.kp + 16) + b * kFp8Block + (lane & 15) * 8) = q;
+                if ((lane & 15) == 0) xsl[u] = static_cast<char>(scale);
+            }
+        }
+        __syncthreads();
+        xl += min(l32, p.m - 1) * (p.kp + 16) + half * 16;
+        xsl += min(l32, p.m - 1) * p.blocks;
+    }
 
     int off[4];
 #pragma unroll
@@ -860,14 +902,22 @@ __global__ void __launch_bounds__(kFewWaves * 64) few_kernel(Fp8Params p)
         const char *at = smem + (wave * R + slot) * F::bytes;
         i32x8 f[2][MT + NT];
         int scale[MT + NT];
-#pragma unroll
-        for (int t = 0; t < MT + NT; ++t) {
+        const int b = first + i * kFewWaves;
+        if constexpr (F::X16) {
 #pragma unroll
             for (int s = 0; s < 2; ++s)
-                f[s][t] = cat(*reinterpret_cast<const i32x4 *>(at + t * 4096 + off[2 * s]),
-                              *reinterpret_cast<const i32x4 *>(at + t * 4096 + off[2 * s + 1]));
-            scale[t] = *reinterpret_cast<const uint8_t *>(at + F::scales_at + (t < MT ? t * 128 : 256 + (t - MT) * 128) + l32 * 4 +
-                                                          ((first + i * kFewWaves) & 3));
+                f[s][0] = cat(*reinterpret_cast<const i32x4 *>(xl + b * kFp8Block + s * 64),
+                              *reinterpret_cast<const i32x4 *>(xl + b * kFp8Block + s * 64 + 32));
+            scale[0] = static_cast<uint8_t>(xsl[b]);
+        }
+#pragma unroll
+        for (int t = F::X16 ? MT : 0; t < MT + NT; ++t) {
+            const char *tile = t < MT ? at + t * 4096 : at + F::w_at + (t - MT) * 4096;
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+                f[s][t] = cat(*reinterpret_cast<const i32x4 *>(tile + off[2 * s]),
+                              *reinterpret_cast<const i32x4 *>(tile + off[2 * s + 1]));
+            scale[t] = *reinterpret_cast<const uint8_t *>(at + F::scales_at + (t < MT ? 256 + t * 128 : (t - MT) * 128) + l32 * 4 + (b & 3));
         }
         // read whole: its place goes to block i + R
         asm volatile("" ::: "memory");
@@ -1029,7 +1079,13 @@ void launch_tiles(const Fp8Params &p, hipStream_t s)
         tile_sum_kernel<T::size, GELU><<<static_cast<unsigned>(p.rest) * (T::size * T::size / 8 / 256), 256, 0, s>>>(p);
 }
 
-int64_t round16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
+bool takes_bf16(const Cut &c, int64_t m, int64_t kp) { return c.tile == 32 && inline_bytes(m, kp) <= kInline; }
+
+// x's blocks, where the call makes them: values (a multiple of 128 bytes), then scales.
+int64_t blocks_bytes(int64_t m, int64_t n, int64_t k)
+{
+    return takes_bf16(cut(m, n, k), m, fp8_blocks(k) * kFp8Block) ? 0 : m * fp8_blocks(k) * kFp8Block + (m * fp8_groups(k) * kFp8Group + 15) / 16 * 16;
+}
 
 // The checks and the launch of both entry points.
 int linear(const char *what, void *y, void *y_scale, bool gelu, const void *x, const void *x_scale, const void *w,
@@ -1050,8 +1106,8 @@ int linear(const char *what, void *y, void *y_scale, bool gelu, const void *x, c
     const int64_t kp = fp8_blocks(k) * kFp8Block, np = fp8_blocks(n) * kFp8Block;
     if (m > (kMax - 1) / kp || n > (kMax - 1) / kp || m > (kMax - 1) / np)
         return fail(LTXK_E_ARG, "%s: x, w or y holds 2^31 values or more", what);
-    const int64_t values = x_scale ? 0 : m * kp, scales = x_scale ? 0 : m * fp8_groups(k) * kFp8Group;
-    const int64_t blocks_at = round16(values) + round16(scales), need = blocks_at + workspace_bytes(m, n, k, gelu);
+    const Cut c = cut(m, n, k);
+    const int64_t blocks_at = x_scale ? 0 : blocks_bytes(m, n, k), need = blocks_at + workspace_bytes(m, n, k, gelu);
     if (need && (!workspace || !aligned16(workspace) || workspace_size < need))
         return fail(LTXK_E_ARG, "%s: the workspace must hold ltxk_linear_fp8_workspace_bytes, 16-byte aligned", what);
     Fp8Params p{};
@@ -1064,8 +1120,10 @@ int linear(const char *what, void *y, void *y_scale, bool gelu, const void *x, c
     p.q = gelu ? static_cast<uint8_t *>(y) : nullptr;
     p.qs = static_cast<uint8_t *>(y_scale);
     p.part = reinterpret_cast<float *>(static_cast<char *>(workspace) + blocks_at);
-    if (!x_scale) {
-        char *q = static_cast<char *>(workspace), *q_scale = q + round16(values);
+    if (!x_scale && takes_bf16(c, m, kp)) {
+        p.x16 = static_cast<const uint16_t *>(x);
+    } else if (!x_scale) {
+        char *q = static_cast<char *>(workspace), *q_scale = q + m * kp;
         const int rc = ltxk_quantize_fp8(q, q_scale, x, m, k, stream);
         if (rc) return rc;
         p.x = reinterpret_cast<const uint8_t *>(q);
@@ -1073,10 +1131,10 @@ int linear(const char *what, void *y, void *y_scale, bool gelu, const void *x, c
     }
     p.m = static_cast<int>(m);
     p.n = static_cast<int>(n);
+    p.k = static_cast<int>(k);
     p.kp = static_cast<int>(kp);
     p.blocks = static_cast<int>(kp / kFp8Block);
     p.np = static_cast<int>(np);
-    const Cut c = cut(m, n, k);
     p.tiles_m = static_cast<int>(c.tiles_m);
     p.tiles_n = static_cast<int>(c.tiles_n);
     p.whole = static_cast<int>(c.whole);
@@ -1103,6 +1161,8 @@ int linear(const char *what, void *y, void *y_scale, bool gelu, const void *x, c
         few_rows<Few<2, 2, 2>>(p, gelu, s);
     } else if (c.tile == 48) {
         few_rows<Few<2, 1, 3>>(p, gelu, s);
+    } else if (p.x16) {
+        few_rows<Few<1, 1, 2, true>>(p, gelu, s);
     } else {
         few_rows<Few<1, 1, 2>>(p, gelu, s);
     }
@@ -1119,8 +1179,7 @@ extern "C" int64_t ltxk_linear_fp8_workspace_bytes(int64_t m, int64_t n, int64_t
     if (m <= 0 || n <= 0 || k <= 0) return 0;
     const int64_t kMax = int64_t{1} << 31;  // sizes that the calls refuse
     if (m >= kMax || n >= kMax || k >= kMax) return 0;
-    const int64_t blocks = quantize ? round16(m * fp8_blocks(k) * kFp8Block) + round16(m * fp8_groups(k) * kFp8Group) : 0;
-    return blocks + workspace_bytes(m, n, k, gelu != 0);
+    return (quantize ? blocks_bytes(m, n, k) : 0) + workspace_bytes(m, n, k, gelu != 0);
 }
 
 extern "C" int ltxk_linear_fp8(void *y, const void *x, const void *x_scale, const void *w, const void *w_scale,

@@ -985,10 +985,10 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: in
     if tk == 0:
         return out.zero_()
     nbytes = _cross_attention_workspace_bytes(b, tq, tk, heads, dh)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
     rc = load().ltxk_cross_attention(out.data_ptr(), q.data_ptr(), qb, qt, k.data_ptr(), kb, kt, v.data_ptr(), vb, vt,
                                      _ptr(keep), keep_stride, _ptr(logits), b, tq, tk, heads, dh, dh ** -0.5,
-                                     ws.data_ptr(), nbytes, _stream(q))
+                                     _ptr(ws), nbytes, _stream(q))
     _check_rc(rc, "cross_attention")
     return out
 

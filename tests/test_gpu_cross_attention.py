@@ -39,7 +39,8 @@ def _against_kept(q, k, v, h, keep, logits, got):
 @pytest.mark.parametrize("kind", ["front", "back", "one", "holes", "empty"])
 @pytest.mark.parametrize("b,tq,tk,h,dh,gated", [
     (1, 1, 1, 2, 64, True), (2, 128, 64, 1, 128, False), (3, 129, 65, 3, 64, True), (2, 127, 333, 2, 128, True),
-    (4, 126, 1024, 4, 64, True), (3, 5, 4099, 3, 128, True), (2, 257, 2050, 2, 64, False), (2, 4100, 700, 8, 128, True)])
+    (4, 126, 1024, 4, 64, True), (3, 5, 4099, 3, 128, True), (2, 70, 8192, 2, 64, True), (2, 3, 8193, 1, 128, False),
+    (3, 40, 9001, 2, 64, True), (2, 257, 2050, 2, 64, False), (2, 4100, 700, 8, 128, True)])
 def test_matches_fp64_over_the_kept_keys(kind, b, tq, tk, h, dh, gated):
     import ltxk
 
