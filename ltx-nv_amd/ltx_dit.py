@@ -193,6 +193,9 @@ class Modality:
     # `positions` (ArgsPreprocessor.rope_tables).  Without them every forward
     # builds the tables from `positions`, as the reference does.
     rope_tables: RopeTables | None = None
+    # Not in the reference API (optional): (B or 1, S) bool, the context tokens of each
+    # batch item to attend to, for prompts of different lengths in one padded batch.
+    context_keep: torch.Tensor | None = None
 
 
 @dataclass
@@ -227,6 +230,7 @@ class TransformerArgs:
     # cross-AdaLN `context * (1 + scale_kv) + shift_kv`, ltx_dit.py:240-246):
     # LTXModel.forward makes every block's in one launch per step.
     block_context: torch.Tensor | None = None
+    context_keep: torch.Tensor | None = None    # (B or 1, S) bool: the context tokens to attend to
 
 
 class ArgsPreprocessor:
@@ -326,6 +330,7 @@ class ArgsPreprocessor:
             x=x, context=context, context_mask=None, timesteps=timestep, embedded_timestep=embedded,
             pe=pe, cross_pe=cross_pe, cross_scale_shift_timestep=cross_ss, cross_gate_timestep=cross_gate,
             enabled=modality.enabled, prompt_timestep=prompt_timestep, pending=pending, timestep_index=index,
+            context_keep=modality.context_keep,
         )
 
 
@@ -501,10 +506,10 @@ class Block(torch.nn.Module):
                 kv_shift = _ada(prompt_sst, 0, args.prompt_timestep)
                 kv_scale = _ada(prompt_sst, 1, args.prompt_timestep)
                 enc = ltxk.modulate(_bf16(args.context), shift=kv_shift, scale=kv_scale)
-            out2 = attn2(q_in, context=enc, mask=args.context_mask)
+            out2 = attn2(q_in, context=enc, mask=args.context_mask, keep=args.context_keep)
             return x_fma, out2, _ada(sst, 8, ts)
         x_fma, x_normed = ltxk.add_norm_modulate(x, out, gate=_ada(sst, 2, ts), eps=eps)
-        return x_fma, attn2(x_normed, context=args.context, mask=args.context_mask), None
+        return x_fma, attn2(x_normed, context=args.context, mask=args.context_mask, keep=args.context_keep), None
 
     @staticmethod
     def _settle(x: torch.Tensor, args: TransformerArgs) -> torch.Tensor:
@@ -695,7 +700,13 @@ class Block(torch.nn.Module):
         Returns (x, None), or (x without the FFN residual, (ffn_out, gate)) when deferring."""
         eps = self.norm_eps
         shift, scale, gate = _ada(sst, 3, ts), _ada(sst, 4, ts), _ada(sst, 5, ts)
-        if pending is not None:
+        if ff.takes_blocks:  # the norm writes what the 8-bit layer reads
+            if pending is not None:
+                out, cgate, mask = pending
+                x, h = ltxk.add_norm_modulate_fp8(x, out, gate=cgate, mask=mask, shift=shift, scale=scale, eps=eps)
+            else:
+                h = ltxk.norm_modulate_fp8(x, shift=shift, scale=scale, eps=eps)
+        elif pending is not None:
             out, cgate, mask = pending
             x, h = ltxk.add_norm_modulate(x, out, gate=cgate, mask=mask, shift=shift, scale=scale, eps=eps)
         else:
@@ -1019,6 +1030,19 @@ class _StepInputs:
     v_rope: RopeTables
     a_rope: RopeTables
     perturbations: PerturbationTable
+    v_keep: torch.Tensor | None = None
+    a_keep: torch.Tensor | None = None
+
+
+def _passes_keep(contexts: dict, stream: str) -> torch.Tensor | None:
+    """(4, S) bool of the passes' context tokens to attend to, from the optional contexts
+    "<stream>_pos_keep" and "<stream>_neg_keep" ((1, S) bool; one alone: the other prompt is whole)."""
+    pos, neg = (contexts.get(f"{stream}_{prompt}_keep") for prompt in ("pos", "neg"))
+    if pos is None and neg is None:
+        return None
+    whole = torch.ones(contexts[f"{stream}_pos"].shape[:2], dtype=torch.bool, device=contexts[f"{stream}_pos"].device)
+    pos, neg = (whole if k is None else k.to(torch.bool).view(whole.shape) for k in (pos, neg))
+    return torch.cat([pos, neg, pos, pos], dim=0)
 
 
 def _step_inputs(model: LTXModel, video_state: LatentState, audio_state: LatentState, contexts: dict,
@@ -1038,6 +1062,7 @@ def _step_inputs(model: LTXModel, video_state: LatentState, audio_state: LatentS
         perturbations=PerturbationTable.of(build_perturbation_config(
             cfg.num_layers, list(PASSES), list(v_params.stg_blocks), list(a_params.stg_blocks),
             video_state.latent.device, video_state.latent.dtype)),
+        v_keep=_passes_keep(contexts, "v"), a_keep=_passes_keep(contexts, "a"),
     )
 
 
@@ -1055,10 +1080,11 @@ def _denoise(model: LTXModel, video_state: LatentState, audio_state: LatentState
     # distinct levels times sigma are the same fp32 products
     video = Modality(latent=video_state.latent.repeat(n, 1, 1), sigma=sigma_b,
                      timesteps=c.v_mask * sigma_b.view(n, 1, 1), positions=c.v_pos, context=c.v_ctx,
-                     keyframes_mask=c.v_keyframes, timestep_rows=c.v_rows.scaled(sigma), rope_tables=c.v_rope)
+                     keyframes_mask=c.v_keyframes, timestep_rows=c.v_rows.scaled(sigma), rope_tables=c.v_rope,
+                     context_keep=c.v_keep)
     audio = Modality(latent=audio_state.latent.repeat(n, 1, 1), sigma=sigma_b,
                      timesteps=c.a_mask * sigma_b.view(n, 1, 1), positions=c.a_pos, context=c.a_ctx,
-                     timestep_rows=c.a_rows.scaled(sigma), rope_tables=c.a_rope)
+                     timestep_rows=c.a_rows.scaled(sigma), rope_tables=c.a_rope, context_keep=c.a_keep)
     vx, ax = model(video, audio, c.perturbations)
     kw = {} if step is None else {"sigma": step[0], "dt": step[1]}
     out = []

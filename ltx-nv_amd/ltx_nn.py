@@ -8,7 +8,8 @@ FeedForward.  RMSNorm, q/k norm + split RoPE, unmasked attention with the
 per-head gate, GELU-tanh, the linear layers of long K that `long_k_tiles` names
 and the projections of few rows (`project`) are ltxk kernels, with fp32
 arithmetic and one bf16 rounding per output.  The other linear layers, `sdpa` and
-masked attention are PyTorch-ROCm's.
+masked attention are PyTorch-ROCm's.  `quantize_fp8` turns the linear layers of
+attentions and feed-forwards into 8-bit ones (Fp8Linear), for inference.
 """
 
 import functools
@@ -494,7 +495,84 @@ def project(x: torch.Tensor, *layers: torch.nn.Linear | None) -> list:
             weights, biases = zip(*plain)
             done = iter(ltxk._launch_layers(x, weights, biases))
             return [None if layer is None else next(done) for layer in layers]
+    if sum(type(layer) is Fp8Linear for layer in real) > 1:
+        blocks = _fp8_input(x)  # quantised once for all of them
+        return [None if layer is None else layer(blocks) if type(layer) is Fp8Linear else linear(layer, x)
+                for layer in layers]
     return [None if layer is None else linear(layer, x) for layer in layers]
+
+
+def _fp8_input(x: torch.Tensor | ltxk.Fp8Blocks) -> ltxk.Fp8Blocks:
+    """x in blocks; refuses to lose a gradient."""
+    if isinstance(x, ltxk.Fp8Blocks):
+        return x
+    _no_gradient(x)
+    return ltxk.quantize_fp8(x.contiguous())
+
+
+def _no_gradient(x: torch.Tensor) -> None:
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("8-bit layers are for inference: they record no gradient (run under torch.no_grad())")
+
+
+class Fp8Linear(torch.nn.Module):
+    """A linear layer whose weight is held in blocks of 128 e4m3 values with a power-of-two
+    scale each (ltxk.Fp8Blocks), half the bytes of bf16 and a little over twice its rate on
+    the matrix cores.  Its input, bf16 or blocks already, is quantised the same way; the
+    output is bf16.  Inference only.  The values are kept as bytes, which `.to(dtype)` leaves
+    as they are."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, device=None):
+        super().__init__()
+        if in_features <= 0 or in_features % 8 or out_features <= 0 or out_features % 8:
+            raise ValueError(f"an 8-bit layer's widths are positive multiples of 8, got {in_features} and {out_features}")
+        self.in_features, self.out_features = in_features, out_features
+        blocks = -(-in_features // ltxk.FP8_BLOCK)
+        self.register_buffer("weight", torch.zeros(out_features, blocks * ltxk.FP8_BLOCK, dtype=torch.uint8, device=device))
+        self.register_buffer("weight_scale", torch.zeros(-(-blocks // ltxk.FP8_GROUP), out_features, ltxk.FP8_GROUP,
+                                                         dtype=torch.uint8, device=device))
+        self.register_buffer("bias", torch.zeros(out_features, dtype=torch.bfloat16, device=device) if bias else None)
+
+    @classmethod
+    def of(cls, layer: torch.nn.Linear) -> "Fp8Linear":
+        """An 8-bit layer from a bf16 one on the GPU."""
+        made = cls(layer.in_features, layer.out_features, layer.bias is not None, device=layer.weight.device)
+        blocks = ltxk.quantize_fp8(layer.weight.detach().contiguous())
+        made.weight, made.weight_scale = blocks.data.view(torch.uint8), blocks.scale
+        if layer.bias is not None:
+            made.bias = layer.bias.detach().clone()
+        return made
+
+    def blocks(self) -> ltxk.Fp8Blocks:
+        return ltxk.Fp8Blocks(self.weight.view(torch.float8_e4m3fn), self.weight_scale,
+                              (self.out_features, self.in_features))
+
+    def forward(self, x: torch.Tensor | ltxk.Fp8Blocks) -> torch.Tensor:
+        if not isinstance(x, ltxk.Fp8Blocks):
+            _no_gradient(x)
+            x = x.contiguous()
+        return ltxk.linear_fp8(x, self.blocks(), self.bias)
+
+    def gelu(self, x: torch.Tensor | ltxk.Fp8Blocks) -> ltxk.Fp8Blocks:
+        """GELU-tanh of the output, in blocks for a following 8-bit layer."""
+        if not isinstance(x, ltxk.Fp8Blocks):
+            _no_gradient(x)
+            x = x.contiguous()
+        return ltxk.linear_gelu_fp8(x, self.blocks(), self.bias)
+
+
+def quantize_fp8(module: torch.nn.Module) -> torch.nn.Module:
+    """Turns the query, key, value and output layers of every Attention in `module` and both layers of every
+    FeedForward into 8-bit ones, in place, and returns it: a model on the GPU in bf16, its weights loaded.  Norms,
+    modulations, gates (a few columns each), embeddings and the layers in front of and behind the blocks stay bf16."""
+    for part in list(module.modules()):
+        names = ("to_q", "to_k", "to_v", "to_out") if isinstance(part, Attention) else \
+            ("proj_in", "proj_out") if isinstance(part, FeedForward) else ()
+        for name in names:
+            layer = getattr(part, name)
+            if type(layer) is torch.nn.Linear and layer.in_features % 8 == 0 and layer.out_features % 8 == 0:
+                setattr(part, name, Fp8Linear.of(layer))
+    return module
 
 
 # ---------------------------------------------------------------------------
@@ -529,7 +607,9 @@ class Attention(torch.nn.Module):
     def forward(self, x: torch.Tensor, context: torch.Tensor | None = None, mask: torch.Tensor | None = None,
                 pe: tuple[torch.Tensor, torch.Tensor] | None = None,
                 k_pe: tuple[torch.Tensor, torch.Tensor] | None = None,
-                perturbation_mask: torch.Tensor | None = None, all_perturbed: bool = False) -> torch.Tensor:
+                perturbation_mask: torch.Tensor | None = None, all_perturbed: bool = False,
+                keep: torch.Tensor | None = None) -> torch.Tensor:
+        """keep (not in the reference): (B or 1, S) bool, the context tokens to attend to (`attend`)."""
         context = x if context is None else context
         h, dh = self.heads, self.dim_head
         if all_perturbed:
@@ -545,23 +625,36 @@ class Attention(torch.nn.Module):
         gates = gates.contiguous() if gates is not None else None
         ltxk.qk_norm_rope(q, k, h, dh, q_weight=self.q_norm.weight, k_weight=self.k_norm.weight,
                           q_pe=pe, k_pe=pe if k_pe is None else k_pe, eps=self.eps)
-        return self.attend(q, k, v, gates, mask, perturbation_mask)
+        return self.attend(q, k, v, gates, mask, perturbation_mask, keep)
 
     @property
     def eps(self) -> float:
         return self.q_norm.eps if self.q_norm.eps is not None else 1e-6
 
     def attend(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, gates: torch.Tensor | None,
-               mask: torch.Tensor | None = None, perturbation_mask: torch.Tensor | None = None) -> torch.Tensor:
+               mask: torch.Tensor | None = None, perturbation_mask: torch.Tensor | None = None,
+               keep: torch.Tensor | None = None) -> torch.Tensor:
         """The part of forward after q/k norm + RoPE (ltx_nn.py:219-236): attention
         on token-major q, k, v (B, T, H*Dh), the head merge [+ perturbation blend]
         [+ per-head gate], then to_out.  Without a mask and for heads of 64 or 128
         that is ltxk_attention with the gate inside it (the blend as an
         ltxk_head_gate pass after it); otherwise torch's SDPA, then ltxk_head_gate.
         Lets a caller prepare the q/k of two attentions in one launch (Block's
-        A2V/V2A)."""
+        A2V/V2A).  `keep`, which takes the place of a mask, names the tokens of k and v to
+        attend to, for contexts of different lengths in one padded batch: that is
+        ltxk_cross_attention, at the cost of the kept tokens alone (zeros where none is kept),
+        or torch's SDPA with it as a boolean mask for what fused_attention_applies excludes."""
         b = q.shape[0]
         h, dh = self.heads, self.dim_head
+        if keep is not None:
+            if mask is not None or perturbation_mask is not None:
+                raise ValueError("keep takes the place of a mask, and goes with no perturbation")
+            if keep.ndim != 2 or keep.shape[0] not in (1, b) or keep.shape[1] != k.shape[1]:
+                raise ValueError(f"keep {tuple(keep.shape)} must be ({b} or 1, {k.shape[1]})")
+            keep = (keep if keep.dtype == torch.bool else keep != 0).contiguous()
+            if fused_attention_applies(q, k, v, h, dh):
+                return linear(self.to_out, ltxk.cross_attention(q, k, v, h, keep, gates))
+            mask = keep[:, None, None, :]
         pm = None
         if perturbation_mask is not None:
             pm = perturbation_mask.reshape(-1).to(torch.bfloat16).contiguous()
@@ -601,7 +694,14 @@ class FeedForward(torch.nn.Module):
         self.proj_in = torch.nn.Linear(dim, inner, bias=bias)
         self.proj_out = torch.nn.Linear(inner, dim_out, bias=bias)
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    @property
+    def takes_blocks(self) -> bool:
+        """Both layers are 8-bit ones: the input may be ltxk.Fp8Blocks."""
+        return type(self.proj_in) is Fp8Linear and type(self.proj_out) is Fp8Linear
+
+    def forward(self, x: torch.Tensor | ltxk.Fp8Blocks) -> torch.Tensor:
+        if self.takes_blocks:  # the hidden values go from layer to layer in blocks
+            return self.proj_out(self.proj_in.gelu(x))
         hdn = linear(self.proj_in, x)
         ltxk.gelu_tanh(hdn, out=hdn)
         return linear(self.proj_out, hdn)
