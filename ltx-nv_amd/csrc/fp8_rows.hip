@@ -9,6 +9,8 @@ namespace ltxk {
 namespace {
 
 constexpr int kBlock = 256;
+constexpr int kPerCu = 3;   // workgroups a compute unit of the streaming form (2: 34 us, 4: 39 on [6144, 4096])
+constexpr int kItems = 64;  // most batch items that it walks
 
 // ------------------------------------------------------------ quantize_fp8 --
 // A wave takes 512 columns (four blocks, 16 lanes of 8 columns each) of a row.
@@ -104,6 +106,119 @@ __global__ void __launch_bounds__(kBlock) add_norm_kernel(NormParams p)
     }
 }
 
+// The same for modulations of one row per batch item: persistent workgroups walk the rows
+// of each item with the item's modulation in registers and the next row on its way while
+// one is reduced and written, up to 512 chunks a row (their registers).  With a residual, a
+// workgroup a row / this form, us: [6144, 4096] 53 / 34 (5.2 TB/s), [4290, 4096] 34 / 26, [3000,
+// 2048] 14 / 12, [1024, 4096] 11 / 11; 4 items of [504, 2048], fewer rows than workgroups, 11 / 13.
+template <int C, bool RESIDUAL>
+__global__ void __launch_bounds__(kBlock) add_norm_stream_kernel(NormParams p)
+{
+    __shared__ float lds[2][kBlock / 64];
+    const int lane = threadIdx.x;
+    const int rows = static_cast<int>(p.rows), tokens = static_cast<int>(p.tokens), G = static_cast<int>(gridDim.x);
+    const uint32_t bytes = static_cast<uint32_t>(p.dim) * 2;
+    int parity = 0;
+    for (int lo = 0; lo < rows; lo += tokens) {
+        const int hi = lo + tokens, at = lo % G, w = static_cast<int>(blockIdx.x);
+        int r = lo + (w >= at ? w - at : w - at + G);  // the first row of the item that is w modulo G
+        if (r >= hi) continue;
+        u32x4 cx[2][C], cf[2][C];
+        auto load = [&](int row, u32x4 (&x)[C], u32x4 (&f)[C]) __attribute__((always_inline)) {
+            const uint32_t range = row < hi ? bytes : 0;  // nothing is read past the item
+            const rsrc_t rx = make_rsrc(p.x + static_cast<int64_t>(row < hi ? row : lo) * p.dim, range);
+            const rsrc_t rf = make_rsrc((RESIDUAL ? p.f : p.x) + static_cast<int64_t>(row < hi ? row : lo) * p.dim, range);
+#pragma unroll
+            for (int k = 0; k < C; ++k) {
+                x[k] = ldb(rx, (lane + k * kBlock) * 16u);
+                if constexpr (RESIDUAL) f[k] = ldb(rf, (lane + k * kBlock) * 16u);
+            }
+        };
+        load(r, cx[0], cf[0]);
+        load(r + G, cx[1], cf[1]);
+        float gt[RESIDUAL ? C : 1][8], sh[C][8], sc[C][8];
+        const int64_t b = lo / tokens;
+#pragma unroll
+        for (int k = 0; k < C; ++k) {
+            const int col = (lane + k * kBlock) * 8;
+            const bool in = col < p.dim;
+            if constexpr (RESIDUAL) ada_load8(p.gate, b, 0, lo, in ? col : 0, 1.f, gt[k]);
+            ada_load8(p.shift, b, 0, lo, in ? col : 0, 0.f, sh[k]);
+            ada_load8(p.scale, b, 0, lo, in ? col : 0, 0.f, sc[k]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (!in) sh[k][j] = 0.f;  // the columns past the last are zeros (their x is)
+        }
+        const float m = RESIDUAL && p.mask ? bf16_to_f32(p.mask[b]) : 1.f;
+        auto step = [&](u32x4 (&x)[C], u32x4 (&f)[C]) __attribute__((always_inline)) {
+            float v[C][8], s2 = 0.f;
+            u32x4 out[C];
+#pragma unroll
+            for (int k = 0; k < C; ++k) {
+                unpack8v(x[k], v[k]);
+                if constexpr (RESIDUAL) {
+                    float fv[8];
+                    unpack8v(f[k], fv);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[k][j] += fv[j] * gt[k][j] * m;
+                    out[k] = pack8v(v[k]);
+                    unpack8v(out[k], v[k]);  // the norm sees the rounded residual
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) s2 = __builtin_fmaf(v[k][j], v[k][j], s2);
+            }
+            load(r + 2 * G, x, f);
+            if constexpr (RESIDUAL) {
+                const rsrc_t rx = make_rsrc(p.x_out + static_cast<int64_t>(r) * p.dim, bytes);
+#pragma unroll
+                for (int k = 0; k < C; ++k) stb(rx, (lane + k * kBlock) * 16u, out[k]);
+            }
+            s2 = wave_sum64(s2);
+            if ((lane & 63) == 0) lds[parity][lane >> 6] = s2;
+            __syncthreads();
+            s2 = (lds[parity][0] + lds[parity][1]) + (lds[parity][2] + lds[parity][3]);
+            parity ^= 1;  // the other row's sums go elsewhere, so that one barrier a row is enough
+            const float rs = rsqrtf(s2 / static_cast<float>(p.dim) + p.eps);
+#pragma unroll
+            for (int k = 0; k < C; ++k) {
+                const int col = (lane + k * kBlock) * 8;
+                float o[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) o[j] = v[k][j] * rs * (1.f + sc[k][j]) + sh[k][j];
+                uint32_t scale;
+                const uint2 q = fp8_quantize8(o, scale);
+                if (col < p.kp) *reinterpret_cast<uint2 *>(p.q + static_cast<int64_t>(r) * p.kp + col) = q;
+                const int block = col / kFp8Block;
+                if ((lane & 15) == 0 && block < (p.blocks + 3) / 4 * 4)
+                    p.q_scale[(static_cast<int64_t>(block / kFp8Group) * p.rows + r) * kFp8Group + block % kFp8Group] =
+                        static_cast<uint8_t>(scale);
+            }
+            r += G;
+            return r < hi;
+        };
+        while (step(cx[0], cf[0]) && step(cx[1], cf[1])) {
+        }
+    }
+}
+
+template <int C>
+void launch_norm(const NormParams &p, hipStream_t s)
+{
+    bool broadcast = true;
+    for (const Ada *a : {&p.gate, &p.shift, &p.scale}) broadcast &= !(a->emb && (a->ts != 0 || a->idx));
+    if constexpr (C <= 2) {
+        const int64_t grid = static_cast<int64_t>(device_cus()) * kPerCu;
+        if (broadcast && p.rows / p.tokens <= kItems && p.tokens > grid) {
+            if (p.f)
+                add_norm_stream_kernel<C, true><<<static_cast<unsigned>(grid), kBlock, 0, s>>>(p);
+            else
+                add_norm_stream_kernel<C, false><<<static_cast<unsigned>(grid), kBlock, 0, s>>>(p);
+            return;
+        }
+    }
+    add_norm_kernel<C><<<static_cast<unsigned>(p.rows), kBlock, 0, s>>>(p);
+}
+
 }  // namespace
 }  // namespace ltxk
 
@@ -171,15 +286,14 @@ extern "C" int ltxk_add_norm_modulate_fp8(void *x_out, void *q, void *q_scale, c
     p.q_scale = static_cast<uint8_t *>(q_scale);
     p.eps = eps;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const unsigned grid = static_cast<unsigned>(rows);
     const int chunks = static_cast<int>(fp8_groups(dim)) * 64;  // a row's threads, the last group's padding too
     if (chunks <= kBlock)
-        add_norm_kernel<1><<<grid, kBlock, 0, s>>>(p);
+        launch_norm<1>(p, s);
     else if (chunks <= 2 * kBlock)
-        add_norm_kernel<2><<<grid, kBlock, 0, s>>>(p);
+        launch_norm<2>(p, s);
     else if (chunks <= 4 * kBlock)
-        add_norm_kernel<4><<<grid, kBlock, 0, s>>>(p);
+        launch_norm<4>(p, s);
     else
-        add_norm_kernel<8><<<grid, kBlock, 0, s>>>(p);
+        launch_norm<8>(p, s);
     return check_launch(what);
 }
