@@ -216,7 +216,8 @@ def test_linear_gelu_matches_fp64(m, n, k, bias):
 
 
 @pytest.mark.parametrize("batch,tokens,dim", [(1, 1, 8), (2, 3, 128), (1, 7, 200), (2, 65, 2048), (1, 130, 4096), (3, 5, 4104),
-                                              (1, 4, 8192), (1, 3, 16384), (2, 9, 640)])
+                                              (1, 4, 8192), (1, 3, 16384), (2, 9, 640), (2, 1601, 264),
+                                              (1, 900, 2056), (3, 800, 4096)])
 @pytest.mark.parametrize("form", ["plain", "residual", "gated", "masked", "indexed", "tokens"])
 def test_add_norm_modulate_fp8(batch, tokens, dim, form):
     """x' equals add_norm_modulate's bit for bit; the blocks hold the fp64 norm of it to within
