@@ -460,6 +460,32 @@ __device__ __forceinline__ void widen(const uint2 &v, float f[4])
     f[3] = __uint_as_float(v.y & 0xffff0000u);
 }
 
+// A 32 x 32 tile whose lane l holds, of row l % 32, columns 8 q + 4 (l / 32) .. + 3 in v[q]: lanes l
+// and l + 32, then l and l + 16, swap, so that lane l holds columns 8 (l / 32) + (l & 16) .. + 7 of
+// rows l % 16 (lo) and l % 16 + 16 (hi): a store of 16 rows of 32 columns each (of 32 rows of 16:
+// 309 against 302 us on [24576, 4096] x 4096).
+__device__ __forceinline__ void rows16(const uint32_t v[4][2], u32x4 &lo, u32x4 &hi)
+{
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const auto first = __builtin_amdgcn_permlane32_swap(v[0][e], v[1][e], false, false);
+        const auto second = __builtin_amdgcn_permlane32_swap(v[2][e], v[3][e], false, false);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const auto rows = __builtin_amdgcn_permlane16_swap(first[i], second[i], false, false);
+            lo[2 * i + e] = rows[0], hi[2 * i + e] = rows[1];
+        }
+    }
+}
+__device__ __forceinline__ void rows16(const uint32_t v[4], uint2 &lo, uint2 &hi)
+{
+    const auto first = __builtin_amdgcn_permlane32_swap(v[0], v[1], false, false);
+    const auto second = __builtin_amdgcn_permlane32_swap(v[2], v[3], false, false);
+    const auto a = __builtin_amdgcn_permlane16_swap(first[0], second[0], false, false);
+    const auto b = __builtin_amdgcn_permlane16_swap(first[1], second[1], false, false);
+    lo = make_uint2(a[0], b[0]), hi = make_uint2(a[1], b[1]);
+}
+
 template <bool GELU>
 __global__ void __launch_bounds__(kBigWaves * 64, 1) big_kernel(Fp8Params p)
 {
@@ -478,12 +504,14 @@ __global__ void __launch_bounds__(kBigWaves * 64, 1) big_kernel(Fp8Params p)
     // 64 wave .. of x's scales and of w's.  Rows past the last repeat it; their results
     // are not stored.
     uint32_t at[kBigLoads], at_s[2];
+    const int first_row = wave * 8 + (lane >> 3);
+    const uint32_t chunk = chunk_pos(first_row, lane & 7) * 16;  // the same 32 rows on
     auto address = [&](const Unit &u) {
 #pragma unroll
         for (int c = 0; c < kBigLoads; ++c) {
-            const int row = (c * kBigWaves + wave) * 8 + (lane >> 3);
+            const int row = first_row + c * kBigWaves * 8;
             const int r = c * kBigWaves * 8 < kBig ? min(u.m0 + row, p.m - 1) : min(u.n0 + row - kBig, p.n - 1);
-            at[c] = static_cast<uint32_t>(r) * static_cast<uint32_t>(p.kp) + chunk_pos(row, lane & 7) * 16;
+            at[c] = static_cast<uint32_t>(r) * static_cast<uint32_t>(p.kp) + chunk;
         }
         at_s[0] = static_cast<uint32_t>(min(u.m0 + wave * 64 + lane, p.m - 1)) * 4;
         at_s[1] = static_cast<uint32_t>(min(u.n0 + wave * 64 + lane, p.n - 1)) * 4;
@@ -652,19 +680,8 @@ __global__ void __launch_bounds__(kBigWaves * 64, 1) big_kernel(Fp8Params p)
                         v[q][0] = pack_bf16x2(f[0], f[1]);
                         v[q][1] = pack_bf16x2(f[2], f[3]);
                     }
-                    // lanes l and l + 32, then l and l + 16, swap: 16 rows of 32 columns a store,
-                    // 64 bytes a row (32 rows of 16: 309 against 302 us on [24576, 4096] x 4096)
                     u32x4 lo, hi;
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const auto first = __builtin_amdgcn_permlane32_swap(v[0][e], v[1][e], false, false);
-                        const auto second = __builtin_amdgcn_permlane32_swap(v[2][e], v[3][e], false, false);
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const auto rows = __builtin_amdgcn_permlane16_swap(first[i], second[i], false, false);
-                            lo[2 * i + e] = rows[0], hi[2 * i + e] = rows[1];
-                        }
-                    }
+                    rows16(v, lo, hi);
                     const int row = m0 + mi * 32 + (lane & 15), col = n0 + ni * 32 + 8 * half + (lane & 16);
                     if (row < p.m && col < p.n)
                         *reinterpret_cast<u32x4 *>(p.y + static_cast<int64_t>(row) * p.n + col) = lo;
@@ -675,26 +692,35 @@ __global__ void __launch_bounds__(kBigWaves * 64, 1) big_kernel(Fp8Params p)
         } else {
             // GELU, and each row's 128 columns, a block
             const int block = n0 / kFp8Block, last = p.np / kFp8Block - 1;
+            uint2 bias[NT][4];
+#pragma unroll
+            for (int ni = 0; ni < NT; ++ni)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) bias[ni][q] = bias4(p, n0 + ni * 32 + 8 * q + 4 * half);
 #pragma unroll
             for (int mi = 0; mi < MT; ++mi) {
                 float g[NT][16], top = 0.f;
-                bool bad = false;
 #pragma unroll
                 for (int ni = 0; ni < NT; ++ni)
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        const int col = n0 + ni * 32 + 8 * q + 4 * half;
                         float b[4];
-                        widen(bias4(p, col), b);
+                        widen(bias[ni][q], b);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float v = gelu(taken(acc[mi][ni][4 * q + e]) + b[e]);
-                            g[ni][4 * q + e] = col < p.n ? v : 0.f;
-                            bad |= v != v;
-                            top = fmaxf(top, fabsf(g[ni][4 * q + e]));
-                        }
+                        for (int e = 0; e < 4; ++e) g[ni][4 * q + e] = gelu(taken(acc[mi][ni][4 * q + e]) + b[e]);
                     }
-                const uint32_t t = bad ? 0x7fffffffu : __float_as_uint(top);
+                if (n0 + 128 > p.n)  // past the last column zeros
+#pragma unroll
+                    for (int ni = 0; ni < NT; ++ni)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+                            if (n0 + ni * 32 + 8 * (r >> 2) + 4 * half >= p.n) g[ni][r] = 0.f;
+                // a NaN does not count in the maximum, and stays one by itself
+#pragma unroll
+                for (int ni = 0; ni < NT; ++ni)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(g[ni][r]));
+                const uint32_t t = __float_as_uint(top);
                 const auto both = __builtin_amdgcn_permlane32_swap(t, t, false, false);
                 const uint32_t scale = fp8_scale(max(static_cast<uint32_t>(both[0]), static_cast<uint32_t>(both[1])));
                 const float inv = fp8_inverse(scale == 255 ? 127 : scale);
@@ -706,16 +732,12 @@ __global__ void __launch_bounds__(kBigWaves * 64, 1) big_kernel(Fp8Params p)
                         const float *f = &g[ni][4 * q];
                         v[q] = scale == 255 ? 0x7f7f7f7fu : fp8_pack4(f[0], f[1], f[2], f[3], inv);
                     }
-                    // as above: 16 rows of 32 columns a store
-                    const auto first = __builtin_amdgcn_permlane32_swap(v[0], v[1], false, false);
-                    const auto second = __builtin_amdgcn_permlane32_swap(v[2], v[3], false, false);
-                    const auto lo = __builtin_amdgcn_permlane16_swap(first[0], second[0], false, false);
-                    const auto hi = __builtin_amdgcn_permlane16_swap(first[1], second[1], false, false);
+                    uint2 lo, hi;
+                    rows16(v, lo, hi);
                     const int row = m0 + mi * 32 + (lane & 15), col = n0 + ni * 32 + 8 * half + (lane & 16);
-                    if (row < p.m && block <= last)
-                        *reinterpret_cast<uint2 *>(p.q + static_cast<int64_t>(row) * p.np + col) = make_uint2(lo[0], hi[0]);
+                    if (row < p.m && block <= last) *reinterpret_cast<uint2 *>(p.q + static_cast<int64_t>(row) * p.np + col) = lo;
                     if (row + 16 < p.m && block <= last)
-                        *reinterpret_cast<uint2 *>(p.q + static_cast<int64_t>(row + 16) * p.np + col) = make_uint2(lo[1], hi[1]);
+                        *reinterpret_cast<uint2 *>(p.q + static_cast<int64_t>(row + 16) * p.np + col) = hi;
                 }
                 const int row = m0 + mi * 32 + l32;
                 const bool in = row < p.m && block <= last;
