@@ -503,7 +503,13 @@ struct FlashCut {
     int64_t q_tiles, tiles, whole, rest, parts;
 };
 
-FlashCut cut(int64_t bh, int64_t tokens_q, int64_t tokens_k)
+// ltxk_cross_attention leaves keys of fewer than kLeastCut tiles whole: the second launch and
+// the fp32 sums take longer than what idles.  126 queries, 4 batch items, 32 heads, us, in two
+// parts / whole: of 64, 512 keys 15 / 12, 1024 22 / 21 (half of them kept 18 / 13); of 128, 1024 30 / 28
+// (25 / 18).
+constexpr int64_t kLeastCut = 24;
+
+FlashCut cut(int64_t bh, int64_t tokens_q, int64_t tokens_k, int64_t least = 0)
 {
     FlashCut c;
     c.q_tiles = (tokens_q + kRows - 1) / kRows;
@@ -511,7 +517,7 @@ FlashCut cut(int64_t bh, int64_t tokens_q, int64_t tokens_k)
     const int64_t all = (bh + 7) / 8 * c.q_tiles;
     c.rest = all % 64;
     c.parts = 1;
-    while (c.parts < 16 && c.rest * c.parts * 2 <= 64 && c.tiles >= c.parts * 2 * 4) c.parts *= 2;
+    while (c.tiles >= least && c.parts < 16 && c.rest * c.parts * 2 <= 64 && c.tiles >= c.parts * 2 * 4) c.parts *= 2;
     if (c.parts == 1) c.rest = 0;
     c.whole = all - c.rest;
     return c;
@@ -559,17 +565,21 @@ int64_t list_bytes(int64_t batch, int64_t tokens_k)
 
 using namespace ltxk;
 
+static int64_t sums_bytes(const FlashCut &c, int64_t head_dim)
+{
+    return 8 * c.rest * c.parts * kRows * (head_dim + 2) * 4;
+}
+
 extern "C" int64_t ltxk_attention_workspace_bytes(int64_t batch, int64_t tokens_q, int64_t tokens_k, int64_t heads,
                                                   int64_t head_dim)
 {
     if (batch <= 0 || tokens_q <= 0 || tokens_k <= 0 || heads <= 0 || head_dim <= 0) return 0;
-    const FlashCut c = cut(batch * heads, tokens_q, tokens_k);
-    return 8 * c.rest * c.parts * kRows * (head_dim + 2) * 4;
+    return sums_bytes(cut(batch * heads, tokens_q, tokens_k), head_dim);
 }
 
 // The checks and the launch of both entry points; `lists` bytes of the workspace are
 // for the kept keys' list.
-static int attend(const char *what, bool round, int64_t lists, void *out, const void *q, int64_t q_bstride, int64_t q_tstride, const void *k,
+static int attend(const char *what, bool round, int64_t least, int64_t lists, void *out, const void *q, int64_t q_bstride, int64_t q_tstride, const void *k,
                   int64_t k_bstride, int64_t k_tstride, const void *v, int64_t v_bstride, int64_t v_tstride,
                   const void *keep, int64_t keep_bstride, const void *logits, int64_t batch, int64_t tokens_q,
                   int64_t tokens_k, int64_t heads, int64_t head_dim, float scale, void *workspace,
@@ -601,13 +611,13 @@ static int attend(const char *what, bool round, int64_t lists, void *out, const 
     if (q_tstride > kMax / 2 || tokens_q > kMax - 256 || (tokens_k + kKeys) > kMax / 2 / k_tstride ||
         (tokens_k + kKeys) > kMax / 2 / v_tstride)
         return fail(LTXK_E_ARG, "%s: a batch item's keys or values span 2^31 bytes or more", what);
-    const FlashCut c = cut(batch * heads, tokens_q, tokens_k);
+    const FlashCut c = cut(batch * heads, tokens_q, tokens_k, least);
     // a launch holds fewer than 2^32 threads
     if (c.whole + c.rest * c.parts >= (int64_t{1} << 32) / (8 * kWaves * 64))
         return fail(LTXK_E_ARG, "%s: too many query tiles", what);
     if ((c.rest || lists) &&
         (!workspace || !aligned16(workspace) ||
-         workspace_bytes < lists + ltxk_attention_workspace_bytes(batch, tokens_q, tokens_k, heads, head_dim)))
+         workspace_bytes < lists + sums_bytes(c, head_dim)))
         return fail(LTXK_E_ARG, "%s: the workspace must hold ltxk_%s_workspace_bytes, 16-byte aligned", what, what);
     FlashParams p{};
     p.q = static_cast<const uint16_t *>(q);
@@ -659,7 +669,7 @@ extern "C" int ltxk_attention(void *out, const void *q, int64_t q_bstride, int64
                               int64_t tokens_k, int64_t heads, int64_t head_dim, float scale, void *workspace,
                               int64_t workspace_bytes, void *stream)
 {
-    return attend("attention", true, 0, out, q, q_bstride, q_tstride, k, k_bstride, k_tstride, v, v_bstride, v_tstride, nullptr,
+    return attend("attention", true, 0, 0, out, q, q_bstride, q_tstride, k, k_bstride, k_tstride, v, v_bstride, v_tstride, nullptr,
                   0, logits, batch, tokens_q, tokens_k, heads, head_dim, scale, workspace, workspace_bytes, stream);
 }
 
@@ -667,7 +677,7 @@ extern "C" int64_t ltxk_cross_attention_workspace_bytes(int64_t batch, int64_t t
                                                         int64_t heads, int64_t head_dim)
 {
     if (batch <= 0 || tokens_q <= 0 || tokens_k <= 0 || heads <= 0 || head_dim <= 0) return 0;
-    return list_bytes(batch, tokens_k) + ltxk_attention_workspace_bytes(batch, tokens_q, tokens_k, heads, head_dim);
+    return list_bytes(batch, tokens_k) + sums_bytes(cut(batch * heads, tokens_q, tokens_k, kLeastCut), head_dim);
 }
 
 extern "C" int ltxk_cross_attention(void *out, const void *q, int64_t q_bstride, int64_t q_tstride, const void *k,
@@ -682,7 +692,7 @@ extern "C" int ltxk_cross_attention(void *out, const void *q, int64_t q_bstride,
     // the list's size once batch and tokens_k are known to be in range
     const int64_t lists = batch > 0 && batch <= (1 << 20) && tokens_k > 0 && tokens_k < 0x7fffffff
                               ? list_bytes(batch, tokens_k) : 0;
-    return attend(what, false, lists, out, q, q_bstride, q_tstride, k, k_bstride, k_tstride, v, v_bstride, v_tstride, keep,
+    return attend(what, false, kLeastCut, lists, out, q, q_bstride, q_tstride, k, k_bstride, k_tstride, v, v_bstride, v_tstride, keep,
                   keep_bstride, logits, batch, tokens_q, tokens_k, heads, head_dim, scale, workspace, workspace_bytes,
                   stream);
 }

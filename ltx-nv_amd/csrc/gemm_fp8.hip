@@ -1044,13 +1044,15 @@ void few_rows(const Fp8Params &p, bool gelu, hipStream_t s)
 
 // The kernel that a product takes, and how it is cut over K.
 //
-// Few rows: up to 32, and outputs of at most 256 tiles of 64 x 64, one a compute unit (tiles of
-// 64 x 32 where there are at most 128).  Cold operands, this kernel / 128 x 128 tiles, us, M x N x
-// K: 126 x 2048 x 2048 7 / 15, 126 x 8192 x 2048 11 / 19, 504 x 2048 x 8192 21 / 25, 256 x 4096 x
-// 4096 15 / 22;  512 tiles, 512 x 4096 x 4096 25 / 25;  1024, 504 x 8192 x 2048 32 / 17.
+// Few rows: up to 32, and outputs of at most 256 tiles of 64 x 64, one a compute unit; tiles of 64 x
+// 32, or 32 x 32, where those are at most 256, too.  Cold operands, this kernel / 128 x 128 tiles, us,
+// M x N x K: 126 x 2048 x 2048 6 / 15, 126 x 2048 x 8192 13 / 19, 126 x 8192 x 2048 11 / 19, 504 x
+// 2048 x 8192 21 / 25, 256 x 4096 x 4096 15 / 22;  512 tiles, 512 x 4096 x 4096 25 / 25;  1024, 504 x
+// 8192 x 2048 32 / 17.  32 x 32 / 64 x 32 / 64 x 64 tiles: 126 x 2048 x 2048 6 / 7 / 9, 252 x 2048 x
+// 2048 - / 7 / 9.
 // K is cut from 128 blocks on where the tiles leave units idle, into parts of at least 16; the
 // second launch costs 5 us: 1 x 1024 x 16384 19 us whole, 12 in 8 parts; 126 x 1024 x 16384 28 and
-// 17; 126 x 2048 x 8192 17 and 17.
+// 17; 16 x 4096 x 16384 25 and 26.
 struct Cut {
     int tile;  // rows of x and of w; few rows: 32, 48 (64 and 32) and 64
     int64_t tiles_m, tiles_n, whole, rest, parts;
@@ -1062,7 +1064,7 @@ Cut cut(int64_t m, int64_t n, int64_t k)
     const int64_t blocks = fp8_blocks(k), tiles64 = (m + 63) / 64 * ((n + 63) / 64);
     c.parts = 1;
     if (m <= 32 || tiles64 <= 256) {
-        const int mt = m <= 32 ? 1 : 2, nt = m <= 32 || tiles64 <= 128 ? 1 : 2;
+        const int mt = m <= 32 || tiles64 <= 64 ? 1 : 2, nt = m <= 32 || tiles64 <= 128 ? 1 : 2;
         c.tile = 16 * (mt + nt);
         c.tiles_m = (m + 32 * mt - 1) / (32 * mt);
         c.tiles_n = (n + 32 * nt - 1) / (32 * nt);
