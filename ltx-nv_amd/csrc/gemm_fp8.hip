@@ -94,23 +94,6 @@ __device__ __forceinline__ u32x4 whole_memory(const void *base)
 
 constexpr int kBand = 4;  // tiles of x that a band of the tile order holds
 
-// A workgroup's tile: SIZE rows of x and as many of w, WM x WN waves.  Steps of 128 values
-// are held in LDS, the first DEEP of a wave's loads for a step (rows of x first, then of
-// w) RD steps deep, the others RS.
-template <int SIZE, int WM_, int WN_, int DEEP, int RD_, int RS_>
-struct Tile {
-    static constexpr int size = SIZE;
-    static constexpr int WM = WM_, WN = WN_, waves = WM * WN;
-    static constexpr int MT = SIZE / WM / 32, NT = SIZE / WN / 32;  // 32-row tiles of a wave
-    static constexpr int L = 2 * SIZE / 8 / waves, LD = DEEP, LS = L - LD;  // loads of a wave for a step
-    static constexpr int RD = RD_, RS = RS_;
-    static constexpr int deep_rows = LD * waves * 8, deep_bytes = LD * waves * 1024, shallow_bytes = LS * waves * 1024;
-    static constexpr int shallow_at = RD * deep_bytes, scale_at = shallow_at + RS * shallow_bytes;
-    static constexpr int lds = scale_at + 4 * SIZE * 4;  // two groups' scales of x and w
-    static_assert(LS == 0 ? RS == RD : RS == 2 && RD == 3, "the waits below");
-    static_assert(deep_rows % (MT * 32) == 0 && (deep_rows <= SIZE || LS == 0), "a wave's rows of x have one depth");
-};
-
 // The rows of x and w that tile t takes: bands kBand tiles of x deep.
 template <int TILE>
 __device__ __forceinline__ void tile_rows(const Fp8Params &p, int t, int &m0, int &n0)
@@ -121,11 +104,16 @@ __device__ __forceinline__ void tile_rows(const Fp8Params &p, int t, int &m0, in
     n0 = at / deep * TILE;
 }
 
-template <typename T, bool GELU>
-__global__ void __launch_bounds__(T::waves * 64, T::waves / 4) tile_kernel(Fp8Params p)
+// 128 x 128 tiles, four waves of 64 x 64, the steps of 128 values four deep in LDS.
+constexpr int kTile = 128, kTileWaves = 4, kTileRing = 4, kTileLoads = 2 * kTile / 8 / kTileWaves;
+constexpr int kTileStep = 2 * kTile * 128, kTileScalesAt = kTileRing * kTileStep;
+constexpr int kTileLds = kTileScalesAt + 2 * 2 * kTile * 4;  // and two groups' scales
+
+template <bool GELU>
+__global__ void __launch_bounds__(kTileWaves * 64, 1) tile_kernel(Fp8Params p)
 {
-    constexpr int MT = T::MT, NT = T::NT, L = T::L, LD = T::LD, LS = T::LS, RD = T::RD, RS = T::RS, TILE = T::size;
-    __shared__ __attribute__((aligned(1024))) char smem[T::lds];
+    constexpr int MT = 2, NT = 2;
+    __shared__ __attribute__((aligned(1024))) char smem[kTileLds];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int l32 = lane & 31, half = lane >> 5;
 
@@ -136,69 +124,56 @@ __global__ void __launch_bounds__(T::waves * 64, T::waves / 4) tile_kernel(Fp8Pa
     if (j < whole_per) {
         tile = xcd * whole_per + j;
     } else {
-        const int per = (p.rest * p.parts + 7) >> 3, unit = xcd * per + j - whole_per;
-        if (j - whole_per >= per || unit >= p.rest * p.parts) return;
+        const int unit = xcd * p.per + j - whole_per;
+        if (unit >= p.rest * p.parts) return;
         part = p.parts == 1 ? -1 : unit / p.rest;
         tile = p.whole + unit % p.rest;
     }
     int m0, n0;
-    tile_rows<TILE>(p, tile, m0, n0);
+    tile_rows<kTile>(p, tile, m0, n0);
     // parts * blocks stays below 2^32: 256 parts at most of fewer than 2^24 blocks
     auto from = [&](int i) { return static_cast<int>(static_cast<uint32_t>(i) * p.blocks / static_cast<uint32_t>(p.parts)); };
     const int first = part < 0 ? 0 : from(part), n = (part < 0 ? p.blocks : from(part + 1)) - first;
 
     const u32x4 xr = whole_memory(p.x), wr = whole_memory(p.w);
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char *)smem));
-    // Load c of a step: rows (c * waves + wave) * 8 .. + 7 of the tile's x and w together.
+    // Load c of a step: rows (4 c + wave) * 8 .. + 7 of the tile's x and w together.
     // Rows past the last repeat it; their results are not stored.
-    uint32_t at[L];
+    uint32_t at[kTileLoads];
 #pragma unroll
-    for (int c = 0; c < L; ++c) {
-        const int row = (c * T::waves + wave) * 8 + (lane >> 3);
-        const bool is_x = c * T::waves * 8 < TILE;
-        at[c] = static_cast<uint32_t>(is_x ? min(m0 + row, p.m - 1) : min(n0 + row - TILE, p.n - 1)) *
+    for (int c = 0; c < kTileLoads; ++c) {
+        const int row = (c * kTileWaves + wave) * 8 + (lane >> 3);
+        const bool is_x = c * kTileWaves * 8 < kTile;
+        at[c] = static_cast<uint32_t>(is_x ? min(m0 + row, p.m - 1) : min(n0 + row - kTile, p.n - 1)) *
                     static_cast<uint32_t>(p.kp) + chunk_pos(row, lane & 7) * 16;
     }
-    // Scales, 64 rows a load: x's first, then w's.
-    constexpr int kScaleLoads = 2 * TILE / 64 / T::waves;
-    static_assert(kScaleLoads * T::waves * 64 == 2 * TILE && TILE / 64 % kScaleLoads == 0, "a wave loads x's or w's");
-    const bool sx = wave * kScaleLoads < TILE / 64;
+    // Scales, 64 rows a wave: x's first, then w's.
+    const bool sx = wave < 2;
     const u32x4 sr = whole_memory(sx ? p.xs : p.ws);
     const int s_rows = sx ? p.m : p.n;
-    uint32_t so[kScaleLoads];
-#pragma unroll
-    for (int c = 0; c < kScaleLoads; ++c)
-        so[c] = static_cast<uint32_t>(min((sx ? m0 : n0 - TILE) + (wave * kScaleLoads + c) * 64 + lane, s_rows - 1)) * 4;
+    const uint32_t so = static_cast<uint32_t>(min((sx ? m0 : n0 - kTile) + wave * 64 + lane, s_rows - 1)) * 4;
     const int groups = (p.blocks + 3) >> 2;
     // A group's scales, into its half of their place; past the last group the last one's, which nothing reads.
     auto load_scales = [&](int group) {
-#pragma unroll
-        for (int c = 0; c < kScaleLoads; ++c)
-            load_lds4(sr, __builtin_amdgcn_readfirstlane(lds0 + T::scale_at + (group & 1) * (2 * TILE * 4) +
-                                                         (wave * kScaleLoads + c) * 256), so[c],
-                      __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(min(group, groups - 1)) * s_rows * 4));
+        load_lds4(sr, __builtin_amdgcn_readfirstlane(lds0 + kTileScalesAt + (group & 1) * (2 * kTile * 4) + wave * 256), so,
+                  __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(min(group, groups - 1)) * s_rows * 4));
     };
-    // Load c of step i, into place `slot` of its ring.
+    // Load c of step i, into place `slot` of the ring.
     auto load = [&](int i, int c, int slot) {
-        const int to = c < LD ? slot * T::deep_bytes + c * T::waves * 1024
-                              : T::shallow_at + slot * T::shallow_bytes + (c - LD) * T::waves * 1024;
-        load_lds16(c * T::waves * 8 < TILE ? xr : wr, __builtin_amdgcn_readfirstlane(lds0 + to + wave * 1024), at[c],
+        load_lds16(c * kTileWaves * 8 < kTile ? xr : wr,
+                   __builtin_amdgcn_readfirstlane(lds0 + slot * kTileStep + (c * kTileWaves + wave) * 1024), at[c],
                    __builtin_amdgcn_readfirstlane((first + i) * kFp8Block));
     };
     load_scales(first >> 2);
     load_scales((first >> 2) + 1);
-    for (int i = 0; i < RD && i < n; ++i) {
-        if (i < RS)
+    for (int i = 0; i < kTileRing && i < n; ++i)
 #pragma unroll
-            for (int c = LD; c < L; ++c) load(i, c, i);
-#pragma unroll
-        for (int c = 0; c < LD; ++c) load(i, c, i);
-    }
+        for (int c = 0; c < kTileLoads; ++c) load(i, c, i);
 
     int off[4];
 #pragma unroll
     for (int s = 0; s < 4; ++s) off[s] = l32 * 128 + chunk_pos(l32, 2 * s + half) * 16;
-    const int wm = wave / T::WN * (MT * 32), wn = wave % T::WN * (NT * 32);  // this wave's rows
+    const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;  // this wave's rows
 
     // acc[i][j]: lane l holds row 32 i + l % 32 of x; register r row 32 j + 8 (r/4) + 4 half + r % 4 of w
     f32x16 acc[MT][NT] = {};
@@ -212,16 +187,11 @@ __global__ void __launch_bounds__(T::waves * 64, T::waves / 4) tile_kernel(Fp8Pa
         const i32x4 *hi = reinterpret_cast<const i32x4 *>(smem + base + off[2 * s + 1]);
         return cat(*lo, *hi);
     };
-    // This wave's rows of x and w in LDS, by the places of a step in the two rings
-    auto rows_at = [&](int row, int deep, int shallow) {
-        return row < T::deep_rows ? deep * T::deep_bytes + row * 128
-                                  : T::shallow_at + shallow * T::shallow_bytes + (row - T::deep_rows) * 128;
-    };
     auto read_x = [&](int base, int s, int t) { xf[s][t] = fragment(base + t * 4096, s); };
     auto read_w = [&](int base, int s, int t) { wf[t] = fragment(base + t * 4096, s); };
-    const int scale_row = T::scale_at + (wm + l32) * 4, scale_row_w = T::scale_at + (TILE + wn + l32) * 4;
+    const int scale_row = kTileScalesAt + (wm + l32) * 4, scale_row_w = kTileScalesAt + (kTile + wn + l32) * 4;
     auto read_scales = [&](int abs) {
-        const char *at = smem + (abs >> 2 & 1) * (2 * TILE * 4) + (abs & 3);
+        const char *at = smem + (abs >> 2 & 1) * (2 * kTile * 4) + (abs & 3);
 #pragma unroll
         for (int t = 0; t < MT; ++t) xs_next[t] = *reinterpret_cast<const uint8_t *>(at + scale_row + t * 128);
 #pragma unroll
@@ -229,24 +199,24 @@ __global__ void __launch_bounds__(T::waves * 64, T::waves / 4) tile_kernel(Fp8Pa
     };
 
     // Loads that may be in flight when a step has to be there: those issued after its last
-    constexpr int kNewer = (RS - 2) * L + (RD - RS) * LD;
-    step_barrier<kNewer + L>(n >= RD);
+    constexpr int kNewer = (kTileRing - 2) * kTileLoads;
+    step_barrier<kNewer + kTileLoads>(n >= kTileRing);
     read_scales(first);
-    int deep = 0, shallow = 0, x_at = rows_at(wm, 0, 0), w_at = rows_at(TILE + wn, 0, 0);
+    int slot = 0, x_at = wm * 128, w_at = (kTile + wn) * 128;  // this step's place, and this wave's rows there
 #pragma unroll
     for (int t = 0; t < MT; ++t) read_x(x_at, 0, t);
 #pragma unroll
     for (int t = 0; t < kEarly; ++t) read_w(w_at, 0, t);
 
-    // Step i, without a branch inside (the compiler would move the products past it).  Between
-    // its products are the loads of steps i + RS (with `near`) and i + RD (with `far`).
-    auto step = [&](int i, auto near, auto far) __attribute__((always_inline)) {
+    // Step i, without a branch inside (the compiler would move the products past it).  With
+    // `more`, the loads of the step that takes its place are between its products.
+    auto step = [&](int i, auto more) __attribute__((always_inline)) {
         // Products before the turn: beside one each the second half of this half step's w is
         // read, the last one covers those reads.  Past it the next half step's x and first half of w.
         constexpr int kProducts = MT * NT, kTurn = NT - kEarly + 1, kSlots = kProducts - kTurn;
-        constexpr int kReads = (MT + kEarly + kSlots - 1) / kSlots, kLoads = (L + kSlots - 1) / kSlots;
-        const int deep_next = deep + 1 == RD ? 0 : deep + 1, shallow_next = shallow + 1 == RS ? 0 : shallow + 1;
-        const int x_next = rows_at(wm, deep_next, shallow_next), w_next = rows_at(TILE + wn, deep_next, shallow_next);
+        constexpr int kReads = (MT + kEarly + kSlots - 1) / kSlots, kLoads = (kTileLoads + kSlots - 1) / kSlots;
+        const int slot_next = (slot + 1) & (kTileRing - 1);
+        const int x_next = slot_next * kTileStep + wm * 128, w_next = slot_next * kTileStep + (kTile + wn) * 128;
 #pragma unroll
         for (int t = 0; t < MT; ++t) xs[t] = xs_next[t];
 #pragma unroll
@@ -258,12 +228,12 @@ __global__ void __launch_bounds__(T::waves * 64, T::waves / 4) tile_kernel(Fp8Pa
                 if (e < kTurn) {
                     if (kEarly + e < NT) read_w(w_at, s, kEarly + e);
                 } else {
-                    // step i + 1 is there, and all waves have read step i whole, so its places
-                    // go to steps i + RS and i + RD
+                    // step i + 1 is there, and all waves have read step i whole, so its place
+                    // goes to step i + kTileRing
                     if (s == 1 && e == kTurn) {
-                        step_barrier<far ? kNewer : 0>(true);
+                        step_barrier<more ? kNewer : 0>(true);
                         __builtin_amdgcn_sched_barrier(0);
-                        if constexpr (near) load_scales(((first + i) >> 2) + 1);
+                        if constexpr (more) load_scales(((first + i) >> 2) + 1);
                         read_scales(first + i + 1);
                     }
 #pragma unroll
@@ -273,38 +243,34 @@ __global__ void __launch_bounds__(T::waves * 64, T::waves / 4) tile_kernel(Fp8Pa
                         else
                             read_w(s == 0 ? w_at : w_next, s ^ 1, t - MT);
                     }
-                    if (s == 1)
+                    if constexpr (more)
+                        if (s == 1)
 #pragma unroll
-                        for (int c = (e - kTurn) * kLoads; c < (e - kTurn + 1) * kLoads && c < L; ++c) {
-                            if constexpr (near)
-                                if (c < LS) load(i + RS, LD + c, shallow);
-                            if constexpr (far)
-                                if (c >= LS) load(i + RD, c - LS, deep);
-                        }
+                            for (int c = (e - kTurn) * kLoads; c < (e - kTurn + 1) * kLoads && c < kTileLoads; ++c)
+                                load(i + kTileRing, c, slot);
                 }
                 const int ni = e / MT, mi = e % MT;
                 acc[mi][ni] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[ni], xf[s][mi], acc[mi][ni], 0, 0, 0,
                                                                              ws[ni], 0, xs[mi]);
                 __builtin_amdgcn_sched_barrier(0);
             }
-        deep = deep_next, shallow = shallow_next, x_at = x_next, w_at = w_next;
+        slot = slot_next, x_at = x_next, w_at = w_next;
     };
     constexpr std::true_type yes{};
     constexpr std::false_type no{};
     int i = 0;
-    for (; i + RD < n; ++i) step(i, yes, yes);
-    if (RS < RD && i + RS < n) step(i++, yes, no);
-    for (; i < n; ++i) step(i, no, no);
+    for (; i + kTileRing < n; ++i) step(i, yes);
+    for (; i < n; ++i) step(i, no);
 
     if (part >= 0) {
-        float *sums = p.part + (static_cast<int64_t>(part) * p.rest + tile - p.whole) * (TILE * TILE);
+        float *sums = p.part + (static_cast<int64_t>(part) * p.rest + tile - p.whole) * (kTile * kTile);
 #pragma unroll
         for (int mi = 0; mi < MT; ++mi)
 #pragma unroll
             for (int ni = 0; ni < NT; ++ni)
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
-                    *reinterpret_cast<f32x4 *>(sums + (wm + mi * 32 + l32) * TILE + wn + ni * 32 + 8 * q + 4 * half) =
+                    *reinterpret_cast<f32x4 *>(sums + (wm + mi * 32 + l32) * kTile + wn + ni * 32 + 8 * q + 4 * half) =
                         f32x4{acc[mi][ni][4 * q], acc[mi][ni][4 * q + 1], acc[mi][ni][4 * q + 2], acc[mi][ni][4 * q + 3]};
         return;
     }
@@ -338,9 +304,8 @@ __global__ void __launch_bounds__(T::waves * 64, T::waves / 4) tile_kernel(Fp8Pa
         }
         return;
     }
-    // GELU, the largest magnitude of each row's block of 128 columns (a wave's, or
-    // that of two waves side by side), the block
-    static_assert(NT * 32 == 128 || NT * 32 == 64, "a block is one wave's or two's");
+    // GELU, the largest magnitude of each row's 128 columns (those of two waves side
+    // by side), the block
     uint32_t top[MT];
 #pragma unroll
     for (int mi = 0; mi < MT; ++mi) {
@@ -357,16 +322,14 @@ __global__ void __launch_bounds__(T::waves * 64, T::waves / 4) tile_kernel(Fp8Pa
         const auto both = __builtin_amdgcn_permlane32_swap(top[mi], top[mi], false, false);
         top[mi] = max(static_cast<uint32_t>(both[0]), static_cast<uint32_t>(both[1]));
     }
-    if constexpr (NT * 32 == 64) {
-        uint32_t *tops = reinterpret_cast<uint32_t *>(smem);
-        __syncthreads();  // all waves are done with the tiles
-        if (half == 0)
+    uint32_t *tops = reinterpret_cast<uint32_t *>(smem);
+    __syncthreads();  // all waves are done with the tiles
+    if (half == 0)
 #pragma unroll
-            for (int mi = 0; mi < MT; ++mi) tops[wave * (MT * 32) + mi * 32 + l32] = top[mi];
-        __syncthreads();
+        for (int mi = 0; mi < MT; ++mi) tops[wave * (MT * 32) + mi * 32 + l32] = top[mi];
+    __syncthreads();
 #pragma unroll
-        for (int mi = 0; mi < MT; ++mi) top[mi] = max(top[mi], tops[(wave ^ 1) * (MT * 32) + mi * 32 + l32]);
-    }
+    for (int mi = 0; mi < MT; ++mi) top[mi] = max(top[mi], tops[(wave ^ 1) * (MT * 32) + mi * 32 + l32]);
     const int block = (n0 + wn) / kFp8Block, last = p.np / kFp8Block - 1;
     if (block > last) return;
 #pragma unroll
@@ -794,8 +757,6 @@ __global__ void __launch_bounds__(256) tile_sum_kernel(Fp8Params p)
     }
 }
 
-typedef Tile<128, 2, 2, 8, 4, 4> Medium;
-
 // ------------------------------------------------------------------ few rows --
 // 32 * MT rows of x and 32 * NT of w a workgroup.  Each of its four waves takes every fourth
 // block of K, through LDS of its own (so that the loads read whole rows of 128 bytes; straight
@@ -803,8 +764,8 @@ typedef Tile<128, 2, 2, 8, 4, 4> Medium;
 // their sums are added in LDS at the end.
 constexpr int kFewWaves = 4;
 
-// X16: x is bf16, and each workgroup quantises all of it into LDS while its first loads of w are
-// on their way: for x of at most kInline bytes there (a launch less).
+// X16: x is bf16, and each workgroup quantises its rows of it into LDS while its first loads of w
+// are on their way: for rows of at most kInline bytes there (a launch less).
 constexpr int kInline = 17408;  // with the ring a third of LDS
 
 template <int MT_, int NT_, int RING_, bool X16_ = false>
@@ -820,7 +781,7 @@ struct Few {
 
 // x in LDS: rows of the values, 16 bytes apart from a multiple of 128 (so that 32 rows cover
 // the banks), then rows of the scales.
-__host__ __device__ inline int64_t inline_bytes(int64_t m, int64_t kp) { return m * (kp + 16 + kp / kFp8Block); }
+__host__ __device__ inline int64_t inline_bytes(int64_t rows, int64_t kp) { return rows * (kp + 16 + kp / kFp8Block); }
 
 // This wave's loads but the newest `n` have landed.
 __device__ __forceinline__ void wait_loads(int n)
@@ -832,9 +793,7 @@ __device__ __forceinline__ void wait_loads(int n)
     LTXK_WAIT(10)
     LTXK_WAIT(14)
     LTXK_WAIT(18)
-    LTXK_WAIT(20)
     LTXK_WAIT(28)
-    LTXK_WAIT(30)
 #undef LTXK_WAIT
     default: __builtin_amdgcn_s_waitcnt(0x0f70);
     }
@@ -884,17 +843,18 @@ __global__ void __launch_bounds__(kFewWaves * 64) few_kernel(Fp8Params p)
         }
     };
     for (int i = 0; i < R && i < n; ++i) load(i, i);
-    char *xl = smem + F::x_at, *xsl = xl + p.m * (p.kp + 16);
+    const int rows = min(32, p.m - m0);
+    char *xl = smem + F::x_at, *xsl = xl + rows * (p.kp + 16);
     if constexpr (F::X16) {
         // a block 16 lanes, as quantize_fp8; the loads of kBatch blocks together
         constexpr int kBatch = 4, kStride = kFewWaves * 4;
-        const int units = p.m * p.blocks;
+        const int units = rows * p.blocks;
         for (int u0 = threadIdx.x >> 4; u0 < units; u0 += kBatch * kStride) {
             u32x4 raw[kBatch];
 #pragma unroll
             for (int i = 0; i < kBatch; ++i) {  // past the last: read again, not stored
                 const int u = min(u0 + i * kStride, units - 1), row = u / p.blocks, col = u % p.blocks * kFp8Block + (lane & 15) * 8;
-                raw[i] = *reinterpret_cast<const u32x4 *>(p.x16 + static_cast<int64_t>(row) * p.k + min(col, p.k - 8));
+                raw[i] = *reinterpret_cast<const u32x4 *>(p.x16 + static_cast<int64_t>(m0 + row) * p.k + min(col, p.k - 8));
                 if (col >= p.k) raw[i] = u32x4{};
             }
 #pragma unroll
@@ -910,8 +870,8 @@ __global__ void __launch_bounds__(kFewWaves * 64) few_kernel(Fp8Params p)
             }
         }
         __syncthreads();
-        xl += min(l32, p.m - 1) * (p.kp + 16) + half * 16;
-        xsl += min(l32, p.m - 1) * p.blocks;
+        xl += min(l32, rows - 1) * (p.kp + 16) + half * 16;
+        xsl += min(l32, rows - 1) * p.blocks;
     }
 
     int off[4];
@@ -1074,7 +1034,7 @@ Cut cut(int64_t m, int64_t n, int64_t k)
     }
     // Tiles: those past the last full wave of the chip are dealt to its units in parts of
     // K of at least 8 steps each.
-    c.tile = (m + 255) / 256 * ((n + 255) / 256) >= 192 && k > 128 ? 256 : 128;
+    c.tile = (m + 255) / 256 * ((n + 255) / 256) >= 192 && k > 128 ? kBig : kTile;
     c.tiles_m = (m + c.tile - 1) / c.tile;
     c.tiles_n = (n + c.tile - 1) / c.tile;
     c.rest = c.tiles_m * c.tiles_n % 256;
@@ -1090,20 +1050,25 @@ Cut cut(int64_t m, int64_t n, int64_t k)
 int64_t workspace_bytes(int64_t m, int64_t n, int64_t k, bool gelu)
 {
     const Cut c = cut(m, n, k);
-    if (c.tile >= 128) return c.parts > 1 ? c.rest * c.parts * c.tile * c.tile * 4 : 0;
+    if (c.tile >= kTile) return c.parts > 1 ? c.rest * c.parts * c.tile * c.tile * 4 : 0;
     return gelu || c.parts > 1 ? c.parts * m * fp8_blocks(n) * kFp8Block * 4 : 0;
 }
 
-template <typename T, bool GELU>
-void launch_tiles(const Fp8Params &p, hipStream_t s)
+template <bool GELU>
+void tiles(const Fp8Params &p, int tile, hipStream_t s)
 {
-    const unsigned grid = 8u * static_cast<unsigned>(p.whole / 8 + (p.rest * p.parts + 7) / 8);
-    tile_kernel<T, GELU><<<grid, T::waves * 64, 0, s>>>(p);
-    if (p.rest && p.parts > 1)
-        tile_sum_kernel<T::size, GELU><<<static_cast<unsigned>(p.rest) * (T::size * T::size / 8 / 256), 256, 0, s>>>(p);
+    const unsigned per = static_cast<unsigned>(p.whole / 8 + p.per);  // of an XCD
+    const unsigned sums = p.parts > 1 ? static_cast<unsigned>(p.rest * tile * tile / 8 / 256) : 0;
+    if (tile == kBig) {
+        big_kernel<GELU><<<8 * std::min<unsigned>(kCus, per), kBigWaves * 64, 0, s>>>(p);
+        if (sums) tile_sum_kernel<kBig, GELU><<<sums, 256, 0, s>>>(p);
+    } else {
+        tile_kernel<GELU><<<8 * per, kTileWaves * 64, 0, s>>>(p);
+        if (sums) tile_sum_kernel<kTile, GELU><<<sums, 256, 0, s>>>(p);
+    }
 }
 
-bool takes_bf16(const Cut &c, int64_t m, int64_t kp) { return c.tile == 32 && inline_bytes(m, kp) <= kInline; }
+bool takes_bf16(const Cut &c, int64_t m, int64_t kp) { return c.tile == 32 && inline_bytes(std::min<int64_t>(m, 32), kp) <= kInline; }
 
 // x's blocks, where the call makes them: values (a multiple of 128 bytes), then scales.
 int64_t blocks_bytes(int64_t m, int64_t n, int64_t k)
@@ -1165,22 +1130,9 @@ int linear(const char *what, void *y, void *y_scale, bool gelu, const void *x, c
     p.rest = static_cast<int>(c.rest);
     p.parts = static_cast<int>(c.parts);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (c.tile == 256) {
+    if (c.tile >= kTile) {
         p.per = static_cast<int>((c.rest * c.parts + 7) / 8);
-        const unsigned grid = 8u * static_cast<unsigned>(std::min<int64_t>(kCus, c.whole / 8 + p.per));
-        if (gelu)
-            big_kernel<true><<<grid, kBigWaves * 64, 0, s>>>(p);
-        else
-            big_kernel<false><<<grid, kBigWaves * 64, 0, s>>>(p);
-        if (c.parts > 1) {
-            const unsigned sums = static_cast<unsigned>(c.rest) * (kBig * kBig / 8 / 256);
-            if (gelu)
-                tile_sum_kernel<kBig, true><<<sums, 256, 0, s>>>(p);
-            else
-                tile_sum_kernel<kBig, false><<<sums, 256, 0, s>>>(p);
-        }
-    } else if (c.tile == 128) {
-        gelu ? launch_tiles<Medium, true>(p, s) : launch_tiles<Medium, false>(p, s);
+        gelu ? tiles<true>(p, c.tile, s) : tiles<false>(p, c.tile, s);
     } else if (c.tile == 64) {
         few_rows<Few<2, 2, 2>>(p, gelu, s);
     } else if (c.tile == 48) {

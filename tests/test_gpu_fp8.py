@@ -215,6 +215,56 @@ def test_linear_gelu_matches_fp64(m, n, k, bias):
     assert torch.equal(got.data.view(torch.uint8), again.data.view(torch.uint8)) and torch.equal(got.scale, again.scale)
 
 
+# Every way that a product is cut: 32 rows that are quantised in the call, a tile of several and over a cut K; K one
+# value past what is; 64 x 32 and 64 x 64 tiles over a cut K; large tiles of two steps, of an odd rest whole and in parts.
+VARIANTS = [(100, 256, 128), (64, 512, 376), (126, 2040, 512), (1, 1024, 17152), (1, 1024, 17160), (31, 520, 16384),
+            (126, 1024, 16384), (250, 1160, 16392), (520, 712, 648), (3001, 4104, 136), (8200, 2056, 520), (4136, 4112, 2056)]
+
+
+@pytest.mark.parametrize("m,n,k", VARIANTS)
+def test_linear_variants_exact(m, n, k):
+    """As above, and equal for x in bf16, of which the blocks' rounding leaves nothing away."""
+    import ltxk
+
+    g = torch.Generator(device=DEV).manual_seed(m + n + k)
+    x, w = _exact_blocks(m, k, g), _exact_blocks(n, k, g)
+    want = x.float().to(F64) @ w.float().to(F64).t().contiguous()
+    assert float((x.float().abs().to(F64) @ w.float().abs().to(F64).t().contiguous()).max()) < 2.0**16
+    bias = torch.randint(-64, 64, (n,), device=DEV, generator=g).to(torch.bfloat16)
+    for b, value in ((None, want), (bias, want + bias.to(F64))):
+        assert torch.equal(ltxk.linear_fp8(x, w, b), value.to(torch.bfloat16))
+        assert torch.equal(ltxk.linear_fp8(x.float().to(torch.bfloat16), w, b), value.to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("m,n,k", VARIANTS)
+def test_linear_gelu_variants_match_fp64(m, n, k):
+    test_linear_gelu_matches_fp64(m, n, k, True)
+
+
+@pytest.mark.parametrize("m,n,k", [(20, 256, 512), (100, 2048, 256), (500, 1024, 512), (1000, 1032, 384), (3001, 4104, 264)])
+def test_not_finite_stays_in_its_row(m, n, k):
+    """A NaN or an infinity in a row of x makes that row of the result NaN, one in a row of w that column; nothing else."""
+    import ltxk
+
+    g = torch.Generator(device=DEV).manual_seed(m)
+    x = torch.randn(m, k, device=DEV, generator=g).to(torch.bfloat16)
+    w = torch.randn(n, k, device=DEV, generator=g).to(torch.bfloat16)
+    clean, clean_gelu = ltxk.linear_fp8(x, ltxk.quantize_fp8(w)), ltxk.linear_gelu_fp8(x, ltxk.quantize_fp8(w)).float()
+    x[3, 5], x[m - 1, k - 1], w[9, 0] = float("nan"), float("inf"), float("-inf")
+    bad = torch.zeros(m, n, dtype=torch.bool, device=DEV)
+    bad[3], bad[m - 1], bad[:, 9] = True, True, True
+    w = ltxk.quantize_fp8(w)
+    for v in (x, ltxk.quantize_fp8(x)):
+        got = ltxk.linear_fp8(v, w)
+        assert torch.equal(got.isnan(), bad) and torch.equal(got[~bad], clean[~bad])
+        got = ltxk.linear_gelu_fp8(v, w).float()
+        assert got[bad].isnan().all()
+        # a block that holds a NaN may be NaN as a whole; the others are what they were
+        bad_blocks = bad.clone()
+        bad_blocks[:, :128] = True
+        assert torch.equal(got[~bad_blocks], clean_gelu[~bad_blocks])
+
+
 @pytest.mark.parametrize("batch,tokens,dim", [(1, 1, 8), (2, 3, 128), (1, 7, 200), (2, 65, 2048), (1, 130, 4096), (3, 5, 4104),
                                               (1, 4, 8192), (1, 3, 16384), (2, 9, 640), (2, 1601, 264),
                                               (1, 900, 2056), (3, 800, 4096)])
