@@ -761,21 +761,26 @@ __global__ void __launch_bounds__(256) tile_sum_kernel(Fp8Params p)
 // 32 * MT rows of x and 32 * NT of w a workgroup.  Each of its four waves takes every fourth
 // block of K, through LDS of its own (so that the loads read whole rows of 128 bytes; straight
 // to registers a load of 16 lanes touches 16 rows), RING blocks ahead and without a barrier;
-// their sums are added in LDS at the end.
+// their sums are added in LDS at the end.  With GELU two waves take the 128 columns of a block side
+// by side and every second block of K, so that the blocks of the result are made there, too.
 constexpr int kFewWaves = 4;
 
 // X16: x is bf16, and each workgroup quantises its rows of it into LDS while its first loads of w
 // are on their way: for rows of at most kInline bytes there (a launch less).
 constexpr int kInline = 17408;  // with the ring a third of LDS
+// In LDS, 16 bytes of each lane, then a gap: 4 rows' 16 chunks of 8 columns cover the banks.
+constexpr int kSumsRow = 68;
 
-template <int MT_, int NT_, int RING_, bool X16_ = false>
+template <int MT_, int NT_, int RING_, bool X16_ = false, bool GELU_ = false>
 struct Few {
     static constexpr int MT = MT_, NT = NT_, RING = RING_;
-    static constexpr bool X16 = X16_;
+    static constexpr bool X16 = X16_, GELU = GELU_;
+    static constexpr int over_n = GELU ? 2 : 1, over_k = kFewWaves / over_n;  // waves
     static constexpr int loads = X16 ? 4 * NT + 1 : 4 * (MT + NT) + 2;  // of a block: 8 rows each, and the scales
     static constexpr int w_at = X16 ? 0 : MT * 4096, scales_at = w_at + NT * 4096, bytes = scales_at + (X16 ? 256 : 512);
-    static constexpr int ring = RING * bytes * kFewWaves, sums = kFewWaves * MT * NT * 4096;
+    static constexpr int ring = RING * bytes * kFewWaves, sums = kFewWaves * MT * NT * 4 * kSumsRow * 16;
     static constexpr int x_at = ring > sums ? ring : sums, lds = x_at + (X16 ? kInline : 0);
+    static_assert(!GELU || (MT == 1 && NT == 2 && !X16), "32 rows of one block");
     static_assert(MT <= 2 && NT <= 2 && loads * (RING - 1) < 64, "a load takes 64 rows of scales, a wait counts to 63");
 };
 
@@ -811,11 +816,12 @@ __global__ void __launch_bounds__(kFewWaves * 64) few_kernel(Fp8Params p)
     const int at_x = blockIdx.x >> 3;
     const int tn = at_x / p.tiles_m / p.parts * 8 + (blockIdx.x & 7), tm = at_x % p.tiles_m, part = at_x / p.tiles_m % p.parts;
     if (tn >= p.tiles_n) return;
-    const int m0 = tm * 32 * MT, n0 = tn * 32 * NT;
-    // blocks of this part, then every fourth of them for this wave
+    const int wn = wave % F::over_n, wk = wave / F::over_n;
+    const int m0 = tm * 32 * MT, n0 = (tn * F::over_n + wn) * 32 * NT;
+    // blocks of this part, then this wave's of them
     const int from = static_cast<int>(static_cast<uint32_t>(part) * p.blocks / p.parts);
     const int to = static_cast<int>(static_cast<uint32_t>(part + 1) * p.blocks / p.parts);
-    const int first = from + wave, n = max(0, (to - first + kFewWaves - 1) / kFewWaves);
+    const int first = from + wk, n = max(0, (to - first + F::over_k - 1) / F::over_k);
 
     const u32x4 xr = whole_memory(p.x), wr = whole_memory(p.w), xsr = whole_memory(p.xs), wsr = whole_memory(p.ws);
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char *)smem)) + wave * R * F::bytes;
@@ -830,7 +836,7 @@ __global__ void __launch_bounds__(kFewWaves * 64) few_kernel(Fp8Params p)
         wo[c] = static_cast<uint32_t>(min(n0 + c * 8 + (lane >> 3), p.n - 1)) * static_cast<uint32_t>(p.kp) + (c & 1 ? chunk_odd : chunk);
     const uint32_t xso = static_cast<uint32_t>(min(m0 + lane, p.m - 1)) * 4, wso = static_cast<uint32_t>(min(n0 + lane, p.n - 1)) * 4;
     auto load = [&](int i, int slot) {
-        const int b = first + i * kFewWaves;
+        const int b = first + i * F::over_k;
         const uint32_t at = lds0 + slot * F::bytes;
         const uint32_t k = __builtin_amdgcn_readfirstlane(b * kFp8Block), g = __builtin_amdgcn_readfirstlane(b >> 2);
 #pragma unroll
@@ -884,7 +890,7 @@ __global__ void __launch_bounds__(kFewWaves * 64) few_kernel(Fp8Params p)
         const char *at = smem + (wave * R + slot) * F::bytes;
         i32x8 f[2][MT + NT];
         int scale[MT + NT];
-        const int b = first + i * kFewWaves;
+        const int b = first + i * F::over_k;
         if constexpr (F::X16) {
 #pragma unroll
             for (int s = 0; s < 2; ++s)
@@ -925,14 +931,44 @@ __global__ void __launch_bounds__(kFewWaves * 64) few_kernel(Fp8Params p)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const f32x16 &a = acc[t / NT][t % NT];
-            sums[((wave * MT * NT + t) * 4 + q) * 64 + lane] = f32x4{a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]};
+            sums[((wave * MT * NT + t) * 4 + q) * kSumsRow + lane] = f32x4{a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]};
         }
     __syncthreads();
+    if constexpr (F::GELU) {
+        // 8 columns a lane, a row's block 16 lanes
+        const int col = tn * kFp8Block + (lane & 15) * 8;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int at = i * 16 + wave * 4 + (lane >> 4), row = m0 + at;
+            float v[8] = {};
+            if (col < p.n) {
+                f32x4 lo = {}, hi = {};
+#pragma unroll
+                for (int w = 0; w < F::over_k; ++w) {
+                    // of the wave that holds these columns: its tile, and four times 8 columns there
+                    const f32x4 *s = sums + (w * F::over_n * NT * 4 + (lane & 15)) * kSumsRow + at;
+                    lo += s[0], hi += s[32];
+                }
+                float b[8] = {};
+                if (p.bias) unpack8v(*reinterpret_cast<const u32x4 *>(p.bias + col), b);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = gelu((e < 4 ? lo[e] : hi[e - 4]) + b[e]);
+            }
+            uint32_t scale;
+            const uint2 q = fp8_quantize8(v, scale);
+            if (row >= p.m) continue;
+            *reinterpret_cast<uint2 *>(p.q + static_cast<int64_t>(row) * p.np + col) = q;
+            if (lane & 15) continue;
+            for (int b = tn; b == tn || (tn == p.tiles_n - 1 && b <= (tn | 3)); ++b)  // the last block's lane fills its group
+                p.qs[(static_cast<int64_t>(b >> 2) * p.m + row) * 4 + (b & 3)] = b == tn ? static_cast<uint8_t>(scale) : 0;
+        }
+        return;
+    }
 #pragma unroll
     for (int t = 0; t < MT * NT; ++t) {  // this wave's q of each tile
         f32x4 v = {};
 #pragma unroll
-        for (int w = 0; w < kFewWaves; ++w) v += sums[((w * MT * NT + t) * 4 + wave) * 64 + lane];
+        for (int w = 0; w < kFewWaves; ++w) v += sums[((w * MT * NT + t) * 4 + wave) * kSumsRow + lane];
         const int row = m0 + t / NT * 32 + l32, col = n0 + t % NT * 32 + 8 * wave + 4 * half;
         if (row >= p.m || col >= p.n) continue;
         if constexpr (SUMS) {
@@ -990,7 +1026,9 @@ template <typename F>
 void few_rows(const Fp8Params &p, bool gelu, hipStream_t s)
 {
     const unsigned grid = 8u * static_cast<unsigned>((p.tiles_n + 7) / 8) * static_cast<unsigned>(p.tiles_m) * static_cast<unsigned>(p.parts);
-    if (gelu || p.parts > 1) {
+    if constexpr (F::GELU) {
+        few_kernel<F, false><<<grid, kFewWaves * 64, 0, s>>>(p);
+    } else if (gelu || p.parts > 1) {
         few_kernel<F, true><<<grid, kFewWaves * 64, 0, s>>>(p);
         const unsigned sums = static_cast<unsigned>((static_cast<int64_t>(p.m) * ((p.np + 511) / 512) + 3) / 4);
         if (gelu)
@@ -1013,16 +1051,31 @@ void few_rows(const Fp8Params &p, bool gelu, hipStream_t s)
 // K is cut from 128 blocks on where the tiles leave units idle, into parts of at least 16; the
 // second launch costs 5 us: 1 x 1024 x 16384 19 us whole, 12 in 8 parts; 126 x 1024 x 16384 28 and
 // 17; 16 x 4096 x 16384 25 and 26.
+//
+// With GELU few rows take a second launch, which makes the blocks of sums in memory, or tiles of 32 x 128
+// that make them themselves, where these are not too few for their K (blocks of it times 6) nor take
+// longer than 32 blocks of K in turn.  Us, with the second launch / one: 126 x 8192 x 2048 13.3 / 10.9, 252 x
+// 4096 x 4096 18.2 / 16.3, 504 x 4096 x 2048 22.3 / 18.3, 8 x 2048 x 256 5.0 / 3.9;  too few, 126 x 2048 x 2048 7.5 /
+// 8.8, 126 x 4096 x 4096 14.2 / 16.3;  too long, 504 x 4096 x 4096 24.0 / 29.1, 504 x 8192 x 2048 19 / 35.
 struct Cut {
     int tile;  // rows of x and of w; few rows: 32, 48 (64 and 32) and 64
+    bool fused;  // few rows with GELU: tiles of 32 x 128, the result's blocks made there
     int64_t tiles_m, tiles_n, whole, rest, parts;
 };
 
-Cut cut(int64_t m, int64_t n, int64_t k)
+Cut cut(int64_t m, int64_t n, int64_t k, bool gelu)
 {
     Cut c{};
     const int64_t blocks = fp8_blocks(k), tiles64 = (m + 63) / 64 * ((n + 63) / 64);
     c.parts = 1;
+    c.tiles_m = (m + 31) / 32;
+    c.tiles_n = fp8_blocks(n);
+    const int64_t tiles = c.tiles_m * c.tiles_n;
+    if (gelu && tiles <= 512 && (tiles + 255) / 256 * blocks <= 32 && tiles >= 6 * blocks) {
+        c.tile = 32;
+        c.fused = true;
+        return c;
+    }
     if (m <= 32 || tiles64 <= 256) {
         const int mt = m <= 32 || tiles64 <= 64 ? 1 : 2, nt = m <= 32 || tiles64 <= 128 ? 1 : 2;
         c.tile = 16 * (mt + nt);
@@ -1049,9 +1102,9 @@ Cut cut(int64_t m, int64_t n, int64_t k)
 
 int64_t workspace_bytes(int64_t m, int64_t n, int64_t k, bool gelu)
 {
-    const Cut c = cut(m, n, k);
+    const Cut c = cut(m, n, k, gelu);
     if (c.tile >= kTile) return c.parts > 1 ? c.rest * c.parts * c.tile * c.tile * 4 : 0;
-    return gelu || c.parts > 1 ? c.parts * m * fp8_blocks(n) * kFp8Block * 4 : 0;
+    return (gelu && !c.fused) || c.parts > 1 ? c.parts * m * fp8_blocks(n) * kFp8Block * 4 : 0;
 }
 
 template <bool GELU>
@@ -1068,12 +1121,12 @@ void tiles(const Fp8Params &p, int tile, hipStream_t s)
     }
 }
 
-bool takes_bf16(const Cut &c, int64_t m, int64_t kp) { return c.tile == 32 && inline_bytes(std::min<int64_t>(m, 32), kp) <= kInline; }
+bool takes_bf16(const Cut &c, int64_t m, int64_t kp) { return c.tile == 32 && !c.fused && inline_bytes(std::min<int64_t>(m, 32), kp) <= kInline; }
 
 // x's blocks, where the call makes them: values (a multiple of 128 bytes), then scales.
-int64_t blocks_bytes(int64_t m, int64_t n, int64_t k)
+int64_t blocks_bytes(int64_t m, int64_t n, int64_t k, bool gelu)
 {
-    return takes_bf16(cut(m, n, k), m, fp8_blocks(k) * kFp8Block) ? 0 : m * fp8_blocks(k) * kFp8Block + (m * fp8_groups(k) * kFp8Group + 15) / 16 * 16;
+    return takes_bf16(cut(m, n, k, gelu), m, fp8_blocks(k) * kFp8Block) ? 0 : m * fp8_blocks(k) * kFp8Block + (m * fp8_groups(k) * kFp8Group + 15) / 16 * 16;
 }
 
 // The checks and the launch of both entry points.
@@ -1095,8 +1148,8 @@ int linear(const char *what, void *y, void *y_scale, bool gelu, const void *x, c
     const int64_t kp = fp8_blocks(k) * kFp8Block, np = fp8_blocks(n) * kFp8Block;
     if (m > (kMax - 1) / kp || n > (kMax - 1) / kp || m > (kMax - 1) / np)
         return fail(LTXK_E_ARG, "%s: x, w or y holds 2^31 values or more", what);
-    const Cut c = cut(m, n, k);
-    const int64_t blocks_at = x_scale ? 0 : blocks_bytes(m, n, k), need = blocks_at + workspace_bytes(m, n, k, gelu);
+    const Cut c = cut(m, n, k, gelu);
+    const int64_t blocks_at = x_scale ? 0 : blocks_bytes(m, n, k, gelu), need = blocks_at + workspace_bytes(m, n, k, gelu);
     if (need && (!workspace || !aligned16(workspace) || workspace_size < need))
         return fail(LTXK_E_ARG, "%s: the workspace must hold ltxk_linear_fp8_workspace_bytes, 16-byte aligned", what);
     Fp8Params p{};
@@ -1133,6 +1186,8 @@ int linear(const char *what, void *y, void *y_scale, bool gelu, const void *x, c
     if (c.tile >= kTile) {
         p.per = static_cast<int>((c.rest * c.parts + 7) / 8);
         gelu ? tiles<true>(p, c.tile, s) : tiles<false>(p, c.tile, s);
+    } else if (c.fused) {
+        few_rows<Few<1, 2, 3, false, true>>(p, gelu, s);
     } else if (c.tile == 64) {
         few_rows<Few<2, 2, 2>>(p, gelu, s);
     } else if (c.tile == 48) {
@@ -1155,7 +1210,7 @@ extern "C" int64_t ltxk_linear_fp8_workspace_bytes(int64_t m, int64_t n, int64_t
     if (m <= 0 || n <= 0 || k <= 0) return 0;
     const int64_t kMax = int64_t{1} << 31;  // sizes that the calls refuse
     if (m >= kMax || n >= kMax || k >= kMax) return 0;
-    return (quantize ? blocks_bytes(m, n, k) : 0) + workspace_bytes(m, n, k, gelu != 0);
+    return (quantize ? blocks_bytes(m, n, k, gelu != 0) : 0) + workspace_bytes(m, n, k, gelu != 0);
 }
 
 extern "C" int ltxk_linear_fp8(void *y, const void *x, const void *x_scale, const void *w, const void *w_scale,
