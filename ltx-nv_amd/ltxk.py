@@ -964,7 +964,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: in
         raise ValueError(f"width {d} is not {heads} heads of 64 or 128")
     keep_stride = 0
     if keep is not None:
-        _dev(keep, "keep", torch.bool if keep.dtype == torch.bool else torch.uint8)
+        _dev(keep, "keep", torch.uint8 if getattr(keep, "dtype", None) == torch.uint8 else torch.bool)
         if keep.ndim != 2 or keep.shape[0] not in (1, b) or keep.shape[1] != tk:
             raise ValueError(f"keep {tuple(keep.shape)} must be ({b} or 1, {tk})")
         if keep.shape[0] > 1:
@@ -1009,7 +1009,7 @@ class Fp8Blocks:
     255 marks a block that held an infinity or NaN.  K is a multiple of 8.  Made by quantize_fp8 and the
     kernels that write blocks; a program that keeps quantised weights may build it from its own tensors."""
 
-    __slots__ = ("data", "scale", "shape")
+    __slots__ = ("shape", "rows", "_data", "_scale", "_both")
 
     def __init__(self, data: torch.Tensor, scale: torch.Tensor, shape):
         shape = tuple(shape)
@@ -1025,21 +1025,48 @@ class Fp8Blocks:
                              f"{(-(-blocks // FP8_GROUP), rows, FP8_GROUP)}")
         if data.get_device() != scale.get_device():
             raise ValueError(f"data is on {data.device}, scale on {scale.device}")
-        self.data, self.scale, self.shape = data, scale, shape
+        self.shape, self.rows, self._data, self._scale, self._both = shape, rows, data, scale, None
 
     @classmethod
     def _made(cls, shape, device) -> "Fp8Blocks":
-        """Uninitialised blocks for a kernel to fill."""
+        """Uninitialised blocks for a kernel to fill, the scales behind the values in one allocation: a result that
+        goes into the next layer needs no tensors, which take the host 1 us each."""
         rows, blocks = _fp8_extent(shape)
         self = object.__new__(cls)
-        self.shape = tuple(shape)
-        self.data = torch.empty(rows, blocks * FP8_BLOCK, device=device, dtype=torch.float8_e4m3fn)
-        self.scale = torch.empty(-(-blocks // FP8_GROUP), rows, FP8_GROUP, device=device, dtype=torch.uint8)
+        self.shape, self.rows, self._data, self._scale = tuple(shape), rows, None, None
+        self._both = torch.empty(rows * (blocks * FP8_BLOCK + -(-blocks // FP8_GROUP) * FP8_GROUP), device=device,
+                                 dtype=torch.uint8)
         return self
+
+    def _pointers(self) -> tuple[int, int]:
+        """Addresses of the values and the scales."""
+        if self._both is None:
+            return self._data.data_ptr(), self._scale.data_ptr()
+        at = self._both.data_ptr()
+        return at, at + self.rows * (-(-self.shape[-1] // FP8_BLOCK) * FP8_BLOCK)
+
+    @property
+    def data(self) -> torch.Tensor:
+        if self._data is None:
+            rows, blocks = _fp8_extent(self.shape)
+            self._data = self._both[:rows * blocks * FP8_BLOCK].view(rows, blocks * FP8_BLOCK).view(torch.float8_e4m3fn)
+        return self._data
+
+    @property
+    def scale(self) -> torch.Tensor:
+        if self._scale is None:
+            rows, blocks = _fp8_extent(self.shape)
+            self._scale = self._both[rows * blocks * FP8_BLOCK:].view(-1, rows, FP8_GROUP) if rows else \
+                self._both.new_empty(-(-blocks // FP8_GROUP), 0, FP8_GROUP)
+        return self._scale
 
     @property
     def device(self) -> torch.device:
-        return self.data.device
+        return self._held().device
+
+    def _held(self) -> torch.Tensor:
+        """A tensor of what is held."""
+        return self._data if self._both is None else self._both
 
     def float(self) -> torch.Tensor:
         """The values held, in fp32 (exact but where they leave fp32's range), by torch operations."""
@@ -1055,9 +1082,11 @@ class Fp8Blocks:
         lead = 1
         for s in shape[:-1]:
             lead *= s
-        if not shape or shape[-1] != self.shape[-1] or lead != self.data.shape[0]:
+        if not shape or shape[-1] != self.shape[-1] or lead != self.rows:
             raise ValueError(f"{self.shape} has no view {shape}: the last dimension stays")
-        return Fp8Blocks(self.data, self.scale, shape)
+        other = object.__new__(Fp8Blocks)
+        other.shape, other.rows, other._data, other._scale, other._both = shape, lead, self._data, self._scale, self._both
+        return other
 
 
 def _fp8_extent(shape) -> tuple[int, int]:
@@ -1069,14 +1098,16 @@ def _fp8_extent(shape) -> tuple[int, int]:
 
 
 def quantize_fp8(x: torch.Tensor) -> Fp8Blocks:
-    """x (..., K) bf16 in blocks; K a positive multiple of 8."""
+    """x (..., K) bf16 in blocks, values and scales in tensors of their own (a weight's are kept and saved apart); K a
+    positive multiple of 8."""
     _dev(x, "x")
     if x.ndim == 0 or x.shape[-1] == 0 or x.shape[-1] % 8:
         raise ValueError(f"x {tuple(x.shape)} must end in a positive multiple of 8")
     _one_device(x)
-    out = Fp8Blocks._made(x.shape, x.device)
-    rc = load().ltxk_quantize_fp8(out.data.data_ptr(), out.scale.data_ptr(), x.data_ptr(), out.data.shape[0],
-                                  x.shape[-1], _stream(x))
+    rows, blocks = _fp8_extent(x.shape)
+    out = Fp8Blocks(torch.empty(rows, blocks * FP8_BLOCK, device=x.device, dtype=torch.float8_e4m3fn),
+                    torch.empty(-(-blocks // FP8_GROUP), rows, FP8_GROUP, device=x.device, dtype=torch.uint8), x.shape)
+    rc = load().ltxk_quantize_fp8(*out._pointers(), x.data_ptr(), rows, x.shape[-1], _stream(x))
     _check_rc(rc, "quantize_fp8")
     return out
 
@@ -1109,12 +1140,15 @@ def _norm_fp8(x, f, gate, mask, shift, scale, eps, x_out):
             raise ValueError(f"mask must hold one value per batch item ({b}), got {mask.numel()}")
     if d == 0 or d % 8:
         raise ValueError(f"x {tuple(x.shape)} must end in a positive multiple of 8")
-    _one_device(x, f, mask, *[o for a in (gate, shift, scale) if a is not None for o in (a.table, a.emb)])
+    _one_device(x, f, mask, x_out)
+    for a in (gate, shift, scale):
+        if a is not None:
+            _one_device(x, a.table, a.emb, a.index.index if a.index is not None else None)
     out = Fp8Blocks._made(x.shape, x.device)
     if x.numel() == 0:
         return x_out, out
     rc = load().ltxk_add_norm_modulate_fp8(
-        _ptr(x_out), out.data.data_ptr(), out.scale.data_ptr(), _ptr(x), _ptr(f), _ada_arg(gate, b, t, d), _ptr(mask),
+        _ptr(x_out), *out._pointers(), _ptr(x), _ptr(f), _ada_arg(gate, b, t, d), _ptr(mask),
         b * t, t, d, eps, _ada_arg(shift, b, t, d), _ada_arg(scale, b, t, d), _stream(x))
     _check_rc(rc, "add_norm_modulate_fp8")
     return x_out, out
@@ -1143,10 +1177,9 @@ def _fp8_linear(x, weight: Fp8Blocks, bias: torch.Tensor | None, gelu: bool):
         _dev(bias, "bias")
         if bias.shape != (n,):
             raise ValueError(f"bias {tuple(bias.shape)} must be ({n},)")
-    data, scale = (x.data, x.scale) if held else (x, None)
-    w = weight.data
-    _one_device(data, w, bias)
-    m = data.shape[0] if held else x.numel() // k
+    w = weight._held()
+    _one_device(w, x._held() if held else x, bias)
+    m = x.rows if held else x.numel() // k
     if gelu:
         out = Fp8Blocks._made((*lead, n), w.device)
     else:
@@ -1154,10 +1187,10 @@ def _fp8_linear(x, weight: Fp8Blocks, bias: torch.Tensor | None, gelu: bool):
     nbytes = _fp8_workspace_bytes(m, n, k, gelu, not held)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=w.device) if nbytes else None
     lib = load()
-    rest = (data.data_ptr(), _ptr(scale), w.data_ptr(), weight.scale.data_ptr(), _ptr(bias), m, n, k, _ptr(ws), nbytes,
+    rest = (*(x._pointers() if held else (x.data_ptr(), None)), *weight._pointers(), _ptr(bias), m, n, k, _ptr(ws), nbytes,
             _stream(w))
     if gelu:
-        _check_rc(lib.ltxk_linear_gelu_fp8(out.data.data_ptr(), out.scale.data_ptr(), *rest), "linear_gelu_fp8")
+        _check_rc(lib.ltxk_linear_gelu_fp8(*out._pointers(), *rest), "linear_gelu_fp8")
     else:
         _check_rc(lib.ltxk_linear_fp8(out.data_ptr(), *rest), "linear_fp8")
     return out
