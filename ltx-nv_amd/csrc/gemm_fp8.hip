@@ -95,25 +95,25 @@ __device__ __forceinline__ u32x4 whole_memory(const void *base)
 constexpr int kBand = 4;  // tiles of x that a band of the tile order holds
 
 // The rows of x and w that tile t takes: bands kBand tiles of x deep.
-template <int TILE>
+template <int TM, int TN>
 __device__ __forceinline__ void tile_rows(const Fp8Params &p, int t, int &m0, int &n0)
 {
     const int band = t / (kBand * p.tiles_n), at = t % (kBand * p.tiles_n);
     const int deep = min(kBand, p.tiles_m - band * kBand);
-    m0 = (band * kBand + at % deep) * TILE;
-    n0 = at / deep * TILE;
+    m0 = (band * kBand + at % deep) * TM;
+    n0 = at / deep * TN;
 }
 
-// 128 x 128 tiles, four waves of 64 x 64, the steps of 128 values four deep in LDS.
-constexpr int kTile = 128, kTileWaves = 4, kTileRing = 4, kTileLoads = 2 * kTile / 8 / kTileWaves;
-constexpr int kTileStep = 2 * kTile * 128, kTileScalesAt = kTileRing * kTileStep;
-constexpr int kTileLds = kTileScalesAt + 2 * 2 * kTile * 4;  // and two groups' scales
+// Tiles of TM x 128, four waves of TM / 2 x 64, the steps of 128 values as deep in LDS as fit.
+constexpr int kTile = 128, kTileWaves = 4;
 
-template <bool GELU>
+template <int TM, bool GELU>
 __global__ void __launch_bounds__(kTileWaves * 64, 1) tile_kernel(Fp8Params p)
 {
-    constexpr int MT = 2, NT = 2;
-    __shared__ __attribute__((aligned(1024))) char smem[kTileLds];
+    constexpr int MT = TM / 64, NT = kTile / 64, ROWS = TM + kTile;
+    constexpr int kRing = TM == kTile ? 4 : 3, kLoads = ROWS / 8 / kTileWaves;  // of a wave for a step
+    constexpr int kStep = ROWS * 128, kScalesAt = kRing * kStep, kGroup = ROWS * 4;
+    __shared__ __attribute__((aligned(1024))) char smem[kScalesAt + 2 * kGroup];  // two groups' scales
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int l32 = lane & 31, half = lane >> 5;
 
@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(kTileWaves * 64, 1) tile_kernel(Fp8Params p)
         tile = p.whole + unit % p.rest;
     }
     int m0, n0;
-    tile_rows<kTile>(p, tile, m0, n0);
+    tile_rows<TM, kTile>(p, tile, m0, n0);
     // parts * blocks stays below 2^32: 256 parts at most of fewer than 2^24 blocks
     auto from = [&](int i) { return static_cast<int>(static_cast<uint32_t>(i) * p.blocks / static_cast<uint32_t>(p.parts)); };
     const int first = part < 0 ? 0 : from(part), n = (part < 0 ? p.blocks : from(part + 1)) - first;
@@ -139,41 +139,43 @@ __global__ void __launch_bounds__(kTileWaves * 64, 1) tile_kernel(Fp8Params p)
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char *)smem));
     // Load c of a step: rows (4 c + wave) * 8 .. + 7 of the tile's x and w together.
     // Rows past the last repeat it; their results are not stored.
-    uint32_t at[kTileLoads];
+    uint32_t at[kLoads];
 #pragma unroll
-    for (int c = 0; c < kTileLoads; ++c) {
+    for (int c = 0; c < kLoads; ++c) {
         const int row = (c * kTileWaves + wave) * 8 + (lane >> 3);
-        const bool is_x = c * kTileWaves * 8 < kTile;
-        at[c] = static_cast<uint32_t>(is_x ? min(m0 + row, p.m - 1) : min(n0 + row - kTile, p.n - 1)) *
+        const bool is_x = c * kTileWaves * 8 < TM;
+        at[c] = static_cast<uint32_t>(is_x ? min(m0 + row, p.m - 1) : min(n0 + row - TM, p.n - 1)) *
                     static_cast<uint32_t>(p.kp) + chunk_pos(row, lane & 7) * 16;
     }
-    // Scales, 64 rows a wave: x's first, then w's.
-    const bool sx = wave < 2;
-    const u32x4 sr = whole_memory(sx ? p.xs : p.ws);
-    const int s_rows = sx ? p.m : p.n;
-    const uint32_t so = static_cast<uint32_t>(min((sx ? m0 : n0 - kTile) + wave * 64 + lane, s_rows - 1)) * 4;
+    // Scales, 64 rows a load: x's, then w's, some of them by two waves.
+    const u32x4 xsr = whole_memory(p.xs), wsr = whole_memory(p.ws);
+    constexpr int kX = TM / 64, kW = kTile / 64;
+    const int sx = wave % kX * 64, sw = wave % kW * 64;
+    const uint32_t xso = static_cast<uint32_t>(min(m0 + sx + lane, p.m - 1)) * 4;
+    const uint32_t wso = static_cast<uint32_t>(min(n0 + sw + lane, p.n - 1)) * 4;
     const int groups = (p.blocks + 3) >> 2;
     // A group's scales, into its half of their place; past the last group the last one's, which nothing reads.
     auto load_scales = [&](int group) {
-        load_lds4(sr, __builtin_amdgcn_readfirstlane(lds0 + kTileScalesAt + (group & 1) * (2 * kTile * 4) + wave * 256), so,
-                  __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(min(group, groups - 1)) * s_rows * 4));
+        const uint32_t to = lds0 + kScalesAt + (group & 1) * kGroup, g = min(group, groups - 1);
+        load_lds4(xsr, __builtin_amdgcn_readfirstlane(to + sx * 4), xso, __builtin_amdgcn_readfirstlane(g * p.m * 4));
+        load_lds4(wsr, __builtin_amdgcn_readfirstlane(to + (TM + sw) * 4), wso, __builtin_amdgcn_readfirstlane(g * p.n * 4));
     };
     // Load c of step i, into place `slot` of the ring.
     auto load = [&](int i, int c, int slot) {
-        load_lds16(c * kTileWaves * 8 < kTile ? xr : wr,
-                   __builtin_amdgcn_readfirstlane(lds0 + slot * kTileStep + (c * kTileWaves + wave) * 1024), at[c],
+        load_lds16(c * kTileWaves * 8 < TM ? xr : wr,
+                   __builtin_amdgcn_readfirstlane(lds0 + slot * kStep + (c * kTileWaves + wave) * 1024), at[c],
                    __builtin_amdgcn_readfirstlane((first + i) * kFp8Block));
     };
     load_scales(first >> 2);
     load_scales((first >> 2) + 1);
-    for (int i = 0; i < kTileRing && i < n; ++i)
+    for (int i = 0; i < kRing && i < n; ++i)
 #pragma unroll
-        for (int c = 0; c < kTileLoads; ++c) load(i, c, i);
+        for (int c = 0; c < kLoads; ++c) load(i, c, i);
 
     int off[4];
 #pragma unroll
     for (int s = 0; s < 4; ++s) off[s] = l32 * 128 + chunk_pos(l32, 2 * s + half) * 16;
-    const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;  // this wave's rows
+    const int wm = (wave >> 1) * (TM / 2), wn = (wave & 1) * 64;  // this wave's rows
 
     // acc[i][j]: lane l holds row 32 i + l % 32 of x; register r row 32 j + 8 (r/4) + 4 half + r % 4 of w
     f32x16 acc[MT][NT] = {};
@@ -189,9 +191,9 @@ __global__ void __launch_bounds__(kTileWaves * 64, 1) tile_kernel(Fp8Params p)
     };
     auto read_x = [&](int base, int s, int t) { xf[s][t] = fragment(base + t * 4096, s); };
     auto read_w = [&](int base, int s, int t) { wf[t] = fragment(base + t * 4096, s); };
-    const int scale_row = kTileScalesAt + (wm + l32) * 4, scale_row_w = kTileScalesAt + (kTile + wn + l32) * 4;
+    const int scale_row = kScalesAt + (wm + l32) * 4, scale_row_w = kScalesAt + (TM + wn + l32) * 4;
     auto read_scales = [&](int abs) {
-        const char *at = smem + (abs >> 2 & 1) * (2 * kTile * 4) + (abs & 3);
+        const char *at = smem + (abs >> 2 & 1) * kGroup + (abs & 3);
 #pragma unroll
         for (int t = 0; t < MT; ++t) xs_next[t] = *reinterpret_cast<const uint8_t *>(at + scale_row + t * 128);
 #pragma unroll
@@ -199,10 +201,10 @@ __global__ void __launch_bounds__(kTileWaves * 64, 1) tile_kernel(Fp8Params p)
     };
 
     // Loads that may be in flight when a step has to be there: those issued after its last
-    constexpr int kNewer = (kTileRing - 2) * kTileLoads;
-    step_barrier<kNewer + kTileLoads>(n >= kTileRing);
+    constexpr int kNewer = (kRing - 2) * kLoads;
+    step_barrier<kNewer + kLoads>(n >= kRing);
     read_scales(first);
-    int slot = 0, x_at = wm * 128, w_at = (kTile + wn) * 128;  // this step's place, and this wave's rows there
+    int slot = 0, x_at = wm * 128, w_at = (TM + wn) * 128;  // this step's place, and this wave's rows there
 #pragma unroll
     for (int t = 0; t < MT; ++t) read_x(x_at, 0, t);
 #pragma unroll
@@ -214,9 +216,9 @@ __global__ void __launch_bounds__(kTileWaves * 64, 1) tile_kernel(Fp8Params p)
         // Products before the turn: beside one each the second half of this half step's w is
         // read, the last one covers those reads.  Past it the next half step's x and first half of w.
         constexpr int kProducts = MT * NT, kTurn = NT - kEarly + 1, kSlots = kProducts - kTurn;
-        constexpr int kReads = (MT + kEarly + kSlots - 1) / kSlots, kLoads = (kTileLoads + kSlots - 1) / kSlots;
-        const int slot_next = (slot + 1) & (kTileRing - 1);
-        const int x_next = slot_next * kTileStep + wm * 128, w_next = slot_next * kTileStep + (kTile + wn) * 128;
+        constexpr int kReads = (MT + kEarly + kSlots - 1) / kSlots, kEach = (kLoads + kSlots - 1) / kSlots;
+        const int slot_next = slot + 1 == kRing ? 0 : slot + 1;
+        const int x_next = slot_next * kStep + wm * 128, w_next = slot_next * kStep + (TM + wn) * 128;
 #pragma unroll
         for (int t = 0; t < MT; ++t) xs[t] = xs_next[t];
 #pragma unroll
@@ -229,7 +231,7 @@ __global__ void __launch_bounds__(kTileWaves * 64, 1) tile_kernel(Fp8Params p)
                     if (kEarly + e < NT) read_w(w_at, s, kEarly + e);
                 } else {
                     // step i + 1 is there, and all waves have read step i whole, so its place
-                    // goes to step i + kTileRing
+                    // goes to step i + kRing
                     if (s == 1 && e == kTurn) {
                         step_barrier<more ? kNewer : 0>(true);
                         __builtin_amdgcn_sched_barrier(0);
@@ -246,8 +248,8 @@ __global__ void __launch_bounds__(kTileWaves * 64, 1) tile_kernel(Fp8Params p)
                     if constexpr (more)
                         if (s == 1)
 #pragma unroll
-                            for (int c = (e - kTurn) * kLoads; c < (e - kTurn + 1) * kLoads && c < kTileLoads; ++c)
-                                load(i + kTileRing, c, slot);
+                            for (int c = (e - kTurn) * kEach; c < (e - kTurn + 1) * kEach && c < kLoads; ++c)
+                                load(i + kRing, c, slot);
                 }
                 const int ni = e / MT, mi = e % MT;
                 acc[mi][ni] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[ni], xf[s][mi], acc[mi][ni], 0, 0, 0,
@@ -259,10 +261,10 @@ __global__ void __launch_bounds__(kTileWaves * 64, 1) tile_kernel(Fp8Params p)
     constexpr std::true_type yes{};
     constexpr std::false_type no{};
     int i = 0;
-    for (; i + kTileRing < n; ++i) step(i, yes);
+    for (; i + kRing < n; ++i) step(i, yes);
     for (; i < n; ++i) step(i, no);
 
-    if (part >= 0) {
+    if (TM == kTile && part >= 0) {
         float *sums = p.part + (static_cast<int64_t>(part) * p.rest + tile - p.whole) * (kTile * kTile);
 #pragma unroll
         for (int mi = 0; mi < MT; ++mi)
@@ -385,7 +387,7 @@ __device__ __forceinline__ Unit unit_at(const Fp8Params &p, int xcd, int j)
         u.part = p.parts == 1 ? -1 : i / p.rest;
         u.tile = p.whole + i % p.rest;
     }
-    tile_rows<kBig>(p, u.tile, u.m0, u.n0);
+    tile_rows<kBig, kBig>(p, u.tile, u.m0, u.n0);
     // parts * blocks stays below 2^32: 256 parts at most of fewer than 2^24 blocks
     auto from = [&](int i) { return static_cast<int>(static_cast<uint32_t>(i) * p.blocks / static_cast<uint32_t>(p.parts)); };
     u.first = u.part < 0 ? 0 : from(u.part);
@@ -723,7 +725,7 @@ __global__ void __launch_bounds__(256) tile_sum_kernel(Fp8Params p)
     constexpr int kPer = TILE * TILE / 8 / 256;  // workgroups a tile
     const int t = blockIdx.x / kPer, i = (blockIdx.x % kPer * 256 + threadIdx.x) * 8;
     int m0, n0;
-    tile_rows<TILE>(p, p.whole + t, m0, n0);
+    tile_rows<TILE, TILE>(p, p.whole + t, m0, n0);
     const int row = m0 + i / TILE, col = n0 + i % TILE;
     if (row >= p.m || col >= (GELU ? p.np : p.n)) return;  // whole blocks of lanes
     float f[8] = {};
@@ -1058,7 +1060,7 @@ void few_rows(const Fp8Params &p, bool gelu, hipStream_t s)
 // 4096 x 4096 18.2 / 16.3, 504 x 4096 x 2048 22.3 / 18.3, 8 x 2048 x 256 5.0 / 3.9;  too few, 126 x 2048 x 2048 7.5 /
 // 8.8, 126 x 4096 x 4096 14.2 / 16.3;  too long, 504 x 4096 x 4096 24.0 / 29.1, 504 x 8192 x 2048 19 / 35.
 struct Cut {
-    int tile;  // rows of x and of w; few rows: 32, 48 (64 and 32) and 64
+    int tile, tile_n;  // rows of x and of w; few rows: 32, 48 (64 and 32) and 64
     bool fused;  // few rows with GELU: tiles of 32 x 128, the result's blocks made there
     int64_t tiles_m, tiles_n, whole, rest, parts;
 };
@@ -1085,14 +1087,22 @@ Cut cut(int64_t m, int64_t n, int64_t k, bool gelu)
             while (c.tiles_m * c.tiles_n * c.parts * 2 <= 256 && blocks >= c.parts * 2 * 16) c.parts *= 2;
         return c;
     }
-    // Tiles: those past the last full wave of the chip are dealt to its units in parts of
-    // K of at least 8 steps each.
-    c.tile = (m + 255) / 256 * ((n + 255) / 256) >= 192 && k > 128 ? kBig : kTile;
+    // Tiles: the kind whose rounds of the chip take least, at 4, 6 and 7 for one of 128 x 128, 256 x
+    // 128 and 256 x 256 (measured, a round of K 4096: 24, 37 and 41 us; 2.2, 1.7 and 1.3 a step of 32
+    // KB that a unit loads, which bounds the smaller ones).  128 x 128 / 256 x 128 / 256 x 256, us, M x N x K: 1024 x 4096 x
+    // 4096 25 / 32 / -, 2048 x 4096 x 4096 44 / 38 / 49, 1500 x 4096 x 2048 32 / 24 / -, 2304 x 4096 x
+    // 4096 59 / 54 / 42, 4290 x 2048 x 4096 53 / 51 / 40.  Those past the last full round are
+    // dealt to its units in parts of K of at least 8 steps each.
+    c.tile = c.tile_n = kTile;
+    auto rounds = [&](int tm, int tn) { return ((m + tm - 1) / tm * ((n + tn - 1) / tn) + 255) / 256; };
+    int64_t least = 4 * rounds(kTile, kTile);
+    if (6 * rounds(kBig, kTile) < least) least = 6 * rounds(kBig, kTile), c.tile = kBig;
+    if (blocks > 1 && 7 * rounds(kBig, kBig) < least) c.tile = c.tile_n = kBig;
     c.tiles_m = (m + c.tile - 1) / c.tile;
-    c.tiles_n = (n + c.tile - 1) / c.tile;
+    c.tiles_n = (n + c.tile_n - 1) / c.tile_n;
     c.rest = c.tiles_m * c.tiles_n % 256;
     c.whole = c.tiles_m * c.tiles_n - c.rest;
-    if (c.rest) {
+    if (c.rest && c.tile == c.tile_n) {  // the least of 256 x 128, over 256 of 128 x 128, leave no unit two
         c.parts = 256 / c.rest;
         if (c.parts > blocks / 8) c.parts = blocks / 8;
         if (c.parts < 1) c.parts = 1;
@@ -1108,15 +1118,17 @@ int64_t workspace_bytes(int64_t m, int64_t n, int64_t k, bool gelu)
 }
 
 template <bool GELU>
-void tiles(const Fp8Params &p, int tile, hipStream_t s)
+void tiles(const Fp8Params &p, const Cut &c, hipStream_t s)
 {
     const unsigned per = static_cast<unsigned>(p.whole / 8 + p.per);  // of an XCD
-    const unsigned sums = p.parts > 1 ? static_cast<unsigned>(p.rest * tile * tile / 8 / 256) : 0;
-    if (tile == kBig) {
+    const unsigned sums = p.parts > 1 ? static_cast<unsigned>(p.rest * c.tile * c.tile / 8 / 256) : 0;
+    if (c.tile_n == kBig) {
         big_kernel<GELU><<<8 * std::min<unsigned>(kCus, per), kBigWaves * 64, 0, s>>>(p);
         if (sums) tile_sum_kernel<kBig, GELU><<<sums, 256, 0, s>>>(p);
+    } else if (c.tile == kBig) {
+        tile_kernel<kBig, GELU><<<8 * per, kTileWaves * 64, 0, s>>>(p);
     } else {
-        tile_kernel<GELU><<<8 * per, kTileWaves * 64, 0, s>>>(p);
+        tile_kernel<kTile, GELU><<<8 * per, kTileWaves * 64, 0, s>>>(p);
         if (sums) tile_sum_kernel<kTile, GELU><<<sums, 256, 0, s>>>(p);
     }
 }
@@ -1185,7 +1197,7 @@ int linear(const char *what, void *y, void *y_scale, bool gelu, const void *x, c
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (c.tile >= kTile) {
         p.per = static_cast<int>((c.rest * c.parts + 7) / 8);
-        gelu ? tiles<true>(p, c.tile, s) : tiles<false>(p, c.tile, s);
+        gelu ? tiles<true>(p, c, s) : tiles<false>(p, c, s);
     } else if (c.fused) {
         few_rows<Few<1, 2, 3, false, true>>(p, gelu, s);
     } else if (c.tile == 64) {
