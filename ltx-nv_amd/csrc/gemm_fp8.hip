@@ -692,12 +692,12 @@ __global__ void __launch_bounds__(kBigWaves * 64, 1) big_kernel(Fp8Params p)
 #pragma unroll
                         for (int r = 0; r < 16; ++r)
                             if (n0 + ni * 32 + 8 * (r >> 2) + 4 * half >= p.n) g[ni][r] = 0.f;
-                // a NaN does not count in the maximum, and stays one by itself
+                // a NaN comes out of the maximum, so that its block is NaN as a whole
 #pragma unroll
                 for (int ni = 0; ni < NT; ++ni)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(g[ni][r]));
-                const uint32_t t = __float_as_uint(top);
+                    for (int r = 0; r < 16; ++r) top = __builtin_elementwise_maximum(top, fabsf(g[ni][r]));
+                const uint32_t t = magnitude(top);
                 const auto both = __builtin_amdgcn_permlane32_swap(t, t, false, false);
                 const uint32_t scale = fp8_scale(max(static_cast<uint32_t>(both[0]), static_cast<uint32_t>(both[1])));
                 const float inv = fp8_inverse(scale == 255 ? 127 : scale);

@@ -267,6 +267,30 @@ def test_not_finite_stays_in_its_row(m, n, k):
         assert torch.equal(got[~bad_blocks], clean_gelu[~bad_blocks])
 
 
+@pytest.mark.parametrize("m,n,k", [(20, 256, 512), (30, 4096, 16384), (126, 4104, 512), (500, 1024, 512), (1000, 1032, 384),
+                                   (2305, 2056, 1000), (3001, 4104, 264), (4136, 4112, 2056)])
+def test_not_finite_takes_its_block(m, n, k):
+    """A NaN, or an infinity, of the hidden values makes its block of 128 NaN, as in quantize_fp8, whichever kernel
+    writes it; every other block is what it was."""
+    import ltxk
+
+    g = torch.Generator(device=DEV).manual_seed(m + 1)
+    x = torch.randn(m, k, device=DEV, generator=g).to(torch.bfloat16)
+    w = ltxk.quantize_fp8((torch.randn(n, k, device=DEV, generator=g) * k**-0.5).to(torch.bfloat16))
+    bias = torch.randn(n, device=DEV, generator=g).to(torch.bfloat16)
+    clean = ltxk.linear_gelu_fp8(x, w, bias)
+    bias[7], bias[n - 5] = float("nan"), float("inf")
+    got = ltxk.linear_gelu_fp8(x, w, bias)
+    last = (n - 1) // 128 * 128
+    v, want = got.float(), clean.float()
+    assert v[:, :128].isnan().all() and v[:, last:].isnan().all()
+    assert torch.equal(v[:, 128:last], want[:, 128:last])
+    # the bytes themselves: NaN values under scale 255
+    assert ((got.data.view(torch.uint8)[:, :128] & 0x7F) == 0x7F).all()
+    groups = got.scale.transpose(0, 1).reshape(m, -1)
+    assert (groups[:, 0] == 255).all() and (groups[:, last // 128] == 255).all() and not groups[:, last // 128 + 1:].any()
+
+
 @pytest.mark.parametrize("batch,tokens,dim", [(1, 1, 8), (2, 3, 128), (1, 7, 200), (2, 65, 2048), (1, 130, 4096), (3, 5, 4104),
                                               (1, 4, 8192), (1, 3, 16384), (2, 9, 640), (2, 1601, 264),
                                               (1, 900, 2056), (3, 800, 4096)])
@@ -394,3 +418,67 @@ def test_captured_run_replays_equal():
         got = [c.clone() for c in captured]
         for a, b in zip(got, call()):
             assert torch.equal(a, b), f"replay {i}"
+
+
+def test_two_streams_at_once():
+    """Calls on two streams have results and workspaces of their own: cut K, quantised x, blocks of the GELU."""
+    import ltxk
+
+    g = torch.Generator(device=DEV).manual_seed(8)
+    shapes = [(300, 520, 4096), (126, 1024, 16384), (64, 2048, 512)]
+    ops = [(torch.randn(m, k, device=DEV, generator=g).to(torch.bfloat16),
+            ltxk.quantize_fp8(torch.randn(n, k, device=DEV, generator=g).to(torch.bfloat16))) for m, n, k in shapes]
+
+    def run():
+        out = [ltxk.linear_fp8(x, w) for x, w in ops]
+        return out + [t for x, w in ops for b in (ltxk.linear_gelu_fp8(x, w),) for t in (b.data.view(torch.uint8), b.scale)]
+
+    want = run()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(6):
+        for s, o in zip(streams, got):
+            with torch.cuda.stream(s):
+                o.append(run())
+    torch.cuda.synchronize()
+    for runs in got:
+        for r in runs:
+            assert all(torch.equal(a, b) for a, b in zip(want, r))
+
+
+def test_binding_refusals():
+    """What the binding refuses of tensors on the GPU, before any launch."""
+    import ltxk
+
+    x = torch.zeros(6, 256, device=DEV, dtype=torch.bfloat16)
+    w = ltxk.quantize_fp8(torch.zeros(16, 256, device=DEV, dtype=torch.bfloat16))
+    bias = torch.zeros(16, device=DEV, dtype=torch.bfloat16)
+    flat = torch.zeros(6 * 256 + 8, device=DEV, dtype=torch.bfloat16)
+    bad = [
+        (ValueError, lambda: ltxk.quantize_fp8(x.float())), (ValueError, lambda: ltxk.quantize_fp8(x[:, :12].contiguous())),
+        (ValueError, lambda: ltxk.quantize_fp8(x[:, :128])), (RuntimeError, lambda: ltxk.quantize_fp8(flat[1:1537].view(6, 256))),
+        (ValueError, lambda: ltxk.linear_fp8(x[:, :128].contiguous(), w)), (ValueError, lambda: ltxk.linear_fp8(x.half(), w)),
+        (ValueError, lambda: ltxk.linear_fp8(x.t(), w)), (ValueError, lambda: ltxk.linear_fp8(x, w, bias[:8])),
+        (ValueError, lambda: ltxk.linear_fp8(x, w, bias.float())), (RuntimeError, lambda: ltxk.linear_fp8(x, w, bias.cpu())),
+        (RuntimeError, lambda: ltxk.linear_fp8(flat[1:1537].view(6, 256), w)), (TypeError, lambda: ltxk.linear_fp8(x, x)),
+        (TypeError, lambda: ltxk.linear_gelu_fp8([1.0], w)),
+        (ValueError, lambda: ltxk.linear_fp8(x, ltxk.quantize_fp8(torch.zeros(12, 256, device=DEV, dtype=torch.bfloat16)))),
+        (ValueError, lambda: ltxk.Fp8Blocks(w.data, w.scale, (16, 128))), (ValueError, lambda: ltxk.Fp8Blocks(w.data, w.scale, (8, 256))),
+        (ValueError, lambda: ltxk.Fp8Blocks(w.data, w.scale[..., :2], (16, 256))),
+        (ValueError, lambda: ltxk.Fp8Blocks(w.data.view(torch.uint8), w.scale, (16, 256))),
+        (ValueError, lambda: w.view(16, 128)), (ValueError, lambda: w.view(4, 8, 256)),
+        (ValueError, lambda: ltxk.add_norm_modulate_fp8(x, x[:3])), (ValueError, lambda: ltxk.add_norm_modulate_fp8(x, None)),
+        (ValueError, lambda: ltxk.add_norm_modulate_fp8(x, x, x_out=x[:3])),
+        (ValueError, lambda: ltxk.norm_modulate_fp8(x, shift=ltxk.AdaRef(bias.view(1, 16), 0))),
+        (TypeError, lambda: ltxk.cross_attention(x[None], x[None], x[None], 4, [True] * 6)),
+        (ValueError, lambda: ltxk.cross_attention(x[None], x[None], x[None], 4, torch.ones(1, 5, device=DEV, dtype=torch.bool))),
+        (ValueError, lambda: ltxk.cross_attention(x[None], x[None], x[None], 4, torch.ones(1, 6, device=DEV))),
+        (ValueError, lambda: ltxk.cross_attention(x[None], x[None], x[None], 3)),
+        (RuntimeError, lambda: ltxk.cross_attention(x[None], x[None], x[None], 4, torch.ones(1, 6, dtype=torch.bool))),
+    ]
+    for i, (error, call) in enumerate(bad):
+        with pytest.raises(error):
+            call()
+            pytest.fail(f"call {i} was not refused")
+    assert not ltxk.linear_fp8(x, w, bias).any()  # the good call still runs
