@@ -437,24 +437,8 @@ __device__ __forceinline__ void widen(const uint2 &v, float f[4])
     f[3] = __uint_as_float(v.y & 0xffff0000u);
 }
 
-// A 32 x 32 tile whose lane l holds, of row l % 32, columns 8 q + 4 (l / 32) .. + 3 in v[q]: lanes l
-// and l + 32, then l and l + 16, swap, so that lane l holds columns 8 (l / 32) + (l & 16) .. + 7 of
-// rows l % 16 (lo) and l % 16 + 16 (hi): a store of 16 rows of 32 columns each (of 32 rows of 16:
-// 309 against 302 us on [24576, 4096] x 4096).
-__device__ __forceinline__ void rows16(const uint32_t v[4][2], u32x4 &lo, u32x4 &hi)
-{
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-        const auto first = __builtin_amdgcn_permlane32_swap(v[0][e], v[1][e], false, false);
-        const auto second = __builtin_amdgcn_permlane32_swap(v[2][e], v[3][e], false, false);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const auto rows = __builtin_amdgcn_permlane16_swap(first[i], second[i], false, false);
-            lo[2 * i + e] = rows[0], hi[2 * i + e] = rows[1];
-        }
-    }
-}
-__device__ __forceinline__ void rows16(const uint32_t v[4], uint2 &lo, uint2 &hi)
+// rows16 of bytes.
+__device__ __forceinline__ void rows16_bytes(const uint32_t v[4], uint2 &lo, uint2 &hi)
 {
     const auto first = __builtin_amdgcn_permlane32_swap(v[0], v[1], false, false);
     const auto second = __builtin_amdgcn_permlane32_swap(v[2], v[3], false, false);
@@ -710,7 +694,7 @@ __global__ void __launch_bounds__(kBigWaves * 64, 1) big_kernel(Fp8Params p)
                         v[q] = scale == 255 ? 0x7f7f7f7fu : fp8_pack4(f[0], f[1], f[2], f[3], inv);
                     }
                     uint2 lo, hi;
-                    rows16(v, lo, hi);
+                    rows16_bytes(v, lo, hi);
                     const int row = m0 + mi * 32 + (lane & 15), col = n0 + ni * 32 + 8 * half + (lane & 16);
                     if (row < p.m && block <= last) *reinterpret_cast<uint2 *>(p.q + static_cast<int64_t>(row) * p.np + col) = lo;
                     if (row + 16 < p.m && block <= last)
