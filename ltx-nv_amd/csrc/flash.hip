@@ -159,8 +159,10 @@ enum Keys { kAll, kKept, kListed };
 constexpr int kMaxListed = 8192;
 
 // The kept of tk keys in their order into `list`, their count returned: 1024 keys a round,
-// four a thread, each wave's by ballots, the waves' counts added up in LDS (`counts`, 8).
-__device__ __forceinline__ int list_kept(const uint8_t *keep, int tk, uint16_t *list, int *counts)
+// four a thread, each wave's by ballots, the waves' counts added up in LDS (`counts`, 8).  `beside` issues
+// loads behind the first round's.
+template <typename F>
+__device__ __forceinline__ int list_kept(const uint8_t *keep, int tk, uint16_t *list, int *counts, F beside)
 {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const uint64_t below = (uint64_t{1} << lane) - 1;
@@ -170,6 +172,7 @@ __device__ __forceinline__ int list_kept(const uint8_t *keep, int tk, uint16_t *
         uint8_t kept[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) kept[j] = i + j < tk ? keep[i + j] : 0;
+        if (first == 0) beside();
         int at = 0, total = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -213,17 +216,32 @@ __global__ void __launch_bounds__(kWaves * 64, 2) flash_kernel(FlashParams p)
     const int unit = j - p.whole, part = split ? unit % p.parts : 0;
     int b, head, first;
     if (!query_tile(p, xcd, split ? p.whole + unit / p.parts : j, b, head, first)) return;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int l32 = lane & 31, half = lane >> 5;
+
+    // Queries: lane l holds query l % 32, elements 16 s + 8 (l/32) .. + 7.  Where the
+    // keys are listed, their latency lies beside the list's: 4 x 6144 queries over 64 / 1024 keys, all kept,
+    // 32 heads of 128, zeros, 93 / 343 us loaded behind the list, 80 / 330 this way.
+    const int row = first + wave * 32 + l32;
+    bf16x8 qf[KS];
+    auto load_q = [&] {
+        const char *qp = reinterpret_cast<const char *>(p.q + b * p.qbs + head * D) +
+                         static_cast<int64_t>(min(row, p.tq - 1)) * p.qts + half * 16;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const bf16x8 *>(qp + s * 32);
+    };
     __shared__ uint16_t kept[KEYS == kKept ? kMaxListed : 1];
     int keys = p.tk;
-    if constexpr (KEYS == kKept) keys = list_kept(p.keep + b * p.keep_bs, p.tk, kept, reinterpret_cast<int *>(k0));
+    if constexpr (KEYS == kKept)
+        keys = list_kept(p.keep + b * p.keep_bs, p.tk, kept, reinterpret_cast<int *>(k0), load_q);
+    else if constexpr (KEPT)
+        load_q();
     if constexpr (KEYS == kListed) keys = p.count[b];
     const int tiles = KEPT ? (keys + kKeys - 1) / kKeys : p.tiles;
     const int t0 = split ? part * tiles / p.parts : 0;
     const int t1 = split ? (part + 1) * tiles / p.parts : tiles;
     const int n = t1 - t0;  // at least one tile (the host takes no more parts than tiles), but where keys are left out
     const int last = p.tk - 1;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int l32 = lane & 31, half = lane >> 5;
     if constexpr (KEPT) {
         if (n == 0) {  // nothing to attend to: a weight of zero, or an output of zero
             if (split) {
@@ -269,15 +287,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) flash_kernel(FlashParams p)
 #pragma unroll
     for (int c = 0; c < kLoads<D>; ++c) load_k(0, c, k0);
 
-    // Queries: lane l holds query l % 32, elements 16 s + 8 (l/32) .. + 7.
-    const int row = first + wave * 32 + l32;
-    bf16x8 qf[KS];
-    {
-        const char *qp = reinterpret_cast<const char *>(p.q + b * p.qbs + head * D) +
-                         static_cast<int64_t>(min(row, p.tq - 1)) * p.qts + half * 16;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const bf16x8 *>(qp + s * 32);
-    }
+    if constexpr (!KEPT) load_q();
 
     // LDS byte offsets of this lane's fragments.  K: row l % 32 (+ 32 u), chunk
     // 2 s + half.  V (transposed reads of 4 keys x 16 columns by 16 lanes): rows
