@@ -13,7 +13,10 @@ constexpr int kPerCu = 3;   // workgroups a compute unit of the streaming form (
 constexpr int kItems = 64;  // most batch items that it walks
 
 // ------------------------------------------------------------ quantize_fp8 --
-// A wave takes 512 columns (four blocks, 16 lanes of 8 columns each) of a row.
+// A wave takes 512 columns (four blocks, 16 lanes of 8 columns each) of a row.  Bound by memory: [24576, 4096]
+// 60 us, 5.0 TB/s (a large copy 4.9; two rows a wave 57, eight 60), [6144, 4096] 17.5, [1024, 4096] 4.4 (two rows
+// 4.6); read without the streaming hint 61, 18.1 and 5.0; written with it 61, 17.4 and 4.0, but the product that
+// reads it next takes 4 us longer at [6144, 4096].
 struct QuantParams {
     const uint16_t *x;
     uint8_t *q, *scale;
@@ -31,7 +34,7 @@ __global__ void __launch_bounds__(kBlock) quantize_kernel(QuantParams p)
     if (group >= p.groups) return;
     const int col = group * 512 + lane * 8;
     u32x4 raw = {};
-    if (col < p.k) raw = *reinterpret_cast<const u32x4 *>(p.x + row * p.k + col);
+    if (col < p.k) raw = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p.x + row * p.k + col));
     float f[8];
     unpack8v(raw, f);
     uint32_t scale;
