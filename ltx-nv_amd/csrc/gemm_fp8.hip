@@ -1088,7 +1088,9 @@ Cut cut(int64_t m, int64_t n, int64_t k, bool gelu)
     // KB that a unit loads, which bounds the smaller ones).  128 x 128 / 256 x 128 / 256 x 256, us, M x N x K: 1024 x 4096 x
     // 4096 25 / 32 / -, 2048 x 4096 x 4096 44 / 38 / 49, 1500 x 4096 x 2048 32 / 24 / -, 2304 x 4096 x
     // 4096 59 / 54 / 42, 4290 x 2048 x 4096 53 / 51 / 40.  Those past the last full round are
-    // dealt to its units in parts of K of at least 8 steps each.
+    // dealt to its units in parts of K where that saves more than it takes.  Two parts / whole: 1024 x 2048 x 2048
+    // 22.6 / 13.3, 6144 x 4096 x 2048 68 / 55, 6144 x 4096 x 4096 100 / 96, 777 x 2048 x 4096 22 / 23, 1024 x 1536 x
+    // 8192 29 / 40;  four / whole: 4290 x 4096 x 4096 74 / 88.
     c.tile = c.tile_n = kTile;
     auto rounds = [&](int tm, int tn) { return ((m + tm - 1) / tm * ((n + tn - 1) / tn) + 255) / 256; };
     int64_t least = 4 * rounds(kTile, kTile);
@@ -1099,9 +1101,14 @@ Cut cut(int64_t m, int64_t n, int64_t k, bool gelu)
     c.rest = c.tiles_m * c.tiles_n % 256;
     c.whole = c.tiles_m * c.tiles_n - c.rest;
     if (c.rest && c.tile == c.tile_n) {  // the least of 256 x 128, over 256 of 128 x 128, leave no unit two
-        c.parts = 256 / c.rest;
-        if (c.parts > blocks / 8) c.parts = blocks / 8;
-        if (c.parts < 1) c.parts = 1;
+        // what the parts save of a tile's steps (us), less what their sums take: a launch, written and read
+        const double step = c.tile == kBig ? 1.3 : 0.75, sums = 2.0 * c.tile * c.tile * 4 * 1e-6 / 4;
+        double most = 0;
+        for (int64_t p = 2; p <= 256 / c.rest && p * 4 <= blocks; ++p) {
+            const double saved = step * static_cast<double>(blocks) * (1.0 - 1.0 / static_cast<double>(p)) - 3.0 -
+                                 sums * static_cast<double>(c.rest * p);
+            if (saved > most) most = saved, c.parts = p;
+        }
     }
     return c;
 }

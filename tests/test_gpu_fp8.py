@@ -217,10 +217,11 @@ def test_linear_gelu_matches_fp64(m, n, k, bias):
 
 # Every way that a product is cut: 32 rows that are quantised in the call, a tile of several and over a cut K; K one
 # value past what is; 64 x 32 and 64 x 64 tiles over a cut K; GELU in tiles of 32 x 128, of one block and at both its
-# borders; 256 x 128 tiles of odd sizes, and of one block; large tiles of two steps, of an odd rest whole and in parts.
+# borders; 256 x 128 tiles of odd sizes, and of one block; large tiles of two steps, of an odd rest whole and in parts; 128 x 128 tiles in parts.
 VARIANTS = [(100, 256, 128), (64, 512, 376), (126, 2040, 512), (1, 1024, 17152), (1, 1024, 17160), (31, 520, 16384),
             (126, 1024, 16384), (250, 1160, 16392), (1, 8, 24),
-            (70, 1000, 512), (252, 4104, 2056), (252, 4096, 4096), (97, 12280, 1000), (520, 712, 648), (2100, 4200, 2568), (2305, 2056, 1000), (3001, 4104, 120), (3001, 4104, 136), (8200, 2056, 520), (4136, 4112, 2056)]
+            (70, 1000, 512), (252, 4104, 2056), (252, 4096, 4096), (97, 12280, 1000), (520, 712, 648), (2100, 4200, 2568), (2305, 2056, 1000), (3001, 4104, 120), (3001, 4104, 136), (8200, 2056, 520), (4136, 4112, 2056),
+            (900, 1544, 8200), (4100, 4104, 4104)]
 
 
 @pytest.mark.parametrize("m,n,k", VARIANTS)
