@@ -12,10 +12,10 @@
 //
 // What bounds it, by the rows of x: memory up to about 32 (the weights are read once: 4 x 36864 x
 // 4096 of 151 MB in 31 us, 4.8 TB/s, what a large copy reaches); the latency of a launch's one round
-// up to a few hundred (126 x 2048 x 2048 in 5 us); the way from the L2 to LDS for one round of tiles (1024 x
-// 4096 x 4096 in 24 us, 268 MB of it, on zeros 24 too); the card's power beyond (24576 x 4096 x 4096 in
-// 312 us, 2.65 PFLOP/s, on zeros 227 us, 3.63; the library's product with a single scale for
-// each operand 292 and 212).
+// up to a few hundred (126 x 2048 x 2048 in 5 us); for one round of tiles its first loads, stores and launch, about 8 us,
+// and LDS, whose reads and writes take 0.32 us of a step's 0.46 (1024 x 4096 x 4096 in 24 us, on zeros 22); the
+// card's power beyond (24576 x 4096 x 4096 in 312 us, 2.65 PFLOP/s, on zeros 227 us, 3.63; the library's
+// product with a single scale for each operand 292 and 212).
 #include "fp8_blocks.h"
 
 #include <algorithm>
@@ -114,8 +114,8 @@ __device__ __forceinline__ void tile_rows(const Fp8Params &p, int t, int &m0, in
 }
 
 // Tiles of TM x 128, four waves of TM / 2 x 64, the steps of 128 values as deep in LDS as fit.
-// Two teams of four waves that take turns at the steps (two waves a SIMD) are 2-6 % slower: the loads
-// bound it, not their latency.
+// Two teams of four waves that take turns at the steps (two waves a SIMD) are 2-6 % slower: LDS bounds
+// a step, not the loads' latency.
 constexpr int kTile = 128, kTileWaves = 4;
 
 template <int TM, bool GELU>
@@ -1084,8 +1084,7 @@ Cut cut(int64_t m, int64_t n, int64_t k, bool gelu)
         return c;
     }
     // Tiles: the kind whose rounds of the chip take least, at 4, 6 and 7 for one of 128 x 128, 256 x
-    // 128 and 256 x 256 (measured, a round of K 4096: 24, 37 and 41 us; 2.2, 1.7 and 1.3 a step of 32
-    // KB that a unit loads, which bounds the smaller ones).  128 x 128 / 256 x 128 / 256 x 256, us, M x N x K: 1024 x 4096 x
+    // 128 and 256 x 256 (a round of K 4096: 24, 37 and 41 us).  128 x 128 / 256 x 128 / 256 x 256, us, M x N x K: 1024 x 4096 x
     // 4096 25 / 32 / -, 2048 x 4096 x 4096 44 / 38 / 49, 1500 x 4096 x 2048 32 / 24 / -, 2304 x 4096 x
     // 4096 59 / 54 / 42, 4290 x 2048 x 4096 53 / 51 / 40.  Those past the last full round are
     // dealt to its units in parts of K where that saves more than it takes.  Two parts / whole: 1024 x 2048 x 2048
