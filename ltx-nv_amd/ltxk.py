@@ -922,17 +922,18 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: int, log
 def _attention_rows(x: torch.Tensor, name: str, b: int, t: int, d: int) -> tuple[int, int]:
     """(batch stride, token stride) of a bf16 (b, t, d) whose rows are contiguous, or an error.  A stride that is never
     taken (one token, one batch item) may be anything in torch: the contiguous one stands for it."""
-    if not isinstance(x, torch.Tensor):
-        raise TypeError(f"{name} must be a torch.Tensor")
-    if x.device.type != "cuda":
-        raise RuntimeError(f"{name} is on {x.device}; ltxk kernels run on the ROCm device only")
-    if x.dtype != torch.bfloat16:
-        raise ValueError(f"{name} has dtype {x.dtype}, expected torch.bfloat16")
-    if x.shape != (b, t, d):
-        raise ValueError(f"{name} is {tuple(x.shape)}, expected {(b, t, d)}")
-    if x.is_contiguous():
-        return t * d, d
+    if not (type(x) is torch.Tensor and x.is_cuda and x.dtype == torch.bfloat16 and x.shape == (b, t, d)):
+        if not isinstance(x, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor")
+        if x.device.type != "cuda":
+            raise RuntimeError(f"{name} is on {x.device}; ltxk kernels run on the ROCm device only")
+        if x.dtype != torch.bfloat16:
+            raise ValueError(f"{name} has dtype {x.dtype}, expected torch.bfloat16")
+        if x.shape != (b, t, d):
+            raise ValueError(f"{name} is {tuple(x.shape)}, expected {(b, t, d)}")
     sb, st, sd = x.stride()
+    if sd == 1 and st == d and sb == t * d:
+        return sb, st
     sb, st = sb if b > 1 else 0, st if t > 1 else d
     if sd != 1 or sb % 8 or st % 8 or st < d:
         raise ValueError(f"{name}'s rows must be contiguous, with batch and token strides (multiples of 8) that cover "
@@ -974,7 +975,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: in
         if logits.shape != (b, tq, heads):
             raise ValueError(f"logits {tuple(logits.shape)} != {(b, tq, heads)}")
     if out is None:
-        out = torch.empty((b, tq, d), device=q.device, dtype=q.dtype)
+        out = q.new_empty((b, tq, d))
     else:
         _dev(out, "out")
         if out.shape != (b, tq, d):
@@ -1183,7 +1184,7 @@ def _fp8_linear(x, weight: Fp8Blocks, bias: torch.Tensor | None, gelu: bool):
     if gelu:
         out = Fp8Blocks._made((*lead, n), w.device)
     else:
-        out = torch.empty((*lead, n), device=w.device, dtype=torch.bfloat16)
+        out = torch.empty((*lead, n), device=w.device, dtype=torch.bfloat16) if held else x.new_empty((*lead, n))
     nbytes = _fp8_workspace_bytes(m, n, k, gelu, not held)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=w.device) if nbytes else None
     lib = load()
