@@ -1072,11 +1072,11 @@ class Fp8Blocks:
     def float(self) -> torch.Tensor:
         """The values held, in fp32 (exact but where they leave fp32's range), by torch operations."""
         rows, blocks = _fp8_extent(self.shape)
-        e = self.scale.transpose(0, 1).reshape(rows, -1)[:, :blocks, None].to(torch.int32)
+        e = self.scale.transpose(0, 1).reshape(rows, -(-blocks // FP8_GROUP) * FP8_GROUP)[:, :blocks, None].to(torch.int32)
         power = torch.where(e == 0, 1 << 22, e << 23).view(torch.float32)  # 2^(e - 127), 2^-127 a subnormal; 255: infinite
         v = self.data.float().view(rows, blocks, FP8_BLOCK) * power
         v = v.masked_fill(e == 255, float("nan"))
-        return v.reshape(rows, -1)[:, :self.shape[-1]].reshape(self.shape)
+        return v.reshape(rows, blocks * FP8_BLOCK)[:, :self.shape[-1]].reshape(self.shape)
 
     def view(self, *shape) -> "Fp8Blocks":
         """The same rows under another leading shape."""

@@ -483,3 +483,26 @@ def test_binding_refusals():
             call()
             pytest.fail(f"call {i} was not refused")
     assert not ltxk.linear_fp8(x, w, bias).any()  # the good call still runs
+
+
+def test_blocks_as_tensors():
+    """Blocks that a kernel made give their tensors when asked, also without rows and past the object's life; a quantised
+    weight's two tensors share no memory, so that they can be saved apart; views hold the same bytes."""
+    import ltxk
+
+    x = torch.randn(6, 264, device=DEV).to(torch.bfloat16)
+    w = ltxk.quantize_fp8(torch.randn(520, 264, device=DEV).to(torch.bfloat16))
+    assert w.data.untyped_storage().data_ptr() != w.scale.untyped_storage().data_ptr()
+    made = ltxk.linear_gelu_fp8(x, w)
+    assert made.data.shape == (6, 640) and made.scale.shape == (2, 6, 4) and made.device == x.device
+    other = ltxk.Fp8Blocks(made.data.clone(), made.scale.clone(), made.shape)
+    w2 = ltxk.quantize_fp8(torch.randn(16, 520, device=DEV).to(torch.bfloat16))
+    want = ltxk.linear_fp8(other, w2)
+    assert torch.equal(ltxk.linear_fp8(made, w2), want)
+    assert torch.equal(ltxk.linear_fp8(made.view(2, 3, 520), w2), want.view(2, 3, 16))
+    data, scale = made.data, made.scale
+    del made
+    assert torch.equal(data.view(torch.uint8), other.data.view(torch.uint8)) and torch.equal(scale, other.scale)
+    empty = ltxk.linear_gelu_fp8(x[:0], w)
+    assert empty.data.shape == (0, 640) and empty.scale.shape == (2, 0, 4) and empty.float().shape == (0, 520)
+    assert ltxk.linear_fp8(empty, w2).shape == (0, 16)
