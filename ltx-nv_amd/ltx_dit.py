@@ -498,6 +498,8 @@ class Block(torch.nn.Module):
             norm_x = ltxk.norm_modulate(x, shift=_ada(sst, 0, ts), scale=_ada(sst, 1, ts), eps=eps)
         out = attn1(norm_x, pe=args.pe, mask=args.self_attention_mask,
                     perturbation_mask=args.self_attn_perturbation_mask, all_perturbed=args.self_attn_all_perturbed)
+        # a module in attn2's place may take the reference's arguments only
+        keep = {} if args.context_keep is None else {"keep": args.context_keep}
         if cross_adaln:
             x_fma, q_in = ltxk.add_norm_modulate(x, out, gate=_ada(sst, 2, ts), shift=_ada(sst, 6, ts),
                                                  scale=_ada(sst, 7, ts), eps=eps)
@@ -506,10 +508,10 @@ class Block(torch.nn.Module):
                 kv_shift = _ada(prompt_sst, 0, args.prompt_timestep)
                 kv_scale = _ada(prompt_sst, 1, args.prompt_timestep)
                 enc = ltxk.modulate(_bf16(args.context), shift=kv_shift, scale=kv_scale)
-            out2 = attn2(q_in, context=enc, mask=args.context_mask, keep=args.context_keep)
+            out2 = attn2(q_in, context=enc, mask=args.context_mask, **keep)
             return x_fma, out2, _ada(sst, 8, ts)
         x_fma, x_normed = ltxk.add_norm_modulate(x, out, gate=_ada(sst, 2, ts), eps=eps)
-        return x_fma, attn2(x_normed, context=args.context, mask=args.context_mask, keep=args.context_keep), None
+        return x_fma, attn2(x_normed, context=args.context, mask=args.context_mask, **keep), None
 
     @staticmethod
     def _settle(x: torch.Tensor, args: TransformerArgs) -> torch.Tensor:
@@ -700,7 +702,7 @@ class Block(torch.nn.Module):
         Returns (x, None), or (x without the FFN residual, (ffn_out, gate)) when deferring."""
         eps = self.norm_eps
         shift, scale, gate = _ada(sst, 3, ts), _ada(sst, 4, ts), _ada(sst, 5, ts)
-        if ff.takes_blocks:  # the norm writes what the 8-bit layer reads
+        if type(ff) is FeedForward and ff.takes_blocks:  # the norm writes what the 8-bit layer reads
             if pending is not None:
                 out, cgate, mask = pending
                 x, h = ltxk.add_norm_modulate_fp8(x, out, gate=cgate, mask=mask, shift=shift, scale=scale, eps=eps)
