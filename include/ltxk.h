@@ -431,7 +431,7 @@ int ltxk_linear_layers(void *const *y, const void *x, const void *const *w, cons
  * largest magnitude of a block and e the least integer with a <= 448 * 2^e, at
  * least -127, a value x is held as q = e4m3(x * 2^-e) (to nearest even), which
  * stands for q * 2^e.  An infinity or NaN makes its whole block NaN.  In memory:
- *   values  [rows, 128*blocks] bytes, blocks = ceil(k/128), zeros past k
+ *   values  [rows, 128*blocks] bytes, blocks = ceil(k/128), zeros past k (but in a NaN block)
  *   scales  [ceil(blocks/4), rows, 4] bytes: e + 127 of block 4*i + j of a row
  *           (255: a NaN block; zeros past the last block)
  * Both 16-byte aligned. */

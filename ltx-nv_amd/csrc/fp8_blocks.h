@@ -10,10 +10,10 @@
 // subnormal range starts up to one binade higher.  And the matrix cores take such
 // scales as operands of the product.  An infinity or NaN makes its whole block NaN.
 //
-// In memory: values (rows, 128 * blocks) bytes, zeros past k; scales e + 127, one
-// byte a block (255: a NaN block), as (ceil(blocks / 4), rows, 4) bytes, so that the
-// scales of neighbouring rows over four blocks are contiguous: a tile's scales are
-// one load, and a lane's four blocks one register.
+// In memory: values (rows, 128 * blocks) bytes, zeros past k (but in a NaN block);
+// scales e + 127, one byte a block (255: a NaN block), as (ceil(blocks / 4), rows, 4)
+// bytes, so that the scales of neighbouring rows over four blocks are contiguous: a
+// tile's scales are one load, and a lane's four blocks one register.
 #pragma once
 
 #include "ltxk_common.h"

@@ -148,9 +148,10 @@ __global__ void __launch_bounds__(kBlock) add_norm_stream_kernel(NormParams p)
             if constexpr (RESIDUAL) ada_load8(p.gate, b, 0, lo, in ? col : 0, 1.f, gt[k]);
             ada_load8(p.shift, b, 0, lo, in ? col : 0, 0.f, sh[k]);
             ada_load8(p.scale, b, 0, lo, in ? col : 0, 0.f, sc[k]);
+            if constexpr (RESIDUAL)
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (!in) sh[k][j] = 0.f;  // the columns past the last are zeros (their x is)
+                for (int j = 0; j < 8; ++j)
+                    if (!in) gt[k][j] = 0.f;  // nothing of column 0's reaches the sum of squares
         }
         const float m = RESIDUAL && p.mask ? bf16_to_f32(p.mask[b]) : 1.f;
         auto step = [&](u32x4 (&x)[C], u32x4 (&f)[C]) __attribute__((always_inline)) {
@@ -186,8 +187,9 @@ __global__ void __launch_bounds__(kBlock) add_norm_stream_kernel(NormParams p)
             for (int k = 0; k < C; ++k) {
                 const int col = (lane + k * kBlock) * 8;
                 float o[8];
+                // zeros past the last column, whatever the row's norm and the modulation are
 #pragma unroll
-                for (int j = 0; j < 8; ++j) o[j] = v[k][j] * rs * (1.f + sc[k][j]) + sh[k][j];
+                for (int j = 0; j < 8; ++j) o[j] = col < p.dim ? v[k][j] * rs * (1.f + sc[k][j]) + sh[k][j] : 0.f;
                 uint32_t scale;
                 const uint2 q = fp8_quantize8(o, scale);
                 if (col < p.kp) *reinterpret_cast<uint2 *>(p.q + static_cast<int64_t>(r) * p.kp + col) = q;

@@ -506,3 +506,40 @@ def test_blocks_as_tensors():
     empty = ltxk.linear_gelu_fp8(x[:0], w)
     assert empty.data.shape == (0, 640) and empty.scale.shape == (2, 0, 4) and empty.float().shape == (0, 520)
     assert ltxk.linear_fp8(empty, w2).shape == (0, 16)
+
+
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("dim", [8, 136, 520, 1032, 2056, 4040])
+def test_norm_padding_beside_values_not_finite(dim, residual):
+    """Rows with a NaN or an infinity, and an infinite modulation of the first column: the columns past the last are
+    zeros in every row all the same (7f in a block that is NaN as a whole), so the last block is NaN for values of
+    its own only, the scale bytes past it are zero, and many rows (which workgroups walk) hold the bytes that
+    few rows (a workgroup each) do."""
+    import ltxk
+
+    g = torch.Generator(device=DEV).manual_seed(dim)
+    tokens, blocks = 1100, -(-dim // 128)
+    x, f = (torch.randn(1, tokens, dim, device=DEV, generator=g).to(torch.bfloat16) for _ in range(2))
+    x[0, 3, 1], x[0, 900, dim - 1], x[0, 1099, 0] = float("nan"), float("inf"), float("-inf")
+    f[0, 5, 2], f[0, 6, 0] = float("nan"), 0.0
+
+    def call(lo, hi, gate, shift, scale):
+        part = [t[:, lo:hi].contiguous() for t in (x, f)]
+        mods = dict(shift=ltxk.AdaRef(shift, 0), scale=ltxk.AdaRef(scale, 0))
+        if residual:
+            return ltxk.add_norm_modulate_fp8(*part, gate=ltxk.AdaRef(gate, 0), **mods)[1]
+        return ltxk.norm_modulate_fp8(part[0], **mods)
+
+    for which in ("none", "gate", "shift", "scale"):
+        mods = {name: torch.full((1, dim), 0.5, dtype=torch.bfloat16, device=DEV) for name in ("gate", "shift", "scale")}
+        if which != "none":
+            mods[which][0, 0] = float("inf")
+        many = call(0, tokens, **mods)
+        scale = many.scale.transpose(0, 1).reshape(tokens, -1)
+        assert not scale[:, blocks:].any(), which
+        tail, bad = many.data.view(torch.uint8)[:, dim:], scale[:, blocks - 1] == 255
+        assert not tail[~bad].any(), which
+        for lo in (0, 400, 898, 1092):
+            few = call(lo, lo + 8, **mods)
+            assert torch.equal(few.scale, many.scale[:, lo:lo + 8]), (which, lo)
+            assert torch.equal(few.data.view(torch.uint8), many.data.view(torch.uint8)[lo:lo + 8]), (which, lo)
