@@ -36,7 +36,7 @@ import torch
 import ltxk
 from common import DEVICE, load_state_dict, read_metadata
 from ltx_nn import (AdaLayerNormSingle, Attention, FeedForward, precompute_freqs_cis, precompute_freqs_cis_compact,
-                    project)
+                    project, reads_blocks)
 from torch_rng import TorchRNG
 
 # ---------------------------------------------------------------------------
@@ -702,7 +702,7 @@ class Block(torch.nn.Module):
         Returns (x, None), or (x without the FFN residual, (ffn_out, gate)) when deferring."""
         eps = self.norm_eps
         shift, scale, gate = _ada(sst, 3, ts), _ada(sst, 4, ts), _ada(sst, 5, ts)
-        if type(ff) is FeedForward and ff.takes_blocks:  # the norm writes what the 8-bit layer reads
+        if reads_blocks(ff):  # the norm writes what the 8-bit layer reads
             if pending is not None:
                 out, cgate, mask = pending
                 x, h = ltxk.add_norm_modulate_fp8(x, out, gate=cgate, mask=mask, shift=shift, scale=scale, eps=eps)

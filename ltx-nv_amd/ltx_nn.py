@@ -495,19 +495,26 @@ def project(x: torch.Tensor, *layers: torch.nn.Linear | None) -> list:
             weights, biases = zip(*plain)
             done = iter(ltxk._launch_layers(x, weights, biases))
             return [None if layer is None else next(done) for layer in layers]
-    if sum(type(layer) is Fp8Linear for layer in real) > 1:
-        blocks = _fp8_input(x)  # quantised once for all of them
-        return [None if layer is None else layer(blocks) if type(layer) is Fp8Linear else linear(layer, x)
-                for layer in layers]
+    shares = [type(layer) is Fp8Linear and _unwatched(layer) for layer in layers]
+    if sum(shares) > 1:
+        _no_gradient(x)
+        blocks = ltxk.quantize_fp8(x.contiguous())  # once for all of them
+        return [None if layer is None else layer(blocks) if share else linear(layer, x)
+                for layer, share in zip(layers, shares)]
     return [None if layer is None else linear(layer, x) for layer in layers]
 
 
-def _fp8_input(x: torch.Tensor | ltxk.Fp8Blocks) -> ltxk.Fp8Blocks:
-    """x in blocks; refuses to lose a gradient."""
-    if isinstance(x, ltxk.Fp8Blocks):
-        return x
-    _no_gradient(x)
-    return ltxk.quantize_fp8(x.contiguous())
+def _unwatched(module: torch.nn.Module) -> bool:
+    """Whether a call of the module is its class's forward and nothing else: no hooks, its
+    own or every module's, and no patched forward.  Blocks of 8-bit values stay between such modules."""
+    own = module.__dict__
+    return not (own["_forward_hooks"] or own["_forward_pre_hooks"] or "forward" in own or _has_any_global_hook())
+
+
+def reads_blocks(ff: torch.nn.Module) -> bool:
+    """Whether a block hands `ff` its input as ltxk.Fp8Blocks: the framework's feed-forward of
+    8-bit layers, unwatched."""
+    return type(ff) is FeedForward and ff.takes_blocks and _unwatched(ff)
 
 
 def _no_gradient(x: torch.Tensor) -> None:
@@ -696,11 +703,12 @@ class FeedForward(torch.nn.Module):
 
     @property
     def takes_blocks(self) -> bool:
-        """Both layers are 8-bit ones: the input may be ltxk.Fp8Blocks."""
-        return type(self.proj_in) is Fp8Linear and type(self.proj_out) is Fp8Linear
+        """Both layers are 8-bit ones that no hook or patched forward watches: the input may be
+        ltxk.Fp8Blocks, and the hidden values are."""
+        return all(type(layer) is Fp8Linear and _unwatched(layer) for layer in (self.proj_in, self.proj_out))
 
     def forward(self, x: torch.Tensor | ltxk.Fp8Blocks) -> torch.Tensor:
-        if self.takes_blocks:  # the hidden values go from layer to layer in blocks
+        if self.takes_blocks:
             return self.proj_out(self.proj_in.gelu(x))
         hdn = linear(self.proj_in, x)
         ltxk.gelu_tanh(hdn, out=hdn)
