@@ -542,7 +542,10 @@ class Fp8Linear(torch.nn.Module):
 
     @classmethod
     def of(cls, layer: torch.nn.Linear) -> "Fp8Linear":
-        """An 8-bit layer from a bf16 one on the GPU."""
+        """An 8-bit layer from a bare bf16 one on the GPU."""
+        if not _bare_linear(layer):
+            raise ValueError("an 8-bit layer is made of a bare torch.nn.Linear of its own shapes: hooks, patched forwards and "
+                             "replaced operands would be lost")
         made = cls(layer.in_features, layer.out_features, layer.bias is not None, device=layer.weight.device)
         blocks = ltxk.quantize_fp8(layer.weight.detach().contiguous())
         made.weight, made.weight_scale = blocks.data.view(torch.uint8), blocks.scale
@@ -568,16 +571,30 @@ class Fp8Linear(torch.nn.Module):
         return ltxk.linear_gelu_fp8(x, self.blocks(), self.bias)
 
 
+def _bare_linear(layer: torch.nn.Module) -> bool:
+    """Whether weight and bias are all that a layer is: a torch.nn.Linear without hooks, a patched
+    forward, parametrizations or operands of other shapes than its own."""
+    if type(layer) is not torch.nn.Linear:
+        return False
+    own, n = layer.__dict__, layer.out_features
+    if any(own[hooks] for hooks in ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks")) \
+            or "forward" in own or "weight" in own or "bias" in own:
+        return False
+    w, b = own["_parameters"].get("weight"), own["_parameters"].get("bias", False)
+    return type(w) in _PLAIN and w.shape == (n, layer.in_features) and (b is None or type(b) in _PLAIN and b.shape == (n,))
+
+
 def quantize_fp8(module: torch.nn.Module) -> torch.nn.Module:
     """Turns the query, key, value and output layers of every Attention in `module` and both layers of every
     FeedForward into 8-bit ones, in place, and returns it: a model on the GPU in bf16, its weights loaded.  Norms,
-    modulations, gates (a few columns each), embeddings and the layers in front of and behind the blocks stay bf16."""
+    modulations, gates (a few columns each), embeddings and the layers in front of and behind the blocks stay bf16, and
+    so do layers that something hangs on (hooks, a patched forward, parametrizations) or whose widths are no multiples of 8."""
     for part in list(module.modules()):
         names = ("to_q", "to_k", "to_v", "to_out") if isinstance(part, Attention) else \
             ("proj_in", "proj_out") if isinstance(part, FeedForward) else ()
         for name in names:
             layer = getattr(part, name)
-            if type(layer) is torch.nn.Linear and layer.in_features % 8 == 0 and layer.out_features % 8 == 0:
+            if _bare_linear(layer) and layer.in_features % 8 == 0 and layer.out_features % 8 == 0:
                 setattr(part, name, Fp8Linear.of(layer))
     return module
 

@@ -96,3 +96,33 @@ def test_hooks_on_a_blocks_feed_forward():
     with torch.no_grad():
         model(v, a, None)
     assert all(seen == TENSORS for seen, _ in hooks)
+
+
+def test_layers_that_hooks_watch_stay_bf16():
+    """A layer with hooks, a patched forward or a replaced operand is not converted, and Fp8Linear.of refuses it: what
+    hangs on it would be lost."""
+    import ltx_nn
+
+    def patched(ff):
+        ff.proj_in.forward = lambda x: x
+
+    def hooked(ff):
+        ff.proj_in.register_forward_hook(lambda *_: None)
+
+    def before(ff):
+        ff.proj_in.register_forward_pre_hook(lambda *_: None)
+
+    def parametrized(ff):
+        torch.nn.utils.parametrizations.weight_norm(ff.proj_in)
+
+    def broadcast(ff):
+        ff.proj_in.bias = torch.nn.Parameter(torch.zeros(1, device=DEV, dtype=BF16))
+
+    for change in (patched, hooked, before, parametrized, broadcast):
+        ff = ltx_nn.FeedForward(128).to(DEV, BF16).requires_grad_(False)
+        change(ff)
+        kept = ff.proj_in
+        ltx_nn.quantize_fp8(ff)
+        assert ff.proj_in is kept and type(ff.proj_out) is ltx_nn.Fp8Linear and not ff.takes_blocks, change.__name__
+        with pytest.raises(ValueError, match="bare"):
+            ltx_nn.Fp8Linear.of(kept)
