@@ -546,12 +546,13 @@ class Fp8Linear(torch.nn.Module):
         if not _bare_linear(layer):
             raise ValueError("an 8-bit layer is made of a bare torch.nn.Linear of its own shapes: hooks, patched forwards and "
                              "replaced operands would be lost")
+        _check_bf16(layer, "the layer")
         made = cls(layer.in_features, layer.out_features, layer.bias is not None, device=layer.weight.device)
         blocks = ltxk.quantize_fp8(layer.weight.detach().contiguous())
         made.weight, made.weight_scale = blocks.data.view(torch.uint8), blocks.scale
         if layer.bias is not None:
             made.bias = layer.bias.detach().clone()
-        return made
+        return made.train(layer.training)
 
     def blocks(self) -> ltxk.Fp8Blocks:
         return ltxk.Fp8Blocks(self.weight.view(torch.float8_e4m3fn), self.weight_scale,
@@ -584,18 +585,32 @@ def _bare_linear(layer: torch.nn.Module) -> bool:
     return type(w) in _PLAIN and w.shape == (n, layer.in_features) and (b is None or type(b) in _PLAIN and b.shape == (n,))
 
 
+def _check_bf16(layer: torch.nn.Linear, name: str) -> None:
+    for t in (layer.weight, layer.bias):
+        if t is not None and not (t.is_cuda and t.dtype == torch.bfloat16):
+            raise ValueError(f"{name} holds {t.dtype} on {t.device}: 8-bit layers are made of bf16 ones on the GPU")
+
+
 def quantize_fp8(module: torch.nn.Module) -> torch.nn.Module:
     """Turns the query, key, value and output layers of every Attention in `module` and both layers of every
     FeedForward into 8-bit ones, in place, and returns it: a model on the GPU in bf16, its weights loaded.  Norms,
     modulations, gates (a few columns each), embeddings and the layers in front of and behind the blocks stay bf16, and
     so do layers that something hangs on (hooks, a patched forward, parametrizations) or whose widths are no multiples of 8."""
-    for part in list(module.modules()):
+    found = []
+    for path, part in module.named_modules():
         names = ("to_q", "to_k", "to_v", "to_out") if isinstance(part, Attention) else \
             ("proj_in", "proj_out") if isinstance(part, FeedForward) else ()
         for name in names:
             layer = getattr(part, name)
-            if _bare_linear(layer) and layer.in_features % 8 == 0 and layer.out_features % 8 == 0:
-                setattr(part, name, Fp8Linear.of(layer))
+            if not (_bare_linear(layer) and layer.in_features % 8 == 0 and layer.out_features % 8 == 0):
+                continue
+            _check_bf16(layer, f"{path}.{name}" if path else name)  # before any layer is replaced
+            found.append((part, name, id(layer)))
+    made = {}  # of layers that several parts share one
+    for part, name, layer in found:
+        if layer not in made:
+            made[layer] = Fp8Linear.of(getattr(part, name))
+        setattr(part, name, made[layer])
     return module
 
 
