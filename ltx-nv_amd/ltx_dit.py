@@ -702,7 +702,7 @@ class Block(torch.nn.Module):
         Returns (x, None), or (x without the FFN residual, (ffn_out, gate)) when deferring."""
         eps = self.norm_eps
         shift, scale, gate = _ada(sst, 3, ts), _ada(sst, 4, ts), _ada(sst, 5, ts)
-        if reads_blocks(ff):  # the norm writes what the 8-bit layer reads
+        if reads_blocks(ff, x, None if pending is None else pending[0]):  # the norm writes what the 8-bit layer reads
             if pending is not None:
                 out, cgate, mask = pending
                 x, h = ltxk.add_norm_modulate_fp8(x, out, gate=cgate, mask=mask, shift=shift, scale=scale, eps=eps)

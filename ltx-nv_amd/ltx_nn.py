@@ -83,6 +83,7 @@ def key_split_partials(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, parts:
 
 _dispatch_modes, _transform = torch._C._len_torch_dispatch_stack, torch._C._functorch.peek_interpreter_stack
 _tracing = torch._C._is_tracing
+_wrapped = torch._C._functorch.is_functorch_wrapped_tensor
 
 
 def eager_call() -> bool:
@@ -511,15 +512,31 @@ def _unwatched(module: torch.nn.Module) -> bool:
     return not (own["_forward_hooks"] or own["_forward_pre_hooks"] or "forward" in own or _has_any_global_hook())
 
 
-def reads_blocks(ff: torch.nn.Module) -> bool:
-    """Whether a block hands `ff` its input as ltxk.Fp8Blocks: the framework's feed-forward of
-    8-bit layers, unwatched."""
-    return type(ff) is FeedForward and ff.takes_blocks and _unwatched(ff)
+def reads_blocks(ff: torch.nn.Module, *inputs: torch.Tensor | None) -> bool:
+    """Whether a block hands `ff` its input as ltxk.Fp8Blocks made of `inputs`: the framework's
+    feed-forward of 8-bit layers, unwatched.  Nothing may be recorded of them then, as of a
+    tensor handed to the layers (`_no_gradient`)."""
+    if not (type(ff) is FeedForward and ff.takes_blocks and _unwatched(ff)):
+        return False
+    _no_gradient(*inputs)
+    return True
 
 
-def _no_gradient(x: torch.Tensor) -> None:
-    if x.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("8-bit layers are for inference: they record no gradient (run under torch.no_grad())")
+def _no_gradient(*inputs: torch.Tensor | None) -> None:
+    """Refuses inputs of 8-bit layers that something is to be recorded of: a gradient, a
+    forward-mode tangent, what a function transform or a tracer sees.  All would be lost."""
+    lost = "trace" if _tracing() else None
+    for x in inputs:
+        if x is None:
+            continue
+        if x.requires_grad and torch.is_grad_enabled():
+            lost = "gradient (run under torch.no_grad())"
+        elif _wrapped(x):
+            lost = "function transform"
+        elif forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None:
+            lost = "forward-mode derivative"
+    if lost is not None:
+        raise RuntimeError(f"8-bit layers are for inference: they record no {lost}")
 
 
 class Fp8Linear(torch.nn.Module):
