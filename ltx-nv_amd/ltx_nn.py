@@ -571,6 +571,16 @@ class Fp8Linear(torch.nn.Module):
             made.bias = layer.bias.detach().clone()
         return made.train(layer.training)
 
+    def _load_from_state_dict(self, state_dict, prefix, metadata, strict, missing, unexpected, errors):
+        """Bytes only: torch would copy a bf16 weight's values into them, converted."""
+        for name in ("weight", "weight_scale"):
+            t = state_dict.get(prefix + name)
+            if t is not None and t.dtype != torch.uint8:
+                errors.append(f"{prefix}{name} is {t.dtype}: an 8-bit layer loads the bytes of another one's state "
+                              "(load a bf16 state before ltx_nn.quantize_fp8)")
+                return
+        super()._load_from_state_dict(state_dict, prefix, metadata, strict, missing, unexpected, errors)
+
     def blocks(self) -> ltxk.Fp8Blocks:
         return ltxk.Fp8Blocks(self.weight.view(torch.float8_e4m3fn), self.weight_scale,
                               (self.out_features, self.in_features))

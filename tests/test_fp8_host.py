@@ -62,3 +62,25 @@ def test_transforms_and_tracers_are_refused():
             torch.func.vmap(call)(x[:, None])
         with pytest.raises(RuntimeError, match="inference"):
             torch.jit.trace(call, x, check_trace=False)
+
+
+@pytest.mark.parametrize("width", [128, 136])  # of 128 columns a bf16 weight has the bytes' shape
+@pytest.mark.parametrize("assign", [False, True])
+@pytest.mark.parametrize("strict", [False, True])
+def test_a_bf16_state_is_refused(width, assign, strict):
+    """A bf16 layer's state (or one cast to another type) is not loaded into an 8-bit layer as if its values were
+    bytes; an 8-bit layer's own is, whichever way."""
+    import ltx_nn
+
+    layer, plain = ltx_nn.Fp8Linear(width, 40), torch.nn.Linear(width, 40).to(BF16)
+    layer.weight.random_(0, 127), layer.weight_scale.fill_(120)
+    held = {name: t.clone() for name, t in layer.state_dict().items()}
+    half = {name: t.half() for name, t in held.items()}
+    values = {**held, "weight": held["weight"].view(torch.float8_e4m3fn)}
+    for state in (plain.state_dict(), half, {**held, "weight": plain.weight.detach()}, values):
+        with pytest.raises(RuntimeError, match="8-bit|size mismatch"):
+            layer.load_state_dict(state, strict=strict, assign=assign)
+        assert all(torch.equal(t, held[name]) and t.dtype == held[name].dtype for name, t in layer.state_dict().items())
+    other = torch.nn.Sequential(ltx_nn.Fp8Linear(width, 40))
+    other.load_state_dict({f"0.{name}": t for name, t in held.items()}, strict=strict, assign=assign)
+    assert all(torch.equal(t, held[name]) for name, t in other[0].state_dict().items())
