@@ -708,8 +708,9 @@ class Attention(torch.nn.Module):
         Lets a caller prepare the q/k of two attentions in one launch (Block's
         A2V/V2A).  `keep`, which takes the place of a mask, names the tokens of k and v to
         attend to, for contexts of different lengths in one padded batch: that is
-        ltxk_cross_attention, at the cost of the kept tokens alone (zeros where none is kept),
-        or torch's SDPA with it as a boolean mask for what fused_attention_applies excludes."""
+        ltxk_cross_attention, at the cost of the kept tokens alone, or torch's SDPA with it as a
+        boolean mask for what fused_attention_applies excludes.  Either way the others may hold
+        anything, and an item without a kept token gives zeros."""
         b = q.shape[0]
         h, dh = self.heads, self.dim_head
         if keep is not None:
@@ -720,7 +721,10 @@ class Attention(torch.nn.Module):
             keep = (keep if keep.dtype == torch.bool else keep != 0).contiguous()
             if fused_attention_applies(q, k, v, h, dh):
                 return linear(self.to_out, ltxk.cross_attention(q, k, v, h, keep, gates))
-            mask = keep[:, None, None, :]
+            # torch multiplies what a mask closes by a weight of zero, and what it does with a row that closes
+            # everything is up to its kernel: left-out tokens become zeros, and an item without a kept one attends to those
+            k, v = (t.masked_fill(~keep.unsqueeze(-1), 0) for t in (k, v))
+            mask = (keep | ~keep.any(-1, keepdim=True))[:, None, None, :]
         pm = None
         if perturbation_mask is not None:
             pm = perturbation_mask.reshape(-1).to(torch.bfloat16).contiguous()

@@ -113,3 +113,31 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for w, o in zip(want, got):
         assert all(torch.equal(w, x) for x in o)
+
+
+@pytest.mark.parametrize("b,tq,tk,h,dh", [(4, 40, 23, 4, 32), (3, 1, 300, 2, 32), (65, 16, 16, 32, 64), (3, 70, 2048, 4, 32)])
+def test_kept_tokens_where_attention_is_torchs(b, tq, tk, h, dh):
+    """Heads that the kernel does not take, and many short sequences: left-out tokens may hold anything there, too,
+    and an item without a kept token gives zeros."""
+    import ltx_nn
+
+    attn = ltx_nn.Attention(h * dh, h * dh, h, dh, apply_gated_attention=True)
+    attn.to_out = torch.nn.Identity()
+    g = torch.Generator(device=DEV).manual_seed(tk)
+    q, k, v = (torch.randn(b, t, h * dh, device=DEV, generator=g).to(torch.bfloat16) for t in (tq, tk, tk))
+    gates = torch.randn(b, tq, h, device=DEV, generator=g).to(torch.bfloat16)
+    keep = torch.rand(b, tk, device=DEV, generator=g) < 0.6
+    keep[0], keep[1] = True, False
+    k[~keep], v[~keep] = float("nan"), float("inf")
+    assert not ltx_nn.fused_attention_applies(q, k, v, h, dh)
+    got = attn.attend(q, k, v, gates, keep=keep)
+    assert not got[1].any()
+    q4, k4, v4 = (t.double().view(b, -1, h, dh).transpose(1, 2).contiguous() for t in (q, k, v))
+    k4, v4 = (t.masked_fill(~keep[:, None, :, None], 0.0) for t in (k4, v4))
+    score = (q4 @ k4.transpose(-1, -2).contiguous()) * dh**-0.5
+    p = torch.exp(score).masked_fill(~keep[:, None, None, :], 0.0)
+    p = p / p.sum(-1, keepdim=True).clamp(min=1e-300)
+    gate = (2 * torch.sigmoid(gates.double())).transpose(1, 2).unsqueeze(-1)
+    want, size = (((p @ t) * gate).transpose(1, 2).reshape(b, tq, h * dh) for t in (v4, v4.abs()))
+    # weights in bf16, the output's rounding and the gated one's: half a step each; a quarter more for the exponentials
+    assert ((got.double() - want).abs() <= size * 2.0**-8 * 3.25 + 1e-30).all()

@@ -1,0 +1,73 @@
+"""Attention(keep=) where it is torch's (CPU): left-out tokens may hold anything there, too, and items without a
+kept token give zeros."""
+
+import math
+
+import pytest
+import torch
+
+
+def _attention(heads, dim_head, gated=False):
+    import ltx_nn
+
+    torch.manual_seed(1)
+    attn = ltx_nn.Attention(64, 64, heads, dim_head, apply_gated_attention=gated)
+    attn.to_out = torch.nn.Identity()
+    return attn
+
+
+def _plain(q, k, v, h, keep):
+    """Softmax attention over the kept keys in fp64, item by item; zeros where nothing is kept."""
+    out = torch.zeros(q.shape, dtype=torch.float64)
+    dh = q.shape[-1] // h
+    for i in range(q.shape[0]):
+        kept = keep[i if keep.shape[0] > 1 else 0]
+        if not kept.any():
+            continue
+        for j in range(h):
+            c = slice(j * dh, (j + 1) * dh)
+            w = torch.softmax(q[i, :, c].double() @ k[i, kept][:, c].double().t() / math.sqrt(dh), -1)
+            out[i, :, c] = w @ v[i, kept][:, c].double()
+    return out
+
+
+@pytest.mark.parametrize("heads,dh", [(2, 32), (1, 64), (3, 24)])
+@pytest.mark.parametrize("tk", [1, 17, 64])
+def test_left_out_tokens_may_hold_anything(heads, dh, tk):
+    attn = _attention(heads, dh)
+    g = torch.Generator().manual_seed(tk)
+    q, k, v = (torch.randn(4, t, heads * dh, generator=g) for t in (5, tk, tk))
+    keep = torch.rand(4, tk, generator=g) < 0.6
+    keep[0], keep[1], keep[2, 0] = True, False, True
+    want = _plain(q, k, v, heads, keep)
+    k[~keep], v[~keep] = float("nan"), float("inf")
+    held = k.clone(), v.clone()
+    for mask in (keep, keep.to(torch.uint8) * 7):
+        got = attn.attend(q, k, v, None, keep=mask).double()
+        # fp32 sums of tk weights and dh products, an exponential of 2 ulp
+        assert (got - want).abs().max() <= 2.0**-23 * (tk + dh + 8) * 4 and not got[1].any()
+    assert all(torch.equal(a.nan_to_num(9.0), b.nan_to_num(9.0)) for a, b in zip(held, (k, v)))  # left as they were
+    one = keep[:1]
+    k, v = k.nan_to_num(0, 0, 0), v.nan_to_num(0, 0, 0)
+    assert torch.equal(attn.attend(q, k, v, None, keep=one), attn.attend(q, k, v, None, keep=one.expand(4, tk)))
+
+
+def test_gradients_of_left_out_tokens_are_zero():
+    """They stay finite where the tokens do not, and beside an item without a kept token."""
+    attn = _attention(2, 32)
+    q, k, v = (torch.randn(3, t, 64) for t in (5, 9, 9))
+    keep = torch.rand(3, 9) < 0.5
+    keep[0], keep[1, 0] = False, True
+    k[~keep], v[~keep] = float("inf"), float("nan")
+    for t in (q, k, v):
+        t.requires_grad_()
+    attn.attend(q, k, v, None, keep=keep).square().sum().backward()
+    assert all(torch.isfinite(t.grad).all() for t in (q, k, v))
+    assert not k.grad[~keep].any() and not v.grad[~keep].any() and not q.grad[0].any() and v.grad[1:][keep[1:]].any()
+
+
+def test_no_tokens_at_all():
+    attn = _attention(2, 32)
+    q, none = torch.randn(2, 5, 64), torch.zeros(2, 0, 64)
+    got = attn.attend(q, none, none, None, keep=torch.zeros(2, 0, dtype=torch.bool))
+    assert got.shape == q.shape and not got.any()
