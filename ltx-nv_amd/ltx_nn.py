@@ -679,6 +679,8 @@ class Attention(torch.nn.Module):
         context = x if context is None else context
         h, dh = self.heads, self.dim_head
         if all_perturbed:
+            if keep is not None:
+                raise ValueError("keep goes with no perturbation")
             v = self.to_v(context)
             gates = self.to_gate_logits(x).contiguous() if self.to_gate_logits is not None else None
             out = v if gates is None else ltxk.head_gate(v, gates)

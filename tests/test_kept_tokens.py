@@ -71,3 +71,14 @@ def test_no_tokens_at_all():
     q, none = torch.randn(2, 5, 64), torch.zeros(2, 0, 64)
     got = attn.attend(q, none, none, None, keep=torch.zeros(2, 0, dtype=torch.bool))
     assert got.shape == q.shape and not got.any()
+
+
+def test_keep_goes_with_no_perturbation():
+    """A perturbed attention passes the values through: there is nothing to leave out."""
+    attn = _attention(2, 32)
+    x, keep = torch.randn(2, 5, 64), torch.ones(2, 5, dtype=torch.bool)
+    with pytest.raises(ValueError, match="no perturbation"):
+        attn(x, keep=keep, all_perturbed=True)
+    with pytest.raises(ValueError, match="no perturbation"):
+        attn.attend(x, x, x, None, keep=keep, perturbation_mask=torch.ones(2, 1, 1))
+    assert torch.equal(attn(x, all_perturbed=True), attn.to_v(x))
