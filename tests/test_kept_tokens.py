@@ -82,3 +82,23 @@ def test_keep_goes_with_no_perturbation():
     with pytest.raises(ValueError, match="no perturbation"):
         attn.attend(x, x, x, None, keep=keep, perturbation_mask=torch.ones(2, 1, 1))
     assert torch.equal(attn(x, all_perturbed=True), attn.to_v(x))
+
+
+def test_passes_take_their_prompts_masks():
+    """run_dit's masks by pass: the positive prompt's for all but the unconditional one; a prompt without a mask is whole."""
+    import ltx_dit
+
+    assert ltx_dit.PASSES == ("cond", "uncond", "ptb", "mod")
+    contexts = {f"{s}_{p}": torch.zeros(1, n, 8) for s, n in (("v", 5), ("a", 3)) for p in ("pos", "neg")}
+    assert ltx_dit._passes_keep(contexts, "v") is None and ltx_dit._passes_keep(contexts, "a") is None
+    pos, neg, audio = (torch.tensor([row]) for row in ([1, 1, 0, 0, 0], [0, 0, 0, 1, 1], [0, 1, 0]))
+    contexts.update(v_pos_keep=pos.bool(), v_neg_keep=neg, a_neg_keep=audio.to(torch.uint8))
+    v, a = (ltx_dit._passes_keep(contexts, s) for s in ("v", "a"))
+    assert v.dtype == a.dtype == torch.bool
+    assert torch.equal(v.int(), torch.cat([pos, neg, pos, pos]).int())
+    assert torch.equal(a.int(), torch.cat([torch.ones_like(audio), audio, torch.ones_like(audio), torch.ones_like(audio)]).int())
+    del contexts["v_neg_keep"]
+    assert torch.equal(ltx_dit._passes_keep(contexts, "v")[1], torch.ones(5, dtype=torch.bool))
+    contexts["v_pos_keep"] = torch.ones(1, 4, dtype=torch.bool)
+    with pytest.raises(RuntimeError):
+        ltx_dit._passes_keep(contexts, "v")
