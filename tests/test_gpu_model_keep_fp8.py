@@ -184,3 +184,33 @@ def test_run_dit_keeps_each_passes_tokens(given):
         other = passes({f"{s}_{n}": contexts[f"{s}_{q}"][:, keeps[f"{s}_{q}"]].contiguous()
                         for s in ("v", "a") for n, q in (("pos", "neg"), ("neg", "neg"))})
         assert min(_distance(got["cond"], other["cond"])) >= 3 * NEAR[False]  # the other prompt's tokens
+
+
+@pytest.mark.parametrize("registers", [0, 32])  # attention masked (torch's), or unmasked once registers fill the padding
+def test_quantized_connector(registers):
+    """The text path's connectors take 8-bit layers like the blocks."""
+    import ltx_nn
+    import ltx_te
+
+    torch.manual_seed(2)
+    connector = ltx_te.Embeddings1DConnector(4, 64, 2, [128], registers, True, True).to(DEV, BF16).requires_grad_(False)
+    for name, p in connector.named_parameters():
+        if name.endswith("norm.weight"):
+            torch.nn.init.ones_(p)
+        else:
+            torch.nn.init.normal_(p, std=p.shape[-1]**-0.5 if p.ndim == 2 and "registers" not in name else 1.0 if p.ndim == 2 else 0.1)
+    x = torch.randn(2, 64, 256, device=DEV).to(BF16)
+    mask = torch.zeros(2, 1, 1, 64, device=DEV, dtype=BF16)
+    mask[1, ..., 40:] = torch.finfo(BF16).min
+    want = connector(x, mask)[0]
+    layers = ltx_nn.quantize_fp8(connector).blocks
+    assert all(b.ff.takes_blocks and type(b.attn1.to_q) is type(b.attn1.to_out) is ltx_nn.Fp8Linear for b in layers)
+    near = 0.1  # the operands' rounding, 0.037 a layer, over four branches as large as the stream they are added to
+    assert _distance([connector(x, mask)[0]], [want])[0] <= near
+    for part in ("attn1.to_out", "ff.proj_out"):
+        held = [b.get_submodule(part).weight.clone() for b in layers]
+        for b in layers:
+            b.get_submodule(part).weight.zero_()
+        assert _distance([connector(x, mask)[0]], [want])[0] >= 2.5 * near, part
+        for b, w in zip(layers, held):
+            b.get_submodule(part).weight.copy_(w)
