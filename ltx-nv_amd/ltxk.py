@@ -1016,8 +1016,8 @@ class Fp8Blocks:
         shape = tuple(shape)
         _dev(data, "data", torch.float8_e4m3fn)
         _dev(scale, "scale", torch.uint8)
-        if not shape or shape[-1] <= 0 or shape[-1] % 8:
-            raise ValueError(f"shape {shape} must end in a positive multiple of 8")
+        if not shape or shape[-1] <= 0 or shape[-1] % 8 or min(shape) < 0:
+            raise ValueError(f"shape {shape} must hold no negative size and end in a positive multiple of 8")
         rows, blocks = _fp8_extent(shape)
         if data.shape != (rows, blocks * FP8_BLOCK):
             raise ValueError(f"data {tuple(data.shape)} does not hold {shape}: expected {(rows, blocks * FP8_BLOCK)}")
@@ -1083,7 +1083,7 @@ class Fp8Blocks:
         lead = 1
         for s in shape[:-1]:
             lead *= s
-        if not shape or shape[-1] != self.shape[-1] or lead != self.rows:
+        if not shape or shape[-1] != self.shape[-1] or lead != self.rows or min(shape) < 0:
             raise ValueError(f"{self.shape} has no view {shape}: the last dimension stays")
         other = object.__new__(Fp8Blocks)
         other.shape, other.rows, other._data, other._scale, other._both = shape, lead, self._data, self._scale, self._both

@@ -115,3 +115,14 @@ def test_binding_refuses_before_the_device():
         ltxk.Fp8Blocks(torch.zeros(4, 128).to(torch.float8_e4m3fn), torch.zeros(1, 4, 4, dtype=torch.uint8), (4, 64))
     with pytest.raises(ValueError, match="tensors"):
         ltxk.cross_attention(x, x, x, 1)
+
+
+def test_blocks_refuse_negative_sizes():
+    """Two of them multiply to a count of rows that fits."""
+    import ltxk
+
+    blocks = ltxk.Fp8Blocks._made((6, 64), "cpu")
+    assert blocks.view(2, 3, 64).shape == (2, 3, 64) and blocks.view(1, 6, 64).rows == 6
+    for shape in ((-2, -3, 64), (-1, -6, 64), (-1, 64), (5, 64), (6, 128), ()):
+        with pytest.raises(ValueError, match="no view"):
+            blocks.view(*shape)
