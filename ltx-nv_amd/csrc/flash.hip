@@ -28,7 +28,7 @@
 // * The running maximum is exact in every tile.  Letting it lag up to 2^8 saves
 //   2-4 %, but then a row's largest weight is no longer exactly 1 and its
 //   rounding shows: relative error 2.26e-3 against 1.87e-3 (torch's 1.87e-3).
-#include "ltxk_common.h"
+#include "tiles.h"
 
 #include <cfloat>
 #include <type_traits>

@@ -17,6 +17,7 @@
 // card's power beyond (24576 x 4096 x 4096 in 312 us, 2.65 PFLOP/s, on zeros 227 us, 3.63; the library's
 // product with a single scale for each operand 292 and 212).
 #include "fp8_blocks.h"
+#include "tiles.h"
 
 #include <algorithm>
 #include <type_traits>

@@ -127,3 +127,11 @@ def test_counter_collection_needs_plain_mode():
                        text=True, timeout=120, cwd=REPO, env=env)
     assert r.returncode == 2
     assert "--plain" in json.loads(r.stdout.strip().splitlines()[-1])["error"]
+
+
+def test_headline_traffic_is_of_the_sources_built_now():
+    """What the row kernels do not use stays out of their sources, or the counters are read anew: otherwise the
+    headline has no measured traffic."""
+    b = _bench()
+    t, note = b.counter_traffic(*b.HEADLINE_KERNEL)
+    assert t is not None, note
