@@ -90,7 +90,6 @@ __device__ __forceinline__ int v_pos(int row, int c)
     return D == 128 ? c ^ (((row & 3) << 2) | ((row >> 2) & 3)) : c ^ ((((row >> 1) & 1) << 2) | ((row >> 2) & 3));
 }
 
-typedef __attribute__((address_space(3))) char lds_char;
 
 // Part j of a wave's share of a 64-row tile: one load instruction moves 64 lanes
 // x 16 bytes straight into LDS.  Rows past the last key repeat it (their scores

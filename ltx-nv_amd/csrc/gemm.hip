@@ -17,19 +17,17 @@
 //   row pieces).
 // * Neighbouring tiles share an XCD and run its K in step: starting each workgroup
 //   elsewhere in K took 1125 us.
-#include "ltxk_common.h"
+#include "tiles.h"
 
 namespace ltxk {
 namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef __attribute__((address_space(3))) char lds_char;
 
 constexpr int kTile = 256;  // rows of x and of w a workgroup
 constexpr int kStep = 64;   // elements of K a step
 constexpr int kWaves = 8;   // 2 along the rows of x, 4 along the rows of w
-constexpr int kBand = 4;    // tiles of x that a band of the tile order holds (8: no difference)
 
 struct GemmParams {
     const uint16_t *x, *w, *bias;
@@ -39,48 +37,6 @@ struct GemmParams {
     int tiles_m, tiles_n;
     int whole, rest, parts;  // tiles that one workgroup takes alone; the others, cut into parts over K
 };
-
-// The rows of x and w that tile t takes: bands kBand tiles of x deep.
-__device__ __forceinline__ void tile_rows(const GemmParams &p, int t, int &m0, int &n0)
-{
-    const int band = t / (kBand * p.tiles_n), at = t % (kBand * p.tiles_n);
-    const int deep = min(kBand, p.tiles_m - band * kBand);
-    m0 = (band * kBand + at % deep) * kTile;
-    n0 = at / deep * kTile;
-}
-
-// LDS position of 16-byte chunk c (8 elements of K) of a tile's row: 16 rows of
-// one chunk column, which a fragment read takes at a time, cover all banks.
-__device__ __forceinline__ int chunk_pos(int row, int c) { return c ^ ((row >> 1) & 7); }
-
-// 64 lanes x 16 bytes from memory straight to LDS at `lds`, through m0.  In assembly
-// because the compiler, which cannot tell the buffers of a ring apart, would wait
-// for every load in flight before each LDS read; it has no output register, and its
-// wait is step_barrier's.  The wait states cover scalar operands that a vector
-// instruction has just written, which the compiler does not see the load read.  It
-// does not see m0 change either (a reserved register, whose clobber it ignores with
-// a warning): nothing else in these kernels may use m0, such as an LDS load builtin,
-// an indexed register or a message, and their assembly holds no other use.
-__device__ __forceinline__ void load_lds(const u32x4 &rsrc, uint32_t lds, uint32_t off, uint32_t soff)
-{
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-                 ::"s"(lds), "v"(off), "s"(rsrc), "s"(soff)
-                 : "memory");
-}
-
-// At most `N` of this wave's loads in flight (none without `more`) and its LDS
-// reads returned, then all waves'.
-template <int N>
-__device__ __forceinline__ void step_barrier(bool more)
-{
-    asm volatile("" ::: "memory");
-    if (more)
-        __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | (N >> 4 << 14));  // vmcnt(N) lgkmcnt(0)
-    else
-        __builtin_amdgcn_s_waitcnt(0x0070);
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-}
 
 __global__ void __launch_bounds__(kWaves * 64, 2) gemm_kernel(GemmParams p)
 {
@@ -105,14 +61,12 @@ __global__ void __launch_bounds__(kWaves * 64, 2) gemm_kernel(GemmParams p)
         tile = p.whole + unit % p.rest;
     }
     int m0, n0;
-    tile_rows(p, tile, m0, n0);
+    tile_rows<kTile, kTile>(p.tiles_m, p.tiles_n, tile, m0, n0);
     const int steps = p.k / kStep;
     const int first = part < 0 ? 0 : static_cast<int>(static_cast<int64_t>(part) * steps / p.parts);
     const int n = (part < 0 ? steps : static_cast<int>(static_cast<int64_t>(part + 1) * steps / p.parts)) - first;
 
-    const uint64_t xa = reinterpret_cast<uint64_t>(p.x), wa = reinterpret_cast<uint64_t>(p.w);
-    const u32x4 xr = {static_cast<uint32_t>(xa), static_cast<uint32_t>(xa >> 32) & 0xffff, 0xffffffffu, 0x00020000u};
-    const u32x4 wr = {static_cast<uint32_t>(wa), static_cast<uint32_t>(wa >> 32) & 0xffff, 0xffffffffu, 0x00020000u};
+    const u32x4 xr = whole_memory(p.x), wr = whole_memory(p.w);
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char *)smem));
     uint32_t xo[L], wo[L];
 #pragma unroll
@@ -123,11 +77,11 @@ __global__ void __launch_bounds__(kWaves * 64, 2) gemm_kernel(GemmParams p)
         wo[j] = static_cast<uint32_t>(min(n0 + row, p.n - 1)) * stride + c;
     }
     auto load_x = [&](int i, int j, int base) {
-        load_lds(xr, __builtin_amdgcn_readfirstlane(lds0 + base + (wave * L + j) * 1024), xo[j],
+        load_lds16(xr, __builtin_amdgcn_readfirstlane(lds0 + base + (wave * L + j) * 1024), xo[j],
                  __builtin_amdgcn_readfirstlane((first + i) * kStep * 2));
     };
     auto load_w = [&](int i, int j, int base) {
-        load_lds(wr, __builtin_amdgcn_readfirstlane(lds0 + base + (wave * L + j) * 1024), wo[j],
+        load_lds16(wr, __builtin_amdgcn_readfirstlane(lds0 + base + (wave * L + j) * 1024), wo[j],
                  __builtin_amdgcn_readfirstlane((first + i) * kStep * 2));
     };
     for (int i = 0; i < 2 && i < n; ++i) {
@@ -214,7 +168,7 @@ __global__ void __launch_bounds__(256) gemm_sum_kernel(GemmParams p)
     constexpr int kBlocks = kTile * kTile / 8 / 256;  // workgroups a tile
     const int t = blockIdx.x / kBlocks, i = (blockIdx.x % kBlocks * 256 + threadIdx.x) * 8;
     int m0, n0;
-    tile_rows(p, p.whole + t, m0, n0);
+    tile_rows<kTile, kTile>(p.tiles_m, p.tiles_n, p.whole + t, m0, n0);
     const int row = m0 + i / kTile, col = n0 + i % kTile;
     if (row >= p.m || col >= p.n) return;
     const float *s = p.part + static_cast<int64_t>(t) * (kTile * kTile) + i;
@@ -302,8 +256,7 @@ __global__ void __launch_bounds__((kFewWaves + 1) * 64, 1) few_rows_kernel(FewPa
 
     // rows past the last repeat it; their results are not stored
     const bool is_x = wave < kFewWaves;
-    const uint64_t base = reinterpret_cast<uint64_t>(is_x ? p.x : g.w);
-    const u32x4 rsrc = {static_cast<uint32_t>(base), static_cast<uint32_t>(base >> 32) & 0xffff, 0xffffffffu, 0x00020000u};
+    const u32x4 rsrc = whole_memory(is_x ? p.x : g.w);
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char *)smem)) +
                           (is_x ? wave * 4096 : kFewX * kXBytes);
     uint32_t go[4];
@@ -316,7 +269,7 @@ __global__ void __launch_bounds__((kFewWaves + 1) * 64, 1) few_rows_kernel(FewPa
     auto load = [&](int i, int slot) {
 #pragma unroll
         for (int j = 0; j < L; ++j)
-            load_lds(rsrc,
+            load_lds16(rsrc,
                      __builtin_amdgcn_readfirstlane(lds0 + slot + (j >> 2) * ((is_x ? kFewRows : kFewCols) * kStep * 2) +
                                                     (j & 3) * 1024),
                      go[j & 3], __builtin_amdgcn_readfirstlane((2 * i + (j >> 2)) * kStep * 2));

@@ -56,63 +56,6 @@ __device__ __forceinline__ float gelu(float x)
 
 // --------------------------------------------------------------------- tiles --
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef __attribute__((address_space(3))) char lds_char;
-
-// LDS position of 16-byte chunk c of a tile's row of 128 values: 16 rows of one
-// chunk column, which a fragment read takes at a time, cover all banks.
-__device__ __forceinline__ int chunk_pos(int row, int c) { return c ^ ((row >> 1) & 7); }
-
-// 64 lanes x 16 (4) bytes from memory straight to LDS at `lds`, through m0.  In assembly
-// because the compiler, which cannot tell the buffers of a ring apart, would wait
-// for every load in flight before each LDS read; it has no output register, and its
-// wait is step_barrier's.  The wait states cover scalar operands that a vector
-// instruction has just written.  Nothing else in the kernel may use m0.
-__device__ __forceinline__ void load_lds16(const u32x4 &rsrc, uint32_t lds, uint32_t off, uint32_t soff)
-{
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-                 ::"s"(lds), "v"(off), "s"(rsrc), "s"(soff)
-                 : "memory");
-}
-__device__ __forceinline__ void load_lds4(const u32x4 &rsrc, uint32_t lds, uint32_t off, uint32_t soff)
-{
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, %3 offen lds"
-                 ::"s"(lds), "v"(off), "s"(rsrc), "s"(soff)
-                 : "memory");
-}
-
-// At most `N` of this wave's loads in flight (none without `more`) and its LDS
-// reads returned, then all waves'.
-template <int N>
-__device__ __forceinline__ void step_barrier(bool more)
-{
-    asm volatile("" ::: "memory");
-    if (more)
-        __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | (N >> 4 << 14));  // vmcnt(N) lgkmcnt(0)
-    else
-        __builtin_amdgcn_s_waitcnt(0x0070);
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-}
-
-__device__ __forceinline__ u32x4 whole_memory(const void *base)
-{
-    const uint64_t a = reinterpret_cast<uint64_t>(base);
-    return u32x4{static_cast<uint32_t>(a), static_cast<uint32_t>(a >> 32) & 0xffff, 0xffffffffu, 0x00020000u};
-}
-
-// Tiles of x that a band of the tile order holds.  24576 x 4096 x 4096 / 6144 x 16384 x 4096, us: 2: 332 / 302,
-// 4: 313 / 300, 8: 317 / 312, 16: 323 / 320.
-constexpr int kBand = 4;
-
-// The rows of x and w that tile t takes: bands kBand tiles of x deep.
-template <int TM, int TN>
-__device__ __forceinline__ void tile_rows(const Fp8Params &p, int t, int &m0, int &n0)
-{
-    const int band = t / (kBand * p.tiles_n), at = t % (kBand * p.tiles_n);
-    const int deep = min(kBand, p.tiles_m - band * kBand);
-    m0 = (band * kBand + at % deep) * TM;
-    n0 = at / deep * TN;
-}
 
 // Tiles of TM x 128, four waves of TM / 2 x 64, the steps of 128 values as deep in LDS as fit.
 // Two teams of four waves that take turns at the steps (two waves a SIMD) are 2-6 % slower: LDS bounds
@@ -142,7 +85,7 @@ __global__ void __launch_bounds__(kTileWaves * 64, 1) tile_kernel(Fp8Params p)
         tile = p.whole + unit % p.rest;
     }
     int m0, n0;
-    tile_rows<TM, kTile>(p, tile, m0, n0);
+    tile_rows<TM, kTile>(p.tiles_m, p.tiles_n, tile, m0, n0);
     // parts * blocks stays below 2^32: 256 parts at most of fewer than 2^24 blocks
     auto from = [&](int i) { return static_cast<int>(static_cast<uint32_t>(i) * p.blocks / static_cast<uint32_t>(p.parts)); };
     const int first = part < 0 ? 0 : from(part), n = (part < 0 ? p.blocks : from(part + 1)) - first;
@@ -400,7 +343,7 @@ __device__ __forceinline__ Unit unit_at(const Fp8Params &p, int xcd, int j)
         u.part = p.parts == 1 ? -1 : i / p.rest;
         u.tile = p.whole + i % p.rest;
     }
-    tile_rows<kBig, kBig>(p, u.tile, u.m0, u.n0);
+    tile_rows<kBig, kBig>(p.tiles_m, p.tiles_n, u.tile, u.m0, u.n0);
     // parts * blocks stays below 2^32: 256 parts at most of fewer than 2^24 blocks
     auto from = [&](int i) { return static_cast<int>(static_cast<uint32_t>(i) * p.blocks / static_cast<uint32_t>(p.parts)); };
     u.first = u.part < 0 ? 0 : from(u.part);
@@ -722,7 +665,7 @@ __global__ void __launch_bounds__(256) tile_sum_kernel(Fp8Params p)
     constexpr int kPer = TILE * TILE / 8 / 256;  // workgroups a tile
     const int t = blockIdx.x / kPer, i = (blockIdx.x % kPer * 256 + threadIdx.x) * 8;
     int m0, n0;
-    tile_rows<TILE, TILE>(p, p.whole + t, m0, n0);
+    tile_rows<TILE, TILE>(p.tiles_m, p.tiles_n, p.whole + t, m0, n0);
     const int row = m0 + i / TILE, col = n0 + i % TILE;
     if (row >= p.m || col >= (GELU ? p.np : p.n)) return;  // whole blocks of lanes
     float f[8] = {};
