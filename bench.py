@@ -78,6 +78,8 @@ def parse() -> argparse.Namespace:
     ap.add_argument("--no-full-step", action="store_true",
                     help="skip the 48-block denoise steps with GEMMs and attention (B=1 and the B=4 guided step)")
     ap.add_argument("--full-steps", type=int, default=2)
+    ap.add_argument("--fp8", action="store_true",
+                    help="the full steps' models with 8-bit linear layers (ltx_nn.quantize_fp8; not the default workload)")
     ap.add_argument("--plain", action="store_true",
                     help="each kernel line runs only warmup + steps calls, no head start or batches "
                          "(counter passes, where every dispatch is serialised)")
@@ -1061,7 +1063,15 @@ def bench_chain(steps: int, blocks: int = 48):
 # ---------------------------------------------------------------------------
 
 
-def bench_guided_step(steps: int, warmup: int = 1):
+def _quantized(model) -> str:
+    """The model's attentions and feed-forwards in 8-bit layers (--fp8)."""
+    import ltx_nn
+
+    ltx_nn.quantize_fp8(model)
+    return "random bf16 weights, the blocks' linear layers in blocks of 128 e4m3 values"
+
+
+def bench_guided_step(steps: int, warmup: int = 1, fp8: bool = False):
     """The reference's denoising loop step at the 48-block model shape
     (ltx_dit.py:565-621): B=4 guidance batch (cond, uncond, STG-perturbed at
     block 28, modality-isolated), x0 + CFG/STG/modality guidance + std rescale +
@@ -1083,6 +1093,7 @@ def bench_guided_step(steps: int, warmup: int = 1):
     with torch.no_grad():
         for p in model.parameters():
             p.normal_(0.0, 0.02, generator=g)
+    weights = _quantized(model) if fp8 else "random bf16 weights"
     vs, as_ = ltx_dit.create_noised_states(1, 121, 512, 768, 24.0, 10, dev, torch.bfloat16)
     r = lambda *shape: (torch.randn(*shape, device=dev, generator=g)).to(torch.bfloat16)  # noqa: E731
     contexts = {"v_pos": r(1, 1024, 4096), "v_neg": r(1, 1024, 4096), "a_pos": r(1, 1024, 2048),
@@ -1116,11 +1127,11 @@ def bench_guided_step(steps: int, warmup: int = 1):
     del model
     torch.cuda.empty_cache()
     return {"workload": "LTX-2.5-shape AV DiT denoising step, 48 blocks, B=4 guidance batch (CFG 3/7, STG block 28, "
-                        "modality 3, rescale 0.7), video 6144x4096, audio 126x2048, text 1024, random bf16 weights",
+                        f"modality 3, rescale 0.7), video 6144x4096, audio 126x2048, text 1024, {weights}",
             "ms_per_step": round(ms, 2), "steps": steps, "latents_finite": finite}
 
 
-def bench_full_step(steps: int, warmup: int = 1):
+def bench_full_step(steps: int, warmup: int = 1, fp8: bool = False):
     """48-block AV model, random N(0, 0.02^2) bf16 weights (seed 123): video
     16x16x24 latent grid = 6144 tokens x 4096 (32 heads x 128), audio 126 tokens x
     2048 (32 x 64), text context 1024 tokens (4096-d video, 2048-d audio), FFN 4x,
@@ -1141,6 +1152,7 @@ def bench_full_step(steps: int, warmup: int = 1):
         for p in model.parameters():
             p.normal_(0.0, 0.02, generator=g)
     n_params = sum(p.numel() for p in model.parameters())
+    weights = _quantized(model) if fp8 else "random bf16 weights"
     rng = TorchRNG(123, dev)
     f, h, w, ta = 16, 16, 24, 126
     v_lat = rng.randn(1, f * h * w, 128, dtype=torch.bfloat16)
@@ -1206,7 +1218,7 @@ def bench_full_step(steps: int, warmup: int = 1):
     del model
     torch.cuda.empty_cache()
     return {"workload": "LTX-2.5-shape AV DiT, 48 blocks, B=1, video 6144x4096, audio 126x2048, text 1024, "
-                        "random bf16 weights", "params": n_params, "ms_per_step": round(ms, 2), "steps": steps,
+                        + weights, "params": n_params, "ms_per_step": round(ms, 2), "steps": steps,
             "graph": graph}
 
 
@@ -1583,10 +1595,10 @@ def main() -> int:
     full = guided = None
     if not args.no_full_step and (not only or "full_step" in only):
         print("[bench] full denoise step (B=1)", file=sys.stderr, flush=True)
-        full = bench_full_step(args.full_steps)
+        full = bench_full_step(args.full_steps, fp8=args.fp8)
     if not args.no_full_step and (not only or "guided_step" in only):
         print("[bench] guided denoising step (B=4)", file=sys.stderr, flush=True)
-        guided = bench_guided_step(args.full_steps)
+        guided = bench_guided_step(args.full_steps, fp8=args.fp8)
     cpu = None
     if not args.no_cpu and not only:
         print("[bench] cpu baselines", file=sys.stderr, flush=True)

@@ -135,3 +135,12 @@ def test_headline_traffic_is_of_the_sources_built_now():
     b = _bench()
     t, note = b.counter_traffic(*b.HEADLINE_KERNEL)
     assert t is not None, note
+
+
+def test_eight_bit_steps_are_asked_for(monkeypatch):
+    """--fp8 is no part of the default workload."""
+    b = _bench()
+    monkeypatch.setattr(sys, "argv", ["bench.py"])
+    assert b.parse().fp8 is False and b.bench_full_step.__defaults__[-1] is False
+    monkeypatch.setattr(sys, "argv", ["bench.py", "--only", "full_step", "--fp8"])
+    assert b.parse().fp8 is True
