@@ -385,7 +385,8 @@ int64_t ltxk_cross_attention_workspace_bytes(int64_t batch, int64_t tokens_q, in
  * in one batch: keep is one byte per key (non-zero: attended) at keep +
  * b*keep_bstride + j, of any pattern (NULL: every key).  Keys and values left out
  * are not read, so they may hold anything; a batch item without a kept key gives
- * zeros.  The work is that of the kept keys.  The gated output rounds once:
+ * zeros.  The work is that of the kept keys.  A kept value that is not finite makes
+ * its column infinite or NaN.  The gated output rounds once:
  *   out[b*Tq + t, h, :] = round(sum * 2*sigmoid(logits[b*Tq + t, h]))
  * Everything else as ltxk_attention, but `workspace` holds
  * ltxk_cross_attention_workspace_bytes.

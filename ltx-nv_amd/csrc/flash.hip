@@ -28,6 +28,10 @@
 // * The running maximum is exact in every tile.  Letting it lag up to 2^8 saves
 //   2-4 %, but then a row's largest weight is no longer exactly 1 and its
 //   rounding shows: relative error 2.26e-3 against 1.87e-3 (torch's 1.87e-3).
+// Few queries over kept keys are bound by memory's latency: a workgroup's tiles follow one
+// another with one tile of loads on its way and a full wait for it, over 1 us a tile where no
+// second workgroup shares its unit (the products of a tile take 0.2): 1 query over 333 keys
+// 7.4-8.9 us, 4 x 126 over 1024 17.  The forms for kept keys spill 39-46 scalar registers.
 #include "tiles.h"
 
 #include <cfloat>
@@ -456,7 +460,9 @@ __global__ void __launch_bounds__(kWaves * 64, 2) flash_kernel(FlashParams p)
     const float gate = p.logits ? head_gate(p.logits[tok]) : 1.f;
     // Stored as 64 bytes of 16 rows each, streaming: 4 x 6144 queries over 64 / 1024 keys, 32 heads of 128,
     // zeros, 8 bytes a lane as they lie 131 / 363 us, 64 a row 108 / 340, streaming 77 / 310 (402 MB of queries
-    // and output take 82 at a large copy's rate); the 8 bytes streaming 512 / 500.
+    // and output take 82 at a large copy's rate); the 8 bytes streaming 512 / 500.  The product that reads the output
+    // next does not miss it in the caches: both together, bytes as they lie / 64 a row / streaming, 6144 x 6144 tokens,
+    // 32 heads of 128, 778 / 777 / 769 us, 4290 458 / 457 / 456, 1024 73 / 73 / 73, 126, heads of 64, 28 / 28 / 28.
     const int r16 = first + wave * 32 + (lane & 15);
     uint16_t *op = p.out + ((static_cast<int64_t>(b) * p.tq + r16) * p.heads + head) * D + 8 * half + (lane & 16);
 #pragma unroll
@@ -525,7 +531,8 @@ struct FlashCut {
 // ltxk_cross_attention leaves keys of fewer than kLeastCut tiles whole: the second launch and
 // the fp32 sums take longer than what idles.  126 queries, 4 batch items, 32 heads, us, in two
 // parts / whole: of 64, 512 keys 15 / 12, 1024 22 / 21 (half of them kept 18 / 13); of 128, 1024 30 / 28
-// (25 / 18).
+// (25 / 18).  Past kMaxListed keys the list is a launch, too: 9000 keys, 0.55 of them kept / all of them
+// without a mask, 32 heads, 126 queries of 64: 40 / 32, 4 x 126 49 / 71, 1024 of 128 111 / 161.
 constexpr int64_t kLeastCut = 24;
 
 FlashCut cut(int64_t bh, int64_t tokens_q, int64_t tokens_k, int64_t least = 0)

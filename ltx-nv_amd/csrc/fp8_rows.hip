@@ -55,7 +55,8 @@ struct NormParams {
 };
 
 // One workgroup a row, C chunks of 8 columns a thread (chunk u = thread + 256 i, so
-// 16 neighbouring lanes hold a block).
+// 16 neighbouring lanes hold a block).  Few rows are bound by the latency of its loads, its
+// sum over the workgroup and its stores, one after another: [126, 2048] 5 us, of 1.8 MB.
 template <int C>
 __global__ void __launch_bounds__(kBlock) add_norm_kernel(NormParams p)
 {
@@ -113,7 +114,9 @@ __global__ void __launch_bounds__(kBlock) add_norm_kernel(NormParams p)
 // of each item with the item's modulation in registers and the next row on its way while
 // one is reduced and written, up to 512 chunks a row (their registers).  With a residual, a
 // workgroup a row / this form, us: [6144, 4096] 53 / 34 (5.2 TB/s), [4290, 4096] 34 / 26, [3000,
-// 2048] 14 / 12, [1024, 4096] 11 / 11; 4 items of [504, 2048], fewer rows than workgroups, 11 / 13.
+// 2048] 14 / 12, [1024, 4096] 11 / 11; 4 items of [504, 2048], fewer rows than workgroups, 11 / 13.  Without a
+// residual this form takes 20-22 on [6144, 4096].  Modulations by token or index, whose rows differ
+// from one row of x to the next, are read for each and keep a workgroup a row: 44-45 with a residual, 28-29 without.
 template <int C, bool RESIDUAL>
 __global__ void __launch_bounds__(kBlock) add_norm_stream_kernel(NormParams p)
 {

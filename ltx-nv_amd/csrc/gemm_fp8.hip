@@ -11,11 +11,12 @@
 // the result's rounding to bf16.  Everything past a group of 8 is fp32.
 //
 // What bounds it, by the rows of x: memory up to about 32 (the weights are read once: 4 x 36864 x
-// 4096 of 151 MB in 31 us, 4.8 TB/s, what a large copy reaches); the latency of a launch's one round
+// 4096 of 151 MB in 31 us, 4.8 TB/s, where kernels that stream rows reach 5.2-6.6: its 1152 workgroups
+// have 768 places, a round and a half); the latency of a launch's one round
 // up to a few hundred (126 x 2048 x 2048 in 5 us); for one round of tiles its first loads, stores and launch, about 8 us,
-// and LDS, whose reads and writes take 0.32 us of a step's 0.46 (1024 x 4096 x 4096 in 24 us, on zeros 22); the
-// card's power beyond (24576 x 4096 x 4096 in 312 us, 2.65 PFLOP/s, on zeros 227 us, 3.63; the library's
-// product with a single scale for each operand 292 and 212).
+// and LDS, whose reads and writes take 0.32 us of a step's 0.46 (1024 x 4096 x 4096 in 23-26 us, on zeros 22); the
+// card's power beyond (24576 x 4096 x 4096 in 287-331 us from card to card, 2.5-2.9 PFLOP/s, on zeros 227 us, 3.63; the
+// library's product with a single scale for each operand 270-292 and 212).
 #include "fp8_blocks.h"
 #include "tiles.h"
 
@@ -110,6 +111,7 @@ __global__ void __launch_bounds__(kTileWaves * 64, 1) tile_kernel(Fp8Params p)
     const uint32_t wso = static_cast<uint32_t>(min(n0 + sw + lane, p.n - 1)) * 4;
     const int groups = (p.blocks + 3) >> 2;
     // A group's scales, into its half of their place; past the last group the last one's, which nothing reads.
+    // Every step loads them (2 of a wave's 10 loads), not one in four, so that the steps are the same code.
     auto load_scales = [&](int group) {
         const uint32_t to = lds0 + kScalesAt + (group & 1) * kGroup, g = min(group, groups - 1);
         load_lds4(xsr, __builtin_amdgcn_readfirstlane(to + sx * 4), xso, __builtin_amdgcn_readfirstlane(g * p.m * 4));
@@ -316,7 +318,9 @@ __global__ void __launch_bounds__(kTileWaves * 64, 1) tile_kernel(Fp8Params p)
 // 64 x 128, whose reads and the loads' writes took all of its cycles), one workgroup a compute
 // unit that takes its tiles (and parts of tiles) one after another: the loads run two steps
 // ahead of the products, into the next tile where this one ends, so that they go on during
-// the epilogue.  24576 x 4096 x 4096: eight waves and a workgroup a tile 380 us, this 312.
+// the epilogue.  24576 x 4096 x 4096, on one card: eight waves and a workgroup a tile 380 us, this 312.
+// GELU's epilogue needs more than the registers hold (6 vector and 14 scalar ones are spilled); the same
+// product with it takes 320-361 us.
 constexpr int kBig = 256, kBigWaves = 4, kBigLoads = 2 * kBig / 8 / kBigWaves;
 constexpr int kDeepLoads = 6;                                  // of a wave: 192 rows of x, three steps in LDS
 constexpr int kNearLoads = kBigLoads - kDeepLoads;             // the other rows of x and w: two steps

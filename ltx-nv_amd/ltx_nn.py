@@ -712,7 +712,9 @@ class Attention(torch.nn.Module):
         attend to, for contexts of different lengths in one padded batch: that is
         ltxk_cross_attention, at the cost of the kept tokens alone, or torch's SDPA with it as a
         boolean mask for what fused_attention_applies excludes.  Either way the others may hold
-        anything, and an item without a kept token gives zeros."""
+        anything, and an item without a kept token gives zeros.  ltxk_cross_attention rounds its
+        gated output once, where ltxk_attention rounds before the gate as well: a bf16 step apart
+        beside the order of sums."""
         b = q.shape[0]
         h, dh = self.heads, self.dim_head
         if keep is not None:
