@@ -614,8 +614,8 @@ def _bare_linear(layer: torch.nn.Module) -> bool:
 
 def _check_bf16(layer: torch.nn.Linear, name: str) -> None:
     for t in (layer.weight, layer.bias):
-        if t is not None and not (t.is_cuda and t.dtype == torch.bfloat16):
-            raise ValueError(f"{name} holds {t.dtype} on {t.device}: 8-bit layers are made of bf16 ones on the GPU")
+        if t is not None and not (t.is_cuda and t.dtype == torch.bfloat16 and t.get_device() == torch.cuda.current_device()):
+            raise ValueError(f"{name} holds {t.dtype} on {t.device}: 8-bit layers are made of bf16 ones on the current GPU")
 
 
 def quantize_fp8(module: torch.nn.Module) -> torch.nn.Module:

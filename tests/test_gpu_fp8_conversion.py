@@ -35,3 +35,19 @@ def test_shared_layers_stay_shared():
     both = torch.nn.ModuleList([ff, other]).eval()
     ltx_nn.quantize_fp8(both)
     assert type(ff.proj_in) is ltx_nn.Fp8Linear and ff.proj_in is other.proj_in and not ff.proj_in.training
+
+
+def test_another_device_leaves_the_model_as_it_was(monkeypatch):
+    """Kernels run on the current device: layers on another one are refused before any is replaced."""
+    import ltx_nn
+
+    ff = ltx_nn.FeedForward(128).to(DEV, BF16).requires_grad_(False)
+    other = torch.nn.ModuleList([ltx_nn.FeedForward(128).to(DEV, BF16).requires_grad_(False), ff])
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    with pytest.raises(ValueError, match="0.proj_in .* on cuda:0.*current GPU"):
+        ltx_nn.quantize_fp8(other)
+    with pytest.raises(ValueError, match="current GPU"):
+        ltx_nn.Fp8Linear.of(ff.proj_in)
+    assert all(type(layer) is torch.nn.Linear for f in other for layer in (f.proj_in, f.proj_out))
+    monkeypatch.undo()
+    assert ltx_nn.quantize_fp8(ff).takes_blocks
