@@ -35,8 +35,8 @@ import torch
 
 import ltxk
 from common import DEVICE, load_state_dict, read_metadata
-from ltx_nn import (AdaLayerNormSingle, Attention, FeedForward, precompute_freqs_cis, precompute_freqs_cis_compact,
-                    project, reads_blocks)
+from ltx_nn import (AdaLayerNormSingle, Attention, FeedForward, check_keep, precompute_freqs_cis,
+                    precompute_freqs_cis_compact, project, reads_blocks)
 from torch_rng import TorchRNG
 
 # ---------------------------------------------------------------------------
@@ -1042,6 +1042,9 @@ def _passes_keep(contexts: dict, stream: str) -> torch.Tensor | None:
     pos, neg = (contexts.get(f"{stream}_{prompt}_keep") for prompt in ("pos", "neg"))
     if pos is None and neg is None:
         return None
+    for keep in (pos, neg):
+        if keep is not None:
+            check_keep(keep)
     whole = torch.ones(contexts[f"{stream}_pos"].shape[:2], dtype=torch.bool, device=contexts[f"{stream}_pos"].device)
     pos, neg = (whole if k is None else k.to(torch.bool).view(whole.shape) for k in (pos, neg))
     return torch.cat([pos, neg, pos, pos], dim=0)

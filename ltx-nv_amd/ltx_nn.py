@@ -646,6 +646,12 @@ def quantize_fp8(module: torch.nn.Module) -> torch.nn.Module:
 # ---------------------------------------------------------------------------
 
 
+def check_keep(keep: torch.Tensor) -> None:
+    """Refuses what looks like an additive mask: its zeros are the tokens to attend to."""
+    if keep.dtype.is_floating_point or keep.dtype.is_complex:
+        raise ValueError(f"keep is {keep.dtype}: bool, or integers that are not zero for the tokens to attend to")
+
+
 class Attention(torch.nn.Module):
     """Multi-head attention with RMS q/k-norm, split RoPE and per-head gating (ltx_nn.py:166-236).
 
@@ -722,6 +728,7 @@ class Attention(torch.nn.Module):
                 raise ValueError("keep takes the place of a mask, and goes with no perturbation")
             if keep.ndim != 2 or keep.shape[0] not in (1, b) or keep.shape[1] != k.shape[1]:
                 raise ValueError(f"keep {tuple(keep.shape)} must be ({b} or 1, {k.shape[1]})")
+            check_keep(keep)
             keep = (keep if keep.dtype == torch.bool else keep != 0).contiguous()
             if fused_attention_applies(q, k, v, h, dh):
                 return linear(self.to_out, ltxk.cross_attention(q, k, v, h, keep, gates))

@@ -102,3 +102,18 @@ def test_passes_take_their_prompts_masks():
     contexts["v_pos_keep"] = torch.ones(1, 4, dtype=torch.bool)
     with pytest.raises(RuntimeError):
         ltx_dit._passes_keep(contexts, "v")
+
+
+def test_additive_masks_are_refused():
+    """Their zeros are what to attend to: read as a keep they would attend to the padding."""
+    import ltx_dit
+
+    attn = _attention(2, 32)
+    x, mask = torch.randn(2, 5, 64), torch.zeros(2, 5)
+    mask[:, 3:] = -math.inf
+    for dtype in (torch.float32, torch.bfloat16):
+        with pytest.raises(ValueError, match="keep is"):
+            attn.attend(x, x, x, None, keep=mask.to(dtype))
+        with pytest.raises(ValueError, match="keep is"):
+            ltx_dit._passes_keep({"v_pos": torch.zeros(1, 5, 8), "v_neg_keep": mask[:1].to(dtype)}, "v")
+    assert torch.equal(attn.attend(x, x, x, None, keep=(mask == 0).long()), attn.attend(x, x, x, None, keep=mask == 0))
