@@ -505,11 +505,14 @@ def project(x: torch.Tensor, *layers: torch.nn.Linear | None) -> list:
     return [None if layer is None else linear(layer, x) for layer in layers]
 
 
-def _unwatched(module: torch.nn.Module) -> bool:
-    """Whether a call of the module is its class's forward and nothing else: no hooks, its
+def _unwatched(*modules: torch.nn.Module) -> bool:
+    """Whether a call of each module is its class's forward and nothing else: no hooks, its
     own or every module's, and no patched forward.  Blocks of 8-bit values stay between such modules."""
-    own = module.__dict__
-    return not (own["_forward_hooks"] or own["_forward_pre_hooks"] or "forward" in own or _has_any_global_hook())
+    for module in modules:
+        own = module.__dict__
+        if own["_forward_hooks"] or own["_forward_pre_hooks"] or "forward" in own:
+            return False
+    return not _has_any_global_hook()
 
 
 def reads_blocks(ff: torch.nn.Module, *inputs: torch.Tensor | None) -> bool:
@@ -528,8 +531,8 @@ def _no_gradient(*inputs: torch.Tensor | None) -> None:
     lost = "trace" if _tracing() else None
     for x in inputs:
         if x is None:
-            continue
-        if x.requires_grad and torch.is_grad_enabled():
+            pass
+        elif x.requires_grad and torch.is_grad_enabled():
             lost = "gradient (run under torch.no_grad())"
         elif _wrapped(x):
             lost = "function transform"
@@ -779,7 +782,8 @@ class FeedForward(torch.nn.Module):
     def takes_blocks(self) -> bool:
         """Both layers are 8-bit ones that no hook or patched forward watches: the input may be
         ltxk.Fp8Blocks, and the hidden values are."""
-        return all(type(layer) is Fp8Linear and _unwatched(layer) for layer in (self.proj_in, self.proj_out))
+        first, second = self.proj_in, self.proj_out
+        return type(first) is type(second) is Fp8Linear and _unwatched(first, second)
 
     def forward(self, x: torch.Tensor | ltxk.Fp8Blocks) -> torch.Tensor:
         if self.takes_blocks:
