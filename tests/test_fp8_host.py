@@ -84,3 +84,17 @@ def test_a_bf16_state_is_refused(width, assign, strict):
     other = torch.nn.Sequential(ltx_nn.Fp8Linear(width, 40))
     other.load_state_dict({f"0.{name}": t for name, t in held.items()}, strict=strict, assign=assign)
     assert all(torch.equal(t, held[name]) for name, t in other[0].state_dict().items())
+
+
+def test_fx_tracing_is_refused():
+    """The kernels bypass the dispatcher: a traced graph would hold their results as constants."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils.flop_counter import FlopCounterMode
+
+    ff, x = _ff(), torch.randn(2, 3, 128).to(BF16)
+    for call in (lambda t: ff(t), lambda t: ff.proj_in(t), lambda t: ff.proj_in.gelu(t), lambda t: _block_ffn(ff, t)):
+        for mode in ("real", "fake"):
+            with pytest.raises(RuntimeError, match="inference"):
+                make_fx(call, tracing_mode=mode)(x)
+        with FlopCounterMode(display=False), pytest.raises(RuntimeError, match="ROCm device"):
+            call(x)  # counts what torch runs: these go on
