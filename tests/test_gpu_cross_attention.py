@@ -141,3 +141,31 @@ def test_kept_tokens_where_attention_is_torchs(b, tq, tk, h, dh):
     want, size = (((p @ t) * gate).transpose(1, 2).reshape(b, tq, h * dh) for t in (v4, v4.abs()))
     # weights in bf16, the output's rounding and the gated one's: half a step each; a quarter more for the exponentials
     assert ((got.double() - want).abs() <= size * 2.0**-8 * 3.25 + 1e-30).all()
+
+
+def test_captured_calls_past_the_listed_keys():
+    """Two graphs, keys listed by a launch of its own and cut over units: replays in turn equal the eager calls."""
+    import ltxk
+
+    g = torch.Generator(device=DEV).manual_seed(6)
+    calls = []
+    for tk in (8193, 9001):
+        q, k, v = (torch.randn(2, t, 128, device=DEV, generator=g).to(torch.bfloat16) for t in (40, tk, tk))
+        keep = torch.rand(2, tk, device=DEV, generator=g) < 0.3
+        side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        with torch.cuda.stream(side):
+            ltxk.cross_attention(q, k, v, 2, keep)
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            out = ltxk.cross_attention(q, k, v, 2, keep)
+        calls.append((graph, out, q, k, v, keep))
+    for i in range(4):
+        for _, _, q, _, _, keep in calls:
+            q.copy_(torch.randn(q.shape, device=DEV, generator=g))
+            keep.copy_(torch.rand(keep.shape, device=DEV, generator=g) < 0.2 * (i + 1))
+            keep[i % 2] &= i > 1  # an item without any
+        for graph, *_ in calls:
+            graph.replay()
+        torch.cuda.synchronize()
+        for _, out, q, k, v, keep in calls:
+            assert torch.equal(out, ltxk.cross_attention(q, k, v, 2, keep)), f"replay {i}"
