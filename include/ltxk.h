@@ -398,6 +398,59 @@ int ltxk_cross_attention(void *out, const void *q, int64_t q_bstride, int64_t q_
                          int64_t tokens_k, int64_t heads, int64_t head_dim, float scale, void *workspace,
                          int64_t workspace_bytes, void *stream);
 
+/* Bytes of workspace ltxk_packed_attention needs for this shape. */
+int64_t ltxk_packed_attention_workspace_bytes(int64_t tokens_q, int64_t tokens_k, int64_t sequences, int64_t heads,
+                                              int64_t kv_heads, int64_t head_dim);
+
+/* Softmax attention over sequences laid end to end, heads of 64, 128 or 256, query
+ * head h over key head h / (heads / kv_heads):
+ *   out[t, h, :] = round(sum_j softmax_j(scale * q[t, h].k[j, h']) v[j, h', :])
+ * Sequence s has queries offsets[s] .. offsets[s+1] - 1 and keys k_offsets[s] ..
+ * k_offsets[s+1] - 1; both arrays are int32 in device memory, sequences + 1
+ * entries, ascending (entries outside the tensors are cut to them).  Its queries
+ * are its newest tokens: the last of n queries stands at the last of m keys, query
+ * t at i = m - n + t.  Causal, it sees keys j <= i, and with a window > 0 of them
+ * those with i - j < window (a window needs the mask); else all of its sequence's.
+ * A query that sees no key gives zeros.  Keys and values that no query of a sequence
+ * sees, and those that a mask closes, change nothing, whatever they hold.  Rows of out
+ * that belong to no sequence are left as they are.
+ * q is bf16 at q + t*q_tstride + h*head_dim (elements; multiples of 8, at least
+ * heads*head_dim, at most 2^23), k and v likewise with kv_heads; out is contiguous
+ * [tokens_q, heads*head_dim] and overlaps no operand.  Scores, softmax and sums are
+ * fp32.  tokens_q*heads and tokens_k stay below 2^31 - 1024.  `workspace`: device
+ * memory of ltxk_packed_attention_workspace_bytes, 16-byte aligned (NULL if that is
+ * 0), in use until the call's work has run.  For the prompts that the language model
+ * in front of the text connectors reads (standalone/ltx_te.py:124-146), and for
+ * clips of different lengths (standalone/ltx_nn.py:22-26). */
+int ltxk_packed_attention(void *out, const void *q, int64_t q_tstride, const void *k, int64_t k_tstride, const void *v,
+                          int64_t v_tstride, const int32_t *offsets, const int32_t *k_offsets, int64_t sequences,
+                          int64_t tokens_q, int64_t tokens_k, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                          int causal, int64_t window, float scale, void *workspace, int64_t workspace_bytes,
+                          void *stream);
+
+/* Bytes of workspace ltxk_prefix_attention needs for this shape. */
+int64_t ltxk_prefix_attention_workspace_bytes(int64_t batch, int64_t tokens_q, int64_t tokens_k, int64_t prefix,
+                                              int64_t heads, int64_t kv_heads, int64_t head_dim);
+
+/* ltxk_packed_attention's softmax for a batch that shares a prefix: the queries of
+ * each item see all `prefix` keys of it, then keys of the item's own.  Item b has
+ * lengths[b] of these (int32 in device memory, cut to 0 .. tokens_k; NULL: tokens_k)
+ * of the tokens_k that k and v hold, its tokens_q queries being the newest of them:
+ * query t stands at i = lengths[b] - tokens_q + t.  Causal, it sees own keys j <= i,
+ * and with i < 0 (padding in front of a shorter item) nothing at all, which gives
+ * zeros; else all of the item's.  Keys and values past an item's length, and those
+ * that the mask closes, change nothing, whatever they hold.
+ * q is bf16 at q + b*q_bstride + t*q_tstride + h*head_dim, k and v likewise, the
+ * prefix's at prefix_k + j*prefix_k_tstride + h'*head_dim; out is contiguous
+ * [batch*tokens_q, heads*head_dim] and overlaps no operand.  batch*tokens_q*heads,
+ * tokens_k and prefix stay below 2^31 - 1024.  Everything else as there. */
+int ltxk_prefix_attention(void *out, const void *q, int64_t q_bstride, int64_t q_tstride, const void *k,
+                          int64_t k_bstride, int64_t k_tstride, const void *v, int64_t v_bstride, int64_t v_tstride,
+                          const void *prefix_k, int64_t prefix_k_tstride, const void *prefix_v,
+                          int64_t prefix_v_tstride, const int32_t *lengths, int64_t batch, int64_t tokens_q,
+                          int64_t tokens_k, int64_t prefix, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                          int causal, float scale, void *workspace, int64_t workspace_bytes, void *stream);
+
 /* Bytes of workspace ltxk_linear needs for this shape (at most 64 MB). */
 int64_t ltxk_linear_workspace_bytes(int64_t m, int64_t n, int64_t k);
 

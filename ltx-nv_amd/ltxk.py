@@ -139,6 +139,18 @@ SIGNATURES = {
         [_c_vp, _c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64,
          _c_i64, _c_i64, _c_i64, _c_i64, _c_float, _c_vp, _c_i64, _c_vp],
     ),
+    "ltxk_packed_attention_workspace_bytes": (_c_i64, [_c_i64] * 6),
+    "ltxk_packed_attention": (
+        _c_int,
+        [_c_vp, _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_vp] + [_c_i64] * 6 +
+        [_c_int, _c_i64, _c_float, _c_vp, _c_i64, _c_vp],
+    ),
+    "ltxk_prefix_attention_workspace_bytes": (_c_i64, [_c_i64] * 7),
+    "ltxk_prefix_attention": (
+        _c_int,
+        [_c_vp, _c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64,
+         _c_vp] + [_c_i64] * 7 + [_c_int, _c_float, _c_vp, _c_i64, _c_vp],
+    ),
     "ltxk_quantize_fp8": (_c_int, [_c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_vp]),
     "ltxk_add_norm_modulate_fp8": (
         _c_int,
@@ -991,6 +1003,157 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: in
                                      _ptr(keep), keep_stride, _ptr(logits), b, tq, tk, heads, dh, dh ** -0.5,
                                      _ptr(ws), nbytes, _stream(q))
     _check_rc(rc, "cross_attention")
+    return out
+
+
+PACKED_HEAD_DIMS = (64, 128, 256)
+
+
+def _grouped_heads(width: int, heads: int, kv_heads: int | None) -> tuple[int, int]:
+    """(key heads, head dimension) of queries `width` wide."""
+    kv_heads = heads if kv_heads is None else kv_heads
+    if heads <= 0 or kv_heads <= 0 or heads % kv_heads:
+        raise ValueError(f"{heads} query heads are not a multiple of {kv_heads} key heads")
+    dh = width // heads
+    if width != heads * dh or dh not in PACKED_HEAD_DIMS:
+        raise ValueError(f"width {width} is not {heads} heads of 64, 128 or 256")
+    return kv_heads, dh
+
+
+def _packed_rows(x: torch.Tensor, name: str, width: int) -> int:
+    """The token stride of a bf16 (T, width) whose rows are contiguous, or an error (a single row's may be anything in
+    torch)."""
+    if not (type(x) is torch.Tensor and x.is_cuda and x.dtype == torch.bfloat16 and x.ndim == 2 and x.shape[1] == width):
+        if not isinstance(x, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor")
+        if x.device.type != "cuda":
+            raise RuntimeError(f"{name} is on {x.device}; ltxk kernels run on the ROCm device only")
+        if x.dtype != torch.bfloat16:
+            raise ValueError(f"{name} has dtype {x.dtype}, expected torch.bfloat16")
+        if x.ndim != 2 or x.shape[1] != width:
+            raise ValueError(f"{name} is {tuple(x.shape)}, expected (T, {width})")
+    st, sd = x.stride()
+    if sd == 1 and st == width:
+        return st
+    st = st if x.shape[0] > 1 else width
+    if sd != 1 or st % 8 or st < width:
+        raise ValueError(f"{name}'s rows must be contiguous, with a token stride (a multiple of 8) that covers them; got "
+                         f"{x.stride()}")
+    return st
+
+
+def _offsets(x: torch.Tensor, name: str, count: int | None = None) -> None:
+    _dev(x, name, torch.int32)
+    if x.ndim != 1 or x.shape[0] == 0 or count is not None and x.shape[0] != count:
+        raise ValueError(f"{name} {tuple(x.shape)} must be ({'sequences + 1' if count is None else count},)")
+
+
+@functools.lru_cache(maxsize=4096)
+def _packed_attention_workspace_bytes(*sizes: int) -> int:
+    return load().ltxk_packed_attention_workspace_bytes(*sizes)
+
+
+@functools.lru_cache(maxsize=4096)
+def _prefix_attention_workspace_bytes(*sizes: int) -> int:
+    return load().ltxk_prefix_attention_workspace_bytes(*sizes)
+
+
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: int, offsets: torch.Tensor,
+                     kv_heads: int | None = None, k_offsets: torch.Tensor | None = None, causal: bool = True,
+                     window: int | None = None, scale: float | None = None,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention over sequences of different lengths laid end to end: q (Tq, H*Dh), k and v (Tk, KVH*Dh), heads of 64, 128
+    or 256, kv_heads dividing heads (None: as many), scale 1/sqrt(Dh) unless given.  Returns (Tq, H*Dh).
+
+    Sequence s has queries offsets[s] .. offsets[s+1] - 1 and keys k_offsets[s] .. k_offsets[s+1] - 1 (None: those of
+    offsets, for as many keys as queries): int32 on the device, S + 1 ascending entries, not read by the host.  Where it
+    has more keys than queries, the queries are its newest tokens.  Causal, a query sees the keys up to its own, with
+    `window` only that many of them; else all of its sequence's.  One that sees none gives zeros.
+
+    q, k and v may be columns of wider rows.  What a mask closes, and rows of no sequence, may hold anything.  Rows of
+    `out` that belong to no sequence are left as they are (undefined in a fresh result)."""
+    if getattr(q, "ndim", 0) != 2:
+        raise ValueError("q must be a (T, H*Dh) tensor")
+    tq, d = q.shape
+    kv_heads, dh = _grouped_heads(d, heads, kv_heads)
+    qt = _packed_rows(q, "q", d)
+    kt = _packed_rows(k, "k", kv_heads * dh)
+    vt = _packed_rows(v, "v", kv_heads * dh)
+    tk = k.shape[0]
+    if v.shape[0] != tk:
+        raise ValueError(f"{tk} keys and {v.shape[0]} values")
+    _offsets(offsets, "offsets")
+    if k_offsets is None:
+        if tk != tq:
+            raise ValueError(f"{tq} queries and {tk} keys need k_offsets")
+        k_offsets = offsets
+    else:
+        _offsets(k_offsets, "k_offsets", offsets.shape[0])
+    if window is not None and (window <= 0 or not causal):
+        raise ValueError("a window must be positive, and needs the causal mask")
+    if out is None:
+        out = q.new_empty((tq, d))
+    else:
+        _dev(out, "out")
+        if out.shape != (tq, d):
+            raise ValueError(f"out {tuple(out.shape)} != {(tq, d)}")
+    _one_device(q, k, v, offsets, k_offsets, out)
+    seqs = offsets.shape[0] - 1
+    if out.numel() == 0 or seqs == 0:
+        return out
+    nbytes = _packed_attention_workspace_bytes(tq, tk, seqs, heads, kv_heads, dh)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    rc = load().ltxk_packed_attention(out.data_ptr(), q.data_ptr(), qt, k.data_ptr(), kt, v.data_ptr(), vt,
+                                      offsets.data_ptr(), k_offsets.data_ptr(), seqs, tq, tk, heads, kv_heads, dh, causal,
+                                      window or 0, dh ** -0.5 if scale is None else scale, _ptr(ws), nbytes, _stream(q))
+    _check_rc(rc, "packed_attention")
+    return out
+
+
+def prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Tensor,
+                     heads: int, kv_heads: int | None = None, lengths: torch.Tensor | None = None, causal: bool = True,
+                     scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of a batch over a prefix that all of it shares, then over keys of each item's own: q (B, Tq, H*Dh), k and
+    v (B, Tk, KVH*Dh), prefix_k and prefix_v (P, KVH*Dh), heads as in `packed_attention`.  Returns (B, Tq, H*Dh).
+
+    lengths (B,) int32 on the device: how many of the Tk own keys each item has so far (None: all).  Its queries are the
+    newest of them: query t stands at lengths[b] - Tq + t.  Causal, it sees the whole prefix and own keys up to its own;
+    queries in front of a shorter item's first token (padding) give zeros.  Else it sees the prefix and all own keys.
+
+    Where few queries an item make it worth it, the prefix is read for all of them at once.  q, k, v and the prefix may be
+    columns of wider rows, k and v views of a larger cache.  What lies past an item's length may hold anything."""
+    if getattr(q, "ndim", 0) != 3 or getattr(k, "ndim", 0) != 3:
+        raise ValueError("q, k and v must be (B, T, H*Dh) tensors")
+    (b, tq, d), tk = q.shape, k.shape[1]
+    kv_heads, dh = _grouped_heads(d, heads, kv_heads)
+    qb, qt = _attention_rows(q, "q", b, tq, d)
+    kb, kt = _attention_rows(k, "k", b, tk, kv_heads * dh)
+    vb, vt = _attention_rows(v, "v", b, tk, kv_heads * dh)
+    pkt = _packed_rows(prefix_k, "prefix_k", kv_heads * dh)
+    pvt = _packed_rows(prefix_v, "prefix_v", kv_heads * dh)
+    prefix = prefix_k.shape[0]
+    if prefix_v.shape[0] != prefix:
+        raise ValueError(f"{prefix} keys and {prefix_v.shape[0]} values in the prefix")
+    if lengths is not None:
+        _dev(lengths, "lengths", torch.int32)
+        if lengths.shape != (b,):
+            raise ValueError(f"lengths {tuple(lengths.shape)} must be ({b},)")
+    if out is None:
+        out = q.new_empty((b, tq, d))
+    else:
+        _dev(out, "out")
+        if out.shape != (b, tq, d):
+            raise ValueError(f"out {tuple(out.shape)} != {(b, tq, d)}")
+    _one_device(q, k, v, prefix_k, prefix_v, lengths, out)
+    if out.numel() == 0:
+        return out
+    nbytes = _prefix_attention_workspace_bytes(b, tq, tk, prefix, heads, kv_heads, dh)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    rc = load().ltxk_prefix_attention(out.data_ptr(), q.data_ptr(), qb, qt, k.data_ptr(), kb, kt, v.data_ptr(), vb, vt,
+                                      prefix_k.data_ptr(), pkt, prefix_v.data_ptr(), pvt, _ptr(lengths), b, tq, tk, prefix,
+                                      heads, kv_heads, dh, causal, dh ** -0.5 if scale is None else scale, _ptr(ws), nbytes,
+                                      _stream(q))
+    _check_rc(rc, "prefix_attention")
     return out
 
 
