@@ -415,7 +415,7 @@ int64_t ltxk_packed_attention_workspace_bytes(int64_t tokens_q, int64_t tokens_k
  * sees, and those that a mask closes, change nothing, whatever they hold.  Rows of out
  * that belong to no sequence are left as they are.
  * q is bf16 at q + t*q_tstride + h*head_dim (elements; multiples of 8, at least
- * heads*head_dim, at most 2^23), k and v likewise with kv_heads; out is contiguous
+ * heads*head_dim, below 2^23), k and v likewise with kv_heads; out is contiguous
  * [tokens_q, heads*head_dim] and overlaps no operand.  Scores, softmax and sums are
  * fp32.  tokens_q*heads and tokens_k stay below 2^31 - 1024.  `workspace`: device
  * memory of ltxk_packed_attention_workspace_bytes, 16-byte aligned (NULL if that is

@@ -5,14 +5,15 @@
 // A query at position i of its sequence's own n keys (its newest ones are the queries')
 // sees keys [lo, hi) of them, hi = i + 1 and lo = max(0, i + 1 - window) where the mask is
 // causal and [0, n) else, behind all of the prefix (if i >= 0).
-#include "ltxk_common.h"
+#include "flash_tiles.h"
 
 #include <cfloat>
+#include <type_traits>
 
 namespace ltxk {
 namespace {
 
-constexpr int kWaves = 4;
+constexpr int kRows = 32 * kWaves;  // rows (a query at one head of the group) of a tile, 32 a wave
 
 struct Params {
     const uint16_t *q, *k, *v, *pk, *pv;
@@ -25,58 +26,144 @@ struct Params {
     int seqs, prefix, heads, kv_heads, group, window;  // window 0: none
     bool causal;
     float scale2;         // scale * log2(e)
-};
-
-// What one sequence's queries attend to, at one key head.
-struct Sequence {
-    const char *q;        // its first query, at the first head of the group
-    int64_t first;        // and that query's row of the output
-    const char *k, *v;    // its first own key
-    int queries, n;       // queries and own keys
+    int tiles, slots;     // row tiles of a key head, and places for them and their parts on an XCD
+    int parts, least;     // the keys of a tile are cut into up to `parts`, of at least `least` tiles each
+    float *part;          // cut tiles: each part's weighted sums of v (kRows x D)
+    float2 *stats;        // and each of its rows' maximum and sum of weights
 };
 
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-// Sequence s, its lengths cut to what the tensors hold whatever the offsets say.
-template <bool PACKED>
-__device__ __forceinline__ Sequence sequence(const Params &p, int s, int kvh, int dim)
+// A tile of rows, what its rows attend to, and where they go.  Rows are a sequence's
+// queries, each at all heads of the group in turn, so that few queries fill a tile's rows
+// and a causal tile spans few of them.
+struct Tile {
+    const char *q;        // the sequence's first query, at the group's first head
+    int64_t token;        // and that query's row of the output
+    const char *k, *v;    // its first own key
+    int queries, n;       // its queries and own keys
+    int first, rows;      // the tile's first row, and the rows of the whole sequence
+    int from, to;         // own keys that some of its rows see
+    int np, tiles;        // key tiles: of the prefix, and in all
+};
+
+// Where sequence s's row tiles begin, if each sequence takes one more than its rows fill:
+// never less than it needs, and known without the others' lengths.
+template <int ROWS>
+__device__ __forceinline__ int first_tile(const Params &p, int s)
 {
-    Sequence r;
-    const int64_t qh = static_cast<int64_t>(kvh) * p.group * dim * 2, kh = static_cast<int64_t>(kvh) * dim * 2;
-    if constexpr (PACKED) {
+    const int64_t q0 = min(max(p.qo[s], 0), p.tq);
+    return static_cast<int>(q0 * p.group / ROWS) + s;
+}
+
+// The last s with first_tile(s) <= t, 64 of them at a time.
+template <int ROWS>
+__device__ __forceinline__ int sequence_of(const Params &p, int t)
+{
+    const int lane = threadIdx.x & 63;
+    int lo = 0, count = p.seqs;
+    while (count > 1) {
+        const int step = (count + 63) / 64, i = lane * step;
+        const uint64_t under = __ballot(i < count && first_tile<ROWS>(p, lo + min(i, count - 1)) <= t);
+        const int at = under ? (63 - __builtin_clzll(under)) * step : 0;
+        lo += at;
+        count = min(step, count - at);
+    }
+    return uniform(lo);
+}
+
+// Row tile t of key head kvh, or false if there is none.
+template <int D, int ROWS>
+__device__ __forceinline__ bool find_tile(const Params &p, int t, int kvh, Tile &r)
+{
+    const int64_t qh = static_cast<int64_t>(kvh) * p.group * D * 2, kh = static_cast<int64_t>(kvh) * D * 2;
+    int tile;
+    if (p.qo) {
+        const int s = sequence_of<ROWS>(p, t);
+        // lengths are cut to what the tensors hold, whatever the offsets say
         const int q0 = min(max(uniform(p.qo[s]), 0), p.tq), q1 = min(uniform(p.qo[s + 1]), p.tq);
         const int k0 = min(max(uniform(p.ko[s]), 0), p.tk), k1 = min(uniform(p.ko[s + 1]), p.tk);
+        tile = t - (static_cast<int>(static_cast<int64_t>(q0) * p.group / ROWS) + s);
         r.queries = max(q1 - q0, 0);
         r.n = max(k1 - k0, 0);
-        r.first = q0;
+        r.token = q0;
         r.q = reinterpret_cast<const char *>(p.q) + static_cast<int64_t>(q0) * p.qts + qh;
         r.k = reinterpret_cast<const char *>(p.k) + static_cast<int64_t>(k0) * p.kts + kh;
         r.v = reinterpret_cast<const char *>(p.v) + static_cast<int64_t>(k0) * p.vts + kh;
     } else {
+        const int s = t % p.seqs;
+        tile = t / p.seqs;
         r.queries = p.tq;
         r.n = p.lengths ? min(max(uniform(p.lengths[s]), 0), p.tk) : p.tk;
-        r.first = static_cast<int64_t>(s) * p.tq;
+        r.token = static_cast<int64_t>(s) * p.tq;
         r.q = reinterpret_cast<const char *>(p.q) + s * p.qbs + qh;
         r.k = reinterpret_cast<const char *>(p.k) + s * p.kbs + kh;
         r.v = reinterpret_cast<const char *>(p.v) + s * p.vbs + kh;
     }
-    return r;
+    r.rows = r.queries * p.group;
+    r.first = tile * ROWS;
+    if (tile < 0 || r.first >= r.rows) return false;
+    const int behind = r.n - r.queries;  // keys in front of the first query's
+    const int last = min(r.first + ROWS, r.rows) - 1;
+    r.to = p.causal ? max(behind + last / p.group + 1, 0) : r.n;
+    r.from = p.window ? min(max(behind + r.first / p.group + 1 - p.window, 0), r.to) : 0;
+    r.np = r.to || !p.causal ? (p.prefix + kKeys - 1) / kKeys : 0;
+    r.tiles = r.np + (r.to - r.from + kKeys - 1) / kKeys;
+    return true;
 }
 
-// The last s with offsets[s] <= token, of `count` sequences (0 if there is none).
-__device__ __forceinline__ int sequence_of(const int *offsets, int count, int token)
+// Into how many parts a tile's keys are cut: short ones into few.
+__device__ __forceinline__ int parts_of(const Params &p, const Tile &r)
 {
-    int lo = 0, hi = count - 1;
-    while (lo < hi) {
-        const int mid = lo + (hi - lo + 1) / 2;
-        if (uniform(offsets[mid]) <= token) lo = mid;
-        else hi = mid - 1;
+    return max(min(p.parts, r.tiles / p.least), 1);
+}
+
+// Row `row` of a tile: its query, head of the group, and the own keys [lo, hi) it sees (and
+// the prefix, if any).
+struct Row {
+    int query, member, lo, hi;
+    bool any;
+};
+__device__ __forceinline__ Row find_row(const Params &p, const Tile &r, int row)
+{
+    Row w;
+    w.query = row / p.group;
+    w.member = row - w.query * p.group;
+    const int pos = r.n - r.queries + w.query;
+    w.hi = p.causal ? max(pos + 1, 0) : r.n;
+    w.lo = p.window ? max(w.hi - p.window, 0) : 0;
+    w.any = w.hi > w.lo || (p.prefix > 0 && !p.causal);
+    return w;
+}
+
+// The 64 keys (values) of key tile g, from memory's `base` on, `valid` of them.
+struct Span {
+    rsrc_t rsrc;
+    uint32_t stride;
+    int valid;
+};
+template <int D, bool V>
+__device__ __forceinline__ Span key_span(const Params &p, const Tile &r, int kvh, int g)
+{
+    const char *base;
+    Span s;
+    if (g < r.np) {
+        s.valid = min(kKeys, p.prefix - g * kKeys);
+        s.stride = V ? p.pvts : p.pkts;
+        base = reinterpret_cast<const char *>(V ? p.pv : p.pk) + static_cast<int64_t>(kvh) * D * 2 +
+               static_cast<int64_t>(g) * kKeys * s.stride;
+    } else {
+        const int at = r.from + (g - r.np) * kKeys;
+        s.valid = min(kKeys, r.to - at);
+        s.stride = V ? p.vts : p.kts;
+        base = (V ? r.v : r.k) + static_cast<int64_t>(at) * s.stride;
     }
-    return lo;
+    s.rsrc = make_rsrc(base, static_cast<uint32_t>(s.valid - 1) * s.stride + 2 * D);
+    return s;
 }
 
 // Adds keys [from, to) to a row's running maximum, sum and weighted values: a lane has the
-// score of one key of 64, then 2 or more columns of the values.
+// score of one key of 64, then one or more columns of the values.
 template <int D>
 __device__ __forceinline__ void attend_keys(const char *q, const char *k, uint32_t ks, const char *v, uint32_t vs, int from,
                                             int to, float scale2, float &mx, float &sum, float (&acc)[D / 64])
@@ -113,44 +200,421 @@ __device__ __forceinline__ void attend_keys(const char *q, const char *k, uint32
     }
 }
 
-// A wave for each query and head.
-template <int D, bool PACKED>
-__global__ void __launch_bounds__(kWaves * 64) row_kernel(Params p)
+// One row over key tiles t0 .. t1 - 1 by a whole wave, only what it sees: for rows whose
+// matrix products met a masked value that is not finite (its weight of zero makes NaN).
+template <int D>
+__device__ __forceinline__ void attend_row(const Params &p, const Tile &r, int kvh, int row, int t0, int t1, float &mx,
+                                           float &sum, float (&acc)[D / 64])
 {
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * kWaves + uniform(threadIdx.x >> 6);
-    const int64_t token = row / p.heads;
-    const int head = static_cast<int>(row % p.heads), kvh = head / p.group;
-    if (token >= static_cast<int64_t>(PACKED ? 1 : p.seqs) * p.tq) return;
-    const int s = PACKED ? sequence_of(p.qo, p.seqs, static_cast<int>(token)) : static_cast<int>(token / p.tq);
-    const Sequence r = sequence<PACKED>(p, s, kvh, D);
-    const int64_t t = token - r.first;
-    if (t < 0 || t >= r.queries) return;  // a row of no sequence
-    const int pos = r.n - r.queries + static_cast<int>(t);
-    const int hi = p.causal ? pos + 1 : r.n, lo = p.window ? max(0, hi - p.window) : 0;
-    const char *q = r.q + t * p.qts + (head - kvh * p.group) * D * 2;
-    float mx = -FLT_MAX, sum = 0.f, acc[D / 64] = {};
-    if (!p.causal || pos >= 0) {
-        const int64_t kh = static_cast<int64_t>(kvh) * D;
-        attend_keys<D>(q, reinterpret_cast<const char *>(p.pk + kh), p.pkts, reinterpret_cast<const char *>(p.pv + kh), p.pvts,
-                       0, p.prefix, p.scale2, mx, sum, acc);
-        attend_keys<D>(q, r.k, p.kts, r.v, p.vts, lo, hi, p.scale2, mx, sum, acc);
-    }
-    const bool none = p.causal ? pos < 0 : p.prefix + r.n == 0;
-    uint16_t *out = p.out + (token * p.heads + head) * D + (threadIdx.x & 63) * (D / 64);
+    const Row w = find_row(p, r, row);
+    const char *q = r.q + static_cast<int64_t>(w.query) * p.qts + w.member * D * 2;
+    const int64_t kh = static_cast<int64_t>(kvh) * D;
+    mx = -FLT_MAX;
+    sum = 0.f;
 #pragma unroll
-    for (int c = 0; c < D / 64; ++c) out[c] = f32_to_bf16(none ? 0.f : acc[c] / sum);
+    for (int c = 0; c < D / 64; ++c) acc[c] = 0.f;
+    if (!w.any) return;
+    attend_keys<D>(q, reinterpret_cast<const char *>(p.pk + kh), p.pkts, reinterpret_cast<const char *>(p.pv + kh), p.pvts,
+                   min(t0, r.np) * kKeys, min(min(t1, r.np) * kKeys, p.prefix), p.scale2, mx, sum, acc);
+    attend_keys<D>(q, r.k, p.kts, r.v, p.vts, max(w.lo, r.from + (max(t0, r.np) - r.np) * kKeys),
+                   min(w.hi, r.from + (max(t1, r.np) - r.np) * kKeys), p.scale2, mx, sum, acc);
+}
+
+// Tile and part of this workgroup.  Workgroups are dealt to the 8 XCDs in turn: of the key
+// heads, as many at a time as divide 8 go to XCDs of their own, whose L2 then holds their
+// keys and values, and each head's tiles are dealt among its XCDs.  The tiles with the most
+// keys (a sequence's last ones) come first.
+__device__ __forceinline__ bool find_work(const Params &p, int &t, int &kvh, int &part)
+{
+    const int xcd = blockIdx.x & 7, j = blockIdx.x >> 3;
+    const int beside = p.kv_heads & -p.kv_heads & 7 ? p.kv_heads & -p.kv_heads : 8, each = 8 / beside;
+    kvh = j / p.slots * beside + xcd % beside;
+    const int slot = p.parts > 1 ? xcd / beside * p.slots + j % p.slots : j % p.slots * each + xcd / beside;
+    t = p.tiles - 1 - slot % p.tiles;
+    part = slot / p.tiles;
+    return part < p.parts;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) tile_kernel(Params p)
+{
+    constexpr int KS = D / 16;               // contraction steps of the scores
+    constexpr int MT = D / 32;               // output tiles
+    constexpr int NK = 2 * KS, NV = 4 * MT;  // K and V fragments of a tile
+    constexpr int kAhead = 4;                // fragments read ahead of the products
+    constexpr int kTileBytes = kKeys * D * 2;
+    __shared__ __attribute__((aligned(1024))) char k0[kTileBytes];
+    __shared__ __attribute__((aligned(1024))) char k1[kTileBytes];
+    __shared__ __attribute__((aligned(1024))) char v0[kTileBytes];
+    __shared__ __attribute__((aligned(1024))) char v1[kTileBytes];
+
+    int t, kvh, part;
+    Tile r;
+    if (!find_work(p, t, kvh, part) || !find_tile<D, kRows>(p, t, kvh, r)) return;
+    const int parts = parts_of(p, r);
+    if (part >= parts) return;
+    const int t0 = static_cast<int>(static_cast<int64_t>(part) * r.tiles / parts);
+    const int n = static_cast<int>(static_cast<int64_t>(part + 1) * r.tiles / parts) - t0;
+    const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int l32 = lane & 31, half = lane >> 5;
+    const int first = r.first + wave * 32, last = r.rows - 1;
+    const Row own = find_row(p, r, min(first + l32, last));
+    const int64_t at = (r.token + own.query) * p.heads + kvh * p.group + own.member;  // this row of the output
+    // rows first .. first + 31 all see own keys up to sure_hi from sure_lo on
+    const int sure_hi = uniform(own.hi), sure_lo = __builtin_amdgcn_readlane(own.lo, 31);
+    uint16_t *const out = p.out;
+
+    if (n == 0) {  // no key for any row
+        for (int i = threadIdx.x; i < kRows * (D / 8); i += kWaves * 64) {
+            const int row = r.first + i / (D / 8);
+            if (row > last) break;
+            const Row w = find_row(p, r, row);
+            *reinterpret_cast<u32x4 *>(out + ((r.token + w.query) * p.heads + kvh * p.group + w.member) * D +
+                                       i % (D / 8) * 8) = u32x4{};
+        }
+        return;
+    }
+
+    // Queries: lane l holds row l % 32, elements 16 s + 8 (l/32) .. + 7.
+    bf16x8 qf[KS];
+    {
+        const char *qp = r.q + static_cast<int64_t>(own.query) * p.qts + own.member * D * 2 + half * 16;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const bf16x8 *>(qp + s * 32);
+    }
+    auto load = [&](auto is_v, const Span &s, int c, char *dst) __attribute__((always_inline)) {
+        constexpr bool V = decltype(is_v)::value;
+        const int at = wave * kLoads<D> + c, row = part_row<D>(c, wave, lane), pos = lane % (D / 8);
+        const uint32_t off = __umul24(min(row, s.valid - 1), s.stride) + (V ? v_pos<D>(row, pos) : k_pos<D>(row, pos)) * 16;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(s.rsrc, (lds_char *)(dst + at * 1024), 16, off, 0, 0, 0);
+    };
+    {
+        const Span s = key_span<D, false>(p, r, kvh, t0);
+#pragma unroll
+        for (int c = 0; c < kLoads<D>; ++c) load(std::false_type{}, s, c, k0);
+    }
+
+    // LDS byte offsets of this lane's fragments.  K: row l % 32 (+ 32 u), chunk
+    // 2 s + half.  V (transposed reads of 4 keys x 16 columns by 16 lanes): rows
+    // 16 s + 8 e + 4 half + (l%16)/4, columns 32 m + 16 (l/16 % 2) + 4 (l % 4).
+    int k_off[KS], v_off[MT][2];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) k_off[s] = l32 * 2 * D + k_pos<D>(l32, 2 * s + half) * 16;
+    const int vi = lane & 15;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int row = 8 * e + 4 * half + (vi >> 2);
+            const int c = 4 * m + 2 * ((lane >> 4) & 1) + ((vi & 3) >> 1);
+            v_off[m][e] = row * 2 * D + v_pos<D>(row, c) * 16 + (vi & 1) * 8;
+        }
+
+    f32x16 o[MT] = {};
+    f32x16 s[2];     // scores, transposed: register i of s[u] is key 32 u + 8 (i/4) + 4 half + i % 4 of row l % 32
+    u32x4 w[4];      // weights, two a register, in the order of the scores
+    float mx = 0.f;  // running maximum of the scaled scores (the same in lanes l and l ^ 32)
+    float sum = 0.f; // this lane's share of the weights' sum
+
+    // Fragment i of a K tile (contraction step i / 2 of keys 32 (i%2) ..) and of a
+    // V tile (keys 16 (i / MT) .., columns 32 (i % MT) ..).
+    auto k_frag = [&](const char *kt, int i) {
+        return *reinterpret_cast<const bf16x8 *>(kt + k_off[i >> 1] + (i & 1) * 64 * D);
+    };
+    auto v_frag = [&](const char *vt, int i) {
+        typedef __attribute__((address_space(3))) bf16x4 lds4;
+        const int m = i % MT, st = i / MT;
+        const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4 *)(vt + v_off[m][0] + st * 32 * D));
+        const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4 *)(vt + v_off[m][1] + st * 32 * D));
+        return cat(lo, hi);
+    };
+    // Matrix phase: a run of the stream of products that a tile takes, the weights
+    // times V of the tile before (0 .. NV - 1), then its scores (NV .. NV + NK - 1),
+    // with the LDS fragments read ahead of them and `loads(j)` between them.
+    auto products = [&](auto from, auto to, const char *vp, const char *kc, auto loads)
+                        __attribute__((always_inline)) {
+        bf16x8 f[NV + NK];
+        auto frag = [&](int j) { f[j] = j < NV ? v_frag(vp, j) : k_frag(kc, j - NV); };
+#pragma unroll
+        for (int j = from; j < from + kAhead; ++j) frag(j);
+#pragma unroll
+        for (int j = from; j < to; ++j) {
+            if (j + kAhead < to) frag(j + kAhead);
+            loads(j - from);
+            if (j < NV) {
+                o[j % MT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[j], __builtin_bit_cast(bf16x8, w[j / MT]),
+                                                                    o[j % MT], 0, 0, 0);
+            } else {
+                const int i = j - NV;
+                s[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[j], qf[i >> 1], i < 2 ? f32x16{} : s[i & 1], 0, 0, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // Vector phase of tile i: its maximum, the rescale of what was summed so far
+    // if a row's maximum grew, its weights.
+    auto softmax = [&](int i) __attribute__((always_inline)) {
+        // keys that not all of the wave's rows see (or that are none) get weight zero
+        const int g = t0 + i, key = r.from + (g - r.np) * kKeys;
+        const bool common = g < r.np;
+        if (common ? p.prefix - g * kKeys < kKeys : key + kKeys > sure_hi || key < sure_lo) {
+            const int hi = (common ? p.prefix - g * kKeys : own.hi - key) - 4 * half;
+            const int lo = (common ? 0 : own.lo - key) - 4 * half;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int j = 32 * u + 8 * (e >> 2) + (e & 3);
+                    if (j >= hi || j < lo) s[u][e] = -INFINITY;
+                }
+        }
+        float m4[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            m4[c] = s[c >> 1][8 * (c & 1)];
+#pragma unroll
+            for (int e = 1; e < 8; ++e) m4[c] = fmaxf(m4[c], s[c >> 1][8 * (c & 1) + e]);
+        }
+        const float m = pair_max(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]))) * p.scale2;
+        if (i == 0) {
+            mx = fmaxf(m, -FLT_MAX);  // finite, so that scores of -inf weigh zero
+        } else if (__any(m > mx)) {
+            const float nm = fmaxf(m, mx);
+            const float a = __builtin_amdgcn_exp2f(mx - nm);
+            mx = nm;
+            sum *= a;
+#pragma unroll
+            for (int c = 0; c < MT; ++c)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[c][e] *= a;
+        }
+        // Scores past kLarge round before the maximum is taken off, as it did: else the
+        // largest weight would be 2^(its rounding) instead of 1.  (Rows that saw no key yet
+        // have a maximum of -FLT_MAX.)
+        float scale2 = p.scale2;
+        if (__any(fabsf(mx) > kLarge)) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[u][e] *= scale2;
+            scale2 = 1.f;
+        }
+        float add[2] = {};
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j >> 3][2 * (j & 7)], scale2, -mx));
+            const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j >> 3][2 * (j & 7) + 1], scale2, -mx));
+            add[0] += x;
+            add[1] += y;
+            w[j >> 2][j & 3] = pack_bf16x2(x, y);
+        }
+        sum += add[0] + add[1];
+    };
+
+    // Tile i: kc holds its keys, vp the values of tile i - 1.  Its values and the
+    // next tile's keys (the last tile's once more after the last) load into the
+    // other buffers between the products.
+    using std::integral_constant;
+    auto tile = [&](int i, auto from, const char *kc, const char *vp, char *kn, char *vn)
+                    __attribute__((always_inline)) {
+        constexpr int kEvery = from == 0 ? 3 : 2;
+        const Span ks = key_span<D, false>(p, r, kvh, t0 + min(i + 1, n - 1)), vs = key_span<D, true>(p, r, kvh, t0 + i);
+        products(from, integral_constant<int, NV + NK>{}, vp, kc, [&](int j) __attribute__((always_inline)) {
+            if (j % kEvery) return;
+            const int c = j / kEvery;
+            if (c < kLoads<D>)
+                load(std::true_type{}, vs, c, vn);
+            else if (c < 2 * kLoads<D>)
+                load(std::false_type{}, ks, c - kLoads<D>, kn);
+        });
+        softmax(i);
+        __builtin_amdgcn_sched_barrier(0);
+        tile_barrier();
+    };
+    constexpr integral_constant<int, 0> whole;
+    tile_barrier();
+    tile(0, integral_constant<int, NV>{}, k0, v1, k1, v0);
+    for (int i = 1; i < n; i += 2) {
+        tile(i, whole, k1, v0, k0, v1);
+        if (i + 1 < n) tile(i + 1, whole, k0, v1, k1, v0);
+    }
+    products(whole, integral_constant<int, NV>{}, n & 1 ? v0 : v1, nullptr, [](int) {});
+
+    // Lane l: row l % 32, columns 32 m + 8 j + 4 half + (0..3) in registers 4 j ..
+    const float total = pair_sum(sum);
+    bool fine = true;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) fine = fine && fabsf(o[m][e]) <= FLT_MAX;
+    const uint64_t odd = __ballot(!fine);
+    uint32_t again = static_cast<uint32_t>(odd) | static_cast<uint32_t>(odd >> 32);  // rows to be done once more
+    const int64_t unit = (static_cast<int64_t>(t) * p.kv_heads + kvh) * p.parts + part;
+    if (parts > 1) {
+        const int64_t u = unit * kRows + wave * 32 + l32;
+        if (first + l32 <= last) {
+            if (half == 0) p.stats[u] = make_float2(mx, total);
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    *reinterpret_cast<f32x4 *>(p.part + u * D + 32 * m + 8 * c + 4 * half) =
+                        f32x4{o[m][4 * c], o[m][4 * c + 1], o[m][4 * c + 2], o[m][4 * c + 3]};
+        }
+    } else {
+        const float inv = 1.f / total;
+        // stored as 64 bytes of 16 rows each
+        const int64_t at0 = __shfl(at, lane & 15, 64), at1 = __shfl(at, (lane & 15) + 16, 64);
+        const int col = 8 * half + (lane & 16);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            uint32_t v[4][2];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                float f[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) f[e] = own.any ? o[m][4 * c + e] * inv : 0.f;
+                v[c][0] = pack_bf16x2(f[0], f[1]);
+                v[c][1] = pack_bf16x2(f[2], f[3]);
+            }
+            u32x4 lo, hi;
+            rows16(v, lo, hi);
+            if (first + (lane & 15) <= last)
+                __builtin_nontemporal_store(lo, reinterpret_cast<u32x4 *>(out + at0 * D + col + 32 * m));
+            if (first + (lane & 15) + 16 <= last)
+                __builtin_nontemporal_store(hi, reinterpret_cast<u32x4 *>(out + at1 * D + col + 32 * m));
+        }
+    }
+    if (again) {
+        __builtin_amdgcn_s_waitcnt(0x0070);
+        asm volatile("" ::: "memory");
+        do {
+            const int i = __builtin_ctz(again), row = first + i;
+            again &= again - 1;
+            if (row > last) continue;
+            float m1, sum1, acc[D / 64];
+            attend_row<D>(p, r, kvh, row, t0, t0 + n, m1, sum1, acc);
+            const int64_t to = __builtin_amdgcn_readlane(static_cast<int>(at), i) & 0xffffffffll |
+                               static_cast<int64_t>(__builtin_amdgcn_readlane(static_cast<int>(at >> 32), i)) << 32;
+            const bool any = find_row(p, r, row).any;
+            const int64_t u = unit * kRows + wave * 32 + i;
+            if (parts > 1 && lane == 0) p.stats[u] = make_float2(m1, sum1);
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) {
+                const int col = lane * (D / 64) + c;
+                if (parts > 1)
+                    p.part[u * D + col] = acc[c];
+                else
+                    out[to * D + col] = f32_to_bf16(any ? acc[c] / sum1 : 0.f);
+            }
+        } while (again);
+    }
+}
+
+// Joins the parts of the cut tiles: 8 columns of one row a thread.
+template <int D>
+__global__ void __launch_bounds__(256) join_kernel(Params p)
+{
+    constexpr int kThreads = kRows * (D / 8);  // of a tile
+    const int64_t tile = static_cast<int64_t>(blockIdx.x) / (kThreads / 256);
+    const int i = blockIdx.x % (kThreads / 256) * 256 + threadIdx.x, c = i % (D / 8), at = i / (D / 8);
+    const int t = static_cast<int>(tile / p.kv_heads), kvh = static_cast<int>(tile % p.kv_heads);
+    Tile r;
+    if (!find_tile<D, kRows>(p, t, kvh, r)) return;
+    const int parts = parts_of(p, r);
+    if (parts == 1 || r.first + at >= r.rows) return;  // the tile's only part has written the output
+    const Row w = find_row(p, r, r.first + at);
+    const int64_t u = tile * p.parts * kRows + at;
+    float m = -INFINITY;
+    for (int k = 0; k < parts; ++k) m = fmaxf(m, p.stats[u + k * kRows].x);
+    float acc[8] = {}, sum = 0.f;
+    for (int k = 0; k < parts; ++k) {
+        const float2 st = p.stats[u + k * kRows];
+        const float f = __builtin_amdgcn_exp2f(st.x - m);
+        const f32x4 *x = reinterpret_cast<const f32x4 *>(p.part + (u + k * kRows) * D + c * 8);
+        const f32x4 lo = x[0], hi = x[1];
+        sum += f * st.y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            acc[e] = __builtin_fmaf(f, lo[e], acc[e]);
+            acc[4 + e] = __builtin_fmaf(f, hi[e], acc[4 + e]);
+        }
+    }
+    const float inv = 1.f / sum;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] = w.any ? acc[e] * inv : 0.f;
+    *reinterpret_cast<u32x4 *>(p.out + ((r.token + w.query) * p.heads + kvh * p.group + w.member) * D + c * 8) = pack8v(acc);
 }
 
 constexpr int64_t kMost = 0x7fffffff - 1024;  // rows that are counted in int
-constexpr int64_t kStride = 1 << 23;          // elements of a token stride: 64 rows within 2^31 bytes
+constexpr int64_t kStride = (1 << 23) - 8;    // elements of a token stride: its bytes are 24 bits
 
-template <bool PACKED>
-void launch(const Params &p, int dim, int64_t rows, hipStream_t s)
+// How a call is cut: row tiles of a key head, and into how many parts at most each one's
+// keys, so that few tiles still fill the chip (two workgroups a compute unit, one with heads
+// of 256), with at least kLeast key tiles a part.
+constexpr int kLeast = 4;
+
+struct Plan {
+    int64_t tiles, parts, slots, blocks;
+};
+
+Plan plan(int64_t tiles, int64_t key_tiles, int64_t kv_heads, int64_t head_dim)
 {
-    const unsigned blocks = static_cast<unsigned>((rows + kWaves - 1) / kWaves);
-    if (dim == 64) row_kernel<64, PACKED><<<blocks, kWaves * 64, 0, s>>>(p);
-    else if (dim == 128) row_kernel<128, PACKED><<<blocks, kWaves * 64, 0, s>>>(p);
-    else row_kernel<256, PACKED><<<blocks, kWaves * 64, 0, s>>>(p);
+    Plan c;
+    c.tiles = tiles;
+    const int64_t room = head_dim == 256 ? 256 : 512;
+    c.parts = 1;
+    while (c.parts < 64 && tiles * kv_heads * c.parts * 2 <= room && key_tiles >= c.parts * 2 * kLeast) c.parts *= 2;
+    const int64_t low = kv_heads & -kv_heads, beside = low < 8 ? low : 8;
+    c.slots = (tiles * c.parts + 8 / beside - 1) / (8 / beside);
+    c.blocks = 8 * c.slots * (kv_heads / beside);
+    return c;
+}
+
+Plan plan_packed(int64_t tokens_q, int64_t tokens_k, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t head_dim)
+{
+    return plan(tokens_q * (heads / kv_heads) / kRows + sequences, (tokens_k / sequences + kKeys - 1) / kKeys, kv_heads, head_dim);
+}
+
+Plan plan_prefix(int64_t batch, int64_t tokens_q, int64_t tokens_k, int64_t prefix, int64_t heads, int64_t kv_heads,
+                 int64_t head_dim)
+{
+    return plan((tokens_q * (heads / kv_heads) + kRows - 1) / kRows * batch,
+                (prefix + kKeys - 1) / kKeys + (tokens_k + kKeys - 1) / kKeys, kv_heads, head_dim);
+}
+
+int64_t parts_bytes(const Plan &c, int64_t kv_heads, int64_t head_dim)
+{
+    return c.parts > 1 ? c.tiles * kv_heads * c.parts * kRows * (head_dim + 2) * 4 : 0;
+}
+
+template <int D>
+void launch(const Params &p, int64_t blocks, hipStream_t s)
+{
+    tile_kernel<D><<<static_cast<unsigned>(blocks), kWaves * 64, 0, s>>>(p);
+    if (p.parts > 1)
+        join_kernel<D><<<static_cast<unsigned>(static_cast<int64_t>(p.tiles) * p.kv_heads * (kRows * D / 8 / 256)), 256, 0, s>>>(p);
+}
+
+// The launch, once the operands are checked and p holds them.
+int run(const char *what, Params &p, const Plan &c, int64_t head_dim, void *workspace, int64_t workspace_bytes, void *stream)
+{
+    // a launch holds fewer than 2^32 threads
+    if (c.blocks >= (int64_t{1} << 32) / (kWaves * 64)) return fail(LTXK_E_ARG, "%s: too many row tiles", what);
+    const int64_t need = parts_bytes(c, p.kv_heads, head_dim);
+    if (need && (!workspace || !aligned16(workspace) || workspace_bytes < need))
+        return fail(LTXK_E_ARG, "%s: the workspace must hold ltxk_%s_workspace_bytes, 16-byte aligned", what, what);
+    p.tiles = static_cast<int>(c.tiles);
+    p.slots = static_cast<int>(c.slots);
+    p.parts = static_cast<int>(c.parts);
+    p.least = kLeast;
+    p.part = static_cast<float *>(workspace);
+    p.stats = reinterpret_cast<float2 *>(p.part + c.tiles * p.kv_heads * c.parts * kRows * head_dim);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (head_dim == 64) launch<64>(p, c.blocks, s);
+    else if (head_dim == 128) launch<128>(p, c.blocks, s);
+    else launch<256>(p, c.blocks, s);
+    return check_launch(what);
 }
 
 // The checks that both entry points share.
@@ -174,7 +638,7 @@ int check_rows(const char *what, const char *name, const void *x, int64_t stride
     if (!aligned16(x) || stride % 8)
         return fail(LTXK_E_ALIGN, "%s: %s must be 16-byte aligned, with strides that are multiples of 8", what, name);
     if (stride < width || stride > kStride)
-        return fail(LTXK_E_ARG, "%s: %s's token stride must be between its width (%lld) and 2^23", what, name,
+        return fail(LTXK_E_ARG, "%s: %s's token stride must be between its width (%lld) and 2^23 - 8", what, name,
                     (long long)width);
     return LTXK_OK;
 }
@@ -187,7 +651,8 @@ using namespace ltxk;
 extern "C" int64_t ltxk_packed_attention_workspace_bytes(int64_t tokens_q, int64_t tokens_k, int64_t sequences,
                                                          int64_t heads, int64_t kv_heads, int64_t head_dim)
 {
-    return 0;
+    if (tokens_q <= 0 || tokens_k < 0 || sequences <= 0 || kv_heads <= 0 || heads < kv_heads || head_dim <= 0) return 0;
+    return parts_bytes(plan_packed(tokens_q, tokens_k, sequences, heads, kv_heads, head_dim), kv_heads, head_dim);
 }
 
 extern "C" int ltxk_packed_attention(void *out, const void *q, int64_t q_tstride, const void *k, int64_t k_tstride,
@@ -234,14 +699,16 @@ extern "C" int ltxk_packed_attention(void *out, const void *q, int64_t q_tstride
     p.group = static_cast<int>(group);
     p.causal = causal != 0;
     p.window = static_cast<int>(window < kMost ? window : 0);  // a window of everything is none
-    launch<true>(p, static_cast<int>(head_dim), tokens_q * heads, static_cast<hipStream_t>(stream));
-    return check_launch(what);
+    return run(what, p, plan_packed(tokens_q, tokens_k, sequences, heads, kv_heads, head_dim), head_dim, workspace,
+               workspace_bytes, stream);
 }
 
 extern "C" int64_t ltxk_prefix_attention_workspace_bytes(int64_t batch, int64_t tokens_q, int64_t tokens_k, int64_t prefix,
                                                          int64_t heads, int64_t kv_heads, int64_t head_dim)
 {
-    return 0;
+    if (batch <= 0 || tokens_q <= 0 || tokens_k < 0 || prefix < 0 || kv_heads <= 0 || heads < kv_heads || head_dim <= 0)
+        return 0;
+    return parts_bytes(plan_prefix(batch, tokens_q, tokens_k, prefix, heads, kv_heads, head_dim), kv_heads, head_dim);
 }
 
 extern "C" int ltxk_prefix_attention(void *out, const void *q, int64_t q_bstride, int64_t q_tstride, const void *k,
@@ -300,6 +767,6 @@ extern "C" int ltxk_prefix_attention(void *out, const void *q, int64_t q_bstride
     p.kv_heads = static_cast<int>(kv_heads);
     p.group = static_cast<int>(group);
     p.causal = causal != 0;
-    launch<false>(p, static_cast<int>(head_dim), batch * tokens_q * heads, static_cast<hipStream_t>(stream));
-    return check_launch(what);
+    return run(what, p, plan_prefix(batch, tokens_q, tokens_k, prefix, heads, kv_heads, head_dim), head_dim, workspace,
+               workspace_bytes, stream);
 }
