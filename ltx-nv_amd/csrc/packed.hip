@@ -13,7 +13,24 @@
 namespace ltxk {
 namespace {
 
-constexpr int kRows = 32 * kWaves;  // rows (a query at one head of the group) of a tile, 32 a wave
+// Rows (a query at one head of the group) of a tile: 32 a wave, which share its keys, or 32
+// that all waves attend with, each over keys of its own.
+constexpr int kRows = 32 * kWaves, kFewRows = 32;
+// Keys that a wave of the latter takes at a time.
+template <int D>
+constexpr int kFewKeys = D == 64 ? 64 : 32;
+
+// The keys of a launch: a sequence's (behind the prefix, if there is one), an item's own
+// alone, or the prefix alone, for the queries of all items.
+enum Keys { kBoth, kOwn, kCommon };
+
+// Parts of cut tiles.
+struct Parts {
+    float *sums;          // each part's weighted sums of v (rows x D)
+    float2 *stats;        // and each of its rows' maximum and sum of weights
+    int tiles, slots;     // row tiles of a key head, and places for them and their parts on an XCD
+    int parts, least;     // the keys of a tile are cut into up to `parts`, of at least `least` tiles each
+};
 
 struct Params {
     const uint16_t *q, *k, *v, *pk, *pv;
@@ -26,10 +43,9 @@ struct Params {
     int seqs, prefix, heads, kv_heads, group, window;  // window 0: none
     bool causal;
     float scale2;         // scale * log2(e)
-    int tiles, slots;     // row tiles of a key head, and places for them and their parts on an XCD
-    int parts, least;     // the keys of a tile are cut into up to `parts`, of at least `least` tiles each
-    float *part;          // cut tiles: each part's weighted sums of v (kRows x D)
-    float2 *stats;        // and each of its rows' maximum and sum of weights
+    Keys keys;
+    bool joined;          // every tile is written as parts
+    Parts cut;
 };
 
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
@@ -45,6 +61,7 @@ struct Tile {
     int first, rows;      // the tile's first row, and the rows of the whole sequence
     int from, to;         // own keys that some of its rows see
     int np, tiles;        // key tiles: of the prefix, and in all
+    bool stacked;         // the queries are those of all items
 };
 
 // Where sequence s's row tiles begin, if each sequence takes one more than its rows fill:
@@ -73,12 +90,20 @@ __device__ __forceinline__ int sequence_of(const Params &p, int t)
 }
 
 // Row tile t of key head kvh, or false if there is none.
-template <int D, int ROWS>
+template <int D, int ROWS, int KEYS>
 __device__ __forceinline__ bool find_tile(const Params &p, int t, int kvh, Tile &r)
 {
     const int64_t qh = static_cast<int64_t>(kvh) * p.group * D * 2, kh = static_cast<int64_t>(kvh) * D * 2;
     int tile;
-    if (p.qo) {
+    r.stacked = p.keys == kCommon;
+    if (r.stacked) {
+        tile = t;
+        r.queries = p.seqs * p.tq;
+        r.n = 0;
+        r.token = 0;
+        r.q = reinterpret_cast<const char *>(p.q) + qh;
+        r.k = r.v = nullptr;
+    } else if (p.qo) {
         const int s = sequence_of<ROWS>(p, t);
         // lengths are cut to what the tensors hold, whatever the offsets say
         const int q0 = min(max(uniform(p.qo[s]), 0), p.tq), q1 = min(uniform(p.qo[s + 1]), p.tq);
@@ -105,18 +130,15 @@ __device__ __forceinline__ bool find_tile(const Params &p, int t, int kvh, Tile 
     if (tile < 0 || r.first >= r.rows) return false;
     const int behind = r.n - r.queries;  // keys in front of the first query's
     const int last = min(r.first + ROWS, r.rows) - 1;
-    r.to = p.causal ? max(behind + last / p.group + 1, 0) : r.n;
+    r.to = p.causal && !r.stacked ? max(behind + last / p.group + 1, 0) : r.n;
     r.from = p.window ? min(max(behind + r.first / p.group + 1 - p.window, 0), r.to) : 0;
-    r.np = r.to || !p.causal ? (p.prefix + kKeys - 1) / kKeys : 0;
-    r.tiles = r.np + (r.to - r.from + kKeys - 1) / kKeys;
+    r.np = r.stacked || (p.keys == kBoth && (r.to || !p.causal)) ? (p.prefix + KEYS - 1) / KEYS : 0;
+    r.tiles = r.np + (r.to - r.from + KEYS - 1) / KEYS;
     return true;
 }
 
 // Into how many parts a tile's keys are cut: short ones into few.
-__device__ __forceinline__ int parts_of(const Params &p, const Tile &r)
-{
-    return max(min(p.parts, r.tiles / p.least), 1);
-}
+__device__ __forceinline__ int parts_of(const Parts &c, int tiles) { return max(min(c.parts, tiles / c.least), 1); }
 
 // Row `row` of a tile: its query, head of the group, and the own keys [lo, hi) it sees (and
 // the prefix, if any).
@@ -136,30 +158,44 @@ __device__ __forceinline__ Row find_row(const Params &p, const Tile &r, int row)
     return w;
 }
 
-// The 64 keys (values) of key tile g, from memory's `base` on, `valid` of them.
+// A row's query.
+__device__ __forceinline__ const char *query(const Params &p, const Tile &r, const Row &w, int dim)
+{
+    const char *q = r.q + w.member * dim * 2;
+    if (!r.stacked) return q + static_cast<int64_t>(w.query) * p.qts;
+    const int item = w.query / p.tq;
+    return q + item * p.qbs + static_cast<int64_t>(w.query - item * p.tq) * p.qts;
+}
+
+// The keys (values) of key tile g, from `base` on, `valid` of them.
 struct Span {
-    rsrc_t rsrc;
+    const char *base;
     uint32_t stride;
     int valid;
 };
-template <int D, bool V>
+template <int D, int KEYS, bool V>
 __device__ __forceinline__ Span key_span(const Params &p, const Tile &r, int kvh, int g)
 {
-    const char *base;
     Span s;
     if (g < r.np) {
-        s.valid = min(kKeys, p.prefix - g * kKeys);
+        s.valid = min(KEYS, p.prefix - g * KEYS);
         s.stride = V ? p.pvts : p.pkts;
-        base = reinterpret_cast<const char *>(V ? p.pv : p.pk) + static_cast<int64_t>(kvh) * D * 2 +
-               static_cast<int64_t>(g) * kKeys * s.stride;
+        s.base = reinterpret_cast<const char *>(V ? p.pv : p.pk) + static_cast<int64_t>(kvh) * D * 2 +
+                 static_cast<int64_t>(g) * KEYS * s.stride;
     } else {
-        const int at = r.from + (g - r.np) * kKeys;
-        s.valid = min(kKeys, r.to - at);
+        const int at = r.from + (g - r.np) * KEYS;
+        s.valid = min(KEYS, r.to - at);
         s.stride = V ? p.vts : p.kts;
-        base = (V ? r.v : r.k) + static_cast<int64_t>(at) * s.stride;
+        s.base = (V ? r.v : r.k) + static_cast<int64_t>(at) * s.stride;
     }
-    s.rsrc = make_rsrc(base, static_cast<uint32_t>(s.valid - 1) * s.stride + 2 * D);
     return s;
+}
+
+// Bytes that a span's loads may reach.
+template <int D>
+__device__ __forceinline__ uint32_t reach(const Span &s)
+{
+    return static_cast<uint32_t>(s.valid - 1) * s.stride + 2 * D;
 }
 
 // Adds keys [from, to) to a row's running maximum, sum and weighted values: a lane has the
@@ -202,22 +238,22 @@ __device__ __forceinline__ void attend_keys(const char *q, const char *k, uint32
 
 // One row over key tiles t0 .. t1 - 1 by a whole wave, only what it sees: for rows whose
 // matrix products met a masked value that is not finite (its weight of zero makes NaN).
-template <int D>
+template <int D, int KEYS>
 __device__ __forceinline__ void attend_row(const Params &p, const Tile &r, int kvh, int row, int t0, int t1, float &mx,
                                            float &sum, float (&acc)[D / 64])
 {
     const Row w = find_row(p, r, row);
-    const char *q = r.q + static_cast<int64_t>(w.query) * p.qts + w.member * D * 2;
+    const char *q = query(p, r, w, D);
     const int64_t kh = static_cast<int64_t>(kvh) * D;
     mx = -FLT_MAX;
     sum = 0.f;
 #pragma unroll
     for (int c = 0; c < D / 64; ++c) acc[c] = 0.f;
-    if (!w.any) return;
+    if (!w.any && !r.stacked) return;
     attend_keys<D>(q, reinterpret_cast<const char *>(p.pk + kh), p.pkts, reinterpret_cast<const char *>(p.pv + kh), p.pvts,
-                   min(t0, r.np) * kKeys, min(min(t1, r.np) * kKeys, p.prefix), p.scale2, mx, sum, acc);
-    attend_keys<D>(q, r.k, p.kts, r.v, p.vts, max(w.lo, r.from + (max(t0, r.np) - r.np) * kKeys),
-                   min(w.hi, r.from + (max(t1, r.np) - r.np) * kKeys), p.scale2, mx, sum, acc);
+                   min(t0, r.np) * KEYS, min(min(t1, r.np) * KEYS, p.prefix), p.scale2, mx, sum, acc);
+    attend_keys<D>(q, r.k, p.kts, r.v, p.vts, max(w.lo, r.from + (max(t0, r.np) - r.np) * KEYS),
+                   min(w.hi, r.from + (max(t1, r.np) - r.np) * KEYS), p.scale2, mx, sum, acc);
 }
 
 // Tile and part of this workgroup.  Workgroups are dealt to the 8 XCDs in turn: of the key
@@ -228,11 +264,53 @@ __device__ __forceinline__ bool find_work(const Params &p, int &t, int &kvh, int
 {
     const int xcd = blockIdx.x & 7, j = blockIdx.x >> 3;
     const int beside = p.kv_heads & -p.kv_heads & 7 ? p.kv_heads & -p.kv_heads : 8, each = 8 / beside;
-    kvh = j / p.slots * beside + xcd % beside;
-    const int slot = p.parts > 1 ? xcd / beside * p.slots + j % p.slots : j % p.slots * each + xcd / beside;
-    t = p.tiles - 1 - slot % p.tiles;
-    part = slot / p.tiles;
-    return part < p.parts;
+    const Parts &c = p.cut;
+    kvh = j / c.slots * beside + xcd % beside;
+    const int slot = c.parts > 1 ? xcd / beside * c.slots + j % c.slots : j % c.slots * each + xcd / beside;
+    t = c.tiles - 1 - slot % c.tiles;
+    part = slot / c.tiles;
+    return part < c.parts;
+}
+
+// The parts' place of a tile's first row.
+__device__ __forceinline__ int64_t part_rows(const Params &p, const Parts &c, int64_t t, int kvh, int part, int rows)
+{
+    return ((t * p.kv_heads + kvh) * c.parts + part) * rows;
+}
+
+// A tile without any key: its rows weigh nothing, or are zero.
+template <int D, int ROWS>
+__device__ __forceinline__ void no_keys(const Params &p, const Tile &r, int kvh, int64_t u, bool joined)
+{
+    for (int i = threadIdx.x; i < ROWS * (D / 8); i += kWaves * 64) {
+        const int at = i / (D / 8), c = i % (D / 8);
+        if (r.first + at >= r.rows) break;
+        const Row w = find_row(p, r, r.first + at);
+        if (!joined)
+            *reinterpret_cast<u32x4 *>(p.out + ((r.token + w.query) * p.heads + kvh * p.group + w.member) * D + c * 8) = u32x4{};
+        else if (c == 0)
+            p.cut.stats[u + at] = make_float2(-FLT_MAX, 0.f);
+    }
+}
+
+// One row over again by a wave: its sums, or its output.
+template <int D, int KEYS>
+__device__ __forceinline__ void again_row(const Params &p, const Tile &r, int kvh, int row, int t0, int t1, int64_t u, bool joined)
+{
+    const int lane = threadIdx.x & 63;
+    float mx, sum, acc[D / 64];
+    attend_row<D, KEYS>(p, r, kvh, row, t0, t1, mx, sum, acc);
+    const Row w = find_row(p, r, row);
+    if (joined && lane == 0) p.cut.stats[u] = make_float2(mx, sum);
+    uint16_t *out = p.out + ((r.token + w.query) * p.heads + kvh * p.group + w.member) * D;
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) {
+        const int col = lane * (D / 64) + c;
+        if (joined)
+            p.cut.sums[u * D + col] = acc[c];
+        else
+            out[col] = f32_to_bf16(w.any ? acc[c] / sum : 0.f);
+    }
 }
 
 template <int D>
@@ -250,9 +328,11 @@ __global__ void __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) tile_kernel(Par
 
     int t, kvh, part;
     Tile r;
-    if (!find_work(p, t, kvh, part) || !find_tile<D, kRows>(p, t, kvh, r)) return;
-    const int parts = parts_of(p, r);
+    if (!find_work(p, t, kvh, part) || !find_tile<D, kRows, kKeys>(p, t, kvh, r)) return;
+    const int parts = parts_of(p.cut, r.tiles);
     if (part >= parts) return;
+    const bool joined = parts > 1 || p.joined;
+    const int64_t unit = part_rows(p, p.cut, t, kvh, part, kRows);
     const int t0 = static_cast<int>(static_cast<int64_t>(part) * r.tiles / parts);
     const int n = static_cast<int>(static_cast<int64_t>(part + 1) * r.tiles / parts) - t0;
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -264,34 +344,26 @@ __global__ void __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) tile_kernel(Par
     const int sure_hi = uniform(own.hi), sure_lo = __builtin_amdgcn_readlane(own.lo, 31);
     uint16_t *const out = p.out;
 
-    if (n == 0) {  // no key for any row
-        for (int i = threadIdx.x; i < kRows * (D / 8); i += kWaves * 64) {
-            const int row = r.first + i / (D / 8);
-            if (row > last) break;
-            const Row w = find_row(p, r, row);
-            *reinterpret_cast<u32x4 *>(out + ((r.token + w.query) * p.heads + kvh * p.group + w.member) * D +
-                                       i % (D / 8) * 8) = u32x4{};
-        }
-        return;
-    }
+    if (n == 0) return no_keys<D, kRows>(p, r, kvh, unit, joined);
 
     // Queries: lane l holds row l % 32, elements 16 s + 8 (l/32) .. + 7.
     bf16x8 qf[KS];
     {
-        const char *qp = r.q + static_cast<int64_t>(own.query) * p.qts + own.member * D * 2 + half * 16;
+        const char *qp = query(p, r, own, D) + half * 16;
 #pragma unroll
         for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const bf16x8 *>(qp + s * 32);
     }
-    auto load = [&](auto is_v, const Span &s, int c, char *dst) __attribute__((always_inline)) {
+    auto load = [&](auto is_v, rsrc_t rsrc, const Span &s, int c, char *dst) __attribute__((always_inline)) {
         constexpr bool V = decltype(is_v)::value;
         const int at = wave * kLoads<D> + c, row = part_row<D>(c, wave, lane), pos = lane % (D / 8);
         const uint32_t off = __umul24(min(row, s.valid - 1), s.stride) + (V ? v_pos<D>(row, pos) : k_pos<D>(row, pos)) * 16;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(s.rsrc, (lds_char *)(dst + at * 1024), 16, off, 0, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_char *)(dst + at * 1024), 16, off, 0, 0, 0);
     };
     {
-        const Span s = key_span<D, false>(p, r, kvh, t0);
+        const Span s = key_span<D, kKeys, false>(p, r, kvh, t0);
+        const rsrc_t rs = make_rsrc(s.base, reach<D>(s));
 #pragma unroll
-        for (int c = 0; c < kLoads<D>; ++c) load(std::false_type{}, s, c, k0);
+        for (int c = 0; c < kLoads<D>; ++c) load(std::false_type{}, rs, s, c, k0);
     }
 
     // LDS byte offsets of this lane's fragments.  K: row l % 32 (+ 32 u), chunk
@@ -418,14 +490,16 @@ __global__ void __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) tile_kernel(Par
     auto tile = [&](int i, auto from, const char *kc, const char *vp, char *kn, char *vn)
                     __attribute__((always_inline)) {
         constexpr int kEvery = from == 0 ? 3 : 2;
-        const Span ks = key_span<D, false>(p, r, kvh, t0 + min(i + 1, n - 1)), vs = key_span<D, true>(p, r, kvh, t0 + i);
+        const Span ks = key_span<D, kKeys, false>(p, r, kvh, t0 + min(i + 1, n - 1));
+        const Span vs = key_span<D, kKeys, true>(p, r, kvh, t0 + i);
+        const rsrc_t kr = make_rsrc(ks.base, reach<D>(ks)), vr = make_rsrc(vs.base, reach<D>(vs));
         products(from, integral_constant<int, NV + NK>{}, vp, kc, [&](int j) __attribute__((always_inline)) {
             if (j % kEvery) return;
             const int c = j / kEvery;
             if (c < kLoads<D>)
-                load(std::true_type{}, vs, c, vn);
+                load(std::true_type{}, vr, vs, c, vn);
             else if (c < 2 * kLoads<D>)
-                load(std::false_type{}, ks, c - kLoads<D>, kn);
+                load(std::false_type{}, kr, ks, c - kLoads<D>, kn);
         });
         softmax(i);
         __builtin_amdgcn_sched_barrier(0);
@@ -449,16 +523,15 @@ __global__ void __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) tile_kernel(Par
         for (int e = 0; e < 16; ++e) fine = fine && fabsf(o[m][e]) <= FLT_MAX;
     const uint64_t odd = __ballot(!fine);
     uint32_t again = static_cast<uint32_t>(odd) | static_cast<uint32_t>(odd >> 32);  // rows to be done once more
-    const int64_t unit = (static_cast<int64_t>(t) * p.kv_heads + kvh) * p.parts + part;
-    if (parts > 1) {
-        const int64_t u = unit * kRows + wave * 32 + l32;
+    if (joined) {
+        const int64_t u = unit + wave * 32 + l32;
         if (first + l32 <= last) {
-            if (half == 0) p.stats[u] = make_float2(mx, total);
+            if (half == 0) p.cut.stats[u] = make_float2(mx, total);
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
-                    *reinterpret_cast<f32x4 *>(p.part + u * D + 32 * m + 8 * c + 4 * half) =
+                    *reinterpret_cast<f32x4 *>(p.cut.sums + u * D + 32 * m + 8 * c + 4 * half) =
                         f32x4{o[m][4 * c], o[m][4 * c + 1], o[m][4 * c + 2], o[m][4 * c + 3]};
         }
     } else {
@@ -488,50 +561,252 @@ __global__ void __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) tile_kernel(Par
     if (again) {
         __builtin_amdgcn_s_waitcnt(0x0070);
         asm volatile("" ::: "memory");
-        do {
-            const int i = __builtin_ctz(again), row = first + i;
-            again &= again - 1;
-            if (row > last) continue;
-            float m1, sum1, acc[D / 64];
-            attend_row<D>(p, r, kvh, row, t0, t0 + n, m1, sum1, acc);
-            const int64_t to = __builtin_amdgcn_readlane(static_cast<int>(at), i) & 0xffffffffll |
-                               static_cast<int64_t>(__builtin_amdgcn_readlane(static_cast<int>(at >> 32), i)) << 32;
-            const bool any = find_row(p, r, row).any;
-            const int64_t u = unit * kRows + wave * 32 + i;
-            if (parts > 1 && lane == 0) p.stats[u] = make_float2(m1, sum1);
-#pragma unroll
-            for (int c = 0; c < D / 64; ++c) {
-                const int col = lane * (D / 64) + c;
-                if (parts > 1)
-                    p.part[u * D + col] = acc[c];
-                else
-                    out[to * D + col] = f32_to_bf16(any ? acc[c] / sum1 : 0.f);
-            }
-        } while (again);
+        for (; again; again &= again - 1) {
+            const int i = __builtin_ctz(again);
+            if (first + i <= last)
+                again_row<D, kKeys>(p, r, kvh, first + i, t0, t0 + n, unit + wave * 32 + i, joined);
+        }
     }
 }
 
-// Joins the parts of the cut tiles: 8 columns of one row a thread.
-template <int D>
-__global__ void __launch_bounds__(256) join_kernel(Params p)
+// At most N loads of this wave in flight; nothing moves over it.
+template <int N>
+__device__ __forceinline__ void wait_loads()
 {
-    constexpr int kThreads = kRows * (D / 8);  // of a tile
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | (N >> 4 << 14));
+    asm volatile("" ::: "memory");
+}
+// This wave's LDS reads have returned; nothing moves over it.
+__device__ __forceinline__ void wait_lds()
+{
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+    asm volatile("" ::: "memory");
+}
+
+// Few rows: each wave takes every fourth tile of kFewKeys keys, through LDS of its own and
+// without barriers, the next keys on their way while the weights are made and the next
+// values while the next scores are; the waves' sums are added up in the end.
+template <int D>
+__global__ void __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) few_kernel(Params p)
+{
+    constexpr int KT = kFewKeys<D>, KU = KT / 32;
+    constexpr int KS = D / 16, MT = D / 32;
+    constexpr int kBytes = KT * D * 2, NL = kBytes / 1024;  // of a tile, and its load instructions
+    __shared__ __attribute__((aligned(1024))) char lds[kWaves][2][kBytes];
+    __shared__ float2 stat[kWaves][kFewRows];
+    __shared__ uint32_t odd;
+
+    int t, kvh, part;
+    Tile r;
+    if (!find_work(p, t, kvh, part) || !find_tile<D, kFewRows, KT>(p, t, kvh, r)) return;
+    const int parts = parts_of(p.cut, r.tiles);
+    if (part >= parts) return;
+    const bool joined = parts > 1 || p.joined;
+    const int64_t unit = part_rows(p, p.cut, t, kvh, part, kFewRows);
+    const int t0 = static_cast<int>(static_cast<int64_t>(part) * r.tiles / parts);
+    const int t1 = static_cast<int>(static_cast<int64_t>(part + 1) * r.tiles / parts);
+    if (t0 == t1) return no_keys<D, kFewRows>(p, r, kvh, unit, joined);
+    const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int l32 = lane & 31, half = lane >> 5;
+    const int rows = min(kFewRows, r.rows - r.first);
+    const Row own = find_row(p, r, r.first + min(l32, rows - 1));
+    const int sure_hi = uniform(own.hi), sure_lo = __builtin_amdgcn_readlane(own.lo, 31);
+    if (threadIdx.x == 0) odd = 0;
+
+    char *const kt = lds[wave][0], *const vt = lds[wave][1];
+    auto load = [&](auto is_v, int g) __attribute__((always_inline)) {
+        constexpr bool V = decltype(is_v)::value;
+        const Span s = key_span<D, KT, V>(p, r, kvh, g);
+        const uint64_t a = reinterpret_cast<uint64_t>(s.base);
+        const u32x4 rsrc = {static_cast<uint32_t>(uniform(static_cast<int>(a))),
+                            static_cast<uint32_t>(uniform(static_cast<int>(a >> 32) & 0xffff)),
+                            static_cast<uint32_t>(uniform(static_cast<int>(reach<D>(s)))), 0x00020000u};
+        const uint32_t to = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char *)(V ? vt : kt)));
+#pragma unroll
+        for (int c = 0; c < NL; ++c) {
+            const int row = c * (1024 / (2 * D)) + lane / (D / 8), pos = lane % (D / 8);
+            const uint32_t off = __umul24(min(row, s.valid - 1), s.stride) + (V ? v_pos<D>(row, pos) : k_pos<D>(row, pos)) * 16;
+            load_lds16(rsrc, to + c * 1024, off, 0);
+        }
+    };
+    int g = t0 + wave;
+    if (g < t1) {
+        load(std::false_type{}, g);
+        load(std::true_type{}, g);
+    }
+    bf16x8 qf[KS];
+    {
+        const char *qp = query(p, r, own, D) + half * 16;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const bf16x8 *>(qp + s * 32);
+    }
+    const int vi = lane & 15;
+    f32x16 o[MT] = {};
+    float mx = -FLT_MAX, sum = 0.f;
+    for (; g < t1; g += kWaves) {
+        const bool more = g + kWaves < t1;
+        wait_loads<NL>();  // the keys are there; the values may be on their way
+        f32x16 s[KU] = {};
+#pragma unroll
+        for (int i = 0; i < KS; ++i)
+#pragma unroll
+            for (int u = 0; u < KU; ++u) {
+                const bf16x8 f = *reinterpret_cast<const bf16x8 *>(kt + (l32 + 32 * u) * 2 * D + k_pos<D>(l32, 2 * i + half) * 16);
+                s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f, qf[i], s[u], 0, 0, 0);
+            }
+        wait_lds();
+        if (more) load(std::false_type{}, g + kWaves);
+
+        const int key = r.from + (g - r.np) * KT;
+        const bool common = g < r.np;
+        if (common ? p.prefix - g * KT < KT : key + KT > sure_hi || key < sure_lo) {
+            const int hi = (common ? p.prefix - g * KT : own.hi - key) - 4 * half;
+            const int lo = (common ? 0 : own.lo - key) - 4 * half;
+#pragma unroll
+            for (int u = 0; u < KU; ++u)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int j = 32 * u + 8 * (e >> 2) + (e & 3);
+                    if (j >= hi || j < lo) s[u][e] = -INFINITY;
+                }
+        }
+        float m = s[0][0];
+#pragma unroll
+        for (int u = 0; u < KU; ++u)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) m = fmaxf(m, s[u][e]);
+        m = pair_max(m) * p.scale2;
+        if (__any(m > mx)) {
+            const float nm = fmaxf(m, mx), a = __builtin_amdgcn_exp2f(mx - nm);
+            mx = nm;
+            sum *= a;
+#pragma unroll
+            for (int c = 0; c < MT; ++c)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[c][e] *= a;
+        }
+        u32x4 w[KU * 2];
+#pragma unroll
+        for (int j = 0; j < KU * 8; ++j) {
+            // rounded before the maximum is taken off, as it was: the largest weight is 1
+            const float x = __builtin_amdgcn_exp2f(s[j >> 3][2 * (j & 7)] * p.scale2 - mx);
+            const float y = __builtin_amdgcn_exp2f(s[j >> 3][2 * (j & 7) + 1] * p.scale2 - mx);
+            sum += x + y;
+            w[j >> 2][j & 3] = pack_bf16x2(x, y);
+        }
+
+        if (more) wait_loads<NL>();  // the values are there
+        else wait_loads<0>();
+        typedef __attribute__((address_space(3))) bf16x4 lds4;
+#pragma unroll
+        for (int st = 0; st < KT / 16; ++st)
+#pragma unroll
+            for (int c = 0; c < MT; ++c) {
+                bf16x4 f[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int row = 8 * e + 4 * half + (vi >> 2);
+                    const int pos = 4 * c + 2 * ((lane >> 4) & 1) + ((vi & 3) >> 1);
+                    f[e] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
+                        (lds4 *)(vt + (row + 16 * st) * 2 * D + v_pos<D>(row, pos) * 16 + (vi & 1) * 8));
+                }
+                o[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(cat(f[0], f[1]), __builtin_bit_cast(bf16x8, w[st]), o[c], 0, 0, 0);
+            }
+        wait_lds();
+        if (more) load(std::true_type{}, g + kWaves);
+    }
+
+    // The waves' sums on one maximum, side by side in LDS: row l % 32, columns
+    // 32 m + 8 j + 4 half + (0..3) in registers 4 j .., 16-byte chunks permuted by the row.
+    const float total = pair_sum(sum);
+    if (half == 0) stat[wave][l32] = make_float2(mx, total);
+    __syncthreads();
+    float top = stat[0][l32].x;
+#pragma unroll
+    for (int i = 1; i < kWaves; ++i) top = fmaxf(top, stat[i][l32].x);
+    const float fade = __builtin_amdgcn_exp2f(mx - top);
+    float *const mine = reinterpret_cast<float *>(lds[wave]);
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            *reinterpret_cast<f32x4 *>(mine + l32 * D + ((8 * m + 2 * c + half) ^ (l32 & (D / 4 - 1))) * 4) =
+                f32x4{o[m][4 * c] * fade, o[m][4 * c + 1] * fade, o[m][4 * c + 2] * fade, o[m][4 * c + 3] * fade};
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows * (D / 8); i += kWaves * 64) {
+        const int at = i / (D / 8), c = i % (D / 8);
+        float2 st[kWaves];
+        float high = -FLT_MAX, all = 0.f, f[8] = {};
+#pragma unroll
+        for (int k = 0; k < kWaves; ++k) st[k] = stat[k][at], high = fmaxf(high, st[k].x);
+#pragma unroll
+        for (int k = 0; k < kWaves; ++k) {
+            all += st[k].y * __builtin_amdgcn_exp2f(st[k].x - high);
+            const float *x = reinterpret_cast<const float *>(lds[k]) + at * D;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const f32x4 y = *reinterpret_cast<const f32x4 *>(x + ((2 * c + h) ^ (at & (D / 4 - 1))) * 4);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) f[4 * h + e] += y[e];
+            }
+        }
+        bool fine = true;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) fine = fine && fabsf(f[e]) <= FLT_MAX;
+        if (!fine) atomicOr(&odd, 1u << at);
+        if (joined) {
+            if (c == 0) p.cut.stats[unit + at] = make_float2(high, all);
+            f32x4 *x = reinterpret_cast<f32x4 *>(p.cut.sums + (unit + at) * D + c * 8);
+            x[0] = f32x4{f[0], f[1], f[2], f[3]};
+            x[1] = f32x4{f[4], f[5], f[6], f[7]};
+        } else {
+            const Row w = find_row(p, r, r.first + at);
+            const float inv = 1.f / all;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = w.any ? f[e] * inv : 0.f;
+            *reinterpret_cast<u32x4 *>(p.out + ((r.token + w.query) * p.heads + kvh * p.group + w.member) * D + c * 8) = pack8v(f);
+        }
+    }
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070);
+    __syncthreads();
+    for (uint32_t again = uniform(odd); again; again &= again - 1) {
+        const int i = __builtin_ctz(again);
+        if (i % kWaves == wave) again_row<D, KT>(p, r, kvh, r.first + i, t0, t1, unit + i, joined);
+    }
+}
+
+// Joins the parts of the cut tiles, and of a prefix's (`common`, tiles of COMMON rows) with
+// those of the items' own keys: 8 columns of one row a thread.
+template <int D, int ROWS, int KEYS, int COMMON>
+__global__ void __launch_bounds__(256) join_kernel(Params p, Parts common)
+{
+    constexpr int kThreads = ROWS * (D / 8);  // of a tile
     const int64_t tile = static_cast<int64_t>(blockIdx.x) / (kThreads / 256);
     const int i = blockIdx.x % (kThreads / 256) * 256 + threadIdx.x, c = i % (D / 8), at = i / (D / 8);
     const int t = static_cast<int>(tile / p.kv_heads), kvh = static_cast<int>(tile % p.kv_heads);
     Tile r;
-    if (!find_tile<D, kRows>(p, t, kvh, r)) return;
-    const int parts = parts_of(p, r);
-    if (parts == 1 || r.first + at >= r.rows) return;  // the tile's only part has written the output
+    if (!find_tile<D, ROWS, KEYS>(p, t, kvh, r)) return;
+    const int parts = parts_of(p.cut, r.tiles);
+    if ((parts == 1 && !p.joined) || r.first + at >= r.rows) return;  // the tile's only part has written the output
     const Row w = find_row(p, r, r.first + at);
-    const int64_t u = tile * p.parts * kRows + at;
-    float m = -INFINITY;
-    for (int k = 0; k < parts; ++k) m = fmaxf(m, p.stats[u + k * kRows].x);
+    const int64_t u = part_rows(p, p.cut, t, kvh, 0, ROWS) + at;
+    int64_t cu = 0;
+    if (COMMON) {
+        const int64_t row = (r.token + w.query) * p.group + w.member;
+        cu = part_rows(p, common, row / COMMON, kvh, 0, COMMON) + row % COMMON;
+    }
+    float m = -FLT_MAX;
+    for (int k = 0; k < parts; ++k) m = fmaxf(m, p.cut.stats[u + k * ROWS].x);
+    if (COMMON)
+        for (int k = 0; k < common.parts; ++k) m = fmaxf(m, common.stats[cu + k * COMMON].x);
     float acc[8] = {}, sum = 0.f;
-    for (int k = 0; k < parts; ++k) {
-        const float2 st = p.stats[u + k * kRows];
+    auto add = [&](float2 st, const float *sums) {
+        if (st.y == 0.f) return;  // a part that saw no key wrote no sums
         const float f = __builtin_amdgcn_exp2f(st.x - m);
-        const f32x4 *x = reinterpret_cast<const f32x4 *>(p.part + (u + k * kRows) * D + c * 8);
+        const f32x4 *x = reinterpret_cast<const f32x4 *>(sums + c * 8);
         const f32x4 lo = x[0], hi = x[1];
         sum += f * st.y;
 #pragma unroll
@@ -539,81 +814,149 @@ __global__ void __launch_bounds__(256) join_kernel(Params p)
             acc[e] = __builtin_fmaf(f, lo[e], acc[e]);
             acc[4 + e] = __builtin_fmaf(f, hi[e], acc[4 + e]);
         }
-    }
+    };
+    for (int k = 0; k < parts; ++k) add(p.cut.stats[u + k * ROWS], p.cut.sums + (u + k * ROWS) * D);
+    if (COMMON)
+        for (int k = 0; k < common.parts; ++k) add(common.stats[cu + k * COMMON], common.sums + (cu + k * COMMON) * D);
+    const bool any = w.any || (COMMON && !p.causal);
     const float inv = 1.f / sum;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] = w.any ? acc[e] * inv : 0.f;
+    for (int e = 0; e < 8; ++e) acc[e] = any ? acc[e] * inv : 0.f;
     *reinterpret_cast<u32x4 *>(p.out + ((r.token + w.query) * p.heads + kvh * p.group + w.member) * D + c * 8) = pack8v(acc);
 }
 
 constexpr int64_t kMost = 0x7fffffff - 1024;  // rows that are counted in int
+constexpr int64_t kShared = 8 << 20;          // bytes of prefix that are worth two launches more
 constexpr int64_t kStride = (1 << 23) - 8;    // elements of a token stride: its bytes are 24 bits
 
-// How a call is cut: row tiles of a key head, and into how many parts at most each one's
-// keys, so that few tiles still fill the chip (two workgroups a compute unit, one with heads
-// of 256), with at least kLeast key tiles a part.
-constexpr int kLeast = 4;
-
-struct Plan {
-    int64_t tiles, parts, slots, blocks;
+// How the tiles of a launch are cut: the keys of each into up to `parts`, so that few tiles
+// still fill the chip (two workgroups a compute unit, one with heads of 256) `rounds` times
+// over, with at least `least` key tiles a part.
+struct Cut {
+    bool few;             // tiles of kFewRows rows
+    int64_t rows, tiles, parts, least, slots, blocks;
 };
 
-Plan plan(int64_t tiles, int64_t key_tiles, int64_t kv_heads, int64_t head_dim)
+Cut cut(bool few, int64_t tiles, int64_t keys, int64_t rounds, int64_t kv_heads, int64_t head_dim)
 {
-    Plan c;
+    Cut c;
+    c.few = few;
+    c.rows = few ? kFewRows : kRows;
     c.tiles = tiles;
-    const int64_t room = head_dim == 256 ? 256 : 512;
     c.parts = 1;
-    while (c.parts < 64 && tiles * kv_heads * c.parts * 2 <= room && key_tiles >= c.parts * 2 * kLeast) c.parts *= 2;
+    c.least = few ? 8 : 4;
+    const int64_t key_tiles = keys / (few && head_dim != 64 ? 32 : 64);
+    const int64_t room = (head_dim == 256 ? 256 : 512) * rounds;
+    while (c.parts < 64 && tiles * kv_heads * c.parts * 2 <= room && key_tiles >= c.parts * 2 * c.least) c.parts *= 2;
     const int64_t low = kv_heads & -kv_heads, beside = low < 8 ? low : 8;
     c.slots = (tiles * c.parts + 8 / beside - 1) / (8 / beside);
     c.blocks = 8 * c.slots * (kv_heads / beside);
     return c;
 }
 
+int64_t parts_bytes(const Cut &c, int64_t kv_heads, int64_t head_dim)
+{
+    return c.tiles * kv_heads * c.parts * c.rows * (head_dim + 2) * 4;
+}
+
+// A call: one launch over all keys, or one over the prefix for all items and one over their
+// own keys, whose parts are joined.
+struct Plan {
+    bool shared;
+    Cut own, common;
+    int64_t bytes;
+};
+
 Plan plan_packed(int64_t tokens_q, int64_t tokens_k, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t head_dim)
 {
-    return plan(tokens_q * (heads / kv_heads) / kRows + sequences, (tokens_k / sequences + kKeys - 1) / kKeys, kv_heads, head_dim);
+    Plan c{};
+    const int64_t rows = tokens_q * (heads / kv_heads);
+    const bool few = rows <= kFewRows * sequences;
+    c.own = cut(few, rows / (few ? kFewRows : kRows) + sequences, tokens_k / sequences, few ? 4 : 1, kv_heads, head_dim);
+    c.bytes = c.own.parts > 1 ? parts_bytes(c.own, kv_heads, head_dim) : 0;
+    return c;
 }
 
 Plan plan_prefix(int64_t batch, int64_t tokens_q, int64_t tokens_k, int64_t prefix, int64_t heads, int64_t kv_heads,
                  int64_t head_dim)
 {
-    return plan((tokens_q * (heads / kv_heads) + kRows - 1) / kRows * batch,
-                (prefix + kKeys - 1) / kKeys + (tokens_k + kKeys - 1) / kKeys, kv_heads, head_dim);
+    Plan c{};
+    const int64_t rows = tokens_q * (heads / kv_heads);
+    const bool few = rows <= kFewRows;
+    const int64_t tile = few ? kFewRows : kRows, tiles = (rows + tile - 1) / tile * batch;
+    c.shared = batch > 1 && rows < kRows && (batch - 1) * prefix * kv_heads * head_dim * 4 > kShared;
+    c.own = cut(few, tiles, (c.shared ? 0 : prefix) + tokens_k, 1, kv_heads, head_dim);
+    c.bytes = c.shared || c.own.parts > 1 ? parts_bytes(c.own, kv_heads, head_dim) : 0;
+    if (c.shared) {
+        const bool few_all = batch * rows <= kFewRows;
+        c.common = cut(few_all, (batch * rows + (few_all ? kFewRows : kRows) - 1) / (few_all ? kFewRows : kRows), prefix, 1,
+                       kv_heads, head_dim);
+        c.bytes += parts_bytes(c.common, kv_heads, head_dim);
+    }
+    return c;
 }
 
-int64_t parts_bytes(const Plan &c, int64_t kv_heads, int64_t head_dim)
+Parts place(const Cut &c, int64_t kv_heads, int64_t head_dim, void *workspace)
 {
-    return c.parts > 1 ? c.tiles * kv_heads * c.parts * kRows * (head_dim + 2) * 4 : 0;
+    Parts r;
+    r.sums = static_cast<float *>(workspace);
+    r.stats = reinterpret_cast<float2 *>(r.sums + c.tiles * kv_heads * c.parts * c.rows * head_dim);
+    r.tiles = static_cast<int>(c.tiles);
+    r.slots = static_cast<int>(c.slots);
+    r.parts = static_cast<int>(c.parts);
+    r.least = static_cast<int>(c.least);
+    return r;
 }
 
 template <int D>
-void launch(const Params &p, int64_t blocks, hipStream_t s)
+void attend(const Params &p, const Cut &c, hipStream_t s)
 {
-    tile_kernel<D><<<static_cast<unsigned>(blocks), kWaves * 64, 0, s>>>(p);
-    if (p.parts > 1)
-        join_kernel<D><<<static_cast<unsigned>(static_cast<int64_t>(p.tiles) * p.kv_heads * (kRows * D / 8 / 256)), 256, 0, s>>>(p);
+    const unsigned blocks = static_cast<unsigned>(c.blocks);
+    if (c.few) few_kernel<D><<<blocks, kWaves * 64, 0, s>>>(p);
+    else tile_kernel<D><<<blocks, kWaves * 64, 0, s>>>(p);
 }
 
-// The launch, once the operands are checked and p holds them.
+template <int D, int ROWS, int KEYS>
+void join(const Params &p, const Plan &c, const Parts &common, hipStream_t s)
+{
+    const unsigned blocks = static_cast<unsigned>(c.own.tiles * p.kv_heads * (ROWS * D / 8 / 256));
+    if (!c.shared) join_kernel<D, ROWS, KEYS, 0><<<blocks, 256, 0, s>>>(p, common);
+    else if (c.common.few) join_kernel<D, ROWS, KEYS, kFewRows><<<blocks, 256, 0, s>>>(p, common);
+    else join_kernel<D, ROWS, KEYS, kRows><<<blocks, 256, 0, s>>>(p, common);
+}
+
+template <int D>
+void launch(Params &p, const Plan &c, void *workspace, hipStream_t s)
+{
+    p.cut = place(c.own, p.kv_heads, D, workspace);
+    Parts common{};
+    if (c.shared) {
+        common = place(c.common, p.kv_heads, D, static_cast<char *>(workspace) + parts_bytes(c.own, p.kv_heads, D));
+        Params all = p;
+        all.cut = common;
+        all.keys = kCommon;
+        all.joined = p.joined = true;
+        attend<D>(all, c.common, s);
+        p.keys = kOwn;
+    }
+    attend<D>(p, c.own, s);
+    if (c.shared || c.own.parts > 1) c.own.few ? join<D, kFewRows, kFewKeys<D>>(p, c, common, s) : join<D, kRows, kKeys>(p, c, common, s);
+}
+
+// The launches, once the operands are checked and p holds them.
 int run(const char *what, Params &p, const Plan &c, int64_t head_dim, void *workspace, int64_t workspace_bytes, void *stream)
 {
     // a launch holds fewer than 2^32 threads
-    if (c.blocks >= (int64_t{1} << 32) / (kWaves * 64)) return fail(LTXK_E_ARG, "%s: too many row tiles", what);
-    const int64_t need = parts_bytes(c, p.kv_heads, head_dim);
-    if (need && (!workspace || !aligned16(workspace) || workspace_bytes < need))
+    const int64_t most = (int64_t{1} << 32) / (kWaves * 64);
+    if (c.own.blocks >= most || (c.shared && c.common.blocks >= most) ||
+        (c.bytes && c.own.tiles * p.kv_heads >= most / (c.own.rows * head_dim / 8 / 256)))
+        return fail(LTXK_E_ARG, "%s: too many row tiles", what);
+    if (c.bytes && (!workspace || !aligned16(workspace) || workspace_bytes < c.bytes))
         return fail(LTXK_E_ARG, "%s: the workspace must hold ltxk_%s_workspace_bytes, 16-byte aligned", what, what);
-    p.tiles = static_cast<int>(c.tiles);
-    p.slots = static_cast<int>(c.slots);
-    p.parts = static_cast<int>(c.parts);
-    p.least = kLeast;
-    p.part = static_cast<float *>(workspace);
-    p.stats = reinterpret_cast<float2 *>(p.part + c.tiles * p.kv_heads * c.parts * kRows * head_dim);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (head_dim == 64) launch<64>(p, c.blocks, s);
-    else if (head_dim == 128) launch<128>(p, c.blocks, s);
-    else launch<256>(p, c.blocks, s);
+    if (head_dim == 64) launch<64>(p, c, workspace, s);
+    else if (head_dim == 128) launch<128>(p, c, workspace, s);
+    else launch<256>(p, c, workspace, s);
     return check_launch(what);
 }
 
@@ -652,7 +995,7 @@ extern "C" int64_t ltxk_packed_attention_workspace_bytes(int64_t tokens_q, int64
                                                          int64_t heads, int64_t kv_heads, int64_t head_dim)
 {
     if (tokens_q <= 0 || tokens_k < 0 || sequences <= 0 || kv_heads <= 0 || heads < kv_heads || head_dim <= 0) return 0;
-    return parts_bytes(plan_packed(tokens_q, tokens_k, sequences, heads, kv_heads, head_dim), kv_heads, head_dim);
+    return plan_packed(tokens_q, tokens_k, sequences, heads, kv_heads, head_dim).bytes;
 }
 
 extern "C" int ltxk_packed_attention(void *out, const void *q, int64_t q_tstride, const void *k, int64_t k_tstride,
@@ -708,7 +1051,7 @@ extern "C" int64_t ltxk_prefix_attention_workspace_bytes(int64_t batch, int64_t 
 {
     if (batch <= 0 || tokens_q <= 0 || tokens_k < 0 || prefix < 0 || kv_heads <= 0 || heads < kv_heads || head_dim <= 0)
         return 0;
-    return parts_bytes(plan_prefix(batch, tokens_q, tokens_k, prefix, heads, kv_heads, head_dim), kv_heads, head_dim);
+    return plan_prefix(batch, tokens_q, tokens_k, prefix, heads, kv_heads, head_dim).bytes;
 }
 
 extern "C" int ltxk_prefix_attention(void *out, const void *q, int64_t q_bstride, int64_t q_tstride, const void *k,

@@ -87,7 +87,8 @@ def test_lengths_and_views():
         _check(want, q, k, v, pk, pv, [150] * 3, 8, 2)
         none = ltxk.prefix_attention(q, k, v, pk, pv, 8, 2, _ints([-5, 0, -2**31]), causal=False)
         _check(none, q, k, v, pk, pv, [0] * 3, 8, 2, causal=False)
-        assert torch.equal(none, ltxk.prefix_attention(q, k[:, :0], v[:, :0], pk, pv, 8, 2, causal=False))
+        none = ltxk.prefix_attention(q, k[:, :0], v[:, :0], pk, pv, 8, 2, causal=False)  # (a call may be cut by its room)
+        _check(none, q, k, v, pk, pv, [0] * 3, 8, 2, causal=False)
         one = ltxk.prefix_attention(q, k[:1].expand(3, 150, 128), v[:1].expand(3, 150, 128), pk, pv, 8, 2, scale=0.25)
         _check(one, q, k[:1].expand(3, 150, 128), v[:1].expand(3, 150, 128), pk, pv, [150] * 3, 8, 2, scale=0.25)
     empty = ltxk.prefix_attention(q, k[:, :0], v[:, :0], pk[:0], pv[:0], 8, 2, causal=False)
