@@ -48,7 +48,14 @@ struct Params {
     Parts cut;
 };
 
+// Values that are the same in all lanes, in scalar registers, as the loads' buffers have to be.
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ const char *uniform(const char *x)
+{
+    const uint64_t a = reinterpret_cast<uint64_t>(x);
+    return reinterpret_cast<const char *>(static_cast<uint64_t>(static_cast<uint32_t>(uniform(static_cast<int>(a >> 32)))) << 32 |
+                                          static_cast<uint32_t>(uniform(static_cast<int>(a))));
+}
 
 // A tile of rows, what its rows attend to, and where they go.  Rows are a sequence's
 // queries, each at all heads of the group in turn, so that few queries fill a tile's rows
@@ -188,6 +195,9 @@ __device__ __forceinline__ Span key_span(const Params &p, const Tile &r, int kvh
         s.stride = V ? p.vts : p.kts;
         s.base = (V ? r.v : r.k) + static_cast<int64_t>(at) * s.stride;
     }
+    s.base = uniform(s.base);
+    s.valid = uniform(s.valid);
+    s.stride = uniform(s.stride);
     return s;
 }
 
@@ -620,9 +630,7 @@ __global__ void __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) few_kernel(Para
         constexpr bool V = decltype(is_v)::value;
         const Span s = key_span<D, KT, V>(p, r, kvh, g);
         const uint64_t a = reinterpret_cast<uint64_t>(s.base);
-        const u32x4 rsrc = {static_cast<uint32_t>(uniform(static_cast<int>(a))),
-                            static_cast<uint32_t>(uniform(static_cast<int>(a >> 32) & 0xffff)),
-                            static_cast<uint32_t>(uniform(static_cast<int>(reach<D>(s)))), 0x00020000u};
+        const u32x4 rsrc = {static_cast<uint32_t>(a), static_cast<uint32_t>(a >> 32) & 0xffff, reach<D>(s), 0x00020000u};
         const uint32_t to = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char *)(V ? vt : kt)));
 #pragma unroll
         for (int c = 0; c < NL; ++c) {
