@@ -44,7 +44,7 @@ struct Params {
     bool causal;
     float scale2;         // scale * log2(e)
     Keys keys;
-    bool joined;          // every tile is written as parts
+    bool joined, few;     // every tile is written as parts; tiles of kFewRows rows
     Parts cut;
 };
 
@@ -270,9 +270,9 @@ __device__ __forceinline__ void attend_row(const Params &p, const Tile &r, int k
 // heads, as many at a time as divide 8 go to XCDs of their own, whose L2 then holds their
 // keys and values, and each head's tiles are dealt among its XCDs.  The tiles with the most
 // keys (a sequence's last ones) come first.
-__device__ __forceinline__ bool find_work(const Params &p, int &t, int &kvh, int &part)
+__device__ __forceinline__ bool find_work(const Params &p, int block, int &t, int &kvh, int &part)
 {
-    const int xcd = blockIdx.x & 7, j = blockIdx.x >> 3;
+    const int xcd = block & 7, j = block >> 3;
     const int beside = p.kv_heads & -p.kv_heads & 7 ? p.kv_heads & -p.kv_heads : 8, each = 8 / beside;
     const Parts &c = p.cut;
     kvh = j / c.slots * beside + xcd % beside;
@@ -323,22 +323,36 @@ __device__ __forceinline__ void again_row(const Params &p, const Tile &r, int kv
     }
 }
 
+// The buffer of a span, for load_lds16.
 template <int D>
-__global__ void __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) tile_kernel(Params p)
+__device__ __forceinline__ u32x4 buffer(const Span &s)
+{
+    const uint64_t a = reinterpret_cast<uint64_t>(s.base);
+    return u32x4{static_cast<uint32_t>(a), static_cast<uint32_t>(a >> 32) & 0xffff, reach<D>(s), 0x00020000u};
+}
+
+__device__ __forceinline__ uint32_t lds_address(const void *x)
+{
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char *)x));
+}
+
+template <int D>
+struct TileLds {
+    char k0[kKeys * D * 2], k1[kKeys * D * 2], v0[kKeys * D * 2], v1[kKeys * D * 2];
+};
+
+template <int D>
+__device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<D> &lds)
 {
     constexpr int KS = D / 16;               // contraction steps of the scores
     constexpr int MT = D / 32;               // output tiles
     constexpr int NK = 2 * KS, NV = 4 * MT;  // K and V fragments of a tile
     constexpr int kAhead = 4;                // fragments read ahead of the products
-    constexpr int kTileBytes = kKeys * D * 2;
-    __shared__ __attribute__((aligned(1024))) char k0[kTileBytes];
-    __shared__ __attribute__((aligned(1024))) char k1[kTileBytes];
-    __shared__ __attribute__((aligned(1024))) char v0[kTileBytes];
-    __shared__ __attribute__((aligned(1024))) char v1[kTileBytes];
+    char *const k0 = lds.k0, *const k1 = lds.k1, *const v0 = lds.v0, *const v1 = lds.v1;
 
     int t, kvh, part;
     Tile r;
-    if (!find_work(p, t, kvh, part) || !find_tile<D, kRows, kKeys>(p, t, kvh, r)) return;
+    if (!find_work(p, block, t, kvh, part) || !find_tile<D, kRows, kKeys>(p, t, kvh, r)) return;
     const int parts = parts_of(p.cut, r.tiles);
     if (part >= parts) return;
     const bool joined = parts > 1 || p.joined;
@@ -363,15 +377,15 @@ __global__ void __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) tile_kernel(Par
 #pragma unroll
         for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const bf16x8 *>(qp + s * 32);
     }
-    auto load = [&](auto is_v, rsrc_t rsrc, const Span &s, int c, char *dst) __attribute__((always_inline)) {
+    auto load = [&](auto is_v, const u32x4 &rsrc, const Span &s, int c, const char *dst) __attribute__((always_inline)) {
         constexpr bool V = decltype(is_v)::value;
         const int at = wave * kLoads<D> + c, row = part_row<D>(c, wave, lane), pos = lane % (D / 8);
         const uint32_t off = __umul24(min(row, s.valid - 1), s.stride) + (V ? v_pos<D>(row, pos) : k_pos<D>(row, pos)) * 16;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_char *)(dst + at * 1024), 16, off, 0, 0, 0);
+        load_lds16(rsrc, lds_address(dst) + at * 1024, off, 0);
     };
     {
         const Span s = key_span<D, kKeys, false>(p, r, kvh, t0);
-        const rsrc_t rs = make_rsrc(s.base, reach<D>(s));
+        const u32x4 rs = buffer<D>(s);
 #pragma unroll
         for (int c = 0; c < kLoads<D>; ++c) load(std::false_type{}, rs, s, c, k0);
     }
@@ -502,7 +516,7 @@ __global__ void __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) tile_kernel(Par
         constexpr int kEvery = from == 0 ? 3 : 2;
         const Span ks = key_span<D, kKeys, false>(p, r, kvh, t0 + min(i + 1, n - 1));
         const Span vs = key_span<D, kKeys, true>(p, r, kvh, t0 + i);
-        const rsrc_t kr = make_rsrc(ks.base, reach<D>(ks)), vr = make_rsrc(vs.base, reach<D>(vs));
+        const u32x4 kr = buffer<D>(ks), vr = buffer<D>(vs);
         products(from, integral_constant<int, NV + NK>{}, vp, kc, [&](int j) __attribute__((always_inline)) {
             if (j % kEvery) return;
             const int c = j / kEvery;
@@ -599,18 +613,24 @@ __device__ __forceinline__ void wait_lds()
 // without barriers, the next keys on their way while the weights are made and the next
 // values while the next scores are; the waves' sums are added up in the end.
 template <int D>
-__global__ void __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) few_kernel(Params p)
+struct FewLds {
+    char tile[kWaves][2][kFewKeys<D> * D * 2];
+    float2 stat[kWaves][kFewRows];
+    uint32_t odd;
+};
+
+template <int D>
+__device__ __forceinline__ void attend_few(const Params &p, int block, FewLds<D> &lds)
 {
     constexpr int KT = kFewKeys<D>, KU = KT / 32;
     constexpr int KS = D / 16, MT = D / 32;
     constexpr int kBytes = KT * D * 2, NL = kBytes / 1024;  // of a tile, and its load instructions
-    __shared__ __attribute__((aligned(1024))) char lds[kWaves][2][kBytes];
-    __shared__ float2 stat[kWaves][kFewRows];
-    __shared__ uint32_t odd;
+    auto &stat = lds.stat;
+    uint32_t &odd = lds.odd;
 
     int t, kvh, part;
     Tile r;
-    if (!find_work(p, t, kvh, part) || !find_tile<D, kFewRows, KT>(p, t, kvh, r)) return;
+    if (!find_work(p, block, t, kvh, part) || !find_tile<D, kFewRows, KT>(p, t, kvh, r)) return;
     const int parts = parts_of(p.cut, r.tiles);
     if (part >= parts) return;
     const bool joined = parts > 1 || p.joined;
@@ -625,13 +645,12 @@ __global__ void __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) few_kernel(Para
     const int sure_hi = uniform(own.hi), sure_lo = __builtin_amdgcn_readlane(own.lo, 31);
     if (threadIdx.x == 0) odd = 0;
 
-    char *const kt = lds[wave][0], *const vt = lds[wave][1];
+    char *const kt = lds.tile[wave][0], *const vt = lds.tile[wave][1];
     auto load = [&](auto is_v, int g) __attribute__((always_inline)) {
         constexpr bool V = decltype(is_v)::value;
         const Span s = key_span<D, KT, V>(p, r, kvh, g);
-        const uint64_t a = reinterpret_cast<uint64_t>(s.base);
-        const u32x4 rsrc = {static_cast<uint32_t>(a), static_cast<uint32_t>(a >> 32) & 0xffff, reach<D>(s), 0x00020000u};
-        const uint32_t to = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char *)(V ? vt : kt)));
+        const u32x4 rsrc = buffer<D>(s);
+        const uint32_t to = lds_address(V ? vt : kt);
 #pragma unroll
         for (int c = 0; c < NL; ++c) {
             const int row = c * (1024 / (2 * D)) + lane / (D / 8), pos = lane % (D / 8);
@@ -735,7 +754,7 @@ __global__ void __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) few_kernel(Para
 #pragma unroll
     for (int i = 1; i < kWaves; ++i) top = fmaxf(top, stat[i][l32].x);
     const float fade = __builtin_amdgcn_exp2f(mx - top);
-    float *const mine = reinterpret_cast<float *>(lds[wave]);
+    float *const mine = reinterpret_cast<float *>(lds.tile[wave]);
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -752,7 +771,7 @@ __global__ void __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) few_kernel(Para
 #pragma unroll
         for (int k = 0; k < kWaves; ++k) {
             all += st[k].y * __builtin_amdgcn_exp2f(st[k].x - high);
-            const float *x = reinterpret_cast<const float *>(lds[k]) + at * D;
+            const float *x = reinterpret_cast<const float *>(lds.tile[k]) + at * D;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const f32x4 y = *reinterpret_cast<const f32x4 *>(x + ((2 * c + h) ^ (at & (D / 4 - 1))) * 4);
@@ -786,15 +805,47 @@ __global__ void __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) few_kernel(Para
     }
 }
 
-// Joins the parts of the cut tiles, and of a prefix's (`common`, tiles of COMMON rows) with
-// those of the items' own keys: 8 columns of one row a thread.
-template <int D, int ROWS, int KEYS, int COMMON>
-__global__ void __launch_bounds__(256) join_kernel(Params p, Parts common)
+// One kind of tile, or both for a prefix and the items' own keys, side by side.
+template <int D>
+__global__ void __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) tile_kernel(Params p)
 {
-    constexpr int kThreads = ROWS * (D / 8);  // of a tile
-    const int64_t tile = static_cast<int64_t>(blockIdx.x) / (kThreads / 256);
-    const int i = blockIdx.x % (kThreads / 256) * 256 + threadIdx.x, c = i % (D / 8), at = i / (D / 8);
-    const int t = static_cast<int>(tile / p.kv_heads), kvh = static_cast<int>(tile % p.kv_heads);
+    __shared__ __attribute__((aligned(1024))) TileLds<D> lds;
+    attend_tile<D>(p, blockIdx.x, lds);
+}
+template <int D>
+__global__ void __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) few_kernel(Params p)
+{
+    __shared__ __attribute__((aligned(1024))) FewLds<D> lds;
+    attend_few<D>(p, blockIdx.x, lds);
+}
+struct BothParams {
+    Params p[2];  // for the prefix's tiles, the first `commons` workgroups, and for the others
+    int commons;
+};
+template <int D>
+__global__ void __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) both_kernel(BothParams both)
+{
+    __shared__ __attribute__((aligned(1024))) union {
+        TileLds<D> tile;
+        FewLds<D> few;
+    } lds;
+    const int i = static_cast<int>(blockIdx.x) < both.commons ? 0 : 1;
+    const Params &p = both.p[i];
+    const int block = blockIdx.x - i * both.commons;
+    if (p.few) attend_few<D>(p, block, lds.few);
+    else attend_tile<D>(p, block, lds.tile);
+}
+
+// Joins the parts of the cut tiles, and of a prefix's (`common`, tiles of COMMON rows) with
+// those of the items' own keys: a row a wave, whose lanes first have a part's maximum and sum
+// each, then 8 columns of every so many parts each.
+template <int D, int ROWS, int KEYS, int COMMON>
+__global__ void __launch_bounds__(256) join_kernel(Params p, Parts common, int groups)
+{
+    constexpr int kLanes = D / 8, kBeside = 64 / kLanes;  // lanes of a part, and parts at a time
+    const int lane = threadIdx.x & 63, c = lane % kLanes, g = lane / kLanes;
+    const int at = static_cast<int>(blockIdx.x) % groups * kWaves + uniform(threadIdx.x >> 6), tile = blockIdx.x / groups;
+    const int t = tile / p.kv_heads, kvh = tile - t * p.kv_heads;
     Tile r;
     if (!find_tile<D, ROWS, KEYS>(p, t, kvh, r)) return;
     const int parts = parts_of(p.cut, r.tiles);
@@ -806,31 +857,42 @@ __global__ void __launch_bounds__(256) join_kernel(Params p, Parts common)
         const int64_t row = (r.token + w.query) * p.group + w.member;
         cu = part_rows(p, common, row / COMMON, kvh, 0, COMMON) + row % COMMON;
     }
-    float m = -FLT_MAX;
-    for (int k = 0; k < parts; ++k) m = fmaxf(m, p.cut.stats[u + k * ROWS].x);
-    if (COMMON)
-        for (int k = 0; k < common.parts; ++k) m = fmaxf(m, common.stats[cu + k * COMMON].x);
-    float acc[8] = {}, sum = 0.f;
-    auto add = [&](float2 st, const float *sums) {
-        if (st.y == 0.f) return;  // a part that saw no key wrote no sums
-        const float f = __builtin_amdgcn_exp2f(st.x - m);
-        const f32x4 *x = reinterpret_cast<const f32x4 *>(sums + c * 8);
-        const f32x4 lo = x[0], hi = x[1];
-        sum += f * st.y;
+    const float2 none = make_float2(-FLT_MAX, 0.f);
+    const float2 st = lane < parts ? p.cut.stats[u + lane * ROWS] : none;
+    const float2 cst = COMMON && lane < common.parts ? common.stats[cu + lane * COMMON] : none;
+    float m = fmaxf(st.x, cst.x);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            acc[e] = __builtin_fmaf(f, lo[e], acc[e]);
-            acc[4 + e] = __builtin_fmaf(f, hi[e], acc[4 + e]);
+    for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    // (a part without a key has a sum of zero, and may have written no sums)
+    const float f = st.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(st.x - m), cf = cst.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(cst.x - m);
+    const float sum = wave_sum64(f * st.y + cf * cst.y);
+    float acc[8] = {};
+    auto add = [&](const float *sums, int64_t first, int rows, int count, float factors) __attribute__((always_inline)) {
+#pragma unroll 4
+        for (int k = g; k < count + g; k += kBeside) {  // as many turns for every lane
+            const float x = __shfl(factors, min(k, count - 1), 64);
+            const f32x4 *y = reinterpret_cast<const f32x4 *>(sums + (first + static_cast<int64_t>(min(k, count - 1)) * rows) * D + c * 8);
+            const f32x4 lo = y[0], hi = y[1];
+            const bool take = k < count && x != 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                acc[e] = take ? __builtin_fmaf(x, lo[e], acc[e]) : acc[e];
+                acc[4 + e] = take ? __builtin_fmaf(x, hi[e], acc[4 + e]) : acc[4 + e];
+            }
         }
     };
-    for (int k = 0; k < parts; ++k) add(p.cut.stats[u + k * ROWS], p.cut.sums + (u + k * ROWS) * D);
-    if (COMMON)
-        for (int k = 0; k < common.parts; ++k) add(common.stats[cu + k * COMMON], common.sums + (cu + k * COMMON) * D);
+    add(p.cut.sums, u, ROWS, parts, f);
+    if (COMMON) add(common.sums, cu, COMMON, common.parts, cf);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+#pragma unroll
+        for (int o = kLanes; o < 64; o <<= 1) acc[e] += __shfl_xor(acc[e], o, 64);
     const bool any = w.any || (COMMON && !p.causal);
     const float inv = 1.f / sum;
 #pragma unroll
     for (int e = 0; e < 8; ++e) acc[e] = any ? acc[e] * inv : 0.f;
-    *reinterpret_cast<u32x4 *>(p.out + ((r.token + w.query) * p.heads + kvh * p.group + w.member) * D + c * 8) = pack8v(acc);
+    if (g == 0)
+        *reinterpret_cast<u32x4 *>(p.out + ((r.token + w.query) * p.heads + kvh * p.group + w.member) * D + c * 8) = pack8v(acc);
 }
 
 constexpr int64_t kMost = 0x7fffffff - 1024;  // rows that are counted in int
@@ -872,7 +934,7 @@ int64_t parts_bytes(const Cut &c, int64_t kv_heads, int64_t head_dim)
 struct Plan {
     bool shared;
     Cut own, common;
-    int64_t bytes;
+    int64_t used, bytes;  // rows of an own tile at most, and the workspace's bytes
 };
 
 Plan plan_packed(int64_t tokens_q, int64_t tokens_k, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t head_dim)
@@ -880,7 +942,8 @@ Plan plan_packed(int64_t tokens_q, int64_t tokens_k, int64_t sequences, int64_t 
     Plan c{};
     const int64_t rows = tokens_q * (heads / kv_heads);
     const bool few = rows <= kFewRows * sequences;
-    c.own = cut(few, rows / (few ? kFewRows : kRows) + sequences, tokens_k / sequences, few ? 4 : 1, kv_heads, head_dim);
+    c.own = cut(few, rows / (few ? kFewRows : kRows) + sequences, tokens_k / sequences, few ? 16 : 1, kv_heads, head_dim);
+    c.used = c.own.rows;
     c.bytes = c.own.parts > 1 ? parts_bytes(c.own, kv_heads, head_dim) : 0;
     return c;
 }
@@ -894,6 +957,7 @@ Plan plan_prefix(int64_t batch, int64_t tokens_q, int64_t tokens_k, int64_t pref
     const int64_t tile = few ? kFewRows : kRows, tiles = (rows + tile - 1) / tile * batch;
     c.shared = batch > 1 && rows < kRows && (batch - 1) * prefix * kv_heads * head_dim * 4 > kShared;
     c.own = cut(few, tiles, (c.shared ? 0 : prefix) + tokens_k, 1, kv_heads, head_dim);
+    c.used = rows < tile ? rows : tile;
     c.bytes = c.shared || c.own.parts > 1 ? parts_bytes(c.own, kv_heads, head_dim) : 0;
     if (c.shared) {
         const bool few_all = batch * rows <= kFewRows;
@@ -916,38 +980,37 @@ Parts place(const Cut &c, int64_t kv_heads, int64_t head_dim, void *workspace)
     return r;
 }
 
-template <int D>
-void attend(const Params &p, const Cut &c, hipStream_t s)
-{
-    const unsigned blocks = static_cast<unsigned>(c.blocks);
-    if (c.few) few_kernel<D><<<blocks, kWaves * 64, 0, s>>>(p);
-    else tile_kernel<D><<<blocks, kWaves * 64, 0, s>>>(p);
-}
-
 template <int D, int ROWS, int KEYS>
 void join(const Params &p, const Plan &c, const Parts &common, hipStream_t s)
 {
-    const unsigned blocks = static_cast<unsigned>(c.own.tiles * p.kv_heads * (ROWS * D / 8 / 256));
-    if (!c.shared) join_kernel<D, ROWS, KEYS, 0><<<blocks, 256, 0, s>>>(p, common);
-    else if (c.common.few) join_kernel<D, ROWS, KEYS, kFewRows><<<blocks, 256, 0, s>>>(p, common);
-    else join_kernel<D, ROWS, KEYS, kRows><<<blocks, 256, 0, s>>>(p, common);
+    const int groups = static_cast<int>((c.used + kWaves - 1) / kWaves);
+    const unsigned blocks = static_cast<unsigned>(c.own.tiles * p.kv_heads * groups);
+    if (!c.shared) join_kernel<D, ROWS, KEYS, 0><<<blocks, 256, 0, s>>>(p, common, groups);
+    else if (c.common.few) join_kernel<D, ROWS, KEYS, kFewRows><<<blocks, 256, 0, s>>>(p, common, groups);
+    else join_kernel<D, ROWS, KEYS, kRows><<<blocks, 256, 0, s>>>(p, common, groups);
 }
 
 template <int D>
 void launch(Params &p, const Plan &c, void *workspace, hipStream_t s)
 {
     p.cut = place(c.own, p.kv_heads, D, workspace);
+    p.few = c.own.few;
     Parts common{};
+    const unsigned blocks = static_cast<unsigned>(c.own.blocks), commons = static_cast<unsigned>(c.common.blocks);
     if (c.shared) {
         common = place(c.common, p.kv_heads, D, static_cast<char *>(workspace) + parts_bytes(c.own, p.kv_heads, D));
+        p.joined = true;
+        p.keys = kOwn;
         Params all = p;
         all.cut = common;
+        all.few = c.common.few;
         all.keys = kCommon;
-        all.joined = p.joined = true;
-        attend<D>(all, c.common, s);
-        p.keys = kOwn;
+        both_kernel<D><<<commons + blocks, kWaves * 64, 0, s>>>(BothParams{{all, p}, static_cast<int>(commons)});
+    } else if (c.own.few) {
+        few_kernel<D><<<blocks, kWaves * 64, 0, s>>>(p);
+    } else {
+        tile_kernel<D><<<blocks, kWaves * 64, 0, s>>>(p);
     }
-    attend<D>(p, c.own, s);
     if (c.shared || c.own.parts > 1) c.own.few ? join<D, kFewRows, kFewKeys<D>>(p, c, common, s) : join<D, kRows, kKeys>(p, c, common, s);
 }
 
@@ -956,8 +1019,7 @@ int run(const char *what, Params &p, const Plan &c, int64_t head_dim, void *work
 {
     // a launch holds fewer than 2^32 threads
     const int64_t most = (int64_t{1} << 32) / (kWaves * 64);
-    if (c.own.blocks >= most || (c.shared && c.common.blocks >= most) ||
-        (c.bytes && c.own.tiles * p.kv_heads >= most / (c.own.rows * head_dim / 8 / 256)))
+    if (c.own.blocks + c.common.blocks >= most || (c.bytes && c.own.tiles * p.kv_heads >= most / (c.used / kWaves + 1)))
         return fail(LTXK_E_ARG, "%s: too many row tiles", what);
     if (c.bytes && (!workspace || !aligned16(workspace) || workspace_bytes < c.bytes))
         return fail(LTXK_E_ARG, "%s: the workspace must hold ltxk_%s_workspace_bytes, 16-byte aligned", what, what);
