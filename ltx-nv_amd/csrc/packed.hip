@@ -28,8 +28,8 @@ enum Keys { kBoth, kOwn, kCommon };
 struct Parts {
     float *sums;          // each part's weighted sums of v (rows x D)
     float2 *stats;        // and each of its rows' maximum and sum of weights
-    int tiles, slots;     // row tiles of a key head, and places for them and their parts on an XCD
-    int parts, least;     // the keys of a tile are cut into up to `parts`, of at least `least` tiles each
+    int units, slots;     // parts of all tiles of a key head (with some that are none), and places for them on an XCD
+    int parts, chunk;     // a tile's keys are cut into up to `parts`, of about `chunk` key tiles each
 };
 
 struct Params {
@@ -68,27 +68,31 @@ struct Tile {
     int first, rows;      // the tile's first row, and the rows of the whole sequence
     int from, to;         // own keys that some of its rows see
     int np, tiles;        // key tiles: of the prefix, and in all
+    int parts;            // into which these are cut
+    int unit, step;       // the first part's unit, and from each to the next
     bool stacked;         // the queries are those of all items
 };
 
-// Where sequence s's row tiles begin, if each sequence takes one more than its rows fill:
-// never less than it needs, and known without the others' lengths.
-template <int ROWS>
-__device__ __forceinline__ int first_tile(const Params &p, int s)
+// Packed sequences: of a sequence with r row tiles and m keys, whose parts take about c r keys
+// (the more tiles the longer), all parts number r ceil(m / (c r)), at most floor(m / c) +
+// floor(rows / ROWS) + 1.  So unit floor(keys before / c) + floor(rows before / ROWS) + s is
+// behind the last one of the sequences before s, and known without their lengths.
+template <int ROWS, int KEYS>
+__device__ __forceinline__ int first_unit(const Params &p, bool cut, int s)
 {
-    const int64_t q0 = min(max(p.qo[s], 0), p.tq);
-    return static_cast<int>(q0 * p.group / ROWS) + s;
+    const int64_t rows = static_cast<int64_t>(min(max(p.qo[s], 0), p.tq)) * p.group;
+    return static_cast<int>(rows / ROWS) + s + (cut ? min(max(p.ko[s], 0), p.tk) / (p.cut.chunk * KEYS) : 0);
 }
 
-// The last s with first_tile(s) <= t, 64 of them at a time.
-template <int ROWS>
-__device__ __forceinline__ int sequence_of(const Params &p, int t)
+// The last s whose first unit is at most `unit`, 64 of them at a time.
+template <int ROWS, int KEYS>
+__device__ __forceinline__ int sequence_of(const Params &p, bool cut, int unit)
 {
     const int lane = threadIdx.x & 63;
     int lo = 0, count = p.seqs;
     while (count > 1) {
         const int step = (count + 63) / 64, i = lane * step;
-        const uint64_t under = __ballot(i < count && first_tile<ROWS>(p, lo + min(i, count - 1)) <= t);
+        const uint64_t under = __ballot(i < count && first_unit<ROWS, KEYS>(p, cut, lo + min(i, count - 1)) <= unit);
         const int at = under ? (63 - __builtin_clzll(under)) * step : 0;
         lo += at;
         count = min(step, count - at);
@@ -96,56 +100,63 @@ __device__ __forceinline__ int sequence_of(const Params &p, int t)
     return uniform(lo);
 }
 
-// Row tile t of key head kvh, or false if there is none.
+// Unit `unit` of key head kvh: its tile and part, or false if there is none.  With `whole` the
+// units are row tiles, whatever their parts.
 template <int D, int ROWS, int KEYS>
-__device__ __forceinline__ bool find_tile(const Params &p, int t, int kvh, Tile &r)
+__device__ __forceinline__ bool find_tile(const Params &p, int unit, int kvh, bool whole, Tile &r, int &part)
 {
     const int64_t qh = static_cast<int64_t>(kvh) * p.group * D * 2, kh = static_cast<int64_t>(kvh) * D * 2;
-    int tile;
+    int tile, parts = p.cut.parts;
+    part = 0;
     r.stacked = p.keys == kCommon;
-    if (r.stacked) {
-        tile = t;
-        r.queries = p.seqs * p.tq;
-        r.n = 0;
-        r.token = 0;
-        r.q = reinterpret_cast<const char *>(p.q) + qh;
-        r.k = r.v = nullptr;
-    } else if (p.qo) {
-        const int s = sequence_of<ROWS>(p, t);
+    if (p.qo) {
+        const bool cut = parts > 1;
+        const int s = sequence_of<ROWS, KEYS>(p, cut && !whole, unit);
         // lengths are cut to what the tensors hold, whatever the offsets say
         const int q0 = min(max(uniform(p.qo[s]), 0), p.tq), q1 = min(uniform(p.qo[s + 1]), p.tq);
         const int k0 = min(max(uniform(p.ko[s]), 0), p.tk), k1 = min(uniform(p.ko[s + 1]), p.tk);
-        tile = t - (static_cast<int>(static_cast<int64_t>(q0) * p.group / ROWS) + s);
         r.queries = max(q1 - q0, 0);
         r.n = max(k1 - k0, 0);
         r.token = q0;
         r.q = reinterpret_cast<const char *>(p.q) + static_cast<int64_t>(q0) * p.qts + qh;
         r.k = reinterpret_cast<const char *>(p.k) + static_cast<int64_t>(k0) * p.kts + kh;
         r.v = reinterpret_cast<const char *>(p.v) + static_cast<int64_t>(k0) * p.vts + kh;
+        r.step = (r.queries * p.group + ROWS - 1) / ROWS;
+        r.unit = uniform(first_unit<ROWS, KEYS>(p, cut, s));
+        tile = unit - (whole ? uniform(first_unit<ROWS, KEYS>(p, false, s)) : r.unit);
+        if (tile < 0 || r.step == 0) return false;
+        if (cut) {
+            const int64_t each = static_cast<int64_t>(p.cut.chunk) * KEYS * r.step;
+            parts = static_cast<int>(min((r.n + each - 1) / each, static_cast<int64_t>(parts)));
+            if (!whole) part = tile / r.step, tile -= part * r.step;
+        }
     } else {
-        const int s = t % p.seqs;
-        tile = t / p.seqs;
-        r.queries = p.tq;
-        r.n = p.lengths ? min(max(uniform(p.lengths[s]), 0), p.tk) : p.tk;
+        const int items = r.stacked ? 1 : p.seqs, s = unit % items;
+        r.queries = r.stacked ? p.seqs * p.tq : p.tq;
+        const int tiles = (r.queries * p.group + ROWS - 1) / ROWS;
+        tile = unit / items;
+        if (!whole) part = tile / tiles, tile -= part * tiles;
+        r.step = items * tiles;
+        r.n = r.stacked ? 0 : p.lengths ? min(max(uniform(p.lengths[s]), 0), p.tk) : p.tk;
         r.token = static_cast<int64_t>(s) * p.tq;
         r.q = reinterpret_cast<const char *>(p.q) + s * p.qbs + qh;
         r.k = reinterpret_cast<const char *>(p.k) + s * p.kbs + kh;
         r.v = reinterpret_cast<const char *>(p.v) + s * p.vbs + kh;
+        r.unit = s;
     }
     r.rows = r.queries * p.group;
     r.first = tile * ROWS;
-    if (tile < 0 || r.first >= r.rows) return false;
+    if (r.first >= r.rows) return false;
+    r.unit += tile * (p.qo || r.stacked ? 1 : p.seqs);
     const int behind = r.n - r.queries;  // keys in front of the first query's
     const int last = min(r.first + ROWS, r.rows) - 1;
     r.to = p.causal && !r.stacked ? max(behind + last / p.group + 1, 0) : r.n;
     r.from = p.window ? min(max(behind + r.first / p.group + 1 - p.window, 0), r.to) : 0;
     r.np = r.stacked || (p.keys == kBoth && (r.to || !p.causal)) ? (p.prefix + KEYS - 1) / KEYS : 0;
     r.tiles = r.np + (r.to - r.from + KEYS - 1) / KEYS;
-    return true;
+    r.parts = max(min(parts, p.qo ? r.tiles : (r.tiles + p.cut.chunk - 1) / p.cut.chunk), 1);
+    return part < r.parts;
 }
-
-// Into how many parts a tile's keys are cut: short ones into few.
-__device__ __forceinline__ int parts_of(const Parts &c, int tiles) { return max(min(c.parts, tiles / c.least), 1); }
 
 // Row `row` of a tile: its query, head of the group, and the own keys [lo, hi) it sees (and
 // the prefix, if any).
@@ -266,26 +277,24 @@ __device__ __forceinline__ void attend_row(const Params &p, const Tile &r, int k
                    min(w.hi, r.from + (max(t1, r.np) - r.np) * KEYS), p.scale2, mx, sum, acc);
 }
 
-// Tile and part of this workgroup.  Workgroups are dealt to the 8 XCDs in turn: of the key
+// Unit and key head of this workgroup.  Workgroups are dealt to the 8 XCDs in turn: of the key
 // heads, as many at a time as divide 8 go to XCDs of their own, whose L2 then holds their
-// keys and values, and each head's tiles are dealt among its XCDs.  The tiles with the most
-// keys (a sequence's last ones) come first.
-__device__ __forceinline__ bool find_work(const Params &p, int block, int &t, int &kvh, int &part)
+// keys and values, and each head's units are dealt among its XCDs, in turn where they are
+// whole tiles (those with the most keys, a sequence's last ones, first), else in runs.
+__device__ __forceinline__ bool find_work(const Params &p, int block, int &unit, int &kvh)
 {
     const int xcd = block & 7, j = block >> 3;
     const int beside = p.kv_heads & -p.kv_heads & 7 ? p.kv_heads & -p.kv_heads : 8, each = 8 / beside;
     const Parts &c = p.cut;
     kvh = j / c.slots * beside + xcd % beside;
-    const int slot = c.parts > 1 ? xcd / beside * c.slots + j % c.slots : j % c.slots * each + xcd / beside;
-    t = c.tiles - 1 - slot % c.tiles;
-    part = slot / c.tiles;
-    return part < c.parts;
+    unit = c.units - 1 - (c.parts > 1 ? xcd / beside * c.slots + j % c.slots : j % c.slots * each + xcd / beside);
+    return unit >= 0;
 }
 
-// The parts' place of a tile's first row.
-__device__ __forceinline__ int64_t part_rows(const Params &p, const Parts &c, int64_t t, int kvh, int part, int rows)
+// The place of a part's first row.
+__device__ __forceinline__ int64_t part_rows(const Params &p, const Tile &r, int kvh, int part, int rows)
 {
-    return ((t * p.kv_heads + kvh) * c.parts + part) * rows;
+    return ((r.unit + static_cast<int64_t>(part) * r.step) * p.kv_heads + kvh) * rows;
 }
 
 // A tile without any key: its rows weigh nothing, or are zero.
@@ -350,15 +359,13 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
     constexpr int kAhead = 4;                // fragments read ahead of the products
     char *const k0 = lds.k0, *const k1 = lds.k1, *const v0 = lds.v0, *const v1 = lds.v1;
 
-    int t, kvh, part;
+    int unit, kvh, part;
     Tile r;
-    if (!find_work(p, block, t, kvh, part) || !find_tile<D, kRows, kKeys>(p, t, kvh, r)) return;
-    const int parts = parts_of(p.cut, r.tiles);
-    if (part >= parts) return;
-    const bool joined = parts > 1 || p.joined;
-    const int64_t unit = part_rows(p, p.cut, t, kvh, part, kRows);
-    const int t0 = static_cast<int>(static_cast<int64_t>(part) * r.tiles / parts);
-    const int n = static_cast<int>(static_cast<int64_t>(part + 1) * r.tiles / parts) - t0;
+    if (!find_work(p, block, unit, kvh) || !find_tile<D, kRows, kKeys>(p, unit, kvh, false, r, part)) return;
+    const bool joined = r.parts > 1 || p.joined;
+    const int64_t place = part_rows(p, r, kvh, part, kRows);
+    const int t0 = static_cast<int>(static_cast<int64_t>(part) * r.tiles / r.parts);
+    const int n = static_cast<int>(static_cast<int64_t>(part + 1) * r.tiles / r.parts) - t0;
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int l32 = lane & 31, half = lane >> 5;
     const int first = r.first + wave * 32, last = r.rows - 1;
@@ -368,7 +375,7 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
     const int sure_hi = uniform(own.hi), sure_lo = __builtin_amdgcn_readlane(own.lo, 31);
     uint16_t *const out = p.out;
 
-    if (n == 0) return no_keys<D, kRows>(p, r, kvh, unit, joined);
+    if (n == 0) return no_keys<D, kRows>(p, r, kvh, place, joined);
 
     // Queries: lane l holds row l % 32, elements 16 s + 8 (l/32) .. + 7.
     bf16x8 qf[KS];
@@ -548,7 +555,7 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
     const uint64_t odd = __ballot(!fine);
     uint32_t again = static_cast<uint32_t>(odd) | static_cast<uint32_t>(odd >> 32);  // rows to be done once more
     if (joined) {
-        const int64_t u = unit + wave * 32 + l32;
+        const int64_t u = place + wave * 32 + l32;
         if (first + l32 <= last) {
             if (half == 0) p.cut.stats[u] = make_float2(mx, total);
 #pragma unroll
@@ -588,7 +595,7 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
         for (; again; again &= again - 1) {
             const int i = __builtin_ctz(again);
             if (first + i <= last)
-                again_row<D, kKeys>(p, r, kvh, first + i, t0, t0 + n, unit + wave * 32 + i, joined);
+                again_row<D, kKeys>(p, r, kvh, first + i, t0, t0 + n, place + wave * 32 + i, joined);
         }
     }
 }
@@ -628,16 +635,14 @@ __device__ __forceinline__ void attend_few(const Params &p, int block, FewLds<D>
     auto &stat = lds.stat;
     uint32_t &odd = lds.odd;
 
-    int t, kvh, part;
+    int unit, kvh, part;
     Tile r;
-    if (!find_work(p, block, t, kvh, part) || !find_tile<D, kFewRows, KT>(p, t, kvh, r)) return;
-    const int parts = parts_of(p.cut, r.tiles);
-    if (part >= parts) return;
-    const bool joined = parts > 1 || p.joined;
-    const int64_t unit = part_rows(p, p.cut, t, kvh, part, kFewRows);
-    const int t0 = static_cast<int>(static_cast<int64_t>(part) * r.tiles / parts);
-    const int t1 = static_cast<int>(static_cast<int64_t>(part + 1) * r.tiles / parts);
-    if (t0 == t1) return no_keys<D, kFewRows>(p, r, kvh, unit, joined);
+    if (!find_work(p, block, unit, kvh) || !find_tile<D, kFewRows, KT>(p, unit, kvh, false, r, part)) return;
+    const bool joined = r.parts > 1 || p.joined;
+    const int64_t place = part_rows(p, r, kvh, part, kFewRows);
+    const int t0 = static_cast<int>(static_cast<int64_t>(part) * r.tiles / r.parts);
+    const int t1 = static_cast<int>(static_cast<int64_t>(part + 1) * r.tiles / r.parts);
+    if (t0 == t1) return no_keys<D, kFewRows>(p, r, kvh, place, joined);
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int l32 = lane & 31, half = lane >> 5;
     const int rows = min(kFewRows, r.rows - r.first);
@@ -784,8 +789,8 @@ __device__ __forceinline__ void attend_few(const Params &p, int block, FewLds<D>
         for (int e = 0; e < 8; ++e) fine = fine && fabsf(f[e]) <= FLT_MAX;
         if (!fine) atomicOr(&odd, 1u << at);
         if (joined) {
-            if (c == 0) p.cut.stats[unit + at] = make_float2(high, all);
-            f32x4 *x = reinterpret_cast<f32x4 *>(p.cut.sums + (unit + at) * D + c * 8);
+            if (c == 0) p.cut.stats[place + at] = make_float2(high, all);
+            f32x4 *x = reinterpret_cast<f32x4 *>(p.cut.sums + (place + at) * D + c * 8);
             x[0] = f32x4{f[0], f[1], f[2], f[3]};
             x[1] = f32x4{f[4], f[5], f[6], f[7]};
         } else {
@@ -801,7 +806,7 @@ __device__ __forceinline__ void attend_few(const Params &p, int block, FewLds<D>
     __syncthreads();
     for (uint32_t again = uniform(odd); again; again &= again - 1) {
         const int i = __builtin_ctz(again);
-        if (i % kWaves == wave) again_row<D, KT>(p, r, kvh, r.first + i, t0, t1, unit + i, joined);
+        if (i % kWaves == wave) again_row<D, KT>(p, r, kvh, r.first + i, t0, t1, place + i, joined);
     }
 }
 
@@ -846,43 +851,48 @@ __global__ void __launch_bounds__(256) join_kernel(Params p, Parts common, int g
     const int lane = threadIdx.x & 63, c = lane % kLanes, g = lane / kLanes;
     const int at = static_cast<int>(blockIdx.x) % groups * kWaves + uniform(threadIdx.x >> 6), tile = blockIdx.x / groups;
     const int t = tile / p.kv_heads, kvh = tile - t * p.kv_heads;
+    int part;
     Tile r;
-    if (!find_tile<D, ROWS, KEYS>(p, t, kvh, r)) return;
-    const int parts = parts_of(p.cut, r.tiles);
-    if ((parts == 1 && !p.joined) || r.first + at >= r.rows) return;  // the tile's only part has written the output
+    if (!find_tile<D, ROWS, KEYS>(p, t, kvh, true, r, part)) return;
+    if ((r.parts == 1 && !p.joined) || r.first + at >= r.rows) return;  // the tile's only part has written the output
     const Row w = find_row(p, r, r.first + at);
-    const int64_t u = part_rows(p, p.cut, t, kvh, 0, ROWS) + at;
-    int64_t cu = 0;
+    // the place of a row's first part, and how far it is to the next part's
+    const int64_t u = part_rows(p, r, kvh, 0, ROWS) + at, step = static_cast<int64_t>(r.step) * p.kv_heads * ROWS;
+    int64_t cu = 0, cstep = 0;
     if (COMMON) {
-        const int64_t row = (r.token + w.query) * p.group + w.member;
-        cu = part_rows(p, common, row / COMMON, kvh, 0, COMMON) + row % COMMON;
+        const int rows = p.seqs * p.tq * p.group, row = static_cast<int>(r.token + w.query) * p.group + w.member;
+        cu = (static_cast<int64_t>(row / COMMON) * p.kv_heads + kvh) * COMMON + row % COMMON;
+        cstep = static_cast<int64_t>((rows + COMMON - 1) / COMMON) * p.kv_heads * COMMON;
     }
-    const float2 none = make_float2(-FLT_MAX, 0.f);
-    const float2 st = lane < parts ? p.cut.stats[u + lane * ROWS] : none;
-    const float2 cst = COMMON && lane < common.parts ? common.stats[cu + lane * COMMON] : none;
-    float m = fmaxf(st.x, cst.x);
+    const int commons = COMMON ? common.parts : 0, count = r.parts + commons;
+    auto stat = [&](int k) {
+        return k < r.parts ? p.cut.stats[u + k * step] : k < count ? common.stats[cu + (k - r.parts) * cstep] : make_float2(-FLT_MAX, 0.f);
+    };
+    float m = -FLT_MAX, sum = 0.f, acc[8] = {};
+    for (int k = lane; k < count; k += 64) m = fmaxf(m, stat(k).x);
 #pragma unroll
     for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-    // (a part without a key has a sum of zero, and may have written no sums)
-    const float f = st.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(st.x - m), cf = cst.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(cst.x - m);
-    const float sum = wave_sum64(f * st.y + cf * cst.y);
-    float acc[8] = {};
-    auto add = [&](const float *sums, int64_t first, int rows, int count, float factors) __attribute__((always_inline)) {
+    for (int k0 = 0; k0 < count; k0 += 64) {
+        // (a part without a key has a sum of zero, and has written no sums)
+        const float2 st = stat(k0 + lane);
+        const float f = st.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(st.x - m);
+        sum += f * st.y;
+        const int here = min(64, count - k0);
 #pragma unroll 4
-        for (int k = g; k < count + g; k += kBeside) {  // as many turns for every lane
-            const float x = __shfl(factors, min(k, count - 1), 64);
-            const f32x4 *y = reinterpret_cast<const f32x4 *>(sums + (first + static_cast<int64_t>(min(k, count - 1)) * rows) * D + c * 8);
-            const f32x4 lo = y[0], hi = y[1];
-            const bool take = k < count && x != 0.f;
+        for (int k = g; k < here + g; k += kBeside) {  // as many turns for every lane
+            const int at_k = k0 + min(k, here - 1);
+            const float x = __shfl(f, min(k, here - 1), 64);
+            const float *sums = at_k < r.parts ? p.cut.sums + (u + at_k * step) * D : common.sums + (cu + (at_k - r.parts) * cstep) * D;
+            const f32x4 lo = *reinterpret_cast<const f32x4 *>(sums + c * 8), hi = *reinterpret_cast<const f32x4 *>(sums + c * 8 + 4);
+            const bool take = k < here && x != 0.f;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 acc[e] = take ? __builtin_fmaf(x, lo[e], acc[e]) : acc[e];
                 acc[4 + e] = take ? __builtin_fmaf(x, hi[e], acc[4 + e]) : acc[4 + e];
             }
         }
-    };
-    add(p.cut.sums, u, ROWS, parts, f);
-    if (COMMON) add(common.sums, cu, COMMON, common.parts, cf);
+    }
+    sum = wave_sum64(sum);
 #pragma unroll
     for (int e = 0; e < 8; ++e)
 #pragma unroll
@@ -895,42 +905,46 @@ __global__ void __launch_bounds__(256) join_kernel(Params p, Parts common, int g
         *reinterpret_cast<u32x4 *>(p.out + ((r.token + w.query) * p.heads + kvh * p.group + w.member) * D + c * 8) = pack8v(acc);
 }
 
-constexpr int64_t kMost = 0x7fffffff - 1024;  // rows that are counted in int
+constexpr int64_t kMost = 1 << 30;            // rows and keys: units and their rows are counted in int
 constexpr int64_t kShared = 8 << 20;          // bytes of prefix that are worth two launches more
 constexpr int64_t kStride = (1 << 23) - 8;    // elements of a token stride: its bytes are 24 bits
 
-// How the tiles of a launch are cut: the keys of each into up to `parts`, so that few tiles
-// still fill the chip (two workgroups a compute unit, one with heads of 256) `rounds` times
-// over, with at least `least` key tiles a part.
+// How the tiles of a launch are cut: where they are too few to fill the chip `rounds` times
+// over (two workgroups a compute unit, one with heads of 256), their keys into parts of at
+// least `least` key tiles.
 struct Cut {
     bool few;             // tiles of kFewRows rows
-    int64_t rows, tiles, parts, least, slots, blocks;
+    int64_t rows, tiles, units, parts, chunk, slots, blocks;
 };
 
-Cut cut(bool few, int64_t tiles, int64_t keys, int64_t rounds, int64_t kv_heads, int64_t head_dim)
+Cut cut(int64_t rows, int64_t tiles, int64_t keys, bool packed, int64_t rounds, int64_t kv_heads, int64_t head_dim)
 {
     Cut c;
-    c.few = few;
-    c.rows = few ? kFewRows : kRows;
+    c.rows = rows;
+    c.few = rows == kFewRows;
     c.tiles = tiles;
-    c.parts = 1;
-    c.least = few ? 8 : 4;
-    const int64_t key_tiles = keys / (few && head_dim != 64 ? 32 : 64);
-    const int64_t room = (head_dim == 256 ? 256 : 512) * rounds;
-    while (c.parts < 64 && tiles * kv_heads * c.parts * 2 <= room && key_tiles >= c.parts * 2 * c.least) c.parts *= 2;
+    const int64_t per = c.few && head_dim != 64 ? 32 : 64;  // keys of a key tile
+    const int64_t room = (head_dim == 256 ? 256 : 512) * rounds / kv_heads + 1, least = c.few ? 8 : 4;
+    // all key tiles of a key head's units (packed: of the sequences, their row tiles taking parts that are longer instead)
+    const int64_t of_all = ((packed ? keys : keys * tiles) + per - 1) / per;
+    c.chunk = (of_all + room - 1) / room;
+    if (c.chunk < least) c.chunk = least;
+    c.parts = ((keys + per - 1) / per + c.chunk - 1) / c.chunk;
+    if (c.parts < 1 || tiles * 2 > room) c.parts = 1;
+    c.units = packed ? tiles + (c.parts > 1 ? keys / (c.chunk * per) : 0) : tiles * c.parts;
     const int64_t low = kv_heads & -kv_heads, beside = low < 8 ? low : 8;
-    c.slots = (tiles * c.parts + 8 / beside - 1) / (8 / beside);
+    c.slots = (c.units + 8 / beside - 1) / (8 / beside);
     c.blocks = 8 * c.slots * (kv_heads / beside);
     return c;
 }
 
 int64_t parts_bytes(const Cut &c, int64_t kv_heads, int64_t head_dim)
 {
-    return c.tiles * kv_heads * c.parts * c.rows * (head_dim + 2) * 4;
+    return c.units * kv_heads * c.rows * (head_dim + 2) * 4;
 }
 
-// A call: one launch over all keys, or one over the prefix for all items and one over their
-// own keys, whose parts are joined.
+// A call: one launch over all keys, or one over the prefix for all items and over their own
+// keys, whose parts are joined.
 struct Plan {
     bool shared;
     Cut own, common;
@@ -940,10 +954,9 @@ struct Plan {
 Plan plan_packed(int64_t tokens_q, int64_t tokens_k, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t head_dim)
 {
     Plan c{};
-    const int64_t rows = tokens_q * (heads / kv_heads);
-    const bool few = rows <= kFewRows * sequences;
-    c.own = cut(few, rows / (few ? kFewRows : kRows) + sequences, tokens_k / sequences, few ? 16 : 1, kv_heads, head_dim);
-    c.used = c.own.rows;
+    const int64_t rows = tokens_q * (heads / kv_heads), tile = rows <= kFewRows * sequences ? kFewRows : kRows;
+    c.own = cut(tile, rows / tile + sequences, tokens_k, true, tile == kFewRows ? 4 : 1, kv_heads, head_dim);
+    c.used = tile;
     c.bytes = c.own.parts > 1 ? parts_bytes(c.own, kv_heads, head_dim) : 0;
     return c;
 }
@@ -952,17 +965,14 @@ Plan plan_prefix(int64_t batch, int64_t tokens_q, int64_t tokens_k, int64_t pref
                  int64_t head_dim)
 {
     Plan c{};
-    const int64_t rows = tokens_q * (heads / kv_heads);
-    const bool few = rows <= kFewRows;
-    const int64_t tile = few ? kFewRows : kRows, tiles = (rows + tile - 1) / tile * batch;
+    const int64_t rows = tokens_q * (heads / kv_heads), tile = rows <= kFewRows ? kFewRows : kRows;
     c.shared = batch > 1 && rows < kRows && (batch - 1) * prefix * kv_heads * head_dim * 4 > kShared;
-    c.own = cut(few, tiles, (c.shared ? 0 : prefix) + tokens_k, 1, kv_heads, head_dim);
+    c.own = cut(tile, (rows + tile - 1) / tile * batch, (c.shared ? 0 : prefix) + tokens_k, false, 1, kv_heads, head_dim);
     c.used = rows < tile ? rows : tile;
     c.bytes = c.shared || c.own.parts > 1 ? parts_bytes(c.own, kv_heads, head_dim) : 0;
     if (c.shared) {
-        const bool few_all = batch * rows <= kFewRows;
-        c.common = cut(few_all, (batch * rows + (few_all ? kFewRows : kRows) - 1) / (few_all ? kFewRows : kRows), prefix, 1,
-                       kv_heads, head_dim);
+        const int64_t of_all = batch * rows <= kFewRows ? kFewRows : kRows;
+        c.common = cut(of_all, (batch * rows + of_all - 1) / of_all, prefix, false, 1, kv_heads, head_dim);
         c.bytes += parts_bytes(c.common, kv_heads, head_dim);
     }
     return c;
@@ -972,11 +982,11 @@ Parts place(const Cut &c, int64_t kv_heads, int64_t head_dim, void *workspace)
 {
     Parts r;
     r.sums = static_cast<float *>(workspace);
-    r.stats = reinterpret_cast<float2 *>(r.sums + c.tiles * kv_heads * c.parts * c.rows * head_dim);
-    r.tiles = static_cast<int>(c.tiles);
+    r.stats = reinterpret_cast<float2 *>(r.sums + c.units * kv_heads * c.rows * head_dim);
+    r.units = static_cast<int>(c.units);
     r.slots = static_cast<int>(c.slots);
     r.parts = static_cast<int>(c.parts);
-    r.least = static_cast<int>(c.least);
+    r.chunk = static_cast<int>(c.chunk);
     return r;
 }
 
