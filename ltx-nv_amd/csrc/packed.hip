@@ -20,6 +20,20 @@ constexpr int kRows = 32 * kWaves, kFewRows = 32;
 template <int D>
 constexpr int kFewKeys = D == 64 ? 64 : 32;
 
+// Weights are 2^(score - reference): the reference is a row's maximum so far, or up to kLag below
+// it, so that what was summed is rarely rescaled.  What is summed up to divide by are the
+// weights as the second product takes them, in bf16, so their rounding cancels where one of
+// them is most of the sum, whatever their size.  References past kHuge round by more than
+// 2^-4: there the scores round first, as the reference did.
+constexpr float kLag = 6.f, kHuge = 1048576.f;
+
+// sum + the two bf16 values of `pair`.
+__device__ __forceinline__ float add_pair(uint32_t pair, float sum)
+{
+    const bf16x2_t ones = {static_cast<__bf16>(1.f), static_cast<__bf16>(1.f)};
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, pair), ones, sum, false);
+}
+
 // The keys of a launch: a sequence's (behind the prefix, if there is one), an item's own
 // alone, or the prefix alone, for the queries of all items.
 enum Keys { kBoth, kOwn, kCommon };
@@ -68,7 +82,7 @@ struct Tile {
     int first, rows;      // the tile's first row, and the rows of the whole sequence
     int from, to;         // own keys that some of its rows see
     int np, tiles;        // key tiles: of the prefix, and in all
-    int parts;            // into which these are cut
+    int parts, each;      // into which these are cut, and key tiles of a part
     int unit, step;       // the first part's unit, and from each to the next
     bool stacked;         // the queries are those of all items
 };
@@ -78,21 +92,21 @@ struct Tile {
 // floor(rows / ROWS) + 1.  So unit floor(keys before / c) + floor(rows before / ROWS) + s is
 // behind the last one of the sequences before s, and known without their lengths.
 template <int ROWS, int KEYS>
-__device__ __forceinline__ int first_unit(const Params &p, bool cut, int s)
+__device__ __forceinline__ int first_unit(const Params &p, int s)
 {
     const int64_t rows = static_cast<int64_t>(min(max(p.qo[s], 0), p.tq)) * p.group;
-    return static_cast<int>(rows / ROWS) + s + (cut ? min(max(p.ko[s], 0), p.tk) / (p.cut.chunk * KEYS) : 0);
+    return static_cast<int>(rows / ROWS) + s + (p.cut.parts > 1 ? min(max(p.ko[s], 0), p.tk) / (p.cut.chunk * KEYS) : 0);
 }
 
-// The last s whose first unit is at most `unit`, 64 of them at a time.
-template <int ROWS, int KEYS>
-__device__ __forceinline__ int sequence_of(const Params &p, bool cut, int unit)
+// The last sequence whose first(s) is at most `x`, 64 of them at a time.
+template <typename F>
+__device__ __forceinline__ int sequence_of(int seqs, int x, F first)
 {
     const int lane = threadIdx.x & 63;
-    int lo = 0, count = p.seqs;
+    int lo = 0, count = seqs;
     while (count > 1) {
         const int step = (count + 63) / 64, i = lane * step;
-        const uint64_t under = __ballot(i < count && first_unit<ROWS, KEYS>(p, cut, lo + min(i, count - 1)) <= unit);
+        const uint64_t under = __ballot(i < count && first(lo + min(i, count - 1)) <= x);
         const int at = under ? (63 - __builtin_clzll(under)) * step : 0;
         lo += at;
         count = min(step, count - at);
@@ -100,18 +114,15 @@ __device__ __forceinline__ int sequence_of(const Params &p, bool cut, int unit)
     return uniform(lo);
 }
 
-// Unit `unit` of key head kvh: its tile and part, or false if there is none.  With `whole` the
-// units are row tiles, whatever their parts.
+// Sequence (item) s at key head kvh: its operands, and its units, of which there are `parts`
+// for a tile at most.
 template <int D, int ROWS, int KEYS>
-__device__ __forceinline__ bool find_tile(const Params &p, int unit, int kvh, bool whole, Tile &r, int &part)
+__device__ __forceinline__ void find_sequence(const Params &p, int s, int kvh, Tile &r)
 {
     const int64_t qh = static_cast<int64_t>(kvh) * p.group * D * 2, kh = static_cast<int64_t>(kvh) * D * 2;
-    int tile, parts = p.cut.parts;
-    part = 0;
+    r.parts = p.cut.parts;
     r.stacked = p.keys == kCommon;
     if (p.qo) {
-        const bool cut = parts > 1;
-        const int s = sequence_of<ROWS, KEYS>(p, cut && !whole, unit);
         // lengths are cut to what the tensors hold, whatever the offsets say
         const int q0 = min(max(uniform(p.qo[s]), 0), p.tq), q1 = min(uniform(p.qo[s + 1]), p.tq);
         const int k0 = min(max(uniform(p.ko[s]), 0), p.tk), k1 = min(uniform(p.ko[s + 1]), p.tk);
@@ -122,31 +133,30 @@ __device__ __forceinline__ bool find_tile(const Params &p, int unit, int kvh, bo
         r.k = reinterpret_cast<const char *>(p.k) + static_cast<int64_t>(k0) * p.kts + kh;
         r.v = reinterpret_cast<const char *>(p.v) + static_cast<int64_t>(k0) * p.vts + kh;
         r.step = (r.queries * p.group + ROWS - 1) / ROWS;
-        r.unit = uniform(first_unit<ROWS, KEYS>(p, cut, s));
-        tile = unit - (whole ? uniform(first_unit<ROWS, KEYS>(p, false, s)) : r.unit);
-        if (tile < 0 || r.step == 0) return false;
-        if (cut) {
-            const int64_t each = static_cast<int64_t>(p.cut.chunk) * KEYS * r.step;
-            parts = static_cast<int>(min((r.n + each - 1) / each, static_cast<int64_t>(parts)));
-            if (!whole) part = tile / r.step, tile -= part * r.step;
+        r.unit = uniform(first_unit<ROWS, KEYS>(p, s));
+        if (r.parts > 1) {
+            const int64_t each = static_cast<int64_t>(p.cut.chunk) * KEYS * max(r.step, 1);
+            r.parts = static_cast<int>(min((r.n + each - 1) / each, static_cast<int64_t>(r.parts)));
         }
     } else {
-        const int items = r.stacked ? 1 : p.seqs, s = unit % items;
+        const int items = r.stacked ? 1 : p.seqs;
         r.queries = r.stacked ? p.seqs * p.tq : p.tq;
-        const int tiles = (r.queries * p.group + ROWS - 1) / ROWS;
-        tile = unit / items;
-        if (!whole) part = tile / tiles, tile -= part * tiles;
-        r.step = items * tiles;
         r.n = r.stacked ? 0 : p.lengths ? min(max(uniform(p.lengths[s]), 0), p.tk) : p.tk;
         r.token = static_cast<int64_t>(s) * p.tq;
         r.q = reinterpret_cast<const char *>(p.q) + s * p.qbs + qh;
         r.k = reinterpret_cast<const char *>(p.k) + s * p.kbs + kh;
         r.v = reinterpret_cast<const char *>(p.v) + s * p.vbs + kh;
+        r.step = (r.queries * p.group + ROWS - 1) / ROWS * items;
         r.unit = s;
     }
     r.rows = r.queries * p.group;
+}
+
+// Row tile `tile` of the sequence: what it attends to, and its parts.
+template <int ROWS, int KEYS>
+__device__ __forceinline__ void take_tile(const Params &p, int tile, Tile &r)
+{
     r.first = tile * ROWS;
-    if (r.first >= r.rows) return false;
     r.unit += tile * (p.qo || r.stacked ? 1 : p.seqs);
     const int behind = r.n - r.queries;  // keys in front of the first query's
     const int last = min(r.first + ROWS, r.rows) - 1;
@@ -154,7 +164,35 @@ __device__ __forceinline__ bool find_tile(const Params &p, int unit, int kvh, bo
     r.from = p.window ? min(max(behind + r.first / p.group + 1 - p.window, 0), r.to) : 0;
     r.np = r.stacked || (p.keys == kBoth && (r.to || !p.causal)) ? (p.prefix + KEYS - 1) / KEYS : 0;
     r.tiles = r.np + (r.to - r.from + KEYS - 1) / KEYS;
-    r.parts = max(min(parts, p.qo ? r.tiles : (r.tiles + p.cut.chunk - 1) / p.cut.chunk), 1);
+    r.parts = max(min(r.parts, p.qo ? r.tiles : (r.tiles + p.cut.chunk - 1) / p.cut.chunk), 1);
+    r.each = r.tiles;
+    if (r.parts > 1) {
+        r.each = (r.tiles + r.parts - 1) / r.parts;
+        r.parts = (r.tiles + r.each - 1) / r.each;
+    }
+}
+
+// Unit `unit` of key head kvh: its tile and part, or false if there is none.
+template <int D, int ROWS, int KEYS>
+__device__ __forceinline__ bool find_tile(const Params &p, int unit, int kvh, Tile &r, int &part)
+{
+    int tile;
+    if (p.qo) {
+        const int s = sequence_of(p.seqs, unit, [&](int i) { return first_unit<ROWS, KEYS>(p, i); });
+        find_sequence<D, ROWS, KEYS>(p, s, kvh, r);
+        if (unit < r.unit || r.step == 0) return false;
+        tile = unit - r.unit;
+        part = p.cut.parts > 1 ? tile / r.step : 0;
+        tile -= part * r.step;
+    } else {
+        const int items = p.keys == kCommon ? 1 : p.seqs, x = unit / items;
+        find_sequence<D, ROWS, KEYS>(p, unit - x * items, kvh, r);
+        const int tiles = r.step / items;
+        part = x / tiles;
+        tile = x - part * tiles;
+    }
+    if (tile * ROWS >= r.rows) return false;
+    take_tile<ROWS, KEYS>(p, tile, r);
     return part < r.parts;
 }
 
@@ -361,11 +399,10 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
 
     int unit, kvh, part;
     Tile r;
-    if (!find_work(p, block, unit, kvh) || !find_tile<D, kRows, kKeys>(p, unit, kvh, false, r, part)) return;
+    if (!find_work(p, block, unit, kvh) || !find_tile<D, kRows, kKeys>(p, unit, kvh, r, part)) return;
     const bool joined = r.parts > 1 || p.joined;
     const int64_t place = part_rows(p, r, kvh, part, kRows);
-    const int t0 = static_cast<int>(static_cast<int64_t>(part) * r.tiles / r.parts);
-    const int n = static_cast<int>(static_cast<int64_t>(part + 1) * r.tiles / r.parts) - t0;
+    const int t0 = part * r.each, n = min(r.each, r.tiles - t0);
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int l32 = lane & 31, half = lane >> 5;
     const int first = r.first + wave * 32, last = r.rows - 1;
@@ -377,24 +414,41 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
 
     if (n == 0) return no_keys<D, kRows>(p, r, kvh, place, joined);
 
-    // Queries: lane l holds row l % 32, elements 16 s + 8 (l/32) .. + 7.
-    bf16x8 qf[KS];
-    {
-        const char *qp = query(p, r, own, D) + half * 16;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const bf16x8 *>(qp + s * 32);
-    }
+    // The keys (values) of tile g on their way into `dst`, a load instruction a call.
     auto load = [&](auto is_v, const u32x4 &rsrc, const Span &s, int c, const char *dst) __attribute__((always_inline)) {
         constexpr bool V = decltype(is_v)::value;
         const int at = wave * kLoads<D> + c, row = part_row<D>(c, wave, lane), pos = lane % (D / 8);
         const uint32_t off = __umul24(min(row, s.valid - 1), s.stride) + (V ? v_pos<D>(row, pos) : k_pos<D>(row, pos)) * 16;
         load_lds16(rsrc, lds_address(dst) + at * 1024, off, 0);
     };
-    {
-        const Span s = key_span<D, kKeys, false>(p, r, kvh, t0);
-        const u32x4 rs = buffer<D>(s);
+    Span ks = key_span<D, kKeys, false>(p, r, kvh, t0), vs = key_span<D, kKeys, true>(p, r, kvh, t0);
+    // on to tile g, or past the last one, where loads get nothing
+    auto next = [&](auto is_v, Span &s, int g) __attribute__((always_inline)) {
+        if (g == r.np) {
+            s = key_span<D, kKeys, decltype(is_v)::value>(p, r, kvh, g);
+        } else {
+            s.base += static_cast<uint64_t>(s.stride) * kKeys;
+            s.valid = min(kKeys, g < r.np ? p.prefix - g * kKeys : r.to - r.from - (g - r.np) * kKeys);
+        }
+    };
+    auto load_all = [&](auto is_v, Span &s, const char *dst) __attribute__((always_inline)) {
+        const u32x4 rsrc = buffer<D>(s);
 #pragma unroll
-        for (int c = 0; c < kLoads<D>; ++c) load(std::false_type{}, rs, s, c, k0);
+        for (int c = 0; c < kLoads<D>; ++c) load(is_v, rsrc, s, c, dst);
+    };
+    load_all(std::false_type{}, ks, k0);
+    if (n > 1) {
+        next(std::false_type{}, ks, t0 + 1);
+        load_all(std::false_type{}, ks, k1);
+    }
+    load_all(std::true_type{}, vs, v0);
+
+    // Queries: lane l holds row l % 32, elements 16 s + 8 (l/32) .. + 7.
+    bf16x8 qf[KS];
+    {
+        const char *qp = query(p, r, own, D) + half * 16;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const bf16x8 *>(qp + s * 32);
     }
 
     // LDS byte offsets of this lane's fragments.  K: row l % 32 (+ 32 u), chunk
@@ -413,11 +467,15 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
             v_off[m][e] = row * 2 * D + v_pos<D>(row, c) * 16 + (vi & 1) * 8;
         }
 
+    struct Scores {
+        f32x16 x[2];       // transposed: register i of x[u] is key 32 u + 8 (i/4) + 4 half + i % 4 of row l % 32
+    };
+    Scores sa, sb;         // of a tile whose weights are being made, and of the next
     f32x16 o[MT] = {};
-    f32x16 s[2];     // scores, transposed: register i of s[u] is key 32 u + 8 (i/4) + 4 half + i % 4 of row l % 32
-    u32x4 w[4];      // weights, two a register, in the order of the scores
-    float mx = 0.f;  // running maximum of the scaled scores (the same in lanes l and l ^ 32)
-    float sum = 0.f; // this lane's share of the weights' sum
+    u32x4 w[4];            // weights, two a register, in the order of the scores
+    float mx = -FLT_MAX;   // running maximum of the scaled scores (the same in lanes l and l ^ 32)
+    float fade = 1.f, scale2 = p.scale2;
+    float sum = 0.f;       // this lane's share of the weights' sum
 
     // Fragment i of a K tile (contraction step i / 2 of keys 32 (i%2) ..) and of a
     // V tile (keys 16 (i / MT) .., columns 32 (i % MT) ..).
@@ -431,34 +489,44 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
         const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4 *)(vt + v_off[m][1] + st * 32 * D));
         return cat(lo, hi);
     };
-    // Matrix phase: a run of the stream of products that a tile takes, the weights
-    // times V of the tile before (0 .. NV - 1), then its scores (NV .. NV + NK - 1),
-    // with the LDS fragments read ahead of them and `loads(j)` between them.
-    auto products = [&](auto from, auto to, const char *vp, const char *kc, auto loads)
-                        __attribute__((always_inline)) {
-        bf16x8 f[NV + NK];
-        auto frag = [&](int j) { f[j] = j < NV ? v_frag(vp, j) : k_frag(kc, j - NV); };
+    // Scores of a tile, `beside(j)` between the products.
+    auto scores = [&](const char *kt, Scores &s, auto beside) __attribute__((always_inline)) {
+        bf16x8 f[NK];
 #pragma unroll
-        for (int j = from; j < from + kAhead; ++j) frag(j);
+        for (int j = 0; j < kAhead; ++j) f[j] = k_frag(kt, j);
 #pragma unroll
-        for (int j = from; j < to; ++j) {
-            if (j + kAhead < to) frag(j + kAhead);
-            loads(j - from);
-            if (j < NV) {
-                o[j % MT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[j], __builtin_bit_cast(bf16x8, w[j / MT]),
-                                                                    o[j % MT], 0, 0, 0);
-            } else {
-                const int i = j - NV;
-                s[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[j], qf[i >> 1], i < 2 ? f32x16{} : s[i & 1], 0, 0, 0);
-            }
+        for (int j = 0; j < NK; ++j) {
+            if (j + kAhead < NK) f[j + kAhead] = k_frag(kt, j + kAhead);
+            s.x[j & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[j], qf[j >> 1], j < 2 ? f32x16{} : s.x[j & 1], 0, 0, 0);
+            beside(j);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    // Vector phase of tile i: its maximum, the rescale of what was summed so far
-    // if a row's maximum grew, its weights.
-    auto softmax = [&](int i) __attribute__((always_inline)) {
-        // keys that not all of the wave's rows see (or that are none) get weight zero
-        const int g = t0 + i, key = r.from + (g - r.np) * kKeys;
+    // The weights times the values.
+    auto values = [&](const char *vt, auto beside) __attribute__((always_inline)) {
+        bf16x8 f[NV];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) f[j] = v_frag(vt, j);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            if (j + kAhead < NV) f[j + kAhead] = v_frag(vt, j + kAhead);
+            o[j % MT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[j], __builtin_bit_cast(bf16x8, w[j / MT]), o[j % MT], 0, 0, 0);
+            beside(j);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // Weights 2 j and 2 j + 1 (of a lane's 32).
+    auto weigh = [&](const Scores &s, int j) __attribute__((always_inline)) {
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s.x[j >> 3][2 * (j & 7)], scale2, -mx));
+        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s.x[j >> 3][2 * (j & 7) + 1], scale2, -mx));
+        uint32_t xy = pack_bf16x2(x, y);
+        asm volatile("" : "+v"(xy));  // made here, beside the products
+        sum = add_pair(xy, sum);
+        w[j >> 2][j & 3] = xy;
+    };
+    // Keys of tile g that not all of the wave's rows see (or that are none) get weight zero.
+    auto mask = [&](Scores &s, int g) __attribute__((always_inline)) {
+        const int key = r.from + (g - r.np) * kKeys;
         const bool common = g < r.np;
         if (common ? p.prefix - g * kKeys < kKeys : key + kKeys > sure_hi || key < sure_lo) {
             const int hi = (common ? p.prefix - g * kKeys : own.hi - key) - 4 * half;
@@ -468,82 +536,90 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     const int j = 32 * u + 8 * (e >> 2) + (e & 3);
-                    if (j >= hi || j < lo) s[u][e] = -INFINITY;
+                    if (j >= hi || j < lo) s.x[u][e] = -INFINITY;
                 }
         }
-        float m4[4];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            m4[c] = s[c >> 1][8 * (c & 1)];
-#pragma unroll
-            for (int e = 1; e < 8; ++e) m4[c] = fmaxf(m4[c], s[c >> 1][8 * (c & 1) + e]);
-        }
-        const float m = pair_max(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]))) * p.scale2;
-        if (i == 0) {
-            mx = fmaxf(m, -FLT_MAX);  // finite, so that scores of -inf weigh zero
-        } else if (__any(m > mx)) {
-            const float nm = fmaxf(m, mx);
-            const float a = __builtin_amdgcn_exp2f(mx - nm);
-            mx = nm;
-            sum *= a;
-#pragma unroll
-            for (int c = 0; c < MT; ++c)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) o[c][e] *= a;
-        }
-        // Scores past kLarge round before the maximum is taken off, as it did: else the
-        // largest weight would be 2^(its rounding) instead of 1.  (Rows that saw no key yet
-        // have a maximum of -FLT_MAX.)
-        float scale2 = p.scale2;
-        if (__any(fabsf(mx) > kLarge)) {
+    };
+    // The reference of the weights after a tile, and what is left of the sums before it.
+    auto raise = [&](Scores &s, float m) __attribute__((always_inline)) {
+        m = pair_max(m) * p.scale2;
+        const float nm = m > mx + kLag ? m : mx;  // finite, so that scores of -inf weigh zero
+        fade = __builtin_amdgcn_exp2f(mx - nm);
+        mx = nm;
+        scale2 = p.scale2;
+        if (__any(fabsf(mx) > kHuge && mx != -FLT_MAX)) {
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) s[u][e] *= scale2;
+                for (int e = 0; e < 16; ++e) s.x[u][e] *= scale2;
             scale2 = 1.f;
         }
-        float add[2] = {};
+    };
+    auto rescale = [&]() __attribute__((always_inline)) {
+        if (!__any(fade != 1.f)) return;
+        sum *= fade;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j >> 3][2 * (j & 7)], scale2, -mx));
-            const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j >> 3][2 * (j & 7) + 1], scale2, -mx));
-            add[0] += x;
-            add[1] += y;
-            w[j >> 2][j & 3] = pack_bf16x2(x, y);
-        }
-        sum += add[0] + add[1];
+        for (int c = 0; c < MT; ++c)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[c][e] *= fade;
     };
 
-    // Tile i: kc holds its keys, vp the values of tile i - 1.  Its values and the
-    // next tile's keys (the last tile's once more after the last) load into the
-    // other buffers between the products.
-    using std::integral_constant;
-    auto tile = [&](int i, auto from, const char *kc, const char *vp, char *kn, char *vn)
+    // Tile i, whose scores sa and maximum are there: the scores of the next tile beside the
+    // weights of this one, then the values beside the next one's maximum.  kn holds the next
+    // tile's keys, vc this one's values; the keys after the next and the next values load
+    // into kc and vn.
+    auto tile = [&](int i, Scores &sc, Scores &sn, const char *kc, const char *kn, const char *vc, const char *vn)
                     __attribute__((always_inline)) {
-        constexpr int kEvery = from == 0 ? 3 : 2;
-        const Span ks = key_span<D, kKeys, false>(p, r, kvh, t0 + min(i + 1, n - 1));
-        const Span vs = key_span<D, kKeys, true>(p, r, kvh, t0 + i);
-        const u32x4 kr = buffer<D>(ks), vr = buffer<D>(vs);
-        products(from, integral_constant<int, NV + NK>{}, vp, kc, [&](int j) __attribute__((always_inline)) {
-            if (j % kEvery) return;
-            const int c = j / kEvery;
-            if (c < kLoads<D>)
-                load(std::true_type{}, vr, vs, c, vn);
-            else if (c < 2 * kLoads<D>)
-                load(std::false_type{}, kr, ks, c - kLoads<D>, kn);
+        rescale();
+        u32x4 kr = {};
+        if (i + 2 < n) {
+            next(std::false_type{}, ks, t0 + i + 2);
+            kr = buffer<D>(ks);
+        }
+        next(std::true_type{}, vs, t0 + i + 1);
+        const u32x4 vr = buffer<D>(vs);
+        scores(kn, sn, [&](int j) __attribute__((always_inline)) {
+            if (j < kLoads<D>) load(std::true_type{}, vr, vs, j, vn);
+            else if (j < 2 * kLoads<D>) load(std::false_type{}, kr, ks, j - kLoads<D>, kc);
+            if (NK >= 16) {
+                if (j % (NK / 16) == 0) weigh(sc, j / (NK / 16));
+            } else {
+                weigh(sc, 2 * j);
+                weigh(sc, 2 * j + 1);
+            }
         });
-        softmax(i);
-        __builtin_amdgcn_sched_barrier(0);
+        mask(sn, t0 + i + 1);
+        float m = -INFINITY;
+        values(vc, [&](int j) __attribute__((always_inline)) {
+#pragma unroll
+            for (int e = 0; e < 32 / NV; ++e) {
+                const int at = j * (32 / NV) + e;
+                m = fmaxf(m, sn.x[at >> 4][at & 15]);
+            }
+            asm volatile("" : "+v"(m));
+        });
+        raise(sn, m);
         tile_barrier();
     };
-    constexpr integral_constant<int, 0> whole;
     tile_barrier();
-    tile(0, integral_constant<int, NV>{}, k0, v1, k1, v0);
-    for (int i = 1; i < n; i += 2) {
-        tile(i, whole, k1, v0, k0, v1);
-        if (i + 1 < n) tile(i + 1, whole, k0, v1, k1, v0);
+    scores(k0, sa, [](int) {});
+    mask(sa, t0);
+    {
+        float m = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) m = fmaxf(m, sa.x[e >> 4][e & 15]);
+        raise(sa, m);
     }
-    products(whole, integral_constant<int, NV>{}, n & 1 ? v0 : v1, nullptr, [](int) {});
+    tile_barrier();
+    for (int i = 0; i + 1 < n; i += 2) {
+        tile(i, sa, sb, k0, k1, v0, v1);
+        if (i + 2 < n) tile(i + 1, sb, sa, k1, k0, v1, v0);
+        else sa = sb;
+    }
+    rescale();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) weigh(sa, j);
+    values(n & 1 ? v0 : v1, [](int) {});
 
     // Lane l: row l % 32, columns 32 m + 8 j + 4 half + (0..3) in registers 4 j ..
     const float total = pair_sum(sum);
@@ -637,11 +713,10 @@ __device__ __forceinline__ void attend_few(const Params &p, int block, FewLds<D>
 
     int unit, kvh, part;
     Tile r;
-    if (!find_work(p, block, unit, kvh) || !find_tile<D, kFewRows, KT>(p, unit, kvh, false, r, part)) return;
+    if (!find_work(p, block, unit, kvh) || !find_tile<D, kFewRows, KT>(p, unit, kvh, r, part)) return;
     const bool joined = r.parts > 1 || p.joined;
     const int64_t place = part_rows(p, r, kvh, part, kFewRows);
-    const int t0 = static_cast<int>(static_cast<int64_t>(part) * r.tiles / r.parts);
-    const int t1 = static_cast<int>(static_cast<int64_t>(part + 1) * r.tiles / r.parts);
+    const int t0 = part * r.each, t1 = min(t0 + r.each, r.tiles);
     if (t0 == t1) return no_keys<D, kFewRows>(p, r, kvh, place, joined);
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int l32 = lane & 31, half = lane >> 5;
@@ -660,7 +735,7 @@ __device__ __forceinline__ void attend_few(const Params &p, int block, FewLds<D>
         for (int c = 0; c < NL; ++c) {
             const int row = c * (1024 / (2 * D)) + lane / (D / 8), pos = lane % (D / 8);
             const uint32_t off = __umul24(min(row, s.valid - 1), s.stride) + (V ? v_pos<D>(row, pos) : k_pos<D>(row, pos)) * 16;
-            load_lds16(rsrc, to + c * 1024, off, 0);
+            load_lds16_stream(rsrc, to + c * 1024, off);
         }
     };
     int g = t0 + wave;
@@ -710,8 +785,8 @@ __device__ __forceinline__ void attend_few(const Params &p, int block, FewLds<D>
 #pragma unroll
             for (int e = 0; e < 16; ++e) m = fmaxf(m, s[u][e]);
         m = pair_max(m) * p.scale2;
-        if (__any(m > mx)) {
-            const float nm = fmaxf(m, mx), a = __builtin_amdgcn_exp2f(mx - nm);
+        if (__any(m > mx + kLag)) {
+            const float nm = m > mx + kLag ? m : mx, a = __builtin_amdgcn_exp2f(mx - nm);
             mx = nm;
             sum *= a;
 #pragma unroll
@@ -722,11 +797,11 @@ __device__ __forceinline__ void attend_few(const Params &p, int block, FewLds<D>
         u32x4 w[KU * 2];
 #pragma unroll
         for (int j = 0; j < KU * 8; ++j) {
-            // rounded before the maximum is taken off, as it was: the largest weight is 1
+            // (the scores round before the reference is taken off, as it did)
             const float x = __builtin_amdgcn_exp2f(s[j >> 3][2 * (j & 7)] * p.scale2 - mx);
             const float y = __builtin_amdgcn_exp2f(s[j >> 3][2 * (j & 7) + 1] * p.scale2 - mx);
-            sum += x + y;
             w[j >> 2][j & 3] = pack_bf16x2(x, y);
+            sum = add_pair(w[j >> 2][j & 3], sum);
         }
 
         if (more) wait_loads<NL>();  // the values are there
@@ -845,24 +920,28 @@ __global__ void __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) both_kernel(Bot
 // those of the items' own keys: a row a wave, whose lanes first have a part's maximum and sum
 // each, then 8 columns of every so many parts each.
 template <int D, int ROWS, int KEYS, int COMMON>
-__global__ void __launch_bounds__(256) join_kernel(Params p, Parts common, int groups)
+__global__ void __launch_bounds__(kWaves * 64) join_kernel(Params p, Parts common, int64_t rows)
 {
     constexpr int kLanes = D / 8, kBeside = 64 / kLanes;  // lanes of a part, and parts at a time
     const int lane = threadIdx.x & 63, c = lane % kLanes, g = lane / kLanes;
-    const int at = static_cast<int>(blockIdx.x) % groups * kWaves + uniform(threadIdx.x >> 6), tile = blockIdx.x / groups;
-    const int t = tile / p.kv_heads, kvh = tile - t * p.kv_heads;
-    int part;
+    const int64_t to = static_cast<int64_t>(blockIdx.x) * kWaves + uniform(threadIdx.x >> 6);  // this row of the output
+    if (to >= rows) return;
+    const int token = static_cast<int>(to / p.heads), head = static_cast<int>(to - static_cast<int64_t>(token) * p.heads);
+    const int kvh = head / p.group;
     Tile r;
-    if (!find_tile<D, ROWS, KEYS>(p, t, kvh, true, r, part)) return;
-    if ((r.parts == 1 && !p.joined) || r.first + at >= r.rows) return;  // the tile's only part has written the output
-    const Row w = find_row(p, r, r.first + at);
+    find_sequence<D, ROWS, KEYS>(p, p.qo ? sequence_of(p.seqs, token, [&](int i) { return p.qo[i]; }) : token / p.tq, kvh, r);
+    if (token < r.token || token >= r.token + r.queries) return;  // of no sequence
+    const int in = static_cast<int>(token - r.token) * p.group + head - kvh * p.group, at = in % ROWS;
+    take_tile<ROWS, KEYS>(p, in / ROWS, r);
+    if (r.parts == 1 && !p.joined) return;  // the tile's only part has written the output
+    const Row w = find_row(p, r, in);
     // the place of a row's first part, and how far it is to the next part's
     const int64_t u = part_rows(p, r, kvh, 0, ROWS) + at, step = static_cast<int64_t>(r.step) * p.kv_heads * ROWS;
     int64_t cu = 0, cstep = 0;
     if (COMMON) {
-        const int rows = p.seqs * p.tq * p.group, row = static_cast<int>(r.token + w.query) * p.group + w.member;
+        const int all = p.seqs * p.tq * p.group, row = token * p.group + w.member;
         cu = (static_cast<int64_t>(row / COMMON) * p.kv_heads + kvh) * COMMON + row % COMMON;
-        cstep = static_cast<int64_t>((rows + COMMON - 1) / COMMON) * p.kv_heads * COMMON;
+        cstep = static_cast<int64_t>((all + COMMON - 1) / COMMON) * p.kv_heads * COMMON;
     }
     const int commons = COMMON ? common.parts : 0, count = r.parts + commons;
     auto stat = [&](int k) {
@@ -901,8 +980,7 @@ __global__ void __launch_bounds__(256) join_kernel(Params p, Parts common, int g
     const float inv = 1.f / sum;
 #pragma unroll
     for (int e = 0; e < 8; ++e) acc[e] = any ? acc[e] * inv : 0.f;
-    if (g == 0)
-        *reinterpret_cast<u32x4 *>(p.out + ((r.token + w.query) * p.heads + kvh * p.group + w.member) * D + c * 8) = pack8v(acc);
+    if (g == 0) *reinterpret_cast<u32x4 *>(p.out + to * D + c * 8) = pack8v(acc);
 }
 
 constexpr int64_t kMost = 1 << 30;            // rows and keys: units and their rows are counted in int
@@ -919,7 +997,7 @@ struct Cut {
 
 Cut cut(int64_t rows, int64_t tiles, int64_t keys, bool packed, int64_t rounds, int64_t kv_heads, int64_t head_dim)
 {
-    Cut c;
+    Cut c{};
     c.rows = rows;
     c.few = rows == kFewRows;
     c.tiles = tiles;
@@ -948,7 +1026,7 @@ int64_t parts_bytes(const Cut &c, int64_t kv_heads, int64_t head_dim)
 struct Plan {
     bool shared;
     Cut own, common;
-    int64_t used, bytes;  // rows of an own tile at most, and the workspace's bytes
+    int64_t bytes;  // of the workspace
 };
 
 Plan plan_packed(int64_t tokens_q, int64_t tokens_k, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t head_dim)
@@ -956,7 +1034,6 @@ Plan plan_packed(int64_t tokens_q, int64_t tokens_k, int64_t sequences, int64_t 
     Plan c{};
     const int64_t rows = tokens_q * (heads / kv_heads), tile = rows <= kFewRows * sequences ? kFewRows : kRows;
     c.own = cut(tile, rows / tile + sequences, tokens_k, true, tile == kFewRows ? 4 : 1, kv_heads, head_dim);
-    c.used = tile;
     c.bytes = c.own.parts > 1 ? parts_bytes(c.own, kv_heads, head_dim) : 0;
     return c;
 }
@@ -968,7 +1045,6 @@ Plan plan_prefix(int64_t batch, int64_t tokens_q, int64_t tokens_k, int64_t pref
     const int64_t rows = tokens_q * (heads / kv_heads), tile = rows <= kFewRows ? kFewRows : kRows;
     c.shared = batch > 1 && rows < kRows && (batch - 1) * prefix * kv_heads * head_dim * 4 > kShared;
     c.own = cut(tile, (rows + tile - 1) / tile * batch, (c.shared ? 0 : prefix) + tokens_k, false, 1, kv_heads, head_dim);
-    c.used = rows < tile ? rows : tile;
     c.bytes = c.shared || c.own.parts > 1 ? parts_bytes(c.own, kv_heads, head_dim) : 0;
     if (c.shared) {
         const int64_t of_all = batch * rows <= kFewRows ? kFewRows : kRows;
@@ -993,11 +1069,11 @@ Parts place(const Cut &c, int64_t kv_heads, int64_t head_dim, void *workspace)
 template <int D, int ROWS, int KEYS>
 void join(const Params &p, const Plan &c, const Parts &common, hipStream_t s)
 {
-    const int groups = static_cast<int>((c.used + kWaves - 1) / kWaves);
-    const unsigned blocks = static_cast<unsigned>(c.own.tiles * p.kv_heads * groups);
-    if (!c.shared) join_kernel<D, ROWS, KEYS, 0><<<blocks, 256, 0, s>>>(p, common, groups);
-    else if (c.common.few) join_kernel<D, ROWS, KEYS, kFewRows><<<blocks, 256, 0, s>>>(p, common, groups);
-    else join_kernel<D, ROWS, KEYS, kRows><<<blocks, 256, 0, s>>>(p, common, groups);
+    const int64_t rows = static_cast<int64_t>(p.qo ? 1 : p.seqs) * p.tq * p.heads;
+    const unsigned blocks = static_cast<unsigned>((rows + kWaves - 1) / kWaves);
+    if (!c.shared) join_kernel<D, ROWS, KEYS, 0><<<blocks, kWaves * 64, 0, s>>>(p, common, rows);
+    else if (c.common.few) join_kernel<D, ROWS, KEYS, kFewRows><<<blocks, kWaves * 64, 0, s>>>(p, common, rows);
+    else join_kernel<D, ROWS, KEYS, kRows><<<blocks, kWaves * 64, 0, s>>>(p, common, rows);
 }
 
 template <int D>
@@ -1029,7 +1105,7 @@ int run(const char *what, Params &p, const Plan &c, int64_t head_dim, void *work
 {
     // a launch holds fewer than 2^32 threads
     const int64_t most = (int64_t{1} << 32) / (kWaves * 64);
-    if (c.own.blocks + c.common.blocks >= most || (c.bytes && c.own.tiles * p.kv_heads >= most / (c.used / kWaves + 1)))
+    if (c.own.blocks + c.common.blocks >= most || (c.bytes && (p.qo ? 1 : p.seqs) * static_cast<int64_t>(p.tq) * p.heads >= most * kWaves))
         return fail(LTXK_E_ARG, "%s: too many row tiles", what);
     if (c.bytes && (!workspace || !aligned16(workspace) || workspace_bytes < c.bytes))
         return fail(LTXK_E_ARG, "%s: the workspace must hold ltxk_%s_workspace_bytes, 16-byte aligned", what, what);

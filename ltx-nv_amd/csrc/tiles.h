@@ -25,6 +25,13 @@ __device__ __forceinline__ void load_lds16(const u32x4 &rsrc, uint32_t lds, uint
                  ::"s"(lds), "v"(off), "s"(rsrc), "s"(soff)
                  : "memory");
 }
+// The same of what is read once.
+__device__ __forceinline__ void load_lds16_stream(const u32x4 &rsrc, uint32_t lds, uint32_t off)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds"
+                 ::"s"(lds), "v"(off), "s"(rsrc)
+                 : "memory");
+}
 __device__ __forceinline__ void load_lds4(const u32x4 &rsrc, uint32_t lds, uint32_t off, uint32_t soff)
 {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, %3 offen lds"
