@@ -395,7 +395,7 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
     constexpr int MT = D / 32;               // output tiles
     constexpr int NK = 2 * KS, NV = 4 * MT;  // K and V fragments of a tile
     constexpr int kAhead = 4;                // fragments read ahead of the products
-    char *const k0 = lds.k0, *const k1 = lds.k1, *const v0 = lds.v0, *const v1 = lds.v1;
+    constexpr int kTileBytes = kKeys * D * 2;
 
     int unit, kvh, part;
     Tile r;
@@ -436,12 +436,12 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
 #pragma unroll
         for (int c = 0; c < kLoads<D>; ++c) load(is_v, rsrc, s, c, dst);
     };
-    load_all(std::false_type{}, ks, k0);
+    load_all(std::false_type{}, ks, lds.k0);
     if (n > 1) {
         next(std::false_type{}, ks, t0 + 1);
-        load_all(std::false_type{}, ks, k1);
+        load_all(std::false_type{}, ks, lds.k1);
     }
-    load_all(std::true_type{}, vs, v0);
+    load_all(std::true_type{}, vs, lds.v0);
 
     // Queries: lane l holds row l % 32, elements 16 s + 8 (l/32) .. + 7.
     bf16x8 qf[KS];
@@ -451,20 +451,22 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
         for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const bf16x8 *>(qp + s * 32);
     }
 
-    // LDS byte offsets of this lane's fragments.  K: row l % 32 (+ 32 u), chunk
-    // 2 s + half.  V (transposed reads of 4 keys x 16 columns by 16 lanes): rows
-    // 16 s + 8 e + 4 half + (l%16)/4, columns 32 m + 16 (l/16 % 2) + 4 (l % 4).
-    int k_off[KS], v_off[MT][2];
+    // LDS addresses of this lane's fragments in the first buffers.  K: row l % 32 (+ 32 u),
+    // chunk 2 s + half.  V (transposed reads of 4 keys x 16 columns by 16 lanes): rows
+    // 16 s + 8 e + 4 half + (l%16)/4, columns 32 m + 16 (l/16 % 2) + 4 (l % 4).  The chunks'
+    // permutations are over 16 of them: what is 256 bytes on in heads of 256 keeps its place.
+    constexpr int KO = KS < 8 ? KS : 8, VO = MT < 4 ? MT : 4;
+    uint32_t k_at[KO], v_at[VO][2];
 #pragma unroll
-    for (int s = 0; s < KS; ++s) k_off[s] = l32 * 2 * D + k_pos<D>(l32, 2 * s + half) * 16;
+    for (int s = 0; s < KO; ++s) k_at[s] = lds_address(lds.k0) + l32 * 2 * D + k_pos<D>(l32, 2 * s + half) * 16;
     const int vi = lane & 15;
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int m = 0; m < VO; ++m)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const int row = 8 * e + 4 * half + (vi >> 2);
             const int c = 4 * m + 2 * ((lane >> 4) & 1) + ((vi & 3) >> 1);
-            v_off[m][e] = row * 2 * D + v_pos<D>(row, c) * 16 + (vi & 1) * 8;
+            v_at[m][e] = lds_address(lds.v0) + row * 2 * D + v_pos<D>(row, c) * 16 + (vi & 1) * 8;
         }
 
     struct Scores {
@@ -478,38 +480,40 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
     float sum = 0.f;       // this lane's share of the weights' sum
 
     // Fragment i of a K tile (contraction step i / 2 of keys 32 (i%2) ..) and of a
-    // V tile (keys 16 (i / MT) .., columns 32 (i % MT) ..).
-    auto k_frag = [&](const char *kt, int i) {
-        return *reinterpret_cast<const bf16x8 *>(kt + k_off[i >> 1] + (i & 1) * 64 * D);
+    // V tile (keys 16 (i / MT) .., columns 32 (i % MT) ..), in the first or second buffer.
+    auto k_frag = [&](int buf, int i) {
+        typedef const __attribute__((address_space(3))) bf16x8 lds8;
+        const int st = i >> 1;
+        return *(lds8 *)(k_at[st % KO] + (buf * kTileBytes + (i & 1) * 64 * D + st / KO * 256));
     };
-    auto v_frag = [&](const char *vt, int i) {
+    auto v_frag = [&](int buf, int i) {
         typedef __attribute__((address_space(3))) bf16x4 lds4;
-        const int m = i % MT, st = i / MT;
-        const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4 *)(vt + v_off[m][0] + st * 32 * D));
-        const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4 *)(vt + v_off[m][1] + st * 32 * D));
+        const int m = i % MT, at = buf * kTileBytes + i / MT * 32 * D + m / VO * 256;
+        const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4 *)(v_at[m % VO][0] + at));
+        const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4 *)(v_at[m % VO][1] + at));
         return cat(lo, hi);
     };
     // Scores of a tile, `beside(j)` between the products.
-    auto scores = [&](const char *kt, Scores &s, auto beside) __attribute__((always_inline)) {
+    auto scores = [&](int buf, Scores &s, auto beside) __attribute__((always_inline)) {
         bf16x8 f[NK];
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) f[j] = k_frag(kt, j);
+        for (int j = 0; j < kAhead; ++j) f[j] = k_frag(buf, j);
 #pragma unroll
         for (int j = 0; j < NK; ++j) {
-            if (j + kAhead < NK) f[j + kAhead] = k_frag(kt, j + kAhead);
+            if (j + kAhead < NK) f[j + kAhead] = k_frag(buf, j + kAhead);
             s.x[j & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[j], qf[j >> 1], j < 2 ? f32x16{} : s.x[j & 1], 0, 0, 0);
             beside(j);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
     // The weights times the values.
-    auto values = [&](const char *vt, auto beside) __attribute__((always_inline)) {
+    auto values = [&](int buf, auto beside) __attribute__((always_inline)) {
         bf16x8 f[NV];
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) f[j] = v_frag(vt, j);
+        for (int j = 0; j < kAhead; ++j) f[j] = v_frag(buf, j);
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            if (j + kAhead < NV) f[j + kAhead] = v_frag(vt, j + kAhead);
+            if (j + kAhead < NV) f[j + kAhead] = v_frag(buf, j + kAhead);
             o[j % MT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[j], __builtin_bit_cast(bf16x8, w[j / MT]), o[j % MT], 0, 0, 0);
             beside(j);
             __builtin_amdgcn_sched_barrier(0);
@@ -565,11 +569,10 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
     };
 
     // Tile i, whose scores sa and maximum are there: the scores of the next tile beside the
-    // weights of this one, then the values beside the next one's maximum.  kn holds the next
-    // tile's keys, vc this one's values; the keys after the next and the next values load
-    // into kc and vn.
-    auto tile = [&](int i, Scores &sc, Scores &sn, const char *kc, const char *kn, const char *vc, const char *vn)
-                    __attribute__((always_inline)) {
+    // weights of this one, then the values beside the next one's maximum.  Buffer 1 - b holds the
+    // next tile's keys, b this one's values; the keys after the next and the next values load
+    // into the other two.
+    auto tile = [&](int i, auto b, Scores &sc, Scores &sn) __attribute__((always_inline)) {
         rescale();
         u32x4 kr = {};
         if (i + 2 < n) {
@@ -578,9 +581,9 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
         }
         next(std::true_type{}, vs, t0 + i + 1);
         const u32x4 vr = buffer<D>(vs);
-        scores(kn, sn, [&](int j) __attribute__((always_inline)) {
-            if (j < kLoads<D>) load(std::true_type{}, vr, vs, j, vn);
-            else if (j < 2 * kLoads<D>) load(std::false_type{}, kr, ks, j - kLoads<D>, kc);
+        scores(1 - b, sn, [&](int j) __attribute__((always_inline)) {
+            if (j < kLoads<D>) load(std::true_type{}, vr, vs, j, b ? lds.v0 : lds.v1);
+            else if (j < 2 * kLoads<D>) load(std::false_type{}, kr, ks, j - kLoads<D>, b ? lds.k1 : lds.k0);
             if (NK >= 16) {
                 if (j % (NK / 16) == 0) weigh(sc, j / (NK / 16));
             } else {
@@ -590,11 +593,11 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
         });
         mask(sn, t0 + i + 1);
         float m = -INFINITY;
-        values(vc, [&](int j) __attribute__((always_inline)) {
+        values(b, [&](int j) __attribute__((always_inline)) {
 #pragma unroll
             for (int e = 0; e < 32 / NV; ++e) {
                 const int at = j * (32 / NV) + e;
-                m = fmaxf(m, sn.x[at >> 4][at & 15]);
+                m = __builtin_elementwise_maximum(m, sn.x[at >> 4][at & 15]);
             }
             asm volatile("" : "+v"(m));
         });
@@ -602,24 +605,25 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
         tile_barrier();
     };
     tile_barrier();
-    scores(k0, sa, [](int) {});
+    scores(0, sa, [](int) {});
     mask(sa, t0);
     {
         float m = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < 32; ++e) m = fmaxf(m, sa.x[e >> 4][e & 15]);
+        for (int e = 0; e < 32; ++e) m = __builtin_elementwise_maximum(m, sa.x[e >> 4][e & 15]);
         raise(sa, m);
     }
     tile_barrier();
     for (int i = 0; i + 1 < n; i += 2) {
-        tile(i, sa, sb, k0, k1, v0, v1);
-        if (i + 2 < n) tile(i + 1, sb, sa, k1, k0, v1, v0);
+        tile(i, std::integral_constant<int, 0>{}, sa, sb);
+        if (i + 2 < n) tile(i + 1, std::integral_constant<int, 1>{}, sb, sa);
         else sa = sb;
     }
     rescale();
 #pragma unroll
     for (int j = 0; j < 16; ++j) weigh(sa, j);
-    values(n & 1 ? v0 : v1, [](int) {});
+    if (n & 1) values(0, [](int) {});
+    else values(1, [](int) {});
 
     // Lane l: row l % 32, columns 32 m + 8 j + 4 half + (0..3) in registers 4 j ..
     const float total = pair_sum(sum);
@@ -783,7 +787,7 @@ __device__ __forceinline__ void attend_few(const Params &p, int block, FewLds<D>
 #pragma unroll
         for (int u = 0; u < KU; ++u)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) m = fmaxf(m, s[u][e]);
+            for (int e = 0; e < 16; ++e) m = __builtin_elementwise_maximum(m, s[u][e]);
         m = pair_max(m) * p.scale2;
         if (__any(m > mx + kLag)) {
             const float nm = m > mx + kLag ? m : mx, a = __builtin_amdgcn_exp2f(mx - nm);
