@@ -16,7 +16,9 @@ namespace {
 // Rows (a query at one head of the group) of a tile: 32 a wave, which share its keys, or 32
 // that all waves attend with, each over keys of its own.
 constexpr int kRows = 32 * kWaves, kFewRows = 32;
-// Keys that a wave of the latter takes at a time.
+// Keys that the former take at a time, and a wave of the latter.
+template <int D>
+constexpr int kTileKeys = D == 256 ? 32 : 64;
 template <int D>
 constexpr int kFewKeys = D == 64 ? 64 : 32;
 
@@ -43,7 +45,8 @@ struct Parts {
     float *sums;          // each part's weighted sums of v (rows x D)
     float2 *stats;        // and each of its rows' maximum and sum of weights
     int units, slots;     // parts of all tiles of a key head (with some that are none), and places for them on an XCD
-    int parts, chunk;     // a tile's keys are cut into up to `parts`, of about `chunk` key tiles each
+    int parts, least;     // a tile's keys are cut into up to `parts`, of at least `least` key tiles each
+    int chunk;            // and of about `chunk` keys (packed: for each row tile of the sequence) each
 };
 
 struct Params {
@@ -88,14 +91,14 @@ struct Tile {
 };
 
 // Packed sequences: of a sequence with r row tiles and m keys, whose parts take about c r keys
-// (the more tiles the longer), all parts number r ceil(m / (c r)), at most floor(m / c) +
+// (the more tiles, the longer), all parts number r ceil(m / (c r)), at most floor(m / c) +
 // floor(rows / ROWS) + 1.  So unit floor(keys before / c) + floor(rows before / ROWS) + s is
 // behind the last one of the sequences before s, and known without their lengths.
-template <int ROWS, int KEYS>
+template <int ROWS>
 __device__ __forceinline__ int first_unit(const Params &p, int s)
 {
     const int64_t rows = static_cast<int64_t>(min(max(p.qo[s], 0), p.tq)) * p.group;
-    return static_cast<int>(rows / ROWS) + s + (p.cut.parts > 1 ? min(max(p.ko[s], 0), p.tk) / (p.cut.chunk * KEYS) : 0);
+    return static_cast<int>(rows / ROWS) + s + (p.cut.parts > 1 ? min(max(p.ko[s], 0), p.tk) / p.cut.chunk : 0);
 }
 
 // The last sequence whose first(s) is at most `x`, 64 of them at a time.
@@ -133,9 +136,9 @@ __device__ __forceinline__ void find_sequence(const Params &p, int s, int kvh, T
         r.k = reinterpret_cast<const char *>(p.k) + static_cast<int64_t>(k0) * p.kts + kh;
         r.v = reinterpret_cast<const char *>(p.v) + static_cast<int64_t>(k0) * p.vts + kh;
         r.step = (r.queries * p.group + ROWS - 1) / ROWS;
-        r.unit = uniform(first_unit<ROWS, KEYS>(p, s));
+        r.unit = uniform(first_unit<ROWS>(p, s));
         if (r.parts > 1) {
-            const int64_t each = static_cast<int64_t>(p.cut.chunk) * KEYS * max(r.step, 1);
+            const int64_t each = static_cast<int64_t>(p.cut.chunk) * max(r.step, 1);
             r.parts = static_cast<int>(min((r.n + each - 1) / each, static_cast<int64_t>(r.parts)));
         }
     } else {
@@ -152,6 +155,19 @@ __device__ __forceinline__ void find_sequence(const Params &p, int s, int kvh, T
     r.rows = r.queries * p.group;
 }
 
+// Into how many parts `tiles` key tiles are cut, of `each` but the last: `most`, if they are long enough.
+__device__ __forceinline__ int parts_of(const Parts &c, int most, int tiles, int &each)
+{
+    const int parts = max(min(most, tiles / c.least), 1);
+    each = (tiles + parts - 1) / parts;
+    return parts > 1 ? (tiles + each - 1) / each : 1;
+}
+template <int KEYS>
+__device__ __forceinline__ int batch_parts(const Parts &c, int tiles)
+{
+    return min(c.parts, (tiles * KEYS + c.chunk - 1) / c.chunk);
+}
+
 // Row tile `tile` of the sequence: what it attends to, and its parts.
 template <int ROWS, int KEYS>
 __device__ __forceinline__ void take_tile(const Params &p, int tile, Tile &r)
@@ -164,12 +180,7 @@ __device__ __forceinline__ void take_tile(const Params &p, int tile, Tile &r)
     r.from = p.window ? min(max(behind + r.first / p.group + 1 - p.window, 0), r.to) : 0;
     r.np = r.stacked || (p.keys == kBoth && (r.to || !p.causal)) ? (p.prefix + KEYS - 1) / KEYS : 0;
     r.tiles = r.np + (r.to - r.from + KEYS - 1) / KEYS;
-    r.parts = max(min(r.parts, p.qo ? r.tiles : (r.tiles + p.cut.chunk - 1) / p.cut.chunk), 1);
-    r.each = r.tiles;
-    if (r.parts > 1) {
-        r.each = (r.tiles + r.parts - 1) / r.parts;
-        r.parts = (r.tiles + r.each - 1) / r.each;
-    }
+    r.parts = parts_of(p.cut, p.qo ? r.parts : batch_parts<KEYS>(p.cut, r.tiles), r.tiles, r.each);
 }
 
 // Unit `unit` of key head kvh: its tile and part, or false if there is none.
@@ -178,7 +189,7 @@ __device__ __forceinline__ bool find_tile(const Params &p, int unit, int kvh, Ti
 {
     int tile;
     if (p.qo) {
-        const int s = sequence_of(p.seqs, unit, [&](int i) { return first_unit<ROWS, KEYS>(p, i); });
+        const int s = sequence_of(p.seqs, unit, [&](int i) { return first_unit<ROWS>(p, i); });
         find_sequence<D, ROWS, KEYS>(p, s, kvh, r);
         if (unit < r.unit || r.step == 0) return false;
         tile = unit - r.unit;
@@ -385,7 +396,8 @@ __device__ __forceinline__ uint32_t lds_address(const void *x)
 
 template <int D>
 struct TileLds {
-    char k0[kKeys * D * 2], k1[kKeys * D * 2], v0[kKeys * D * 2], v1[kKeys * D * 2];
+    static constexpr int kBytes = kTileKeys<D> * D * 2;
+    char k0[kBytes], k1[kBytes], v0[kBytes], v1[kBytes];
 };
 
 template <int D>
@@ -393,13 +405,14 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
 {
     constexpr int KS = D / 16;               // contraction steps of the scores
     constexpr int MT = D / 32;               // output tiles
-    constexpr int NK = 2 * KS, NV = 4 * MT;  // K and V fragments of a tile
-    constexpr int kAhead = 4;                // fragments read ahead of the products
-    constexpr int kTileBytes = kKeys * D * 2;
+    constexpr int KT = kTileKeys<D>, KU = KT / 32;
+    constexpr int NK = KU * KS, NV = KT / 16 * MT;  // K and V fragments of a tile
+    constexpr int kAhead = D == 256 ? 2 : 4;                // fragments read ahead of the products
+    constexpr int kTileBytes = KT * D * 2, kParts = kTileBytes / 1024 / kWaves;  // of a tile, and a wave's loads for it
 
     int unit, kvh, part;
     Tile r;
-    if (!find_work(p, block, unit, kvh) || !find_tile<D, kRows, kKeys>(p, unit, kvh, r, part)) return;
+    if (!find_work(p, block, unit, kvh) || !find_tile<D, kRows, KT>(p, unit, kvh, r, part)) return;
     const bool joined = r.parts > 1 || p.joined;
     const int64_t place = part_rows(p, r, kvh, part, kRows);
     const int t0 = part * r.each, n = min(r.each, r.tiles - t0);
@@ -417,31 +430,26 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
     // The keys (values) of tile g on their way into `dst`, a load instruction a call.
     auto load = [&](auto is_v, const u32x4 &rsrc, const Span &s, int c, const char *dst) __attribute__((always_inline)) {
         constexpr bool V = decltype(is_v)::value;
-        const int at = wave * kLoads<D> + c, row = part_row<D>(c, wave, lane), pos = lane % (D / 8);
+        const int at = wave * kParts + c, row = at * (1024 / (2 * D)) + lane / (D / 8), pos = lane % (D / 8);
         const uint32_t off = __umul24(min(row, s.valid - 1), s.stride) + (V ? v_pos<D>(row, pos) : k_pos<D>(row, pos)) * 16;
         load_lds16(rsrc, lds_address(dst) + at * 1024, off, 0);
     };
-    Span ks = key_span<D, kKeys, false>(p, r, kvh, t0), vs = key_span<D, kKeys, true>(p, r, kvh, t0);
+    Span ks = key_span<D, KT, false>(p, r, kvh, t0), vs = key_span<D, KT, true>(p, r, kvh, t0);
     // on to tile g, or past the last one, where loads get nothing
     auto next = [&](auto is_v, Span &s, int g) __attribute__((always_inline)) {
         if (g == r.np) {
-            s = key_span<D, kKeys, decltype(is_v)::value>(p, r, kvh, g);
+            s = key_span<D, KT, decltype(is_v)::value>(p, r, kvh, g);
         } else {
-            s.base += static_cast<uint64_t>(s.stride) * kKeys;
-            s.valid = min(kKeys, g < r.np ? p.prefix - g * kKeys : r.to - r.from - (g - r.np) * kKeys);
+            s.base += static_cast<uint64_t>(s.stride) * KT;
+            s.valid = min(KT, g < r.np ? p.prefix - g * KT : r.to - r.from - (g - r.np) * KT);
         }
     };
     auto load_all = [&](auto is_v, Span &s, const char *dst) __attribute__((always_inline)) {
         const u32x4 rsrc = buffer<D>(s);
 #pragma unroll
-        for (int c = 0; c < kLoads<D>; ++c) load(is_v, rsrc, s, c, dst);
+        for (int c = 0; c < kParts; ++c) load(is_v, rsrc, s, c, dst);
     };
     load_all(std::false_type{}, ks, lds.k0);
-    if (n > 1) {
-        next(std::false_type{}, ks, t0 + 1);
-        load_all(std::false_type{}, ks, lds.k1);
-    }
-    load_all(std::true_type{}, vs, lds.v0);
 
     // Queries: lane l holds row l % 32, elements 16 s + 8 (l/32) .. + 7.
     bf16x8 qf[KS];
@@ -455,13 +463,14 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
     // chunk 2 s + half.  V (transposed reads of 4 keys x 16 columns by 16 lanes): rows
     // 16 s + 8 e + 4 half + (l%16)/4, columns 32 m + 16 (l/16 % 2) + 4 (l % 4).  The chunks'
     // permutations are over 16 of them: what is 256 bytes on in heads of 256 keeps its place.
-    constexpr int KO = KS < 8 ? KS : 8, VO = MT < 4 ? MT : 4;
-    uint32_t k_at[KO], v_at[VO][2];
+    // (In heads of 256 the first chunk's address gives the others': registers are short.)
+    constexpr int KO = KS < 8 ? KS : 8, VO = MT < 4 ? MT : 4, KA = D == 256 ? 1 : KO, VA = D == 256 ? 1 : VO;
+    uint32_t k_at[KA], v_at[VA][2];
 #pragma unroll
-    for (int s = 0; s < KO; ++s) k_at[s] = lds_address(lds.k0) + l32 * 2 * D + k_pos<D>(l32, 2 * s + half) * 16;
+    for (int s = 0; s < KA; ++s) k_at[s] = lds_address(lds.k0) + l32 * 2 * D + k_pos<D>(l32, 2 * s + half) * 16;
     const int vi = lane & 15;
 #pragma unroll
-    for (int m = 0; m < VO; ++m)
+    for (int m = 0; m < VA; ++m)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const int row = 8 * e + 4 * half + (vi >> 2);
@@ -470,44 +479,41 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
         }
 
     struct Scores {
-        f32x16 x[2];       // transposed: register i of x[u] is key 32 u + 8 (i/4) + 4 half + i % 4 of row l % 32
+        f32x16 x[KU];      // transposed: register i of x[u] is key 32 u + 8 (i/4) + 4 half + i % 4 of row l % 32
     };
-    Scores sa, sb;         // of a tile whose weights are being made, and of the next
     f32x16 o[MT] = {};
-    u32x4 w[4];            // weights, two a register, in the order of the scores
+    u32x4 w[KT / 16];      // weights, two a register, in the order of the scores
     float mx = -FLT_MAX;   // running maximum of the scaled scores (the same in lanes l and l ^ 32)
     float fade = 1.f, scale2 = p.scale2;
     float sum = 0.f;       // this lane's share of the weights' sum
 
-    // Fragment i of a K tile (contraction step i / 2 of keys 32 (i%2) ..) and of a
+    // Fragment i of a K tile (contraction step i / KU of keys 32 (i % KU) ..) and of a
     // V tile (keys 16 (i / MT) .., columns 32 (i % MT) ..), in the first or second buffer.
     auto k_frag = [&](int buf, int i) {
         typedef const __attribute__((address_space(3))) bf16x8 lds8;
-        const int st = i >> 1;
-        return *(lds8 *)(k_at[st % KO] + (buf * kTileBytes + (i & 1) * 64 * D + st / KO * 256));
+        const int st = i / KU;
+        return *(lds8 *)((k_at[st % KA] ^ (KA == 1 ? st % KO * 32 : 0)) + (buf * kTileBytes + i % KU * 64 * D + st / KO * 256));
     };
     auto v_frag = [&](int buf, int i) {
         typedef __attribute__((address_space(3))) bf16x4 lds4;
-        const int m = i % MT, at = buf * kTileBytes + i / MT * 32 * D + m / VO * 256;
-        const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4 *)(v_at[m % VO][0] + at));
-        const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4 *)(v_at[m % VO][1] + at));
+        const int m = i % MT, x = VA == 1 ? m % VO * 64 : 0, at = buf * kTileBytes + i / MT * 32 * D + m / VO * 256;
+        const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4 *)((v_at[m % VA][0] ^ x) + at));
+        const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4 *)((v_at[m % VA][1] ^ x) + at));
         return cat(lo, hi);
     };
-    // Scores of a tile, `beside(j)` between the products.
-    auto scores = [&](int buf, Scores &s, auto beside) __attribute__((always_inline)) {
+    auto scores = [&](int buf, Scores &s) __attribute__((always_inline)) {
         bf16x8 f[NK];
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) f[j] = k_frag(buf, j);
 #pragma unroll
         for (int j = 0; j < NK; ++j) {
             if (j + kAhead < NK) f[j + kAhead] = k_frag(buf, j + kAhead);
-            s.x[j & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[j], qf[j >> 1], j < 2 ? f32x16{} : s.x[j & 1], 0, 0, 0);
-            beside(j);
+            s.x[j % KU] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[j], qf[j / KU], j < KU ? f32x16{} : s.x[j % KU], 0, 0, 0);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
     // The weights times the values.
-    auto values = [&](int buf, auto beside) __attribute__((always_inline)) {
+    auto values = [&](int buf) __attribute__((always_inline)) {
         bf16x8 f[NV];
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) f[j] = v_frag(buf, j);
@@ -515,28 +521,25 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
         for (int j = 0; j < NV; ++j) {
             if (j + kAhead < NV) f[j + kAhead] = v_frag(buf, j + kAhead);
             o[j % MT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[j], __builtin_bit_cast(bf16x8, w[j / MT]), o[j % MT], 0, 0, 0);
-            beside(j);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    // Weights 2 j and 2 j + 1 (of a lane's 32).
+    // Weights 2 j and 2 j + 1 of a lane's.
     auto weigh = [&](const Scores &s, int j) __attribute__((always_inline)) {
         const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s.x[j >> 3][2 * (j & 7)], scale2, -mx));
         const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s.x[j >> 3][2 * (j & 7) + 1], scale2, -mx));
-        uint32_t xy = pack_bf16x2(x, y);
-        asm volatile("" : "+v"(xy));  // made here, beside the products
-        sum = add_pair(xy, sum);
-        w[j >> 2][j & 3] = xy;
+        w[j >> 2][j & 3] = pack_bf16x2(x, y);
+        sum = add_pair(w[j >> 2][j & 3], sum);
     };
     // Keys of tile g that not all of the wave's rows see (or that are none) get weight zero.
     auto mask = [&](Scores &s, int g) __attribute__((always_inline)) {
-        const int key = r.from + (g - r.np) * kKeys;
+        const int key = r.from + (g - r.np) * KT;
         const bool common = g < r.np;
-        if (common ? p.prefix - g * kKeys < kKeys : key + kKeys > sure_hi || key < sure_lo) {
-            const int hi = (common ? p.prefix - g * kKeys : own.hi - key) - 4 * half;
+        if (common ? p.prefix - g * KT < KT : key + KT > sure_hi || key < sure_lo) {
+            const int hi = (common ? p.prefix - g * KT : own.hi - key) - 4 * half;
             const int lo = (common ? 0 : own.lo - key) - 4 * half;
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < KU; ++u)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     const int j = 32 * u + 8 * (e >> 2) + (e & 3);
@@ -545,7 +548,10 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
         }
     };
     // The reference of the weights after a tile, and what is left of the sums before it.
-    auto raise = [&](Scores &s, float m) __attribute__((always_inline)) {
+    auto raise = [&](Scores &s) __attribute__((always_inline)) {
+        float m = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 16 * KU; ++e) m = __builtin_elementwise_maximum(m, s.x[e >> 4][e & 15]);
         m = pair_max(m) * p.scale2;
         const float nm = m > mx + kLag ? m : mx;  // finite, so that scores of -inf weigh zero
         fade = __builtin_amdgcn_exp2f(mx - nm);
@@ -553,7 +559,7 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
         scale2 = p.scale2;
         if (__any(fabsf(mx) > kHuge && mx != -FLT_MAX)) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < KU; ++u)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s.x[u][e] *= scale2;
             scale2 = 1.f;
@@ -568,62 +574,41 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
             for (int e = 0; e < 16; ++e) o[c][e] *= fade;
     };
 
-    // Tile i, whose scores sa and maximum are there: the scores of the next tile beside the
-    // weights of this one, then the values beside the next one's maximum.  Buffer 1 - b holds the
-    // next tile's keys, b this one's values; the keys after the next and the next values load
-    // into the other two.
-    auto tile = [&](int i, auto b, Scores &sc, Scores &sn) __attribute__((always_inline)) {
-        rescale();
-        u32x4 kr = {};
-        if (i + 2 < n) {
-            next(std::false_type{}, ks, t0 + i + 2);
+    // Tile i, whose keys are in buffer b: the weights of the tile before times its values, then
+    // the scores; its values and the next tile's keys load into the other buffers meanwhile.
+    Scores s;
+    auto tile = [&](int i, auto b) __attribute__((always_inline)) {
+        u32x4 kr = {};  // (an empty buffer: the load gets nothing)
+        if (i + 1 < n) {
+            next(std::false_type{}, ks, t0 + i + 1);
             kr = buffer<D>(ks);
         }
-        next(std::true_type{}, vs, t0 + i + 1);
+        if (i) next(std::true_type{}, vs, t0 + i);
         const u32x4 vr = buffer<D>(vs);
-        scores(1 - b, sn, [&](int j) __attribute__((always_inline)) {
-            if (j < kLoads<D>) load(std::true_type{}, vr, vs, j, b ? lds.v0 : lds.v1);
-            else if (j < 2 * kLoads<D>) load(std::false_type{}, kr, ks, j - kLoads<D>, b ? lds.k1 : lds.k0);
-            if (NK >= 16) {
-                if (j % (NK / 16) == 0) weigh(sc, j / (NK / 16));
-            } else {
-                weigh(sc, 2 * j);
-                weigh(sc, 2 * j + 1);
-            }
-        });
-        mask(sn, t0 + i + 1);
-        float m = -INFINITY;
-        values(b, [&](int j) __attribute__((always_inline)) {
 #pragma unroll
-            for (int e = 0; e < 32 / NV; ++e) {
-                const int at = j * (32 / NV) + e;
-                m = __builtin_elementwise_maximum(m, sn.x[at >> 4][at & 15]);
-            }
-            asm volatile("" : "+v"(m));
-        });
-        raise(sn, m);
+        for (int c = 0; c < kParts; ++c) load(std::true_type{}, vr, vs, c, b ? lds.v1 : lds.v0);
+#pragma unroll
+        for (int c = 0; c < kParts; ++c) load(std::false_type{}, kr, ks, c, b ? lds.k0 : lds.k1);
+        if (D == 256) asm volatile("" : "+v"(k_at[0]), "+v"(v_at[0][0]), "+v"(v_at[0][1]));
+        if (i) values(1 - b);
+        scores(b, s);
+        mask(s, t0 + i);
+        raise(s);
+        rescale();
+#pragma unroll
+        for (int j = 0; j < 8 * KU; ++j) weigh(s, j);
         tile_barrier();
     };
     tile_barrier();
-    scores(0, sa, [](int) {});
-    mask(sa, t0);
-    {
-        float m = -INFINITY;
-#pragma unroll
-        for (int e = 0; e < 32; ++e) m = __builtin_elementwise_maximum(m, sa.x[e >> 4][e & 15]);
-        raise(sa, m);
+    for (int i = 0; i < n; i += 2) {
+        tile(i, std::integral_constant<int, 0>{});
+        if (i + 1 < n) tile(i + 1, std::integral_constant<int, 1>{});
     }
-    tile_barrier();
-    for (int i = 0; i + 1 < n; i += 2) {
-        tile(i, std::integral_constant<int, 0>{}, sa, sb);
-        if (i + 2 < n) tile(i + 1, std::integral_constant<int, 1>{}, sb, sa);
-        else sa = sb;
-    }
-    rescale();
+    if (!(n & 1)) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) weigh(sa, j);
-    if (n & 1) values(0, [](int) {});
-    else values(1, [](int) {});
+        for (int m = 0; m < VA; ++m) v_at[m][0] += kTileBytes, v_at[m][1] += kTileBytes;
+    }
+    values(0);
 
     // Lane l: row l % 32, columns 32 m + 8 j + 4 half + (0..3) in registers 4 j ..
     const float total = pair_sum(sum);
@@ -675,7 +660,7 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
         for (; again; again &= again - 1) {
             const int i = __builtin_ctz(again);
             if (first + i <= last)
-                again_row<D, kKeys>(p, r, kvh, first + i, t0, t0 + n, place + wave * 32 + i, joined);
+                again_row<D, KT>(p, r, kvh, first + i, t0, t0 + n, place + wave * 32 + i, joined);
         }
     }
 }
@@ -891,7 +876,7 @@ __device__ __forceinline__ void attend_few(const Params &p, int block, FewLds<D>
 
 // One kind of tile, or both for a prefix and the items' own keys, side by side.
 template <int D>
-__global__ void __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) tile_kernel(Params p)
+__global__ void __launch_bounds__(kWaves * 64, 2) tile_kernel(Params p)
 {
     __shared__ __attribute__((aligned(1024))) TileLds<D> lds;
     attend_tile<D>(p, blockIdx.x, lds);
@@ -942,12 +927,17 @@ __global__ void __launch_bounds__(kWaves * 64) join_kernel(Params p, Parts commo
     // the place of a row's first part, and how far it is to the next part's
     const int64_t u = part_rows(p, r, kvh, 0, ROWS) + at, step = static_cast<int64_t>(r.step) * p.kv_heads * ROWS;
     int64_t cu = 0, cstep = 0;
+    int commons = 0;
     if (COMMON) {
         const int all = p.seqs * p.tq * p.group, row = token * p.group + w.member;
         cu = (static_cast<int64_t>(row / COMMON) * p.kv_heads + kvh) * COMMON + row % COMMON;
         cstep = static_cast<int64_t>((all + COMMON - 1) / COMMON) * p.kv_heads * COMMON;
+        constexpr int CK = COMMON == kFewRows ? kFewKeys<D> : kTileKeys<D>;
+        const int tiles = (p.prefix + CK - 1) / CK;
+        int each;
+        commons = parts_of(common, batch_parts<CK>(common, tiles), tiles, each);
     }
-    const int commons = COMMON ? common.parts : 0, count = r.parts + commons;
+    const int count = r.parts + commons;
     auto stat = [&](int k) {
         return k < r.parts ? p.cut.stats[u + k * step] : k < count ? common.stats[cu + (k - r.parts) * cstep] : make_float2(-FLT_MAX, 0.f);
     };
@@ -991,29 +981,42 @@ constexpr int64_t kMost = 1 << 30;            // rows and keys: units and their 
 constexpr int64_t kShared = 8 << 20;          // bytes of prefix that are worth two launches more
 constexpr int64_t kStride = (1 << 23) - 8;    // elements of a token stride: its bytes are 24 bits
 
-// How the tiles of a launch are cut: where they are too few to fill the chip `rounds` times
-// over (two workgroups a compute unit, one with heads of 256), their keys into parts of at
-// least `least` key tiles.
+// How the tiles of a launch are cut: where they are too few to fill half of the chip `rounds`
+// times over (two workgroups a compute unit, one of few rows with heads of 256), their keys
+// into parts of at least kLeast.
+constexpr int64_t kLeast = 256;
+
 struct Cut {
     bool few;             // tiles of kFewRows rows
-    int64_t rows, tiles, units, parts, chunk, slots, blocks;
+    int64_t rows, units, parts, least, chunk, slots, blocks;
 };
 
-Cut cut(int64_t rows, int64_t tiles, int64_t keys, bool packed, int64_t rounds, int64_t kv_heads, int64_t head_dim)
+// `tiles` row tiles of a key head over up to `keys` keys each, or (sequences > 0) packed ones over
+// all of `keys` together.
+Cut cut(int64_t rows, int64_t tiles, int64_t keys, int64_t sequences, int64_t rounds, int64_t kv_heads, int64_t head_dim)
 {
     Cut c{};
     c.rows = rows;
     c.few = rows == kFewRows;
-    c.tiles = tiles;
-    const int64_t per = c.few && head_dim != 64 ? 32 : 64;  // keys of a key tile
-    const int64_t room = (head_dim == 256 ? 256 : 512) * rounds / kv_heads + 1, least = c.few ? 8 : 4;
-    // all key tiles of a key head's units (packed: of the sequences, their row tiles taking parts that are longer instead)
-    const int64_t of_all = ((packed ? keys : keys * tiles) + per - 1) / per;
-    c.chunk = (of_all + room - 1) / room;
-    if (c.chunk < least) c.chunk = least;
-    c.parts = ((keys + per - 1) / per + c.chunk - 1) / c.chunk;
-    if (c.parts < 1 || tiles * 2 > room) c.parts = 1;
-    c.units = packed ? tiles + (c.parts > 1 ? keys / (c.chunk * per) : 0) : tiles * c.parts;
+    const int64_t per = head_dim == 256 || (c.few && head_dim == 128) ? 32 : 64;  // keys of a key tile
+    const int64_t room = (head_dim == 256 && c.few ? 256 : 512) * rounds / kv_heads;
+    c.least = kLeast / per;
+    c.parts = 1;
+    c.chunk = keys > 0 ? keys : 1;
+    c.units = tiles;
+    if (tiles * 2 <= room && sequences) {
+        // (a sequence's row tiles take longer parts instead of more)
+        const int64_t each = (tiles + sequences - 1) / sequences, chunk = keys / (room - tiles) + 1;
+        c.chunk = chunk > kLeast / each ? chunk : kLeast / each + 1;
+        c.parts = (keys + c.chunk - 1) / c.chunk;
+        c.units = tiles + keys / c.chunk;
+    } else if (tiles * 2 <= room) {
+        c.chunk = keys * tiles / room / per * per + per;
+        if (c.chunk < kLeast) c.chunk = kLeast;
+        c.parts = (keys + per + c.chunk - 1) / c.chunk;
+        c.units = tiles * c.parts;
+    }
+    if (c.parts < 2) c.parts = 1, c.units = tiles;
     const int64_t low = kv_heads & -kv_heads, beside = low < 8 ? low : 8;
     c.slots = (c.units + 8 / beside - 1) / (8 / beside);
     c.blocks = 8 * c.slots * (kv_heads / beside);
@@ -1037,7 +1040,7 @@ Plan plan_packed(int64_t tokens_q, int64_t tokens_k, int64_t sequences, int64_t 
 {
     Plan c{};
     const int64_t rows = tokens_q * (heads / kv_heads), tile = rows <= kFewRows * sequences ? kFewRows : kRows;
-    c.own = cut(tile, rows / tile + sequences, tokens_k, true, tile == kFewRows ? 4 : 1, kv_heads, head_dim);
+    c.own = cut(tile, rows / tile + sequences, tokens_k, sequences, tile == kFewRows ? 4 : 1, kv_heads, head_dim);
     c.bytes = c.own.parts > 1 ? parts_bytes(c.own, kv_heads, head_dim) : 0;
     return c;
 }
@@ -1048,11 +1051,11 @@ Plan plan_prefix(int64_t batch, int64_t tokens_q, int64_t tokens_k, int64_t pref
     Plan c{};
     const int64_t rows = tokens_q * (heads / kv_heads), tile = rows <= kFewRows ? kFewRows : kRows;
     c.shared = batch > 1 && rows < kRows && (batch - 1) * prefix * kv_heads * head_dim * 4 > kShared;
-    c.own = cut(tile, (rows + tile - 1) / tile * batch, (c.shared ? 0 : prefix) + tokens_k, false, 1, kv_heads, head_dim);
+    c.own = cut(tile, (rows + tile - 1) / tile * batch, (c.shared ? 0 : prefix) + tokens_k, 0, 1, kv_heads, head_dim);
     c.bytes = c.shared || c.own.parts > 1 ? parts_bytes(c.own, kv_heads, head_dim) : 0;
     if (c.shared) {
         const int64_t of_all = batch * rows <= kFewRows ? kFewRows : kRows;
-        c.common = cut(of_all, (batch * rows + of_all - 1) / of_all, prefix, false, 1, kv_heads, head_dim);
+        c.common = cut(of_all, (batch * rows + of_all - 1) / of_all, prefix, 0, 1, kv_heads, head_dim);
         c.bytes += parts_bytes(c.common, kv_heads, head_dim);
     }
     return c;
@@ -1066,6 +1069,7 @@ Parts place(const Cut &c, int64_t kv_heads, int64_t head_dim, void *workspace)
     r.units = static_cast<int>(c.units);
     r.slots = static_cast<int>(c.slots);
     r.parts = static_cast<int>(c.parts);
+    r.least = static_cast<int>(c.least);
     r.chunk = static_cast<int>(c.chunk);
     return r;
 }
@@ -1101,7 +1105,7 @@ void launch(Params &p, const Plan &c, void *workspace, hipStream_t s)
     } else {
         tile_kernel<D><<<blocks, kWaves * 64, 0, s>>>(p);
     }
-    if (c.shared || c.own.parts > 1) c.own.few ? join<D, kFewRows, kFewKeys<D>>(p, c, common, s) : join<D, kRows, kKeys>(p, c, common, s);
+    if (c.shared || c.own.parts > 1) c.own.few ? join<D, kFewRows, kFewKeys<D>>(p, c, common, s) : join<D, kRows, kTileKeys<D>>(p, c, common, s);
 }
 
 // The launches, once the operands are checked and p holds them.

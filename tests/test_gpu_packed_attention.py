@@ -82,6 +82,23 @@ def test_masked_values_may_hold_anything(dh, mask):
         assert bool(got[queries[0] - 2:queries[0]].isnan().all())
 
 
+@pytest.mark.parametrize("dh", [64, 128, 256])
+@pytest.mark.parametrize("queries,heads", [([1, 1], 2), ([9, 40], 4), ([300], 2), ([1] * 30, 8)])
+def test_every_cut_of_the_keys(queries, heads, dh):
+    import ltxk
+
+    g = torch.Generator(device=DEV).manual_seed(heads)
+    q = _draw(g, sum(queries), heads * dh, 1.5)
+    for most in list(range(1, 2400, 157)) + list(range(2400, 9000, 601)):
+        keys = [most * (i + 1) // len(queries) for i in range(len(queries))]
+        k, v = _draw(g, sum(keys), 2 * dh), _draw(g, sum(keys), 2 * dh)
+        qo, ko = _offsets(queries), _offsets(keys)
+        got = ltxk.packed_attention(q, k, v, heads, qo, 2, ko)
+        for s in {0, len(queries) - 1}:
+            rows, at = slice(int(qo[s]), int(qo[s + 1])), slice(int(ko[s]), int(ko[s + 1]))
+            assert_near(got[rows], *one_sequence(q[rows], k[at], v[at], heads, 2), f"{most} keys, sequence {s}")
+
+
 def test_views_scale_and_equal_offsets():
     """Columns of one projection's rows, and lengths shared by queries and keys, give the same bits; a scale of its own."""
     import ltxk

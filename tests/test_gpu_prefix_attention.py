@@ -53,6 +53,21 @@ def test_matches_fp64(tq, prefix, room, lengths, heads, kv_heads, dh, causal):
     _check(got, q, k, v, pk, pv, lengths, heads, kv_heads, causal=causal)
 
 
+@pytest.mark.parametrize("dh", [64, 128, 256])
+@pytest.mark.parametrize("b,tq", [(2, 1), (40, 1), (12, 5), (3, 70)])
+def test_every_cut_of_a_prefix(b, tq, dh):
+    """Prefixes of every number of key tiles, last tiles of every length, cut into parts of every size."""
+    import ltxk
+
+    g = torch.Generator(device=DEV).manual_seed(b)
+    pk, pv = _draw(g, 9000, 2 * dh), _draw(g, 9000, 2 * dh)
+    q, k, v = _draw(g, b, tq, 4 * dh, scale=1.5), _draw(g, b, 80, 2 * dh), _draw(g, b, 80, 2 * dh)
+    lengths = [80, 79] + [70 + i % 9 for i in range(b - 2)]
+    for prefix in list(range(1, 2400, 157)) + list(range(2400, 9000, 601)):
+        got = ltxk.prefix_attention(q, k, v, pk[:prefix], pv[:prefix], 4, 2, _ints(lengths))
+        _check(got[-2:], q[-2:], k[-2:], v[-2:], pk[:prefix], pv[:prefix], lengths[-2:], 4, 2)
+
+
 @pytest.mark.parametrize("tq,prefix", [(4, 200), (4, 9000), (150, 200)])
 def test_masked_values_may_hold_anything(tq, prefix):
     import ltxk
