@@ -612,12 +612,12 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
 
     // Lane l: row l % 32, columns 32 m + 8 j + 4 half + (0..3) in registers 4 j ..
     const float total = pair_sum(sum);
-    bool fine = true;
+    float size = 0.f;
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) fine = fine && fabsf(o[m][e]) <= FLT_MAX;
-    const uint64_t odd = __ballot(!fine);
+        for (int e = 0; e < 16; ++e) size = __builtin_elementwise_maximum(size, fabsf(o[m][e]));  // (NaN stays NaN)
+    const uint64_t odd = __ballot(!(size <= FLT_MAX));
     uint32_t again = static_cast<uint32_t>(odd) | static_cast<uint32_t>(odd >> 32);  // rows to be done once more
     if (joined) {
         const int64_t u = place + wave * 32 + l32;
@@ -631,7 +631,7 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
                         f32x4{o[m][4 * c], o[m][4 * c + 1], o[m][4 * c + 2], o[m][4 * c + 3]};
         }
     } else {
-        const float inv = 1.f / total;
+        const float inv = own.any ? 1.f / total : 0.f;
         // stored as 64 bytes of 16 rows each
         const int64_t at0 = __shfl(at, lane & 15, 64), at1 = __shfl(at, (lane & 15) + 16, 64);
         const int col = 8 * half + (lane & 16);
@@ -642,7 +642,7 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
             for (int c = 0; c < 4; ++c) {
                 float f[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) f[e] = own.any ? o[m][4 * c + e] * inv : 0.f;
+                for (int e = 0; e < 4; ++e) f[e] = o[m][4 * c + e] * inv;
                 v[c][0] = pack_bf16x2(f[0], f[1]);
                 v[c][1] = pack_bf16x2(f[2], f[3]);
             }
