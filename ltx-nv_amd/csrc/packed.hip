@@ -347,10 +347,10 @@ __device__ __forceinline__ int64_t part_rows(const Params &p, const Tile &r, int
 }
 
 // A tile without any key: its rows weigh nothing, or are zero.
-template <int D, int ROWS>
+template <int D, int ROWS, int WAVES>
 __device__ __forceinline__ void no_keys(const Params &p, const Tile &r, int kvh, int64_t u, bool joined)
 {
-    for (int i = threadIdx.x; i < ROWS * (D / 8); i += kWaves * 64) {
+    for (int i = threadIdx.x; i < ROWS * (D / 8); i += WAVES * 64) {
         const int at = i / (D / 8), c = i % (D / 8);
         if (r.first + at >= r.rows) break;
         const Row w = find_row(p, r, r.first + at);
@@ -394,20 +394,44 @@ __device__ __forceinline__ uint32_t lds_address(const void *x)
     return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char *)x));
 }
 
-template <int D>
+// At most N loads of this wave in flight; nothing moves over it.
+template <int N>
+__device__ __forceinline__ void wait_loads()
+{
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | (N >> 4 << 14));
+    asm volatile("" ::: "memory");
+}
+// This wave's LDS reads have returned; nothing moves over it.
+__device__ __forceinline__ void wait_lds()
+{
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+    asm volatile("" ::: "memory");
+}
+
+template <int D, int GROUPS>
 struct TileLds {
     static constexpr int kBytes = kTileKeys<D> * D * 2;
-    char k0[kBytes], k1[kBytes], v0[kBytes], v1[kBytes];
+    union {
+        struct {
+            char k0[kBytes], k1[kBytes], v0[kBytes], v1[kBytes];
+        } of[GROUPS];
+        float sums[GROUPS == 1 ? 1 : kRows * D];
+    };
+    float2 stats[GROUPS == 1 ? 1 : kRows];
 };
 
-template <int D>
-__device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<D> &lds)
+// A tile of kRows rows by GROUPS times four waves: each group takes every so many key tiles,
+// through LDS of its own, and their sums are added up in the end.
+template <int D, int GROUPS>
+__device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<D, GROUPS> &whole)
 {
     constexpr int KS = D / 16;               // contraction steps of the scores
     constexpr int MT = D / 32;               // output tiles
     constexpr int KT = kTileKeys<D>, KU = KT / 32;
     constexpr int NK = KU * KS, NV = KT / 16 * MT;  // K and V fragments of a tile
-    constexpr int kAhead = D == 256 ? 2 : 4;                // fragments read ahead of the products
+    constexpr int kAhead = D == 256 ? 2 : 4;        // fragments read ahead of the products
     constexpr int kTileBytes = KT * D * 2, kParts = kTileBytes / 1024 / kWaves;  // of a tile, and a wave's loads for it
 
     int unit, kvh, part;
@@ -415,8 +439,10 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
     if (!find_work(p, block, unit, kvh) || !find_tile<D, kRows, KT>(p, unit, kvh, r, part)) return;
     const bool joined = r.parts > 1 || p.joined;
     const int64_t place = part_rows(p, r, kvh, part, kRows);
-    const int t0 = part * r.each, n = min(r.each, r.tiles - t0);
-    const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int t0 = part * r.each, all = min(r.each, r.tiles - t0);
+    const int any = uniform(threadIdx.x >> 6), group = GROUPS == 1 ? 0 : any / kWaves, wave = GROUPS == 1 ? any : any % kWaves;
+    const int lane = threadIdx.x & 63, n = (all - group + GROUPS - 1) / GROUPS;  // the group's tiles
+    auto &lds = whole.of[group];
     const int l32 = lane & 31, half = lane >> 5;
     const int first = r.first + wave * 32, last = r.rows - 1;
     const Row own = find_row(p, r, min(first + l32, last));
@@ -425,7 +451,7 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
     const int sure_hi = uniform(own.hi), sure_lo = __builtin_amdgcn_readlane(own.lo, 31);
     uint16_t *const out = p.out;
 
-    if (n == 0) return no_keys<D, kRows>(p, r, kvh, place, joined);
+    if (all == 0) return no_keys<D, kRows, GROUPS * kWaves>(p, r, kvh, place, joined);
 
     // The keys (values) of tile g on their way into `dst`, a load instruction a call.
     auto load = [&](auto is_v, const u32x4 &rsrc, const Span &s, int c, const char *dst) __attribute__((always_inline)) {
@@ -434,10 +460,11 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
         const uint32_t off = __umul24(min(row, s.valid - 1), s.stride) + (V ? v_pos<D>(row, pos) : k_pos<D>(row, pos)) * 16;
         load_lds16(rsrc, lds_address(dst) + at * 1024, off, 0);
     };
-    Span ks = key_span<D, KT, false>(p, r, kvh, t0), vs = key_span<D, KT, true>(p, r, kvh, t0);
-    // on to tile g, or past the last one, where loads get nothing
-    auto next = [&](auto is_v, Span &s, int g) __attribute__((always_inline)) {
-        if (g == r.np) {
+    Span ks = key_span<D, KT, false>(p, r, kvh, t0 + min(group, all - 1)), vs = key_span<D, KT, true>(p, r, kvh, t0 + min(group, all - 1));
+    // on to the group's tile i
+    auto next = [&](auto is_v, Span &s, int i) __attribute__((always_inline)) {
+        const int g = t0 + group + i * GROUPS;
+        if (GROUPS > 1 || g == r.np) {
             s = key_span<D, KT, decltype(is_v)::value>(p, r, kvh, g);
         } else {
             s.base += static_cast<uint64_t>(s.stride) * KT;
@@ -449,7 +476,7 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
 #pragma unroll
         for (int c = 0; c < kParts; ++c) load(is_v, rsrc, s, c, dst);
     };
-    load_all(std::false_type{}, ks, lds.k0);
+    if (n) load_all(std::false_type{}, ks, lds.k0);
 
     // Queries: lane l holds row l % 32, elements 16 s + 8 (l/32) .. + 7.
     bf16x8 qf[KS];
@@ -580,10 +607,10 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
     auto tile = [&](int i, auto b) __attribute__((always_inline)) {
         u32x4 kr = {};  // (an empty buffer: the load gets nothing)
         if (i + 1 < n) {
-            next(std::false_type{}, ks, t0 + i + 1);
+            next(std::false_type{}, ks, i + 1);
             kr = buffer<D>(ks);
         }
-        if (i) next(std::true_type{}, vs, t0 + i);
+        if (i) next(std::true_type{}, vs, i);
         const u32x4 vr = buffer<D>(vs);
 #pragma unroll
         for (int c = 0; c < kParts; ++c) load(std::true_type{}, vr, vs, c, b ? lds.v1 : lds.v0);
@@ -592,26 +619,58 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
         if (D == 256) asm volatile("" : "+v"(k_at[0]), "+v"(v_at[0][0]), "+v"(v_at[0][1]));
         if (i) values(1 - b);
         scores(b, s);
-        mask(s, t0 + i);
+        mask(s, t0 + group + i * GROUPS);
         raise(s);
         rescale();
 #pragma unroll
         for (int j = 0; j < 8 * KU; ++j) weigh(s, j);
-        tile_barrier();
     };
     tile_barrier();
-    for (int i = 0; i < n; i += 2) {
-        tile(i, std::integral_constant<int, 0>{});
-        if (i + 1 < n) tile(i + 1, std::integral_constant<int, 1>{});
+    const int turns = (all + GROUPS - 1) / GROUPS;  // as many barriers for each group
+    for (int i = 0; i < turns; i += 2) {
+        if (GROUPS == 1 || i < n) tile(i, std::integral_constant<int, 0>{});
+        tile_barrier();
+        if (i + 1 < turns) {
+            if (GROUPS == 1 || i + 1 < n) tile(i + 1, std::integral_constant<int, 1>{});
+            tile_barrier();
+        }
     }
     if (!(n & 1)) {
 #pragma unroll
         for (int m = 0; m < VA; ++m) v_at[m][0] += kTileBytes, v_at[m][1] += kTileBytes;
     }
-    values(0);
+    if (GROUPS == 1 || n) values(0);
 
     // Lane l: row l % 32, columns 32 m + 8 j + 4 half + (0..3) in registers 4 j ..
-    const float total = pair_sum(sum);
+    float total = pair_sum(sum);
+    if constexpr (GROUPS > 1) {
+        // The second group's sums on the first one's: 16-byte chunks of a row permuted by the row.
+        tile_barrier();
+        const int at = wave * 32 + l32;
+        f32x4 *const row = reinterpret_cast<f32x4 *>(whole.sums + at * D);
+        if (group) {
+            if (half == 0) whole.stats[at] = make_float2(mx, total);
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    row[(8 * m + 2 * c + half) ^ (l32 & (D / 4 - 1))] = f32x4{o[m][4 * c], o[m][4 * c + 1], o[m][4 * c + 2], o[m][4 * c + 3]};
+        }
+        tile_barrier();
+        if (group) return;
+        const float2 other = whole.stats[at];
+        const float top = fmaxf(mx, other.x), f = __builtin_amdgcn_exp2f(mx - top), g = __builtin_amdgcn_exp2f(other.x - top);
+        mx = top;
+        total = total * f + other.y * g;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const f32x4 x = row[(8 * m + 2 * c + half) ^ (l32 & (D / 4 - 1))];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[m][4 * c + e] = __builtin_fmaf(x[e], g, o[m][4 * c + e] * f);
+            }
+    }
     float size = 0.f;
 #pragma unroll
     for (int m = 0; m < MT; ++m)
@@ -660,25 +719,9 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
         for (; again; again &= again - 1) {
             const int i = __builtin_ctz(again);
             if (first + i <= last)
-                again_row<D, KT>(p, r, kvh, first + i, t0, t0 + n, place + wave * 32 + i, joined);
+                again_row<D, KT>(p, r, kvh, first + i, t0, t0 + all, place + wave * 32 + i, joined);
         }
     }
-}
-
-// At most N loads of this wave in flight; nothing moves over it.
-template <int N>
-__device__ __forceinline__ void wait_loads()
-{
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | (N >> 4 << 14));
-    asm volatile("" ::: "memory");
-}
-// This wave's LDS reads have returned; nothing moves over it.
-__device__ __forceinline__ void wait_lds()
-{
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0xc07f);
-    asm volatile("" ::: "memory");
 }
 
 // Few rows: each wave takes every fourth tile of kFewKeys keys, through LDS of its own and
@@ -706,7 +749,7 @@ __device__ __forceinline__ void attend_few(const Params &p, int block, FewLds<D>
     const bool joined = r.parts > 1 || p.joined;
     const int64_t place = part_rows(p, r, kvh, part, kFewRows);
     const int t0 = part * r.each, t1 = min(t0 + r.each, r.tiles);
-    if (t0 == t1) return no_keys<D, kFewRows>(p, r, kvh, place, joined);
+    if (t0 == t1) return no_keys<D, kFewRows, kWaves>(p, r, kvh, place, joined);
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int l32 = lane & 31, half = lane >> 5;
     const int rows = min(kFewRows, r.rows - r.first);
@@ -875,11 +918,11 @@ __device__ __forceinline__ void attend_few(const Params &p, int block, FewLds<D>
 }
 
 // One kind of tile, or both for a prefix and the items' own keys, side by side.
-template <int D>
-__global__ void __launch_bounds__(kWaves * 64, 2) tile_kernel(Params p)
+template <int D, int GROUPS>
+__global__ void __launch_bounds__(GROUPS * kWaves * 64, 2) tile_kernel(Params p)
 {
-    __shared__ __attribute__((aligned(1024))) TileLds<D> lds;
-    attend_tile<D>(p, blockIdx.x, lds);
+    __shared__ __attribute__((aligned(1024))) TileLds<D, GROUPS> lds;
+    attend_tile<D, GROUPS>(p, blockIdx.x, lds);
 }
 template <int D>
 __global__ void __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) few_kernel(Params p)
@@ -895,14 +938,14 @@ template <int D>
 __global__ void __launch_bounds__(kWaves * 64, D == 256 ? 1 : 2) both_kernel(BothParams both)
 {
     __shared__ __attribute__((aligned(1024))) union {
-        TileLds<D> tile;
+        TileLds<D, 1> tile;
         FewLds<D> few;
     } lds;
     const int i = static_cast<int>(blockIdx.x) < both.commons ? 0 : 1;
     const Params &p = both.p[i];
     const int block = blockIdx.x - i * both.commons;
     if (p.few) attend_few<D>(p, block, lds.few);
-    else attend_tile<D>(p, block, lds.tile);
+    else attend_tile<D, 1>(p, block, lds.tile);
 }
 
 // Joins the parts of the cut tiles, and of a prefix's (`common`, tiles of COMMON rows) with
@@ -984,7 +1027,7 @@ constexpr int64_t kStride = (1 << 23) - 8;    // elements of a token stride: its
 // How the tiles of a launch are cut: where they are too few to fill half of the chip `rounds`
 // times over (two workgroups a compute unit, one of few rows with heads of 256), their keys
 // into parts of at least kLeast.
-constexpr int64_t kLeast = 256;
+constexpr int64_t kLeast = 256, kWorth = 768;
 
 struct Cut {
     bool few;             // tiles of kFewRows rows
@@ -999,18 +1042,19 @@ Cut cut(int64_t rows, int64_t tiles, int64_t keys, int64_t sequences, int64_t ro
     c.rows = rows;
     c.few = rows == kFewRows;
     const int64_t per = head_dim == 256 || (c.few && head_dim == 128) ? 32 : 64;  // keys of a key tile
-    const int64_t room = (head_dim == 256 && c.few ? 256 : 512) * rounds / kv_heads;
+    const int64_t room = (c.few && head_dim != 256 ? 512 : 256) * rounds / kv_heads;
     c.least = kLeast / per;
     c.parts = 1;
     c.chunk = keys > 0 ? keys : 1;
     c.units = tiles;
-    if (tiles * 2 <= room && sequences) {
+    if (tiles * 2 > room || keys < (sequences ? sequences : 1) * kWorth) {
+    } else if (sequences) {
         // (a sequence's row tiles take longer parts instead of more)
         const int64_t each = (tiles + sequences - 1) / sequences, chunk = keys / (room - tiles) + 1;
         c.chunk = chunk > kLeast / each ? chunk : kLeast / each + 1;
         c.parts = (keys + c.chunk - 1) / c.chunk;
         c.units = tiles + keys / c.chunk;
-    } else if (tiles * 2 <= room) {
+    } else {
         c.chunk = keys * tiles / room / per * per + per;
         if (c.chunk < kLeast) c.chunk = kLeast;
         c.parts = (keys + per + c.chunk - 1) / c.chunk;
@@ -1102,8 +1146,10 @@ void launch(Params &p, const Plan &c, void *workspace, hipStream_t s)
         both_kernel<D><<<commons + blocks, kWaves * 64, 0, s>>>(BothParams{{all, p}, static_cast<int>(commons)});
     } else if (c.own.few) {
         few_kernel<D><<<blocks, kWaves * 64, 0, s>>>(p);
+    } else if (c.own.units * p.kv_heads <= 256) {
+        tile_kernel<D, 2><<<blocks, 2 * kWaves * 64, 0, s>>>(p);
     } else {
-        tile_kernel<D><<<blocks, kWaves * 64, 0, s>>>(p);
+        tile_kernel<D, 1><<<blocks, kWaves * 64, 0, s>>>(p);
     }
     if (c.shared || c.own.parts > 1) c.own.few ? join<D, kFewRows, kFewKeys<D>>(p, c, common, s) : join<D, kRows, kTileKeys<D>>(p, c, common, s);
 }
