@@ -817,8 +817,8 @@ __device__ __forceinline__ void attend_few(const Params &p, int block, FewLds<D>
 #pragma unroll
             for (int e = 0; e < 16; ++e) m = __builtin_elementwise_maximum(m, s[u][e]);
         m = pair_max(m) * p.scale2;
-        if (__any(m > mx + kLag)) {
-            const float nm = m > mx + kLag ? m : mx, a = __builtin_amdgcn_exp2f(mx - nm);
+        if (__any(m > mx)) {
+            const float nm = m > mx ? m : mx, a = __builtin_amdgcn_exp2f(mx - nm);
             mx = nm;
             sum *= a;
 #pragma unroll
@@ -966,6 +966,7 @@ __global__ void __launch_bounds__(kWaves * 64) join_kernel(Params p, Parts commo
     const int in = static_cast<int>(token - r.token) * p.group + head - kvh * p.group, at = in % ROWS;
     take_tile<ROWS, KEYS>(p, in / ROWS, r);
     if (r.parts == 1 && !p.joined) return;  // the tile's only part has written the output
+    if (r.unit + (r.parts - 1) * r.step >= p.cut.units) return;  // (offsets that do not ascend)
     const Row w = find_row(p, r, in);
     // the place of a row's first part, and how far it is to the next part's
     const int64_t u = part_rows(p, r, kvh, 0, ROWS) + at, step = static_cast<int64_t>(r.step) * p.kv_heads * ROWS;
@@ -1020,14 +1021,15 @@ __global__ void __launch_bounds__(kWaves * 64) join_kernel(Params p, Parts commo
     if (g == 0) *reinterpret_cast<u32x4 *>(p.out + to * D + c * 8) = pack8v(acc);
 }
 
-constexpr int64_t kMost = 1 << 30;            // rows and keys: units and their rows are counted in int
-constexpr int64_t kShared = 8 << 20;          // bytes of prefix that are worth two launches more
+constexpr int64_t kMost = 1 << 29;            // rows and keys, which are counted in int (a prefix's and own keys together)
+constexpr int64_t kShared = 96 << 20;         // bytes of prefix not read again that are worth their sums and a second launch
 constexpr int64_t kStride = (1 << 23) - 8;    // elements of a token stride: its bytes are 24 bits
 
-// How the tiles of a launch are cut: where they are too few to fill half of the chip `rounds`
-// times over (two workgroups a compute unit, one of few rows with heads of 256), their keys
-// into parts of at least kLeast.
-constexpr int64_t kLeast = 256, kWorth = 768;
+// How the tiles of a launch are cut: where they are too few to fill half of the chip (two
+// workgroups a compute unit of few rows, but one with heads of 256; one, of two groups, of
+// other tiles), their keys into parts of at least kLeast; and single rows of packed sequences,
+// which may be of any length, into parts of no more than 5/4 of the average.
+constexpr int64_t kLeast = 256;
 
 struct Cut {
     bool few;             // tiles of kFewRows rows
@@ -1036,25 +1038,28 @@ struct Cut {
 
 // `tiles` row tiles of a key head over up to `keys` keys each, or (sequences > 0) packed ones over
 // all of `keys` together.
-Cut cut(int64_t rows, int64_t tiles, int64_t keys, int64_t sequences, int64_t rounds, int64_t kv_heads, int64_t head_dim)
+Cut cut(int64_t rows, int64_t tiles, int64_t keys, int64_t sequences, int64_t kv_heads, int64_t head_dim)
 {
     Cut c{};
     c.rows = rows;
     c.few = rows == kFewRows;
     const int64_t per = head_dim == 256 || (c.few && head_dim == 128) ? 32 : 64;  // keys of a key tile
-    const int64_t room = (c.few && head_dim != 256 ? 512 : 256) * rounds / kv_heads;
+    const int64_t room = (c.few && head_dim != 256 ? 512 : 256) / kv_heads;
+    const int64_t average = sequences ? keys / sequences : keys;
     c.least = kLeast / per;
     c.parts = 1;
     c.chunk = keys > 0 ? keys : 1;
     c.units = tiles;
-    if (tiles * 2 > room || keys < (sequences ? sequences : 1) * kWorth) {
-    } else if (sequences) {
+    // (fewer keys are done before their parts are joined)
+    const bool worth = average >= (!c.few ? 768 : head_dim == 64 ? 1280 : head_dim == 128 ? 768 : 512), fills = tiles * 2 > room;
+    if (worth && sequences && !(fills && !c.few) && tiles <= 4 * room) {
         // (a sequence's row tiles take longer parts instead of more)
-        const int64_t each = (tiles + sequences - 1) / sequences, chunk = keys / (room - tiles) + 1;
-        c.chunk = chunk > kLeast / each ? chunk : kLeast / each + 1;
+        const int64_t each = (tiles + sequences - 1) / sequences;
+        c.chunk = fills ? average * 3 / 4 : keys / (room - tiles) + 1;
+        if (c.chunk <= kLeast / each) c.chunk = kLeast / each + 1;
         c.parts = (keys + c.chunk - 1) / c.chunk;
         c.units = tiles + keys / c.chunk;
-    } else {
+    } else if (worth && !sequences && !fills) {
         c.chunk = keys * tiles / room / per * per + per;
         if (c.chunk < kLeast) c.chunk = kLeast;
         c.parts = (keys + per + c.chunk - 1) / c.chunk;
@@ -1072,36 +1077,50 @@ int64_t parts_bytes(const Cut &c, int64_t kv_heads, int64_t head_dim)
     return c.units * kv_heads * c.rows * (head_dim + 2) * 4;
 }
 
+// Two groups of waves a tile where a unit has no other tile beside it (causal ones are half as
+// long as the longest, on average), but for a few key tiles, which take less than the sums.
+int groups_of(const Cut &c, int64_t keys, bool causal, int64_t kv_heads)
+{
+    return c.units * kv_heads <= (causal ? 512 : 256) && keys >= 256 ? 2 : 1;
+}
+
 // A call: one launch over all keys, or one over the prefix for all items and over their own
 // keys, whose parts are joined.
 struct Plan {
     bool shared;
+    int groups;           // of a tile's waves
     Cut own, common;
     int64_t bytes;  // of the workspace
 };
 
-Plan plan_packed(int64_t tokens_q, int64_t tokens_k, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t head_dim)
+Plan plan_packed(int64_t tokens_q, int64_t tokens_k, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                 bool causal)
 {
     Plan c{};
-    const int64_t rows = tokens_q * (heads / kv_heads), tile = rows <= kFewRows * sequences ? kFewRows : kRows;
-    c.own = cut(tile, rows / tile + sequences, tokens_k, sequences, tile == kFewRows ? 4 : 1, kv_heads, head_dim);
+    const int64_t rows = tokens_q * (heads / kv_heads), tile = rows * head_dim <= 2048 * sequences ? kFewRows : kRows;
+    c.own = cut(tile, rows / tile + sequences, tokens_k, sequences, kv_heads, head_dim);
     c.bytes = c.own.parts > 1 ? parts_bytes(c.own, kv_heads, head_dim) : 0;
+    c.groups = groups_of(c.own, tokens_k / sequences, causal, kv_heads);
     return c;
 }
 
 Plan plan_prefix(int64_t batch, int64_t tokens_q, int64_t tokens_k, int64_t prefix, int64_t heads, int64_t kv_heads,
-                 int64_t head_dim)
+                 int64_t head_dim, bool causal)
 {
     Plan c{};
     const int64_t rows = tokens_q * (heads / kv_heads), tile = rows <= kFewRows ? kFewRows : kRows;
-    c.shared = batch > 1 && rows < kRows && (batch - 1) * prefix * kv_heads * head_dim * 4 > kShared;
-    c.own = cut(tile, (rows + tile - 1) / tile * batch, (c.shared ? 0 : prefix) + tokens_k, 0, 1, kv_heads, head_dim);
-    c.bytes = c.shared || c.own.parts > 1 ? parts_bytes(c.own, kv_heads, head_dim) : 0;
-    if (c.shared) {
+    const int64_t tiles = (rows + tile - 1) / tile * batch;
+    if (batch > 1 && rows < kRows && prefix) {
         const int64_t of_all = batch * rows <= kFewRows ? kFewRows : kRows;
-        c.common = cut(of_all, (batch * rows + of_all - 1) / of_all, prefix, 0, 1, kv_heads, head_dim);
-        c.bytes += parts_bytes(c.common, kv_heads, head_dim);
+        c.common = cut(of_all, (batch * rows + of_all - 1) / of_all, prefix, 0, kv_heads, head_dim);
+        const int64_t sums = 2 * batch * rows * c.common.parts * kv_heads * head_dim * 4;
+        c.shared = (batch - 1) * prefix * kv_heads * head_dim * 4 > kShared + sums;
+        if (!c.shared) c.common = Cut{};
     }
+    c.own = cut(tile, tiles, (c.shared ? 0 : prefix) + tokens_k, 0, kv_heads, head_dim);
+    if (c.shared || c.own.parts > 1) c.bytes = parts_bytes(c.own, kv_heads, head_dim);
+    if (c.shared) c.bytes += parts_bytes(c.common, kv_heads, head_dim);
+    c.groups = groups_of(c.own, prefix + tokens_k, causal, kv_heads);
     return c;
 }
 
@@ -1146,7 +1165,7 @@ void launch(Params &p, const Plan &c, void *workspace, hipStream_t s)
         both_kernel<D><<<commons + blocks, kWaves * 64, 0, s>>>(BothParams{{all, p}, static_cast<int>(commons)});
     } else if (c.own.few) {
         few_kernel<D><<<blocks, kWaves * 64, 0, s>>>(p);
-    } else if (c.own.units * p.kv_heads <= 256) {
+    } else if (c.groups == 2) {
         tile_kernel<D, 2><<<blocks, 2 * kWaves * 64, 0, s>>>(p);
     } else {
         tile_kernel<D, 1><<<blocks, kWaves * 64, 0, s>>>(p);
@@ -1205,7 +1224,7 @@ extern "C" int64_t ltxk_packed_attention_workspace_bytes(int64_t tokens_q, int64
                                                          int64_t heads, int64_t kv_heads, int64_t head_dim)
 {
     if (tokens_q <= 0 || tokens_k < 0 || sequences <= 0 || kv_heads <= 0 || heads < kv_heads || head_dim <= 0) return 0;
-    return plan_packed(tokens_q, tokens_k, sequences, heads, kv_heads, head_dim).bytes;
+    return plan_packed(tokens_q, tokens_k, sequences, heads, kv_heads, head_dim, false).bytes;
 }
 
 extern "C" int ltxk_packed_attention(void *out, const void *q, int64_t q_tstride, const void *k, int64_t k_tstride,
@@ -1252,7 +1271,7 @@ extern "C" int ltxk_packed_attention(void *out, const void *q, int64_t q_tstride
     p.group = static_cast<int>(group);
     p.causal = causal != 0;
     p.window = static_cast<int>(window < kMost ? window : 0);  // a window of everything is none
-    return run(what, p, plan_packed(tokens_q, tokens_k, sequences, heads, kv_heads, head_dim), head_dim, workspace,
+    return run(what, p, plan_packed(tokens_q, tokens_k, sequences, heads, kv_heads, head_dim, p.causal), head_dim, workspace,
                workspace_bytes, stream);
 }
 
@@ -1261,7 +1280,7 @@ extern "C" int64_t ltxk_prefix_attention_workspace_bytes(int64_t batch, int64_t 
 {
     if (batch <= 0 || tokens_q <= 0 || tokens_k < 0 || prefix < 0 || kv_heads <= 0 || heads < kv_heads || head_dim <= 0)
         return 0;
-    return plan_prefix(batch, tokens_q, tokens_k, prefix, heads, kv_heads, head_dim).bytes;
+    return plan_prefix(batch, tokens_q, tokens_k, prefix, heads, kv_heads, head_dim, false).bytes;
 }
 
 extern "C" int ltxk_prefix_attention(void *out, const void *q, int64_t q_bstride, int64_t q_tstride, const void *k,
@@ -1320,6 +1339,6 @@ extern "C" int ltxk_prefix_attention(void *out, const void *q, int64_t q_bstride
     p.kv_heads = static_cast<int>(kv_heads);
     p.group = static_cast<int>(group);
     p.causal = causal != 0;
-    return run(what, p, plan_prefix(batch, tokens_q, tokens_k, prefix, heads, kv_heads, head_dim), head_dim, workspace,
+    return run(what, p, plan_prefix(batch, tokens_q, tokens_k, prefix, heads, kv_heads, head_dim, p.causal), head_dim, workspace,
                workspace_bytes, stream);
 }
