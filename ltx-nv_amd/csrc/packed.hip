@@ -45,6 +45,7 @@ struct Parts {
     float *sums;          // each part's weighted sums of v (rows x D)
     float2 *stats;        // and each of its rows' maximum and sum of weights
     int units, slots;     // parts of all tiles of a key head (with some that are none), and places for them on an XCD
+    int rows;             // a part's, as many as a tile has at most
     int parts, least;     // a tile's keys are cut into up to `parts`, of at least `least` key tiles each
     int chunk;            // and of about `chunk` keys (packed: for each row tile of the sequence) each
 };
@@ -341,9 +342,9 @@ __device__ __forceinline__ bool find_work(const Params &p, int block, int &unit,
 }
 
 // The place of a part's first row.
-__device__ __forceinline__ int64_t part_rows(const Params &p, const Tile &r, int kvh, int part, int rows)
+__device__ __forceinline__ int64_t part_rows(const Params &p, const Tile &r, int kvh, int part)
 {
-    return ((r.unit + static_cast<int64_t>(part) * r.step) * p.kv_heads + kvh) * rows;
+    return ((r.unit + static_cast<int64_t>(part) * r.step) * p.kv_heads + kvh) * p.cut.rows;
 }
 
 // A tile without any key: its rows weigh nothing, or are zero.
@@ -438,7 +439,7 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
     Tile r;
     if (!find_work(p, block, unit, kvh) || !find_tile<D, kRows, KT>(p, unit, kvh, r, part)) return;
     const bool joined = r.parts > 1 || p.joined;
-    const int64_t place = part_rows(p, r, kvh, part, kRows);
+    const int64_t place = part_rows(p, r, kvh, part);
     const int t0 = part * r.each, all = min(r.each, r.tiles - t0);
     const int any = uniform(threadIdx.x >> 6), group = GROUPS == 1 ? 0 : any / kWaves, wave = GROUPS == 1 ? any : any % kWaves;
     const int lane = threadIdx.x & 63, n = (all - group + GROUPS - 1) / GROUPS;  // the group's tiles
@@ -747,7 +748,7 @@ __device__ __forceinline__ void attend_few(const Params &p, int block, FewLds<D>
     Tile r;
     if (!find_work(p, block, unit, kvh) || !find_tile<D, kFewRows, KT>(p, unit, kvh, r, part)) return;
     const bool joined = r.parts > 1 || p.joined;
-    const int64_t place = part_rows(p, r, kvh, part, kFewRows);
+    const int64_t place = part_rows(p, r, kvh, part);
     const int t0 = part * r.each, t1 = min(t0 + r.each, r.tiles);
     if (t0 == t1) return no_keys<D, kFewRows, kWaves>(p, r, kvh, place, joined);
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -969,13 +970,13 @@ __global__ void __launch_bounds__(kWaves * 64) join_kernel(Params p, Parts commo
     if (r.unit + (r.parts - 1) * r.step >= p.cut.units) return;  // (offsets that do not ascend)
     const Row w = find_row(p, r, in);
     // the place of a row's first part, and how far it is to the next part's
-    const int64_t u = part_rows(p, r, kvh, 0, ROWS) + at, step = static_cast<int64_t>(r.step) * p.kv_heads * ROWS;
+    const int64_t u = part_rows(p, r, kvh, 0) + at, step = static_cast<int64_t>(r.step) * p.kv_heads * p.cut.rows;
     int64_t cu = 0, cstep = 0;
     int commons = 0;
     if (COMMON) {
         const int all = p.seqs * p.tq * p.group, row = token * p.group + w.member;
-        cu = (static_cast<int64_t>(row / COMMON) * p.kv_heads + kvh) * COMMON + row % COMMON;
-        cstep = static_cast<int64_t>((all + COMMON - 1) / COMMON) * p.kv_heads * COMMON;
+        cu = (static_cast<int64_t>(row / COMMON) * p.kv_heads + kvh) * common.rows + row % COMMON;
+        cstep = static_cast<int64_t>((all + COMMON - 1) / COMMON) * p.kv_heads * common.rows;
         constexpr int CK = COMMON == kFewRows ? kFewKeys<D> : kTileKeys<D>;
         const int tiles = (p.prefix + CK - 1) / CK;
         int each;
@@ -1034,6 +1035,7 @@ constexpr int64_t kLeast = 256;
 struct Cut {
     bool few;             // tiles of kFewRows rows
     int64_t rows, units, parts, least, chunk, slots, blocks;
+    int64_t used;         // rows of a tile at most
 };
 
 // `tiles` row tiles of a key head over up to `keys` keys each, or (sequences > 0) packed ones over
@@ -1041,7 +1043,7 @@ struct Cut {
 Cut cut(int64_t rows, int64_t tiles, int64_t keys, int64_t sequences, int64_t kv_heads, int64_t head_dim)
 {
     Cut c{};
-    c.rows = rows;
+    c.rows = c.used = rows;
     c.few = rows == kFewRows;
     const int64_t per = head_dim == 256 || (c.few && head_dim == 128) ? 32 : 64;  // keys of a key tile
     const int64_t room = (c.few && head_dim != 256 ? 512 : 256) / kv_heads;
@@ -1074,7 +1076,7 @@ Cut cut(int64_t rows, int64_t tiles, int64_t keys, int64_t sequences, int64_t kv
 
 int64_t parts_bytes(const Cut &c, int64_t kv_heads, int64_t head_dim)
 {
-    return c.units * kv_heads * c.rows * (head_dim + 2) * 4;
+    return (c.units * kv_heads * c.used * (head_dim + 2) * 4 + 15) / 16 * 16;
 }
 
 // Two groups of waves a tile where a unit has no other tile beside it (causal ones are half as
@@ -1118,6 +1120,7 @@ Plan plan_prefix(int64_t batch, int64_t tokens_q, int64_t tokens_k, int64_t pref
         if (!c.shared) c.common = Cut{};
     }
     c.own = cut(tile, tiles, (c.shared ? 0 : prefix) + tokens_k, 0, kv_heads, head_dim);
+    if (rows < tile) c.own.used = rows;
     if (c.shared || c.own.parts > 1) c.bytes = parts_bytes(c.own, kv_heads, head_dim);
     if (c.shared) c.bytes += parts_bytes(c.common, kv_heads, head_dim);
     c.groups = groups_of(c.own, prefix + tokens_k, causal, kv_heads);
@@ -1128,10 +1131,11 @@ Parts place(const Cut &c, int64_t kv_heads, int64_t head_dim, void *workspace)
 {
     Parts r;
     r.sums = static_cast<float *>(workspace);
-    r.stats = reinterpret_cast<float2 *>(r.sums + c.units * kv_heads * c.rows * head_dim);
+    r.stats = reinterpret_cast<float2 *>(r.sums + c.units * kv_heads * c.used * head_dim);
     r.units = static_cast<int>(c.units);
     r.slots = static_cast<int>(c.slots);
     r.parts = static_cast<int>(c.parts);
+    r.rows = static_cast<int>(c.used);
     r.least = static_cast<int>(c.least);
     r.chunk = static_cast<int>(c.chunk);
     return r;
