@@ -529,26 +529,24 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
         const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4 *)((v_at[m % VA][1] ^ x) + at));
         return cat(lo, hi);
     };
-    auto scores = [&](int buf, Scores &s) __attribute__((always_inline)) {
-        bf16x8 f[NK];
+    // Matrix phase: a run of the stream of products that a tile takes, the weights
+    // times V of the tile before (0 .. NV - 1), then its scores (NV .. NV + NK - 1),
+    // with the LDS fragments read ahead of them and `loads(j)` between them.
+    auto products = [&](auto from, auto to, int vbuf, int kbuf, Scores &s, auto loads) __attribute__((always_inline)) {
+        bf16x8 f[NV + NK];
+        auto frag = [&](int j) { f[j] = j < NV ? v_frag(vbuf, j) : k_frag(kbuf, j - NV); };
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) f[j] = k_frag(buf, j);
+        for (int j = from; j < from + kAhead; ++j) frag(j);
 #pragma unroll
-        for (int j = 0; j < NK; ++j) {
-            if (j + kAhead < NK) f[j + kAhead] = k_frag(buf, j + kAhead);
-            s.x[j % KU] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[j], qf[j / KU], j < KU ? f32x16{} : s.x[j % KU], 0, 0, 0);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-    };
-    // The weights times the values.
-    auto values = [&](int buf) __attribute__((always_inline)) {
-        bf16x8 f[NV];
-#pragma unroll
-        for (int j = 0; j < kAhead; ++j) f[j] = v_frag(buf, j);
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            if (j + kAhead < NV) f[j + kAhead] = v_frag(buf, j + kAhead);
-            o[j % MT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[j], __builtin_bit_cast(bf16x8, w[j / MT]), o[j % MT], 0, 0, 0);
+        for (int j = from; j < to; ++j) {
+            if (j + kAhead < to) frag(j + kAhead);
+            loads(j - from);
+            if (j < NV) {
+                o[j % MT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[j], __builtin_bit_cast(bf16x8, w[j / MT]), o[j % MT], 0, 0, 0);
+            } else {
+                const int i = j - NV;
+                s.x[i % KU] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[j], qf[i / KU], i < KU ? f32x16{} : s.x[i % KU], 0, 0, 0);
+            }
             __builtin_amdgcn_sched_barrier(0);
         }
     };
@@ -603,36 +601,43 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
     };
 
     // Tile i, whose keys are in buffer b: the weights of the tile before times its values, then
-    // the scores; its values and the next tile's keys load into the other buffers meanwhile.
+    // the scores; its values and the next tile's keys load into the other buffers between the
+    // products.
+    using std::integral_constant;
     Scores s;
-    auto tile = [&](int i, auto b) __attribute__((always_inline)) {
+    auto tile = [&](int i, auto from, auto b) __attribute__((always_inline)) {
+        constexpr int kEvery = from == 0 ? 3 : 2;
         u32x4 kr = {};  // (an empty buffer: the load gets nothing)
         if (i + 1 < n) {
             next(std::false_type{}, ks, i + 1);
             kr = buffer<D>(ks);
         }
-        if (i) next(std::true_type{}, vs, i);
+        if (from == 0) next(std::true_type{}, vs, i);
         const u32x4 vr = buffer<D>(vs);
-#pragma unroll
-        for (int c = 0; c < kParts; ++c) load(std::true_type{}, vr, vs, c, b ? lds.v1 : lds.v0);
-#pragma unroll
-        for (int c = 0; c < kParts; ++c) load(std::false_type{}, kr, ks, c, b ? lds.k0 : lds.k1);
         if (D == 256) asm volatile("" : "+v"(k_at[0]), "+v"(v_at[0][0]), "+v"(v_at[0][1]));
-        if (i) values(1 - b);
-        scores(b, s);
+        products(from, integral_constant<int, NV + NK>{}, 1 - b, b, s, [&](int j) __attribute__((always_inline)) {
+            if (j % kEvery) return;
+            const int c = j / kEvery;
+            if (c < kParts) load(std::true_type{}, vr, vs, c, b ? lds.v1 : lds.v0);
+            else if (c < 2 * kParts) load(std::false_type{}, kr, ks, c - kParts, b ? lds.k0 : lds.k1);
+        });
         mask(s, t0 + group + i * GROUPS);
         raise(s);
         rescale();
 #pragma unroll
         for (int j = 0; j < 8 * KU; ++j) weigh(s, j);
     };
+    constexpr integral_constant<int, 0> whole_tile, first_buffer;
+    constexpr integral_constant<int, 1> second_buffer;
     tile_barrier();
     const int turns = (all + GROUPS - 1) / GROUPS;  // as many barriers for each group
-    for (int i = 0; i < turns; i += 2) {
-        if (GROUPS == 1 || i < n) tile(i, std::integral_constant<int, 0>{});
+    if (GROUPS == 1 || n) tile(0, integral_constant<int, NV>{}, first_buffer);
+    tile_barrier();
+    for (int i = 1; i < turns; i += 2) {
+        if (GROUPS == 1 || i < n) tile(i, whole_tile, second_buffer);
         tile_barrier();
         if (i + 1 < turns) {
-            if (GROUPS == 1 || i + 1 < n) tile(i + 1, std::integral_constant<int, 1>{});
+            if (GROUPS == 1 || i + 1 < n) tile(i + 1, whole_tile, first_buffer);
             tile_barrier();
         }
     }
@@ -640,7 +645,7 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
 #pragma unroll
         for (int m = 0; m < VA; ++m) v_at[m][0] += kTileBytes, v_at[m][1] += kTileBytes;
     }
-    if (GROUPS == 1 || n) values(0);
+    if (GROUPS == 1 || n) products(whole_tile, integral_constant<int, NV>{}, 0, 0, s, [](int) {});
 
     // Lane l: row l % 32, columns 32 m + 8 j + 4 half + (0..3) in registers 4 j ..
     float total = pair_sum(sum);
