@@ -1,10 +1,32 @@
 // Attention over sequences laid end to end, and over a prefix that a batch shares: grouped
-// heads (query head h reads key head h / (heads / kv_heads)), causal or not, fp32 scores,
-// softmax and sums, one rounding to bf16.
+// heads (query head h reads key head h / (heads / kv_heads)), causal or not:
 //
+//   out[t, h, :] = round_bf16(sum_j p_j v_j / sum_j p_j),  p_j = 2^(scale log2(e) q.k_j - r)
+//
+// over the keys j that query t sees, r a reference that the quotient does not depend on.
 // A query at position i of its sequence's own n keys (its newest ones are the queries')
 // sees keys [lo, hi) of them, hi = i + 1 and lo = max(0, i + 1 - window) where the mask is
-// causal and [0, n) else, behind all of the prefix (if i >= 0).
+// causal and [0, n) else, behind all of the prefix (if i >= 0).  Scores, references, sums
+// and output are fp32; p is rounded to bf16 for the second product, and so are the p that
+// are summed.
+//
+// A row is a query at one head of its group, so that one tile of keys serves all heads of
+// the group, few queries fill a tile of rows, and a causal tile spans few of them.  Tiles of
+// 128 rows share key tiles in LDS, 32 rows a wave (the scores transposed, so that a lane has a
+// row's weights as the second product takes them).  Up to 32 rows are attended by all four
+// waves, each over keys of its own.  What bounds them:
+// * Tiles, long: power and, with half of the time, what is not a product.  6144 x 6144 tokens,
+//   32 heads of 128, no mask, 610 us (1.01 PFLOP/s; ltxk_attention 621 on the same card), on zeros 524
+//   (430).  Causal, 12288 tokens over 8 key heads: 1140-1270 us from card to card, 0.97-1.08.  Heads of 256 in
+//   a window of 1024: 360-430 us for 20078 tokens, 0.68-0.82.
+// * Tiles, few: the latency of a tile's chain of products, exponentials and products again, about
+//   1.4 us for 64 keys (32 with heads of 256) where no second workgroup shares the unit, with 3 us ahead (which
+//   sequence, first keys, queries) and 1-2 behind.  Deeper rings of tiles (three on their way instead of one) change
+//   nothing; the weights of a tile beside the scores of the next, 47 against 51 us on prompts of 1024 and
+//   333 tokens, heads of 256, but 5 % slower where the chip is full; two groups of waves, 39.
+// * Few rows: memory, 5.5 TB/s on 64 tokens over 125624 keys (97 us with the join of their parts, 5); short ones
+//   the same latencies.
+// * Units that turn out to be none, which lengths on the device cost: 2-3 us of a workgroup's place each.
 #include "flash_tiles.h"
 
 #include <cfloat>
@@ -16,17 +38,21 @@ namespace {
 // Rows (a query at one head of the group) of a tile: 32 a wave, which share its keys, or 32
 // that all waves attend with, each over keys of its own.
 constexpr int kRows = 32 * kWaves, kFewRows = 32;
-// Keys that the former take at a time, and a wave of the latter.
+// Keys that the former take at a time, and a wave of the latter.  (32 with heads of 256 let two
+// workgroups share a unit: 20078 tokens in a window of 1024 367 us, 475 with 64 and one.)
 template <int D>
 constexpr int kTileKeys = D == 256 ? 32 : 64;
 template <int D>
 constexpr int kFewKeys = D == 64 ? 64 : 32;
 
-// Weights are 2^(score - reference): the reference is a row's maximum so far, or up to kLag below
-// it, so that what was summed is rarely rescaled.  What is summed up to divide by are the
-// weights as the second product takes them, in bf16, so their rounding cancels where one of
-// them is most of the sum, whatever their size.  References past kHuge round by more than
-// 2^-4: there the scores round first, as the reference did.
+// Tiles of kRows rows take a row's maximum so far, or up to kLag below it, as the reference, so that
+// what was summed is rarely rescaled: 12288 causal tokens 1141 us, 1225 with the maximum in every
+// tile, four clips 1730 / 1925, a window with heads of 256 359 / 391.  The largest weight is then not
+// always 1, and its rounding adds to the error: 1.92e-3 to 2.33e-3 in all against 1.87e-3 to 2.18e-3
+// (the output's own rounding is 1.66e-3).  Few rows, which wait for memory, take the maximum.
+// The weights are summed as the second product takes them, so that their rounding cancels where
+// one of them is most of the sum.  References past kHuge round by more than 2^-4: there the scores
+// round first, as the reference did.
 constexpr float kLag = 6.f, kHuge = 1048576.f;
 
 // sum + the two bf16 values of `pair`.
@@ -166,7 +192,7 @@ __device__ __forceinline__ int parts_of(const Parts &c, int most, int tiles, int
 template <int KEYS>
 __device__ __forceinline__ int batch_parts(const Parts &c, int tiles)
 {
-    return min(c.parts, (tiles * KEYS + c.chunk - 1) / c.chunk);
+    return c.parts > 1 ? min(c.parts, (tiles * KEYS + c.chunk - 1) / c.chunk) : 1;
 }
 
 // Row tile `tile` of the sequence: what it attends to, and its parts.
@@ -269,7 +295,7 @@ __device__ __forceinline__ uint32_t reach(const Span &s)
     return static_cast<uint32_t>(s.valid - 1) * s.stride + 2 * D;
 }
 
-// Adds keys [from, to) to a row's running maximum, sum and weighted values: a lane has the
+// Adds keys [from, to) to a row's maximum, sum and weighted values: a lane has the
 // score of one key of 64, then one or more columns of the values.
 template <int D>
 __device__ __forceinline__ void attend_keys(const char *q, const char *k, uint32_t ks, const char *v, uint32_t vs, int from,
@@ -411,6 +437,7 @@ __device__ __forceinline__ void wait_lds()
     asm volatile("" ::: "memory");
 }
 
+// LDS of tiles of kRows rows: two stages of keys and values a group, or in the end its sums.
 template <int D, int GROUPS>
 struct TileLds {
     static constexpr int kBytes = kTileKeys<D> * D * 2;
@@ -424,7 +451,8 @@ struct TileLds {
 };
 
 // A tile of kRows rows by GROUPS times four waves: each group takes every so many key tiles,
-// through LDS of its own, and their sums are added up in the end.
+// through LDS of its own, and their sums are added up in the end.  Two groups on a unit of their
+// own overlap one's products with the other's weights.
 template <int D, int GROUPS>
 __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<D, GROUPS> &whole)
 {
@@ -730,9 +758,7 @@ __device__ __forceinline__ void attend_tile(const Params &p, int block, TileLds<
     }
 }
 
-// Few rows: each wave takes every fourth tile of kFewKeys keys, through LDS of its own and
-// without barriers, the next keys on their way while the weights are made and the next
-// values while the next scores are; the waves' sums are added up in the end.
+// LDS of tiles of few rows: keys and values of each wave, then its sums.
 template <int D>
 struct FewLds {
     char tile[kWaves][2][kFewKeys<D> * D * 2];
@@ -740,6 +766,10 @@ struct FewLds {
     uint32_t odd;
 };
 
+// A tile of few rows: each wave takes every fourth tile of kFewKeys keys, through LDS of its own
+// and without barriers, the next keys on their way while the weights are made and the next
+// values while the next scores are; the waves' sums are added up in the end.  What is read is read
+// by no other workgroup: streaming loads, 95 against 109 us on 64 tokens over 125624 keys.
 template <int D>
 __device__ __forceinline__ void attend_few(const Params &p, int block, FewLds<D> &lds)
 {
@@ -835,7 +865,7 @@ __device__ __forceinline__ void attend_few(const Params &p, int block, FewLds<D>
         u32x4 w[KU * 2];
 #pragma unroll
         for (int j = 0; j < KU * 8; ++j) {
-            // (the scores round before the reference is taken off, as it did)
+            // (the scores round before the maximum is taken off, as it did)
             const float x = __builtin_amdgcn_exp2f(s[j >> 3][2 * (j & 7)] * p.scale2 - mx);
             const float y = __builtin_amdgcn_exp2f(s[j >> 3][2 * (j & 7) + 1] * p.scale2 - mx);
             w[j >> 2][j & 3] = pack_bf16x2(x, y);
@@ -1028,13 +1058,21 @@ __global__ void __launch_bounds__(kWaves * 64) join_kernel(Params p, Parts commo
 }
 
 constexpr int64_t kMost = 1 << 29;            // rows and keys, which are counted in int (a prefix's and own keys together)
-constexpr int64_t kShared = 96 << 20;         // bytes of prefix not read again that are worth their sums and a second launch
+// Bytes of a prefix not read again that are worth their sums and a second launch.  32 heads of 128 over 8, own keys
+// 64, one query an item, us, shared / not: 4 items, prefix 4096 14.6 / 14.5, 16384 25 / 31; 32 items, 1024 18 / 16, 4096
+// 22 / 35, 16384 32 / 147; 16 items of 8 queries, 2048 25 / 22, 8192 41 / 48, of 28, 48 / 41 and 98 / 92.
+constexpr int64_t kShared = 96 << 20;
 constexpr int64_t kStride = (1 << 23) - 8;    // elements of a token stride: its bytes are 24 bits
 
-// How the tiles of a launch are cut: where they are too few to fill half of the chip (two
-// workgroups a compute unit of few rows, but one with heads of 256; one, of two groups, of
-// other tiles), their keys into parts of at least kLeast; and single rows of packed sequences,
-// which may be of any length, into parts of no more than 5/4 of the average.
+// How the tiles of a launch are cut.  Where they are too few to fill half of the chip (two
+// workgroups a compute unit of few rows, but one with heads of 256; one, of two groups, of other
+// tiles), their keys go into parts of at least kLeast, if there are enough of them: joining takes a
+// second launch, 4-5 us.  One row of 8 key heads over n keys, us, cut / whole: heads of 64, 1024 9.4 / 8.9,
+// 1536 9.4 / 11; of 128, 512 10.4 / 8.7, 768 10.5 / 10.8, 1024 10.4 / 12.8; of 256, 300 15.5 / 13.3, 512
+// 15.2 / 15.8, 1024 15 / 25.  100 queries, heads of 128, 512 22 / 17, 768 21 / 20, 1536 22 / 31.
+// Few rows of packed sequences, whose lengths may differ, go into parts of 3/4 of the average, so that the
+// longest do not end last: 64 tokens over 100 to 8192 keys 97 us, in parts of 5/4 108, whole 140; over 300 to
+// 3000 (one row a key head, heads of 128) 61 / 66 / -, over 900 to 1100 56 / 56 / -, of exactly 1024 58 / - / 45.
 constexpr int64_t kLeast = 256;
 
 struct Cut {
@@ -1057,7 +1095,6 @@ Cut cut(int64_t rows, int64_t tiles, int64_t keys, int64_t sequences, int64_t kv
     c.parts = 1;
     c.chunk = keys > 0 ? keys : 1;
     c.units = tiles;
-    // (fewer keys are done before their parts are joined)
     const bool worth = average >= (!c.few ? 768 : head_dim == 64 ? 1280 : head_dim == 128 ? 768 : 512), fills = tiles * 2 > room;
     if (worth && sequences && !(fills && !c.few) && tiles <= 4 * room) {
         // (a sequence's row tiles take longer parts instead of more)
@@ -1085,7 +1122,9 @@ int64_t parts_bytes(const Cut &c, int64_t kv_heads, int64_t head_dim)
 }
 
 // Two groups of waves a tile where a unit has no other tile beside it (causal ones are half as
-// long as the longest, on average), but for a few key tiles, which take less than the sums.
+// long as the longest, on average), but for a few keys, which take less than adding up: one sequence,
+// 32 heads over 8, us, one / two groups: causal, heads of 64, 128 tokens 7.4 / 7.9, 500 14 / 12, 1000 23 / 19,
+// 2000 39 / 35; of 256, 13 / 16, 26 / 25, 46 / 40, 98 / 86; without a mask, heads of 128, 1000 29 / 25, 2000 75 / 82.
 int groups_of(const Cut &c, int64_t keys, bool causal, int64_t kv_heads)
 {
     return c.units * kv_heads <= (causal ? 512 : 256) && keys >= 256 ? 2 : 1;
@@ -1100,6 +1139,9 @@ struct Plan {
     int64_t bytes;  // of the workspace
 };
 
+// Tiles of few rows, where the sequences have few on average.  64 sequences of 1024 keys, us, few / 128 rows, whole:
+// heads of 128, 4 rows 45 / 46, 16 53 / 47, 32 64 / 48; of 64, 20 / 28, 19 / 28, 22 / 28; of 256, 88 / 103, 112 / 103, 134 / 103.
+// (A sequence has floor(rows / 32) + 1 units, so that 32 rows make one of two units none.)
 Plan plan_packed(int64_t tokens_q, int64_t tokens_k, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t head_dim,
                  bool causal)
 {
