@@ -99,6 +99,27 @@ def test_every_cut_of_the_keys(queries, heads, dh):
             assert_near(got[rows], *one_sequence(q[rows], k[at], v[at], heads, 2), f"{most} keys, sequence {s}")
 
 
+@pytest.mark.parametrize("queries,keys,heads,kv_heads,dh", [
+    ([1, 0, 2] * 1700, None, 4, 2, 64), ([0] * 4100 + [5] + [0] * 4100 + [3], None, 2, 1, 128),
+    ([1] * 100 + [2000], [700] * 100 + [2000], 8, 2, 128), ([900] + [1] * 60, [900] + [50, 6000] * 30, 4, 4, 64),
+    ([1], [150_000], 2, 1, 64), ([2], [40_000], 3, 1, 256), ([1] * 3, [100_000, 3, 40_000], 8, 8, 128)])
+def test_many_and_unequal_sequences(queries, keys, heads, kv_heads, dh):
+    """Thousands of sequences, most of them empty; one prompt among single tokens; keys in hundreds of parts."""
+    import ltxk
+
+    g = torch.Generator(device=DEV).manual_seed(len(queries))
+    qo, ko = _offsets(queries), _offsets(keys or queries)
+    q, k, v = _draw(g, sum(queries), heads * dh, 1.5), _draw(g, int(ko[-1]), kv_heads * dh), _draw(g, int(ko[-1]), kv_heads * dh)
+    out = torch.full_like(q, float("nan"))
+    got = ltxk.packed_attention(q, k, v, heads, qo, kv_heads, None if keys is None else ko, out=out)
+    assert bool(got.isfinite().all())
+    at, kt = qo.tolist(), ko.tolist()
+    some = [s for s, n in enumerate(queries) if n]
+    for s in {*some[:6], *some[-6:], *some[:: max(1, len(some) // 20)]}:
+        rows, cols = slice(at[s], at[s + 1]), slice(kt[s], kt[s + 1])
+        assert_near(got[rows], *one_sequence(q[rows], k[cols], v[cols], heads, kv_heads), f"sequence {s}")
+
+
 def test_views_scale_and_equal_offsets():
     """Columns of one projection's rows, and lengths shared by queries and keys, give the same bits; a scale of its own."""
     import ltxk

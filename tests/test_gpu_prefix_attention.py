@@ -68,6 +68,22 @@ def test_every_cut_of_a_prefix(b, tq, dh):
         _check(got[-2:], q[-2:], k[-2:], v[-2:], pk[:prefix], pv[:prefix], lengths[-2:], 4, 2)
 
 
+@pytest.mark.parametrize("b,tq,prefix,room,heads,kv_heads,dh", [
+    (1500, 1, 2000, 20, 4, 2, 128), (300, 3, 3000, 400, 4, 1, 64), (2, 1, 120_000, 9000, 8, 1, 128), (90, 9, 900, 64, 6, 2, 256),
+    (1, 700, 5000, 700, 4, 2, 128)])
+def test_many_items_and_long_prefixes(b, tq, prefix, room, heads, kv_heads, dh):
+    import ltxk
+
+    g = torch.Generator(device=DEV).manual_seed(b)
+    q, k, v = _draw(g, b, tq, heads * dh, scale=1.5), _draw(g, b, room, kv_heads * dh), _draw(g, b, room, kv_heads * dh)
+    pk, pv = _draw(g, prefix, kv_heads * dh), _draw(g, prefix, kv_heads * dh)
+    lengths = [(37 * i) % (room + 1) for i in range(b)]
+    got = ltxk.prefix_attention(q, k, v, pk, pv, heads, kv_heads, _ints(lengths), out=torch.full_like(q, float("nan")))
+    assert bool(got.isfinite().all())
+    for i in {0, 1 % b, b - 1, *range(0, b, max(1, b // 12))}:
+        _check(got[i:i + 1], q[i:i + 1], k[i:i + 1], v[i:i + 1], pk, pv, lengths[i:i + 1], heads, kv_heads)
+
+
 @pytest.mark.parametrize("tq,prefix", [(4, 200), (4, 9000), (150, 200)])
 def test_masked_values_may_hold_anything(tq, prefix):
     import ltxk
