@@ -17,15 +17,17 @@
 // waves, each over keys of its own.  What bounds them:
 // * Tiles, long: power and, with half of the time, what is not a product.  6144 x 6144 tokens,
 //   32 heads of 128, no mask, 610 us (1.01 PFLOP/s; ltxk_attention 621 on the same card), on zeros 524
-//   (430).  Causal, 12288 tokens over 8 key heads: 1140-1270 us from card to card, 0.97-1.08.  Heads of 256 in
-//   a window of 1024: 360-430 us for 20078 tokens, 0.68-0.82.
+//   (430).  Causal, 12288 tokens over 8 key heads: 1140-1250 us from card to card, 0.99-1.08.  Heads of 256 in
+//   a window of 1024: 353-430 us for 20078 tokens, 0.68-0.83.
 // * Tiles, few: the latency of a tile's chain of products, exponentials and products again, about
 //   1.4 us for 64 keys (32 with heads of 256) where no second workgroup shares the unit, with 3 us ahead (which
 //   sequence, first keys, queries) and 1-2 behind.  Deeper rings of tiles (three on their way instead of one) change
 //   nothing; the weights of a tile beside the scores of the next, 47 against 51 us on prompts of 1024 and
-//   333 tokens, heads of 256, but 5 % slower where the chip is full; two groups of waves, 39.
+//   333 tokens, heads of 256, but 5 % slower where the chip is full; two groups of waves, 38.
 // * Few rows: memory, 5.5 TB/s on 64 tokens over 125624 keys (97 us with the join of their parts, 5); short ones
 //   the same latencies.
+// * A prefix beside own keys: 64 items of a query, 32 heads of 128 over 8, prefix 8192, own up to 1024, 33 us and 6.5 to
+//   join: the latencies of both kinds of tile on places that they share.
 // * Units that turn out to be none, which lengths on the device cost: 2-3 us of a workgroup's place each.
 #include "flash_tiles.h"
 
@@ -1093,8 +1095,9 @@ __global__ void __launch_bounds__(kWaves * 64) join_kernel(Params p, Parts commo
 
 constexpr int64_t kMost = 1 << 29;            // rows and keys, which are counted in int (a prefix's and own keys together)
 // Bytes of a prefix not read again that are worth their sums and a second launch.  32 heads of 128 over 8, own keys
-// 64, one query an item, us, shared / not: 4 items, prefix 4096 14.6 / 14.5, 16384 25 / 31; 32 items, 1024 18 / 16, 4096
-// 22 / 35, 16384 32 / 147; 16 items of 8 queries, 2048 25 / 22, 8192 41 / 48, of 28, 48 / 41 and 98 / 92.
+// 64, us, shared / not: one query, 4 items, prefix 4096 11.8 / 14.4 (48 MB; not shared), 16384 22 / 31; 32 items, 512
+// 20 / 10, 1024 15.7 / 16.4 (124 MB), 4096 19 / 32, 16384 36 / 122; 16 items of 8 queries, 2048 22 / 21 (120 MB), 8192
+// 38 / 44, of 28, 42 / 41 and 88 / 89.
 constexpr int64_t kShared = 96 << 20;
 constexpr int64_t kStride = (1 << 23) - 8;    // elements of a token stride: its bytes are 24 bits
 
