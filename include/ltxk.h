@@ -398,7 +398,7 @@ int ltxk_cross_attention(void *out, const void *q, int64_t q_bstride, int64_t q_
                          int64_t tokens_k, int64_t heads, int64_t head_dim, float scale, void *workspace,
                          int64_t workspace_bytes, void *stream);
 
-/* Bytes of workspace ltxk_packed_attention needs for this shape. */
+/* Bytes of workspace ltxk_packed_attention needs for this shape (0 for one that it refuses). */
 int64_t ltxk_packed_attention_workspace_bytes(int64_t tokens_q, int64_t tokens_k, int64_t sequences, int64_t heads,
                                               int64_t kv_heads, int64_t head_dim);
 
@@ -428,7 +428,7 @@ int ltxk_packed_attention(void *out, const void *q, int64_t q_tstride, const voi
                           int causal, int64_t window, float scale, void *workspace, int64_t workspace_bytes,
                           void *stream);
 
-/* Bytes of workspace ltxk_prefix_attention needs for this shape. */
+/* Bytes of workspace ltxk_prefix_attention needs for this shape (0 for one that it refuses). */
 int64_t ltxk_prefix_attention_workspace_bytes(int64_t batch, int64_t tokens_q, int64_t tokens_k, int64_t prefix,
                                               int64_t heads, int64_t kv_heads, int64_t head_dim);
 

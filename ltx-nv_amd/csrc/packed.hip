@@ -1094,6 +1094,7 @@ __global__ void __launch_bounds__(kWaves * 64) join_kernel(Params p, Parts commo
 }
 
 constexpr int64_t kMost = 1 << 29;            // rows and keys, which are counted in int (a prefix's and own keys together)
+constexpr int64_t kMostItems = 1 << 20;       // sequences, or items of a batch
 // Bytes of a prefix not read again that are worth their sums and a second launch.  32 heads of 128 over 8, own keys
 // 64, us, shared / not: one query, 4 items, prefix 4096 11.8 / 14.4 (48 MB; not shared), 16384 22 / 31; 32 items, 512
 // 20 / 10, 1024 15.7 / 16.4 (124 MB), 4096 19 / 32, 16384 36 / 122; 16 items of 8 queries, 2048 22 / 21 (120 MB), 8192
@@ -1319,6 +1320,13 @@ int check_sizes(const char *what, int64_t tokens_q, int64_t tokens_k, int64_t he
     return LTXK_OK;
 }
 
+// Sizes that a call takes and has work with.
+bool sizes_fit(int64_t batch, int64_t tokens_q, int64_t tokens_k, int64_t prefix, int64_t heads, int64_t kv_heads, int64_t head_dim)
+{
+    return heads > 0 && heads <= (1 << 16) && kv_heads > 0 && heads % kv_heads == 0 && tokens_q > 0 && tokens_q <= kMost / heads / batch &&
+           tokens_k >= 0 && tokens_k <= kMost && prefix >= 0 && prefix <= kMost && (head_dim == 64 || head_dim == 128 || head_dim == 256);
+}
+
 int check_rows(const char *what, const char *name, const void *x, int64_t stride, int64_t width)
 {
     if (!x) return fail(LTXK_E_ARG, "%s: null %s", what, name);
@@ -1338,7 +1346,7 @@ using namespace ltxk;
 extern "C" int64_t ltxk_packed_attention_workspace_bytes(int64_t tokens_q, int64_t tokens_k, int64_t sequences,
                                                          int64_t heads, int64_t kv_heads, int64_t head_dim)
 {
-    if (tokens_q <= 0 || tokens_k < 0 || sequences <= 0 || kv_heads <= 0 || heads < kv_heads || head_dim <= 0) return 0;
+    if (sequences <= 0 || sequences > kMostItems || !sizes_fit(1, tokens_q, tokens_k, 0, heads, kv_heads, head_dim)) return 0;
     return plan_packed(tokens_q, tokens_k, sequences, heads, kv_heads, head_dim, false).bytes;
 }
 
@@ -1352,7 +1360,7 @@ extern "C" int ltxk_packed_attention(void *out, const void *q, int64_t q_tstride
     clear_error();
     Params p{};
     if (int rc = check_sizes(what, tokens_q, tokens_k, heads, kv_heads, head_dim, scale, &p.scale2)) return rc;
-    if (sequences < 0 || sequences > (1 << 20))
+    if (sequences < 0 || sequences > kMostItems)
         return fail(LTXK_E_ARG, "%s: between 0 and 2^20 sequences (got %lld)", what, (long long)sequences);
     if (window < 0 || (window && !causal))
         return fail(LTXK_E_ARG, "%s: a window must be positive, and needs the causal mask", what);
@@ -1393,8 +1401,7 @@ extern "C" int ltxk_packed_attention(void *out, const void *q, int64_t q_tstride
 extern "C" int64_t ltxk_prefix_attention_workspace_bytes(int64_t batch, int64_t tokens_q, int64_t tokens_k, int64_t prefix,
                                                          int64_t heads, int64_t kv_heads, int64_t head_dim)
 {
-    if (batch <= 0 || tokens_q <= 0 || tokens_k < 0 || prefix < 0 || kv_heads <= 0 || heads < kv_heads || head_dim <= 0)
-        return 0;
+    if (batch <= 0 || batch > kMostItems || !sizes_fit(batch, tokens_q, tokens_k, prefix, heads, kv_heads, head_dim)) return 0;
     return plan_prefix(batch, tokens_q, tokens_k, prefix, heads, kv_heads, head_dim, false).bytes;
 }
 
@@ -1410,7 +1417,7 @@ extern "C" int ltxk_prefix_attention(void *out, const void *q, int64_t q_bstride
     clear_error();
     Params p{};
     if (int rc = check_sizes(what, tokens_q, tokens_k, heads, kv_heads, head_dim, scale, &p.scale2)) return rc;
-    if (batch < 0 || batch > (1 << 20) || prefix < 0)
+    if (batch < 0 || batch > kMostItems || prefix < 0)
         return fail(LTXK_E_ARG, "%s: bad shape batch=%lld prefix=%lld", what, (long long)batch, (long long)prefix);
     if (batch == 0 || tokens_q == 0) return LTXK_OK;
     const int64_t group = heads / kv_heads;

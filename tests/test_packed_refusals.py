@@ -139,3 +139,17 @@ def test_binding_refuses_tensors():
     prefix(ValueError, "must be", lengths=_gpu(3, dtype=torch.int32))
     prefix(ValueError, "out", out=_gpu(2, 2, 512))
     prefix(TypeError, "Tensor", prefix_k=None)
+
+
+@pytest.mark.parametrize("kw", [dict(tq=1 << 62), dict(tk=1 << 62), dict(items=1 << 62), dict(heads=1 << 62), dict(kv_heads=3),
+                                dict(head_dim=96), dict(tq=0), dict(tq=-1), dict(items=0), dict(prefix=1 << 62), dict(kv_heads=0)])
+def test_workspaces_of_refused_sizes(kw):
+    """A size that a call refuses needs none, however large: no sum or quotient of it is taken."""
+    _, lib = _lib()
+    a = {**dict(items=4, tq=8, tk=4096, prefix=1 << 16, heads=8, kv_heads=2, head_dim=128), **kw}
+    assert lib.ltxk_prefix_attention_workspace_bytes(a["items"], a["tq"], a["tk"], a["prefix"], a["heads"], a["kv_heads"],
+                                                     a["head_dim"]) == 0
+    if "prefix" not in kw:
+        assert lib.ltxk_packed_attention_workspace_bytes(a["tq"], a["tk"], a["items"], a["heads"], a["kv_heads"],
+                                                         a["head_dim"]) == 0
+    assert lib.ltxk_prefix_attention_workspace_bytes(4, 8, 4096, 1 << 16, 8, 2, 128) > 0
