@@ -120,6 +120,30 @@ def test_many_and_unequal_sequences(queries, keys, heads, kv_heads, dh):
         assert_near(got[rows], *one_sequence(q[rows], k[cols], v[cols], heads, kv_heads), f"sequence {s}")
 
 
+@pytest.mark.parametrize("seed", range(30))
+def test_any_sizes(seed):
+    """Sizes of all magnitudes, with more keys than queries, fewer, and none, in every mask."""
+    import random
+
+    import ltxk
+
+    r, g = random.Random(seed), torch.Generator(device=DEV).manual_seed(seed)
+    dh, kv_heads, group = r.choice((64, 128, 256)), r.choice((1, 2, 3, 4, 8, 16)), r.choice((1, 1, 2, 3, 4, 8))
+    seqs, causal = int(2 ** r.uniform(0, 7)), r.random() < 0.7
+    most_q, most_k = r.choice((1, 3, 40, 700)), int(2 ** r.uniform(1, 12))
+    queries = [r.randint(0, most_q) for _ in range(seqs)]
+    keys = [r.randint(0, most_k) + (n if r.random() < 0.8 else 0) for n in queries]
+    heads, qo, ko = kv_heads * group, _offsets(queries), _offsets(keys)
+    kw = dict(causal=causal, window=r.choice((None, None, 1, 37, 500)) if causal else None)
+    q, k, v = _draw(g, sum(queries), heads * dh, 1.5), _draw(g, sum(keys), kv_heads * dh), _draw(g, sum(keys), kv_heads * dh)
+    got = ltxk.packed_attention(q, k, v, heads, qo, kv_heads, ko, out=torch.full_like(q, float("nan")), **kw)
+    assert bool(got.isfinite().all())
+    at, kt = qo.tolist(), ko.tolist()
+    for s in {0, seqs - 1, *range(0, seqs, max(1, seqs // 8))}:
+        rows, cols = slice(at[s], at[s + 1]), slice(kt[s], kt[s + 1])
+        assert_near(got[rows], *one_sequence(q[rows], k[cols], v[cols], heads, kv_heads, **kw), f"sequence {s}")
+
+
 def test_views_scale_and_equal_offsets():
     """Columns of one projection's rows, and lengths shared by queries and keys, give the same bits; a scale of its own."""
     import ltxk

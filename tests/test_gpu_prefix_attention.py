@@ -84,6 +84,28 @@ def test_many_items_and_long_prefixes(b, tq, prefix, room, heads, kv_heads, dh):
         _check(got[i:i + 1], q[i:i + 1], k[i:i + 1], v[i:i + 1], pk, pv, lengths[i:i + 1], heads, kv_heads)
 
 
+@pytest.mark.parametrize("seed", range(30))
+def test_any_sizes(seed):
+    """Sizes of all magnitudes: each way to share a prefix, to cut it and own keys, and to lay out few and many rows."""
+    import random
+
+    import ltxk
+
+    r, g = random.Random(seed), torch.Generator(device=DEV).manual_seed(seed)
+    dh, kv_heads, group = r.choice((64, 128, 256)), r.choice((1, 2, 3, 4, 8, 16)), r.choice((1, 1, 2, 3, 4, 8))
+    b, tq = int(2 ** r.uniform(0, 7)), r.choice((1, 1, 1, 2, 5, 9, 30, 70))
+    prefix, room = int(2 ** r.uniform(0, 15)) - 1, int(2 ** r.uniform(0, 11)) - 1
+    while b * room * kv_heads * dh > 1 << 27:
+        room //= 2
+    heads, lengths, causal = kv_heads * group, [r.randint(0, room) for _ in range(b)], r.random() < 0.7
+    q, k, v = _draw(g, b, tq, heads * dh, scale=1.5), _draw(g, b, room, kv_heads * dh), _draw(g, b, room, kv_heads * dh)
+    pk, pv = _draw(g, prefix, kv_heads * dh), _draw(g, prefix, kv_heads * dh)
+    got = ltxk.prefix_attention(q, k, v, pk, pv, heads, kv_heads, _ints(lengths), causal, out=torch.full_like(q, float("nan")))
+    assert bool(got.isfinite().all())
+    for i in {0, b - 1, *range(0, b, max(1, b // 6))}:
+        _check(got[i:i + 1], q[i:i + 1], k[i:i + 1], v[i:i + 1], pk, pv, lengths[i:i + 1], heads, kv_heads, causal=causal)
+
+
 @pytest.mark.parametrize("tq,prefix", [(4, 200), (4, 9000), (150, 200)])
 def test_masked_values_may_hold_anything(tq, prefix):
     import ltxk
