@@ -1252,7 +1252,8 @@ void join(const Params &p, const Plan &c, const Parts &common, hipStream_t s)
     const int64_t rows = static_cast<int64_t>(p.qo ? 1 : p.seqs) * p.tq * p.heads;
     const unsigned blocks = static_cast<unsigned>((rows + kWaves - 1) / kWaves);
     if (!c.shared) join_kernel<D, ROWS, KEYS, 0><<<blocks, kWaves * 64, 0, s>>>(p, common, rows);
-    else if (c.common.few) join_kernel<D, ROWS, KEYS, kFewRows><<<blocks, kWaves * 64, 0, s>>>(p, common, rows);
+    // (stacked rows are few only where an item's are)
+    else if (c.common.few) join_kernel<D, kFewRows, kFewKeys<D>, kFewRows><<<blocks, kWaves * 64, 0, s>>>(p, common, rows);
     else join_kernel<D, ROWS, KEYS, kRows><<<blocks, kWaves * 64, 0, s>>>(p, common, rows);
 }
 
