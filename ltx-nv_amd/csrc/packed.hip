@@ -375,6 +375,9 @@ __device__ __forceinline__ int64_t part_rows(const Params &p, const Tile &r, int
     return ((r.unit + static_cast<int64_t>(part) * r.step) * p.kv_heads + kvh) * p.cut.rows;
 }
 
+// A sum of weights that says that a part has no key, and has written no weighted values.
+constexpr float kNoKeys = -1.f;
+
 // A tile without any key: its rows weigh nothing, or are zero.
 template <int D, int ROWS, int WAVES>
 __device__ __forceinline__ void no_keys(const Params &p, const Tile &r, int kvh, int64_t u, bool joined)
@@ -386,7 +389,7 @@ __device__ __forceinline__ void no_keys(const Params &p, const Tile &r, int kvh,
         if (!joined)
             *reinterpret_cast<u32x4 *>(p.out + ((r.token + w.query) * p.heads + kvh * p.group + w.member) * D + c * 8) = u32x4{};
         else if (c == 0)
-            p.cut.stats[u + at] = make_float2(-FLT_MAX, 0.f);
+            p.cut.stats[u + at] = make_float2(-FLT_MAX, kNoKeys);
     }
 }
 
@@ -1055,17 +1058,18 @@ __global__ void __launch_bounds__(kWaves * 64) join_kernel(Params p, Parts commo
     }
     const int count = r.parts + commons;
     auto stat = [&](int k) {
-        return k < r.parts ? p.cut.stats[u + k * step] : k < count ? common.stats[cu + (k - r.parts) * cstep] : make_float2(-FLT_MAX, 0.f);
+        return k < r.parts ? p.cut.stats[u + k * step] : k < count ? common.stats[cu + (k - r.parts) * cstep] : make_float2(-FLT_MAX, kNoKeys);
     };
     float m = -FLT_MAX, sum = 0.f, acc[8] = {};
     for (int k = lane; k < count; k += 64) m = fmaxf(m, stat(k).x);
 #pragma unroll
     for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
     for (int k0 = 0; k0 < count; k0 += 64) {
-        // (a part without a key has a sum of zero, and has written no sums)
+        // (a part whose weights are all zero still brings the values that are not finite)
         const float2 st = stat(k0 + lane);
-        const float f = st.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(st.x - m);
-        sum += f * st.y;
+        const bool none = st.y == kNoKeys;
+        const float f = none ? kNoKeys : __builtin_amdgcn_exp2f(st.x - m);
+        sum += none ? 0.f : f * st.y;
         const int here = min(64, count - k0);
 #pragma unroll 4
         for (int k = g; k < here + g; k += kBeside) {  // as many turns for every lane
@@ -1073,7 +1077,7 @@ __global__ void __launch_bounds__(kWaves * 64) join_kernel(Params p, Parts commo
             const float x = __shfl(f, min(k, here - 1), 64);
             const float *sums = at_k < r.parts ? p.cut.sums + (u + at_k * step) * D : common.sums + (cu + (at_k - r.parts) * cstep) * D;
             const f32x4 lo = *reinterpret_cast<const f32x4 *>(sums + c * 8), hi = *reinterpret_cast<const f32x4 *>(sums + c * 8 + 4);
-            const bool take = k < here && x != 0.f;
+            const bool take = k < here && x != kNoKeys;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 acc[e] = take ? __builtin_fmaf(x, lo[e], acc[e]) : acc[e];
