@@ -417,7 +417,9 @@ int64_t ltxk_packed_attention_workspace_bytes(int64_t tokens_q, int64_t tokens_k
  * q is bf16 at q + t*q_tstride + h*head_dim (elements; multiples of 8, at least
  * heads*head_dim, below 2^23), k and v likewise with kv_heads; out is contiguous
  * [tokens_q, heads*head_dim] and overlaps no operand.  Scores, softmax and sums are
- * fp32.  tokens_q*heads and tokens_k are at most 2^29.  `workspace`: device
+ * fp32.  tokens_q*heads and tokens_k are at most 2^29, and a launch holds fewer than 2^32
+ * threads, which it does where tokens_q*heads/32 + (sequences+7)*kv_heads is below 2^24
+ * (sequences is at most 2^20).  `workspace`: device
  * memory of ltxk_packed_attention_workspace_bytes, 16-byte aligned (NULL if that is
  * 0), in use until the call's work has run.  For the prompts that the language model
  * in front of the text connectors reads (standalone/ltx_te.py:124-146), and for
@@ -443,7 +445,8 @@ int64_t ltxk_prefix_attention_workspace_bytes(int64_t batch, int64_t tokens_q, i
  * q is bf16 at q + b*q_bstride + t*q_tstride + h*head_dim, k and v likewise, the
  * prefix's at prefix_k + j*prefix_k_tstride + h'*head_dim; out is contiguous
  * [batch*tokens_q, heads*head_dim] and overlaps no operand.  batch*tokens_q*heads,
- * tokens_k and prefix are at most 2^29.  Everything else as there. */
+ * tokens_k and prefix are at most 2^29, and batch*tokens_q*heads/32 + (batch+7)*kv_heads
+ * below 2^24 always fits a launch (batch is at most 2^20).  Everything else as there. */
 int ltxk_prefix_attention(void *out, const void *q, int64_t q_bstride, int64_t q_tstride, const void *k,
                           int64_t k_bstride, int64_t k_tstride, const void *v, int64_t v_bstride, int64_t v_tstride,
                           const void *prefix_k, int64_t prefix_k_tstride, const void *prefix_v,

@@ -1099,6 +1099,7 @@ __global__ void __launch_bounds__(kWaves * 64) join_kernel(Params p, Parts commo
 
 constexpr int64_t kMost = 1 << 29;            // rows and keys, which are counted in int (a prefix's and own keys together)
 constexpr int64_t kMostItems = 1 << 20;       // sequences, or items of a batch
+constexpr int64_t kMostBlocks = (int64_t{1} << 32) / (kWaves * 64);  // workgroups: a launch holds fewer than 2^32 threads
 // Bytes of a prefix not read again that are worth their sums and a second launch.  32 heads of 128 over 8, own keys
 // 64, us, shared / not: one query, 4 items, prefix 4096 11.8 / 14.4 (48 MB; not shared), 16384 22 / 31; 32 items, 512
 // 20 / 10, 1024 15.7 / 16.4 (124 MB), 4096 19 / 32, 16384 36 / 122; 16 items of 8 queries, 2048 22 / 21 (120 MB), 8192
@@ -1189,6 +1190,12 @@ struct Plan {
     int64_t bytes;  // of the workspace
 };
 
+// Whether a call's launches hold its workgroups and, joined, a wave for each of its rows.
+bool launches_fit(const Plan &c, int64_t rows)
+{
+    return c.own.blocks + c.common.blocks < kMostBlocks && (c.bytes == 0 || rows < kMostBlocks * kWaves);
+}
+
 // Tiles of few rows, where the sequences have few on average.  64 sequences of 1024 keys, us, few / 128 rows, whole:
 // heads of 128, 4 rows 45 / 46, 16 53 / 47, 32 64 / 48; of 64, 20 / 28, 19 / 28, 22 / 28; of 256, 88 / 103, 112 / 103, 134 / 103.
 // (A sequence has floor(rows / 32) + 1 units, so that 32 rows make one of two units none.)
@@ -1209,13 +1216,13 @@ Plan plan_packed(int64_t tokens_q, int64_t tokens_k, int64_t sequences, int64_t 
 // Against as many places for each as if alone, 80 calls of random sizes take 0.97 of the time: heads of 128 over 8,
 // 64 items of 1 query, prefix 8192, own 1024 46.4 -> 40.5 us, 6 of 8 over 34625, own 372 100 -> 76; heads of 256, 7
 // items of 5, 4290, own 1536 38 -> 34; but 116 of 8 over 35576, own 774 428 -> 455.
-Plan plan_prefix(int64_t batch, int64_t tokens_q, int64_t tokens_k, int64_t prefix, int64_t heads, int64_t kv_heads,
-                 int64_t head_dim, bool causal)
+Plan plan_batch(int64_t batch, int64_t tokens_q, int64_t tokens_k, int64_t prefix, int64_t heads, int64_t kv_heads,
+                int64_t head_dim, bool causal, bool may_share)
 {
     Plan c{};
     const int64_t rows = tokens_q * (heads / kv_heads), tile = rows <= kFewRows ? kFewRows : kRows;
     const int64_t tiles = (rows + tile - 1) / tile * batch;
-    if (batch > 1 && rows < kRows && prefix) {
+    if (may_share && batch > 1 && rows < kRows && prefix) {
         const int64_t of_all = batch * rows <= kFewRows ? kFewRows : kRows;
         const int64_t stacked = (batch * rows + of_all - 1) / of_all, room = places(kFewRows, head_dim) / kv_heads;
         const int64_t theirs = stacked * turns(of_all, prefix, head_dim), others = tiles * turns(tile, tokens_k, head_dim);
@@ -1234,6 +1241,15 @@ Plan plan_prefix(int64_t batch, int64_t tokens_q, int64_t tokens_k, int64_t pref
     if (c.shared) c.bytes += parts_bytes(c.common, kv_heads, head_dim);
     c.groups = groups_of(c.own, prefix + tokens_k, causal, kv_heads);
     return c;
+}
+
+// A prefix is shared where its join and its tiles beside the items' own still fit.
+Plan plan_prefix(int64_t batch, int64_t tokens_q, int64_t tokens_k, int64_t prefix, int64_t heads, int64_t kv_heads,
+                 int64_t head_dim, bool causal)
+{
+    const Plan c = plan_batch(batch, tokens_q, tokens_k, prefix, heads, kv_heads, head_dim, causal, true);
+    if (!c.shared || launches_fit(c, batch * tokens_q * heads)) return c;
+    return plan_batch(batch, tokens_q, tokens_k, prefix, heads, kv_heads, head_dim, causal, false);
 }
 
 Parts place(const Cut &c, int64_t kv_heads, int64_t head_dim, void *workspace)
@@ -1297,9 +1313,7 @@ void launch(Params &p, const Plan &c, void *workspace, hipStream_t s)
 // The launches, once the operands are checked and p holds them.
 int run(const char *what, Params &p, const Plan &c, int64_t head_dim, void *workspace, int64_t workspace_bytes, void *stream)
 {
-    // a launch holds fewer than 2^32 threads
-    const int64_t most = (int64_t{1} << 32) / (kWaves * 64);
-    if (c.own.blocks + c.common.blocks >= most || (c.bytes && (p.qo ? 1 : p.seqs) * static_cast<int64_t>(p.tq) * p.heads >= most * kWaves))
+    if (!launches_fit(c, (p.qo ? 1 : p.seqs) * static_cast<int64_t>(p.tq) * p.heads))
         return fail(LTXK_E_ARG, "%s: too many row tiles", what);
     if (c.bytes && (!workspace || !aligned16(workspace) || workspace_bytes < c.bytes))
         return fail(LTXK_E_ARG, "%s: the workspace must hold ltxk_%s_workspace_bytes, 16-byte aligned", what, what);
@@ -1352,7 +1366,8 @@ extern "C" int64_t ltxk_packed_attention_workspace_bytes(int64_t tokens_q, int64
                                                          int64_t heads, int64_t kv_heads, int64_t head_dim)
 {
     if (sequences <= 0 || sequences > kMostItems || !sizes_fit(1, tokens_q, tokens_k, 0, heads, kv_heads, head_dim)) return 0;
-    return plan_packed(tokens_q, tokens_k, sequences, heads, kv_heads, head_dim, false).bytes;
+    const Plan c = plan_packed(tokens_q, tokens_k, sequences, heads, kv_heads, head_dim, false);
+    return launches_fit(c, tokens_q * heads) ? c.bytes : 0;
 }
 
 extern "C" int ltxk_packed_attention(void *out, const void *q, int64_t q_tstride, const void *k, int64_t k_tstride,
@@ -1407,7 +1422,8 @@ extern "C" int64_t ltxk_prefix_attention_workspace_bytes(int64_t batch, int64_t 
                                                          int64_t heads, int64_t kv_heads, int64_t head_dim)
 {
     if (batch <= 0 || batch > kMostItems || !sizes_fit(batch, tokens_q, tokens_k, prefix, heads, kv_heads, head_dim)) return 0;
-    return plan_prefix(batch, tokens_q, tokens_k, prefix, heads, kv_heads, head_dim, false).bytes;
+    const Plan c = plan_prefix(batch, tokens_q, tokens_k, prefix, heads, kv_heads, head_dim, false);
+    return launches_fit(c, batch * tokens_q * heads) ? c.bytes : 0;
 }
 
 extern "C" int ltxk_prefix_attention(void *out, const void *q, int64_t q_bstride, int64_t q_tstride, const void *k,
