@@ -83,8 +83,6 @@ def key_split_partials(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, parts:
 
 _dispatch_modes, _transform = torch._C._len_torch_dispatch_stack, torch._C._functorch.peek_interpreter_stack
 _tracing = torch._C._is_tracing
-_mode, _PROXY = torch._C._get_dispatch_mode, torch._C._TorchDispatchModeKey.PROXY
-_wrapped = torch._C._functorch.is_functorch_wrapped_tensor
 
 
 def eager_call() -> bool:
@@ -529,16 +527,7 @@ def reads_blocks(ff: torch.nn.Module, *inputs: torch.Tensor | None) -> bool:
 def _no_gradient(*inputs: torch.Tensor | None) -> None:
     """Refuses inputs of 8-bit layers that something is to be recorded of: a gradient, a
     forward-mode tangent, what a function transform or a tracer sees.  All would be lost."""
-    lost = "trace" if _tracing() or _mode(_PROXY) is not None else None
-    for x in inputs:
-        if x is None:
-            pass
-        elif x.requires_grad and torch.is_grad_enabled():
-            lost = "gradient (run under torch.no_grad())"
-        elif _wrapped(x):
-            lost = "function transform"
-        elif forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None:
-            lost = "forward-mode derivative"
+    lost = ltxk.lost_record(*inputs)
     if lost is not None:
         raise RuntimeError(f"8-bit layers are for inference: they record no {lost}")
 

@@ -15,6 +15,7 @@ import sys
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_PATH = pathlib.Path(__file__).resolve().with_name("libltxk.so")
 
@@ -1006,6 +1007,44 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: in
     return out
 
 
+_dispatch_modes, _transform = torch._C._len_torch_dispatch_stack, torch._C._functorch.peek_interpreter_stack
+_tracing = torch._C._is_tracing
+_mode, _PROXY = torch._C._get_dispatch_mode, torch._C._TorchDispatchModeKey.PROXY
+_wrapped = torch._C._functorch.is_functorch_wrapped_tensor
+
+
+def lost_record(*inputs: torch.Tensor | None) -> str | None:
+    """What is to be recorded of a call on `inputs` and would be lost in one that torch's dispatcher does not see: a
+    gradient, a forward-mode tangent, what a function transform or a tracer sees."""
+    lost = "trace" if _tracing() or _mode(_PROXY) is not None else None
+    grad, dual = torch.is_grad_enabled(), forward_ad._current_level >= 0
+    for x in inputs:
+        if not isinstance(x, torch.Tensor):
+            pass
+        elif grad and x.requires_grad:
+            lost = "gradient (run under torch.no_grad())"
+        elif _wrapped(x):
+            lost = "function transform"
+        elif dual and forward_ad.unpack_dual(x).tangent is not None:
+            lost = "forward-mode derivative"
+    return lost
+
+
+def _inference_only(what: str, *inputs: torch.Tensor) -> None:
+    # the common case in a few reads: nothing records
+    if not _dispatch_modes() and _transform() is None and forward_ad._current_level < 0 and not _tracing():
+        if not torch.is_grad_enabled():
+            return
+        for x in inputs:
+            if getattr(x, "requires_grad", False):
+                break
+        else:
+            return
+    lost = lost_record(*inputs)
+    if lost is not None:
+        raise RuntimeError(f"{what} is for inference: it records no {lost}")
+
+
 PACKED_HEAD_DIMS = (64, 128, 256)
 
 
@@ -1071,9 +1110,11 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: i
     `window` only that many of them; else all of its sequence's.  One that sees none gives zeros.
 
     q, k and v may be columns of wider rows.  What a mask closes, and rows of no sequence, may hold anything.  Rows of
-    `out` that belong to no sequence are left as they are (undefined in a fresh result)."""
+    `out` that belong to no sequence are left as they are (undefined in a fresh result).  For inference: operands of
+    which a gradient is to be recorded are refused (run under torch.no_grad())."""
     if getattr(q, "ndim", 0) != 2:
         raise ValueError("q must be a (T, H*Dh) tensor")
+    _inference_only("packed_attention", q, k, v)
     tq, d = q.shape
     kv_heads, dh = _grouped_heads(d, heads, kv_heads)
     qt = _packed_rows(q, "q", d)
@@ -1121,9 +1162,11 @@ def prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, prefix_k
     queries in front of a shorter item's first token (padding) give zeros.  Else it sees the prefix and all own keys.
 
     Where few queries an item make it worth it, the prefix is read for all of them at once.  q, k, v and the prefix may be
-    columns of wider rows, k and v views of a larger cache.  What lies past an item's length may hold anything."""
+    columns of wider rows, k and v views of a larger cache.  What lies past an item's length may hold anything.  For
+    inference, as `packed_attention`."""
     if getattr(q, "ndim", 0) != 3 or getattr(k, "ndim", 0) != 3:
         raise ValueError("q, k and v must be (B, T, H*Dh) tensors")
+    _inference_only("prefix_attention", q, k, v, prefix_k, prefix_v)
     (b, tq, d), tk = q.shape, k.shape[1]
     kv_heads, dh = _grouped_heads(d, heads, kv_heads)
     qb, qt = _attention_rows(q, "q", b, tq, d)
