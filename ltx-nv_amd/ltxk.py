@@ -1046,6 +1046,7 @@ def _inference_only(what: str, *inputs: torch.Tensor) -> None:
 
 
 PACKED_HEAD_DIMS = (64, 128, 256)
+MAX_WINDOW = 1 << 29  # all keys that a call may have: what an int64 does not hold would come out as another window
 
 
 def _grouped_heads(width: int, heads: int, kv_heads: int | None) -> tuple[int, int]:
@@ -1146,7 +1147,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: i
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
     rc = load().ltxk_packed_attention(out.data_ptr(), q.data_ptr(), qt, k.data_ptr(), kt, v.data_ptr(), vt,
                                       offsets.data_ptr(), k_offsets.data_ptr(), seqs, tq, tk, heads, kv_heads, dh, causal,
-                                      window or 0, dh ** -0.5 if scale is None else scale, _ptr(ws), nbytes, _stream(q))
+                                      min(window or 0, MAX_WINDOW), dh ** -0.5 if scale is None else scale, _ptr(ws),
+                                      nbytes, _stream(q))
     _check_rc(rc, "packed_attention")
     return out
 
