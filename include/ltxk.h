@@ -413,7 +413,9 @@ int64_t ltxk_packed_attention_workspace_bytes(int64_t tokens_q, int64_t tokens_k
  * those with i - j < window (a window needs the mask); else all of its sequence's.
  * A query that sees no key gives zeros.  Keys and values that no query of a sequence
  * sees, and those that a mask closes, change nothing, whatever they hold.  Rows of out
- * that belong to no sequence are left as they are.
+ * that belong to no sequence are left as they are.  A value that is not finite makes what
+ * sees it not finite, however little it weighs, and so may values of which 2^6 times the sum
+ * of magnitudes passes the largest fp32.
  * q is bf16 at q + t*q_tstride + h*head_dim (elements; multiples of 8, at least
  * heads*head_dim, below 2^23), k and v likewise with kv_heads; out is contiguous
  * [tokens_q, heads*head_dim] and overlaps no operand.  Scores, softmax and sums are

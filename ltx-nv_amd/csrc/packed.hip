@@ -15,20 +15,23 @@
 // 128 rows share key tiles in LDS, 32 rows a wave (the scores transposed, so that a lane has a
 // row's weights as the second product takes them).  Up to 32 rows are attended by all four
 // waves, each over keys of its own.  What bounds them:
-// * Tiles, long: power and, with half of the time, what is not a product.  6144 x 6144 tokens,
-//   32 heads of 128, no mask, 610 us (1.01 PFLOP/s; ltxk_attention 621 on the same card), on zeros 524
-//   (430).  Causal, 12288 tokens over 8 key heads: 1140-1250 us from card to card, 0.99-1.08.  Heads of 256 in
-//   a window of 1024: 353-430 us for 20078 tokens, 0.68-0.83.
+// * Tiles, long: with half of the time what is not a product (the matrix cores are busy 48 %, with heads of
+//   256 42 %), then power.  6144 x 6144 tokens, 32 heads of 128, no mask, 610 us (1.01 PFLOP/s; ltxk_attention
+//   599-621), of which the products at a large one's 1.5 PFLOP/s would take 412 and zeros, which draw less power,
+//   521 (ltxk_attention 427).  Causal, 12288 tokens over 8 key heads: 1140-1260 us from card to card, 0.98-1.08.
+//   Heads of 256 in a window of 1024: 353-430 us for 20078 tokens, 0.68-0.83.
 // * Tiles, few: the latency of a tile's chain of products, exponentials and products again, about
 //   1.4 us for 64 keys (32 with heads of 256) where no second workgroup shares the unit, with 3 us ahead (which
 //   sequence, first keys, queries) and 1-2 behind.  Deeper rings of tiles (three on their way instead of one) change
 //   nothing; the weights of a tile beside the scores of the next, 47 against 51 us on prompts of 1024 and
 //   333 tokens, heads of 256, but 5 % slower where the chip is full; two groups of waves, 38.
-// * Few rows: memory, 5.5 TB/s on 64 tokens over 125624 keys (97 us with the join of their parts, 5); short ones
-//   the same latencies.
+// * Few rows: memory, 5.3-5.4 TB/s on 64 tokens over 125624 keys (516 MB in 95-98 us with the join of their parts, 5;
+//   5.7 without); short ones the same latencies.
 // * A prefix beside own keys: 64 items of a query, 32 heads of 128 over 8, prefix 8192, own up to 1024, 33 us and 6.5 to
 //   join: the latencies of both kinds of tile on places that they share.
-// * Units that turn out to be none, which lengths on the device cost: 2-3 us of a workgroup's place each.
+// * Units that turn out to be none, which lengths on the device cost: 2-3 us of a workgroup's place each.  A call is
+//   cut by its keys, of which a window leaves few, and its join then finds nothing to do: 4 tokens of 16 heads of 256 in
+//   a window of 1024 of 4096 keys 18.4 us, over these 1024 alone 16.1; one of 8 heads of 128, of 100000, 12.7 / 12.6.
 #include "flash_tiles.h"
 
 #include <cfloat>
@@ -959,8 +962,8 @@ __device__ __forceinline__ void attend_few(const Params &p, int block, FewLds<D>
 }
 
 // Parameters of which the compiler knows what the kind of call fixes, so that it keeps fewer in
-// scalar registers, which spill all the same (guidance 38.7 -> 37.7 us, 12288 tokens 1220 -> 1213; a prefix and own
-// keys side by side 50.6 -> 46.7, 42.9 -> 40, 43.4 -> 37.9).
+// scalar registers, of which up to 88 spill all the same, 96-156 with a prefix and own keys side by side (guidance
+// 38.7 -> 37.7 us, 12288 tokens 1220 -> 1213; side by side 50.6 -> 46.7, 42.9 -> 40, 43.4 -> 37.9).
 enum Call { kSequences, kItems, kItemsOwn, kPrefixOfAll };
 template <Call CALL>
 __device__ __forceinline__ Params known(const Params &given)

@@ -1110,8 +1110,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: i
     has more keys than queries, the queries are its newest tokens.  Causal, a query sees the keys up to its own, with
     `window` only that many of them; else all of its sequence's.  One that sees none gives zeros.
 
-    q, k and v may be columns of wider rows.  What a mask closes, and rows of no sequence, may hold anything.  Rows of
-    `out` that belong to no sequence are left as they are (undefined in a fresh result).  For inference: operands of
+    q, k and v may be columns of wider rows.  What a mask closes, and rows of no sequence, may hold anything.  `out`
+    overlaps no operand; its rows that belong to no sequence are left as they are (undefined in a fresh result).  For inference: operands of
     which a gradient is to be recorded are refused (run under torch.no_grad())."""
     if getattr(q, "ndim", 0) != 2:
         raise ValueError("q must be a (T, H*Dh) tensor")
@@ -1164,8 +1164,8 @@ def prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, prefix_k
     queries in front of a shorter item's first token (padding) give zeros.  Else it sees the prefix and all own keys.
 
     Where few queries an item make it worth it, the prefix is read for all of them at once.  q, k, v and the prefix may be
-    columns of wider rows, k and v views of a larger cache.  What lies past an item's length may hold anything.  For
-    inference, as `packed_attention`."""
+    columns of wider rows, k and v views of a larger cache.  What lies past an item's length may hold anything.  `out`
+    overlaps no operand.  For inference, as `packed_attention`."""
     if getattr(q, "ndim", 0) != 3 or getattr(k, "ndim", 0) != 3:
         raise ValueError("q, k and v must be (B, T, H*Dh) tensors")
     _inference_only("prefix_attention", q, k, v, prefix_k, prefix_v)
